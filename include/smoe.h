@@ -497,6 +497,32 @@ int smoe_moe_prefill_block(smoe_handle* h, const smoe_expert_shape* shape, const
                            float* hidden_out, void* workspace, uint64_t workspace_bytes);
 
 /* ------------------------------------------------------------------ */
+/* Around the block: norms, 8-bit rows                                  */
+/* ------------------------------------------------------------------ */
+
+/* Per row t < n_tokens: r = x[t] + residual[t], y = r / sqrt(mean(r^2) +
+ * eps) * norm_w, the step between two blocks that smoe_moe_decode_layers
+ * chains for one token (rms_norm_bf16_n_tokens_cpu, backend/cpu/mod.rs:
+ * 406-430, after the residual's addition), for the rows of a batch or a
+ * prompt. sum_out[t] = r; out[t] = y; out_q[t] = y in 8 bits with one scale
+ * per q_group values (32, 64 or 128; 0: one per row), the rows smoe_qmm_i8
+ * takes: scale = max|y| / 127, code = y / scale rounded to nearest even; a
+ * group with an infinity or NaN has scale NaN and codes 0, one whose largest
+ * magnitude is below 2^-119 scale 0 and codes 0.
+ * x: device [n_tokens, hidden], bf16 when x_is_bf16 else f32; residual:
+ * device f32 or NULL (r = x); norm_w: device bf16[hidden] or NULL (ones);
+ * sum_out: device f32, out: device bf16 when out_is_bf16 else f32, out_q:
+ * device int8, each [n_tokens, hidden] or NULL, out and out_q not both;
+ * out_scales: device f32[n_tokens, hidden / q_group], with out_q. All 16-byte
+ * aligned. sum_out or out may be the buffer of x or residual where the types
+ * are the same; else outputs overlap nothing. hidden 1..16384 (a multiple of
+ * q_group), else SMOE_ERR_UNSUPPORTED_SHAPE (SMOE_ERR_IN_DIM_NOT_MULTIPLE).
+ * Enqueue-only, allocates nothing, capturable in a HIP graph. */
+int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* residual, const void* norm_w,
+                 float eps, uint32_t n_tokens, uint32_t hidden, float* sum_out, void* out, int out_is_bf16,
+                 int8_t* out_q, float* out_scales, uint32_t q_group);
+
+/* ------------------------------------------------------------------ */
 /* Expert arena loader: packed_experts/layer_NN.bin -> device memory    */
 /* ------------------------------------------------------------------ */
 

@@ -35,6 +35,19 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+def _misfit(device, *checks):
+    """Whether a tensor is not what a call reads or writes: checks of (tensor
+    or None, element types, elements it has to hold), dense and on `device`."""
+    return any(t is not None and (str(t.dtype).rpartition(".")[2] not in types or not t.is_contiguous()
+                                  or t.device.type != "cuda" or t.device.index != device or t.numel() < n)
+               for t, types, n in checks)
+
+
+_F32 = ("float32",)
+_BF16 = ("bfloat16", "int16", "uint16")  # bf16 also as its bits
+_INVALID = _abi.CODES["SMOE_ERR_INVALID_ARG"]
+
+
 @dataclass(frozen=True)
 class ExpertLayout:
     """Packed-expert layout `[gate | up | down]`, each block
@@ -294,6 +307,21 @@ class Kernels:
                                            _ptr(weights), _ptr(x), int(x_is_bf16), n_tokens, k, _ptr(shared),
                                            _ptr(gate), _ptr(h_mid), _ptr(hidden_out), _ptr(workspace),
                                            0 if workspace is None else workspace.numel() * workspace.element_size())
+
+    # -- around the block ---------------------------------------------------------
+    def rmsnorm(self, x, residual, norm_w, eps, n_tokens, hidden, sum_out=None, out=None, out_q=None,
+                out_scales=None, q_group=0):
+        """r = x + residual (sum_out), RMSNorm(r) * norm_w as f32 or bf16 (out, by
+        its type) and / or in 8 bits with scales (out_q, out_scales; q_group 0:
+        one scale per row). x: f32 or bf16 rows."""
+        n = n_tokens * hidden
+        if _misfit(self.device, (x, _F32 + _BF16, n), (residual, _F32, n), (norm_w, _BF16, hidden), (sum_out, _F32, n),
+                   (out, _F32 + _BF16, n), (out_q, ("int8",), n),
+                   (out_scales, _F32, n_tokens * (hidden // (q_group or hidden or 1)))):
+            return _INVALID
+        return _lib.smoe_rmsnorm(self.h, _ptr(x), int(x is not None and x.element_size() == 2), _ptr(residual),
+                                 _ptr(norm_w), C.c_float(eps), n_tokens, hidden, _ptr(sum_out), _ptr(out),
+                                 int(out is not None and out.element_size() == 2), _ptr(out_q), _ptr(out_scales), q_group)
 
     # -- expert files -------------------------------------------------------------
     def load_file(self, path, dst, offset=0, nbytes=0):

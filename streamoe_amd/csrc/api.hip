@@ -941,6 +941,34 @@ int smoe_moe_prefill_block(smoe_handle* h, const smoe_expert_shape* shape, const
   return hip_status(launch_prefill(a, (uint32_t)n_cu, h->stream));
 }
 
+int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* residual, const void* norm_w,
+                 float eps, uint32_t n_tokens, uint32_t hidden, float* sum_out, void* out, int out_is_bf16,
+                 int8_t* out_q, float* out_scales, uint32_t q_group) {
+  if (!h || !x || !n_tokens || !hidden || (!out && !out_q) || (!out_q != !out_scales)) return SMOE_ERR_INVALID_ARG;
+  if (out_q && q_group) {
+    if (int rc = check_group(q_group)) return rc;
+    if (hidden % q_group) return SMOE_ERR_IN_DIM_NOT_MULTIPLE;
+  }
+  if (hidden > kNormMaxHidden || n_tokens > 0x7FFFFFFFu) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  for (const void* p : {x, (const void*)residual, norm_w, (const void*)sum_out, (const void*)out, (const void*)out_q,
+                        (const void*)out_scales})
+    if (!aligned(p, 0, 16)) return SMOE_ERR_MISALIGNED;
+  if (int rc = use_device(h)) return rc;
+  NormArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.w = (const uint16_t*)norm_w;
+  a.eps = eps;
+  a.hidden = hidden;
+  a.sum = sum_out;
+  a.out = out;
+  a.out_bf16 = out_is_bf16;
+  a.q = out_q;
+  a.scales = out_scales;
+  a.group = q_group;
+  return hip_status(launch_rmsnorm(a, x_is_bf16 != 0, n_tokens, h->stream));
+}
+
 int smoe_synth_experts(smoe_handle* h, void* base, uint32_t n_experts, uint64_t stride,
                        const smoe_expert_shape* shape, uint64_t seed, float scale_sigma,
                        float bias_sigma) {

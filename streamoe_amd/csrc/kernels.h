@@ -289,6 +289,22 @@ hipError_t launch_ph_down(const BlobGeom& routed, const BlobGeom& shared, const 
                           const FfnTable& tab_val, uint32_t n_slots, const float* act, const float* h_mid,
                           const float* shared_out, float* hidden_out, hipStream_t st, bool ordered = false,
                           uint32_t n_tokens = 1, uint32_t astride = 0);
+// Residual addition + RMSNorm + 8-bit rows (norm.hip); row t at + t hidden.
+constexpr uint32_t kNormMaxHidden = 16384;  // 64 values per thread
+struct NormArgs {
+  const void* x;          // [n, hidden] f32 or bf16
+  const float* residual;  // or null
+  const uint16_t* w;      // bf16 [hidden], or null
+  float eps;
+  uint32_t hidden;
+  float* sum;             // x + residual, or null
+  void* out;              // f32 or bf16, or null
+  int out_bf16;
+  int8_t* q;              // codes, or null
+  float* scales;          // [n, hidden / group], one per row with group 0
+  uint32_t group;         // 0, 32, 64 or 128
+};
+hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
 // Streaming-read diagnostic over `bytes` (multiple of 16) with
 // kStreamBlocks blocks; sink: kStreamBlocks u32.
 constexpr uint32_t kStreamBlocks = 2048;

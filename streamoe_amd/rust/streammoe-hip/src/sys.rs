@@ -6,6 +6,9 @@
 
 use std::os::raw::{c_char, c_int, c_void};
 
+/// The header's 8-bit codes.
+pub type int8_t = i8;
+
 pub const SMOE_MAX_K: u32 = 16;
 pub const SMOE_ABI_VERSION: u32 = 2;
 
@@ -149,6 +152,10 @@ extern "C" {
                                   x: *const c_void, x_is_bf16: c_int, n_tokens: u32, k: u32,
                                   shared_expert: *const c_void, shared_gate: *const f32, h_mid: *const f32,
                                   hidden_out: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn smoe_rmsnorm(h: *mut smoe_handle, x: *const c_void, x_is_bf16: c_int, residual: *const f32,
+                        norm_w: *const c_void, eps: f32, n_tokens: u32, hidden: u32, sum_out: *mut f32,
+                        out: *mut c_void, out_is_bf16: c_int, out_q: *mut int8_t, out_scales: *mut f32,
+                        q_group: u32) -> c_int;
     pub fn smoe_layer_file_layout(file_bytes: u64, n_experts: u32, hidden: u32, inter: u32, group: u32,
                                   declared_size: u64, declared_stride: u64,
                                   out: *mut smoe_file_layout) -> c_int;
