@@ -523,6 +523,66 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
                  int8_t* out_q, float* out_scales, uint32_t q_group);
 
 /* ------------------------------------------------------------------ */
+/* Beam search behind the LM head                                       */
+/* ------------------------------------------------------------------ */
+
+/* Device workspace bytes smoe_beam_select needs (0 for zero sizes). */
+uint64_t smoe_beam_select_workspace_size(uint32_t n_requests, uint32_t n_beams, uint32_t vocab, uint32_t n_picks);
+
+/* One step of n_requests beam searches: per request the n_picks best
+ * continuations (row, token) of its n_beams rows of logits by
+ *   scores[row] + logits[row, token] - log sum_v exp(logits[row, v]),
+ * best first. Ties go to the lower row, then the lower token; values are
+ * compared in f64 and, within a row, by their logits. A continuation without a
+ * value (a logit of -inf or NaN, any of a row that has only those or holds
+ * +inf, any of a row whose score is -inf or NaN) counts as -inf. A row with
+ * done[row] != 0 has ended: it keeps its score with pad_token, its other
+ * continuations count as -inf.
+ * logits: device f32[n_requests * n_beams, vocab] (16-byte aligned); scores:
+ * device f32[n_requests * n_beams]; done: device uint8[n_requests * n_beams]
+ * or NULL. out_scores: device f32[n_requests, n_picks]; out_rows: device int32,
+ * the logits' row a pick continues (request * n_beams + beam, what
+ * smoe_beam_reorder takes); out_tokens: device int32. out_scores may be
+ * scores when n_picks == n_beams; nothing else overlaps. workspace: device, of
+ * smoe_beam_select_workspace_size bytes, 256-byte aligned, one call's at a
+ * time. n_beams 1..16, vocab up to 2^28 (SMOE_ERR_UNSUPPORTED_SHAPE); n_picks
+ * 1..32 and at most n_beams * vocab (SMOE_ERR_BAD_K). No counterpart in the
+ * reference, whose sampling is greedy (io/gpu_lm_head.rs:130-193). The same
+ * bits on every run. Enqueue-only, allocates nothing, capturable in a HIP
+ * graph. */
+int smoe_beam_select(smoe_handle* h, const float* logits, const float* scores, const uint8_t* done,
+                     uint32_t pad_token, uint32_t n_requests, uint32_t n_beams, uint32_t vocab,
+                     uint32_t n_picks, float* out_scores, int32_t* out_rows, int32_t* out_tokens,
+                     void* workspace, uint64_t workspace_bytes);
+
+/* One state tensor of the beams, as bytes: row r holds n_pieces pieces of
+ * piece_bytes, piece p at src + r * src_row_stride + p * src_piece_stride
+ * (the used part of a cache of several heads; one piece for a dense row). */
+typedef struct {
+  const void* src; /* device */
+  void* dst;       /* device, another buffer */
+  uint64_t src_row_stride;
+  uint64_t dst_row_stride;
+  uint64_t src_piece_stride;
+  uint64_t dst_piece_stride;
+  uint64_t piece_bytes;
+  uint32_t n_pieces;
+  uint32_t reserved; /* 0 */
+} smoe_beam_state;
+
+/* dst row i = src row rows[i] for i < n_rows, in each of n_states tensors
+ * (states: host array, read during the call; rows: device int32[n_rows], each
+ * in [0, src_rows)). A source row may be taken any number of times; bytes of
+ * dst outside the pieces stay. A row index out of range is found on the
+ * device: its rows stay as they were and the next smoe_sync returns
+ * SMOE_ERR_INVALID_ARG. src and dst of a state must not overlap, nor rows or
+ * pieces of dst (SMOE_ERR_INVALID_ARG); a state's dst must not overlap
+ * another state. Addresses and strides of any alignment (16 bytes are the
+ * fast case). Enqueue-only, allocates nothing, capturable in a HIP graph. */
+int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_states, const int32_t* rows,
+                      uint32_t n_rows, uint32_t src_rows);
+
+/* ------------------------------------------------------------------ */
 /* Expert arena loader: packed_experts/layer_NN.bin -> device memory    */
 /* ------------------------------------------------------------------ */
 

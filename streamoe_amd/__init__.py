@@ -115,6 +115,33 @@ class QuantWeights:
 
 
 @dataclass
+class BeamState:
+    """One state tensor of the beams for Kernels.beam_reorder: rows [n, bytes ..]
+    or, with the pieces of a row on axis 1, [n, pieces, room ..]; the first
+    `used` bytes of every piece are copied from src to dst (default: all). Axes
+    from the last piece axis on are dense; rows and pieces may have any stride."""
+
+    src: object
+    dst: object
+    used: int = None
+
+    def c(self):
+        s, d = self.src, self.dst
+        if (s.device != d.device or s.device.type != "cuda" or s.dtype != d.dtype or s.dim() not in (2, 3)
+                or s.shape[1:] != d.shape[1:] or s.stride(-1) != 1 or d.stride(-1) != 1):
+            raise SmoeError(_INVALID, "BeamState")
+        size = s.element_size()
+        pieces = s.shape[1] if s.dim() == 3 else 1
+        room = s.shape[-1] * size
+        used = room if self.used is None else self.used
+        if not 0 <= used <= room:
+            raise SmoeError(_INVALID, "BeamState: used")
+        piece = (lambda t: t.stride(1) * size) if s.dim() == 3 else (lambda t: 0)
+        return _abi.BeamStateC(s.data_ptr(), d.data_ptr(), s.stride(0) * size, d.stride(0) * size, piece(s), piece(d),
+                               used, pieces, 0)
+
+
+@dataclass
 class ExpertPayload:
     """Per-token host inputs of a K-expert dispatch (expert_forward.rs:123-139)."""
 
@@ -322,6 +349,35 @@ class Kernels:
         return _lib.smoe_rmsnorm(self.h, _ptr(x), int(x is not None and x.element_size() == 2), _ptr(residual),
                                  _ptr(norm_w), C.c_float(eps), n_tokens, hidden, _ptr(sum_out), _ptr(out),
                                  int(out is not None and out.element_size() == 2), _ptr(out_q), _ptr(out_scales), q_group)
+
+    # -- beam search --------------------------------------------------------------
+    def beam_select_workspace_size(self, n_requests, n_beams, vocab, n_picks):
+        return _lib.smoe_beam_select_workspace_size(n_requests, n_beams, vocab, n_picks)
+
+    def beam_select(self, logits, scores, done, pad_token, n_requests, n_beams, vocab, n_picks, out_scores, out_rows,
+                    out_tokens, workspace):
+        """The n_picks best continuations of each request's beams (value, row of
+        the logits, token); done: uint8 flags of ended beams, or None."""
+        rows, picks = n_requests * n_beams, n_requests * n_picks
+        if _misfit(self.device, (logits, _F32, rows * vocab), (scores, _F32, rows), (done, ("uint8", "bool"), rows),
+                   (out_scores, _F32, picks), (out_rows, ("int32",), picks), (out_tokens, ("int32",), picks)):
+            return _INVALID
+        return _lib.smoe_beam_select(self.h, _ptr(logits), _ptr(scores), _ptr(done), pad_token, n_requests, n_beams,
+                                     vocab, n_picks, _ptr(out_scores), _ptr(out_rows), _ptr(out_tokens),
+                                     _ptr(workspace),
+                                     0 if workspace is None else workspace.numel() * workspace.element_size())
+
+    def beam_reorder(self, states, rows):
+        """dst row i = src row rows[i] of every BeamState, for the rows of `rows`
+        (int32, as beam_select's out_rows)."""
+        n = rows.numel()
+        if not states or _misfit(self.device, (rows, ("int32",), 1)):
+            return _INVALID
+        src_rows = min(s.src.shape[0] for s in states)
+        if any(s.dst.shape[0] < n or s.dst.device.index != self.device for s in states):
+            return _INVALID
+        arr = (_abi.BeamStateC * len(states))(*[s.c() for s in states])
+        return _lib.smoe_beam_reorder(self.h, arr, len(states), _ptr(rows), n, src_rows)
 
     # -- expert files -------------------------------------------------------------
     def load_file(self, path, dst, offset=0, nbytes=0):

@@ -85,6 +85,20 @@ class Layer(C.Structure):
     ]
 
 
+class BeamStateC(C.Structure):
+    _fields_ = [
+        ("src", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("src_row_stride", C.c_uint64),
+        ("dst_row_stride", C.c_uint64),
+        ("src_piece_stride", C.c_uint64),
+        ("dst_piece_stride", C.c_uint64),
+        ("piece_bytes", C.c_uint64),
+        ("n_pieces", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
 class FileLayout(C.Structure):
     _fields_ = [
         ("bits", C.c_uint32),
@@ -136,6 +150,9 @@ PROTOTYPES = {
     "smoe_moe_prefill_block": (_I, [_P, C.POINTER(ExpertShape), _P, _U64, _U32, _P, _P, _P, _I, _U32, _U32, _P,
                                     _P, _P, _P, _P, _U64]),
     "smoe_rmsnorm": (_I, [_P, _P, _I, _P, _P, C.c_float, _U32, _U32, _P, _P, _I, _P, _P, _U32]),
+    "smoe_beam_select_workspace_size": (_U64, [_U32, _U32, _U32, _U32]),
+    "smoe_beam_select": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _P, _P, _U64]),
+    "smoe_beam_reorder": (_I, [_P, C.POINTER(BeamStateC), _U32, _P, _U32, _U32]),
     "smoe_layer_file_layout": (_I, [_U64, _U32, _U32, _U32, _U32, _U64, _U64, C.POINTER(FileLayout)]),
     "smoe_load_file": (_I, [_P, C.c_char_p, _U64, _U64, _P, _U64, C.POINTER(_U64)]),
     "smoe_stream_read": (_I, [_P, _P, C.c_uint64, _P]),

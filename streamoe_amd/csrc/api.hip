@@ -969,6 +969,106 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
   return hip_status(launch_rmsnorm(a, x_is_bf16 != 0, n_tokens, h->stream));
 }
 
+static int check_beam(uint32_t n_requests, uint32_t n_beams, uint32_t vocab, uint32_t n_picks) {
+  if (!n_requests || !n_beams || !vocab) return SMOE_ERR_INVALID_ARG;
+  if (n_beams > kBeamMaxBeams || vocab > kBeamMaxVocab) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (n_picks < 1 || n_picks > kBeamMaxPicks || n_picks > (uint64_t)n_beams * vocab) return SMOE_ERR_BAD_K;
+  // One block per row and slice.
+  if ((uint64_t)n_requests * n_beams * kBeamMaxSlices > 0x7FFFFFFFull) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  return SMOE_OK;
+}
+
+uint64_t smoe_beam_select_workspace_size(uint32_t n_requests, uint32_t n_beams, uint32_t vocab, uint32_t n_picks) {
+  if (check_beam(n_requests, n_beams, vocab, n_picks)) return 0;
+  return beam_workspace(n_requests, n_beams, vocab, n_picks, nullptr, nullptr);
+}
+
+int smoe_beam_select(smoe_handle* h, const float* logits, const float* scores, const uint8_t* done,
+                     uint32_t pad_token, uint32_t n_requests, uint32_t n_beams, uint32_t vocab,
+                     uint32_t n_picks, float* out_scores, int32_t* out_rows, int32_t* out_tokens,
+                     void* workspace, uint64_t workspace_bytes) {
+  if (!h || !logits || !scores || !out_scores || !out_rows || !out_tokens || !workspace) return SMOE_ERR_INVALID_ARG;
+  if (int rc = check_beam(n_requests, n_beams, vocab, n_picks)) return rc;
+  if (done && pad_token >= vocab) return SMOE_ERR_INVALID_ARG;
+  if (out_scores == scores && n_picks != n_beams) return SMOE_ERR_INVALID_ARG;
+  if (!aligned(logits, 0, 16) || !aligned(scores, 0, 4) || !aligned(out_scores, 0, 4) || !aligned(out_rows, 0, 4) ||
+      !aligned(out_tokens, 0, 4) || !aligned(workspace, 0, 256))
+    return SMOE_ERR_MISALIGNED;
+  BeamArgs a{};
+  if (workspace_bytes < beam_workspace(n_requests, n_beams, vocab, n_picks, &a, (uint8_t*)workspace))
+    return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  if (int rc = use_device(h)) return rc;
+  a.logits = logits;
+  a.scores = scores;
+  a.done = done;
+  a.rows = n_requests * n_beams;
+  a.beams = n_beams;
+  a.vocab = vocab;
+  a.picks = n_picks;
+  a.pad = pad_token;
+  a.out_scores = out_scores;
+  a.out_rows = out_rows;
+  a.out_tokens = out_tokens;
+  return hip_status(launch_beam_select(a, h->stream));
+}
+
+// Bytes from the first to behind the last of rows x pieces; false: past 2^63.
+static bool beam_extent(uint32_t rows, uint64_t row, uint32_t pieces, uint64_t piece, uint64_t bytes, uint64_t* out) {
+  const unsigned __int128 e =
+      (unsigned __int128)(rows - 1) * row + (unsigned __int128)(pieces - 1) * piece + bytes;
+  *out = (uint64_t)e;
+  return e < ((unsigned __int128)1 << 63);
+}
+
+int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_states, const int32_t* rows,
+                      uint32_t n_rows, uint32_t src_rows) {
+  if (!h || !states || !n_states || !rows || !n_rows || !src_rows) return SMOE_ERR_INVALID_ARG;
+  if (!aligned(rows, 0, 4)) return SMOE_ERR_MISALIGNED;
+  // Two passes over the states: every one is checked before any is enqueued.
+  constexpr uint32_t kBatch = 64;
+  BeamCopy c[kBatch];
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass)
+      if (int rc = use_device(h)) return rc;
+    for (uint32_t i0 = 0; i0 < n_states; i0 += kBatch) {
+      uint32_t n = 0;
+      for (uint32_t i = i0; i < n_states && i < i0 + kBatch; ++i) {
+        const smoe_beam_state& s = states[i];
+        BeamCopy& o = c[n++];
+        o = {(const uint8_t*)s.src, (uint8_t*)s.dst,     s.src_row_stride, s.dst_row_stride, s.src_piece_stride,
+             s.dst_piece_stride,    s.piece_bytes,       s.n_pieces,       1u};
+        const uint64_t both = (uint64_t)(uintptr_t)s.src | (uint64_t)(uintptr_t)s.dst | s.src_row_stride |
+                              s.dst_row_stride | s.src_piece_stride | s.dst_piece_stride;
+        o.unit = both % 16 == 0 ? 16u : both % 4 == 0 ? 4u : 1u;
+        if (pass) continue;
+        if (!s.src || !s.dst || !s.n_pieces || s.reserved) return SMOE_ERR_INVALID_ARG;
+        if (!s.piece_bytes) continue;
+        uint64_t from, to, row, col;
+        if (!beam_extent(src_rows, s.src_row_stride, s.n_pieces, s.src_piece_stride, s.piece_bytes, &from) ||
+            !beam_extent(n_rows, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes, &to) ||
+            !beam_extent(1, 0, s.n_pieces, s.dst_piece_stride, s.piece_bytes, &row) ||
+            !beam_extent(n_rows, s.dst_row_stride, 1, 0, s.piece_bytes, &col))
+          return SMOE_ERR_INVALID_ARG;
+        const uint64_t src = (uint64_t)(uintptr_t)s.src, dst = (uint64_t)(uintptr_t)s.dst;
+        if (src < dst + to && dst < src + from) return SMOE_ERR_INVALID_ARG;
+        // Rows one after another, each holding its pieces, or the other way round.
+        const bool by_row = (n_rows == 1 || s.dst_row_stride >= row) &&
+                            (s.n_pieces == 1 || s.dst_piece_stride >= s.piece_bytes);
+        const bool by_piece = (s.n_pieces == 1 || s.dst_piece_stride >= col) &&
+                              (n_rows == 1 || s.dst_row_stride >= s.piece_bytes);
+        if (!by_row && !by_piece) return SMOE_ERR_INVALID_ARG;
+        if ((unsigned __int128)((s.piece_bytes >> 14) + 1) * s.n_pieces * n_rows > kBeamCopyMaxBlocks)
+          return SMOE_ERR_UNSUPPORTED_SHAPE;
+      }
+      if (pass) {
+        const hipError_t e = launch_beam_copy(c, n, rows, n_rows, src_rows, h->err, h->stream);
+        if (e != hipSuccess) return SMOE_ERR_HIP;
+      }
+    }
+  }
+  return SMOE_OK;
+}
+
 int smoe_synth_experts(smoe_handle* h, void* base, uint32_t n_experts, uint64_t stride,
                        const smoe_expert_shape* shape, uint64_t seed, float scale_sigma,
                        float bias_sigma) {

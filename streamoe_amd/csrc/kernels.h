@@ -305,6 +305,39 @@ struct NormArgs {
   uint32_t group;         // 0, 32, 64 or 128
 };
 hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
+// Beam search step (beam.hip).
+constexpr uint32_t kBeamMaxBeams = 16, kBeamMaxPicks = 32, kBeamMaxVocab = 1u << 28;
+constexpr uint32_t kBeamMaxSlices = 64;  // of one beam's logits
+struct BeamStat {
+  double sum;  // of exp(logit - max) over a slice
+  float max;
+  uint32_t pad;
+};
+struct BeamArgs {
+  const float* logits;   // [rows, vocab], rows = requests * beams
+  const float* scores;   // [rows]
+  const uint8_t* done;   // [rows], or null
+  uint32_t rows, beams, vocab, picks, pad;
+  float* out_scores;     // [requests, picks]
+  int32_t *out_rows, *out_tokens;
+  // Workspace (beam_workspace): per row and slice, of `tiles` tiles each.
+  uint32_t slices, tiles;
+  BeamStat* stats;
+  unsigned long long* cand;  // picks keys each, in falling order, 0 past the last
+};
+uint64_t beam_workspace(uint32_t requests, uint32_t beams, uint32_t vocab, uint32_t picks, BeamArgs* a, uint8_t* base);
+hipError_t launch_beam_select(const BeamArgs& a, hipStream_t st);
+// One state tensor of a reordering: `pieces` pieces of `bytes` bytes in every row.
+struct BeamCopy {
+  const uint8_t* src;
+  uint8_t* dst;
+  uint64_t src_row, dst_row, src_piece, dst_piece, bytes;  // strides in bytes
+  uint32_t pieces, unit;                                   // unit: 16, 4 or 1, what addresses and strides divide by
+};
+constexpr uint64_t kBeamCopyMaxBlocks = 1u << 30;  // per launch
+uint64_t beam_copy_blocks(const BeamCopy& s, uint32_t n_rows);
+hipError_t launch_beam_copy(const BeamCopy* states, uint32_t n, const int32_t* rows, uint32_t n_rows,
+                            uint32_t src_rows, uint32_t* err, hipStream_t st);
 // Streaming-read diagnostic over `bytes` (multiple of 16) with
 // kStreamBlocks blocks; sink: kStreamBlocks u32.
 constexpr uint32_t kStreamBlocks = 2048;

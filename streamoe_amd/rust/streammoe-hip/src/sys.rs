@@ -6,8 +6,9 @@
 
 use std::os::raw::{c_char, c_int, c_void};
 
-/// The header's 8-bit codes.
+/// The header's 8-bit types.
 pub type int8_t = i8;
+pub type uint8_t = u8;
 
 pub const SMOE_MAX_K: u32 = 16;
 pub const SMOE_ABI_VERSION: u32 = 2;
@@ -89,6 +90,20 @@ pub struct smoe_file_layout {
     pub stride: u64,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct smoe_beam_state {
+    pub src: *const c_void,
+    pub dst: *mut c_void,
+    pub src_row_stride: u64,
+    pub dst_row_stride: u64,
+    pub src_piece_stride: u64,
+    pub dst_piece_stride: u64,
+    pub piece_bytes: u64,
+    pub n_pieces: u32,
+    pub reserved: u32,
+}
+
 extern "C" {
     pub fn smoe_strerror(status: c_int) -> *const c_char;
     pub fn smoe_abi_version() -> u32;
@@ -156,6 +171,13 @@ extern "C" {
                         norm_w: *const c_void, eps: f32, n_tokens: u32, hidden: u32, sum_out: *mut f32,
                         out: *mut c_void, out_is_bf16: c_int, out_q: *mut int8_t, out_scales: *mut f32,
                         q_group: u32) -> c_int;
+    pub fn smoe_beam_select_workspace_size(n_requests: u32, n_beams: u32, vocab: u32, n_picks: u32) -> u64;
+    pub fn smoe_beam_select(h: *mut smoe_handle, logits: *const f32, scores: *const f32, done: *const uint8_t,
+                            pad_token: u32, n_requests: u32, n_beams: u32, vocab: u32, n_picks: u32,
+                            out_scores: *mut f32, out_rows: *mut i32, out_tokens: *mut i32,
+                            workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn smoe_beam_reorder(h: *mut smoe_handle, states: *const smoe_beam_state, n_states: u32, rows: *const i32,
+                             n_rows: u32, src_rows: u32) -> c_int;
     pub fn smoe_layer_file_layout(file_bytes: u64, n_experts: u32, hidden: u32, inter: u32, group: u32,
                                   declared_size: u64, declared_stride: u64,
                                   out: *mut smoe_file_layout) -> c_int;
