@@ -523,6 +523,48 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
                  int8_t* out_q, float* out_scales, uint32_t q_group);
 
 /* ------------------------------------------------------------------ */
+/* Low-rank adapters beside a shared projection                         */
+/* ------------------------------------------------------------------ */
+
+/* The adapters of one projection: A_i [max_rank, in_dim] and B_i [out_dim,
+ * max_rank], bf16 rows, of which the first ranks[i] rows of A_i and columns of
+ * B_i count (what lies behind them is not used and may hold anything). */
+typedef struct {
+  const void* a;        /* device bf16, A_i at a + i * a_stride */
+  const void* b;        /* device bf16, B_i at b + i * b_stride */
+  uint64_t a_stride;    /* bytes, a multiple of 16, at least A_i's size */
+  uint64_t b_stride;    /* bytes, a multiple of 16, at least B_i's size */
+  const float* scale;   /* device f32[n_adapters] */
+  const int32_t* ranks; /* device int32[n_adapters], each 0..max_rank, or NULL: max_rank */
+  uint32_t n_adapters;  /* 1..4096 */
+  uint32_t max_rank;    /* a multiple of 8, up to 128 */
+} smoe_adapters;
+
+/* Device workspace bytes smoe_lora needs (0 for sizes it does not take). */
+uint64_t smoe_lora_workspace_size(const smoe_adapters* adapters, uint32_t n_tokens);
+
+/* y[t] = base[t] + scale[a] * B_a (A_a x[t]) with a = ids[t] per row
+ * t < n_tokens, and y[t] = base[t] where ids[t] is -1: many requests' adapters
+ * beside one projection (base = what smoe_qmm, smoe_qmm_i8 or smoe_qmv gave).
+ * ids: device int32[n_tokens], in any order; x: device [n_tokens, in_dim],
+ * bf16 when x_is_bf16 else f32; base: device f32[n_tokens, out_dim] or NULL
+ * (zeros), may be y; y: device f32[n_tokens, out_dim]. x, a, b 16-byte
+ * aligned, in_dim a multiple of 8; out_dim any (multiples of 4 with y and base
+ * on 16 bytes are the fast case). On bf16 MFMA with f32 sums; f32 x and the
+ * low-rank values between the products enter as bf16 pairs (off by at most
+ * 2^-16 of each value); a row with an infinity or NaN gives NaN. An id or a
+ * rank out of range is found on the device: the next smoe_sync returns
+ * SMOE_ERR_INVALID_ARG, the row's y is base (the rank is clamped). n_tokens up
+ * to 65536, in_dim up to 65536, else SMOE_ERR_UNSUPPORTED_SHAPE. workspace:
+ * device, smoe_lora_workspace_size bytes, 256-byte aligned, one call's at a
+ * time. A row's bits do not depend on the other rows' adapters. Enqueue-only,
+ * allocates nothing, capturable in a HIP graph. No counterpart in the
+ * reference. */
+int smoe_lora(smoe_handle* h, const smoe_adapters* adapters, const int32_t* ids, const void* x, int x_is_bf16,
+              const float* base, float* y, uint32_t out_dim, uint32_t in_dim, uint32_t n_tokens,
+              void* workspace, uint64_t workspace_bytes);
+
+/* ------------------------------------------------------------------ */
 /* Beam search behind the LM head                                       */
 /* ------------------------------------------------------------------ */
 

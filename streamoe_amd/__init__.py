@@ -115,6 +115,30 @@ class QuantWeights:
 
 
 @dataclass
+class Adapters:
+    """The low-rank adapters of one projection: a [n, max_rank, in_dim] and b
+    [n, out_dim, max_rank] in bf16, scale f32[n], ranks int32[n] or None (all
+    max_rank). The adapters may lie apart (any stride of axis 0)."""
+
+    a: object
+    b: object
+    scale: object
+    ranks: object = None
+
+    def c(self):
+        a, b = self.a, self.b
+        n, r = a.shape[0], a.shape[1]
+        if (a.dim() != 3 or b.dim() != 3 or b.shape[0] != n or b.shape[2] != r or not a[0].is_contiguous()
+                or not b[0].is_contiguous() or _misfit(a.device.index, (a[0], _BF16, 1), (b[0], _BF16, 1),
+                                                       (self.scale, _F32, n), (self.ranks, ("int32",), n))):
+            raise SmoeError(_INVALID, "Adapters")
+        # A lone adapter's stride says nothing: its size.
+        step = lambda t: (t.stride(0) if n > 1 else t[0].numel()) * 2
+        return _abi.AdaptersC(a.data_ptr(), b.data_ptr(), step(a), step(b), self.scale.data_ptr(),
+                              None if self.ranks is None else self.ranks.data_ptr(), n, r)
+
+
+@dataclass
 class BeamState:
     """One state tensor of the beams for Kernels.beam_reorder: rows [n, bytes ..]
     or, with the pieces of a row on axis 1, [n, pieces, room ..]; the first
@@ -349,6 +373,23 @@ class Kernels:
         return _lib.smoe_rmsnorm(self.h, _ptr(x), int(x is not None and x.element_size() == 2), _ptr(residual),
                                  _ptr(norm_w), C.c_float(eps), n_tokens, hidden, _ptr(sum_out), _ptr(out),
                                  int(out is not None and out.element_size() == 2), _ptr(out_q), _ptr(out_scales), q_group)
+
+    # -- low-rank adapters ---------------------------------------------------------
+    def lora_workspace_size(self, adapters: Adapters, n_tokens):
+        ac = adapters.c()
+        return _lib.smoe_lora_workspace_size(C.byref(ac), n_tokens)
+
+    def lora(self, adapters: Adapters, ids, x, base, y, out_dim, in_dim, n_tokens, workspace):
+        """y[t] = base[t] + scale[a] b[a] (a[a] x[t]), a = ids[t] (-1: none); base
+        None (zeros) or y itself; x f32 or bf16 rows."""
+        ac = adapters.c()
+        if (adapters.a.device.index != self.device or adapters.a.shape[2] != in_dim or adapters.b.shape[1] != out_dim
+                or _misfit(self.device, (ids, ("int32",), n_tokens), (x, _F32 + _BF16, n_tokens * in_dim),
+                           (base, _F32, n_tokens * out_dim), (y, _F32, n_tokens * out_dim))):
+            return _INVALID
+        return _lib.smoe_lora(self.h, C.byref(ac), _ptr(ids), _ptr(x), int(x is not None and x.element_size() == 2),
+                              _ptr(base), _ptr(y), out_dim, in_dim, n_tokens, _ptr(workspace),
+                              0 if workspace is None else workspace.numel() * workspace.element_size())
 
     # -- beam search --------------------------------------------------------------
     def beam_select_workspace_size(self, n_requests, n_beams, vocab, n_picks):

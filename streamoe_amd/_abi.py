@@ -85,6 +85,19 @@ class Layer(C.Structure):
     ]
 
 
+class AdaptersC(C.Structure):
+    _fields_ = [
+        ("a", C.c_void_p),
+        ("b", C.c_void_p),
+        ("a_stride", C.c_uint64),
+        ("b_stride", C.c_uint64),
+        ("scale", C.c_void_p),
+        ("ranks", C.c_void_p),
+        ("n_adapters", C.c_uint32),
+        ("max_rank", C.c_uint32),
+    ]
+
+
 class BeamStateC(C.Structure):
     _fields_ = [
         ("src", C.c_void_p),
@@ -150,6 +163,8 @@ PROTOTYPES = {
     "smoe_moe_prefill_block": (_I, [_P, C.POINTER(ExpertShape), _P, _U64, _U32, _P, _P, _P, _I, _U32, _U32, _P,
                                     _P, _P, _P, _P, _U64]),
     "smoe_rmsnorm": (_I, [_P, _P, _I, _P, _P, C.c_float, _U32, _U32, _P, _P, _I, _P, _P, _U32]),
+    "smoe_lora_workspace_size": (_U64, [C.POINTER(AdaptersC), _U32]),
+    "smoe_lora": (_I, [_P, C.POINTER(AdaptersC), _P, _P, _I, _P, _P, _U32, _U32, _U32, _P, _U64]),
     "smoe_beam_select_workspace_size": (_U64, [_U32, _U32, _U32, _U32]),
     "smoe_beam_select": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _P, _P, _U64]),
     "smoe_beam_reorder": (_I, [_P, C.POINTER(BeamStateC), _U32, _P, _U32, _U32]),

@@ -969,6 +969,56 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
   return hip_status(launch_rmsnorm(a, x_is_bf16 != 0, n_tokens, h->stream));
 }
 
+static int check_adapters(const smoe_adapters* s, uint32_t n_tokens) {
+  if (!s || !n_tokens || !s->n_adapters || !s->max_rank) return SMOE_ERR_INVALID_ARG;
+  if (s->max_rank % 8 || s->max_rank > kLoraMaxRank || s->n_adapters > kLoraMaxAdapters || n_tokens > kLoraMaxTokens)
+    return SMOE_ERR_UNSUPPORTED_SHAPE;
+  return SMOE_OK;
+}
+
+uint64_t smoe_lora_workspace_size(const smoe_adapters* adapters, uint32_t n_tokens) {
+  if (check_adapters(adapters, n_tokens)) return 0;
+  return lora_workspace(adapters->n_adapters, adapters->max_rank, n_tokens, nullptr, nullptr);
+}
+
+int smoe_lora(smoe_handle* h, const smoe_adapters* adapters, const int32_t* ids, const void* x, int x_is_bf16,
+              const float* base, float* y, uint32_t out_dim, uint32_t in_dim, uint32_t n_tokens,
+              void* workspace, uint64_t workspace_bytes) {
+  if (!h || !ids || !x || !y || !out_dim || !in_dim || !workspace) return SMOE_ERR_INVALID_ARG;
+  if (int rc = check_adapters(adapters, n_tokens)) return rc;
+  const smoe_adapters& s = *adapters;
+  if (!s.a || !s.b || !s.scale) return SMOE_ERR_INVALID_ARG;
+  if (in_dim % 8 || in_dim > kLoraMaxIn || out_dim > 0x7FFFFF00u) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (s.a_stride < (uint64_t)s.max_rank * in_dim * 2 || s.b_stride < (uint64_t)s.max_rank * out_dim * 2)
+    return SMOE_ERR_INVALID_ARG;
+  if (!aligned(s.a, 0, 16) || !aligned(s.b, 0, 16) || s.a_stride % 16 || s.b_stride % 16 || !aligned(x, 0, 16) ||
+      !aligned(s.scale, 0, 4) || !aligned(s.ranks, 0, 4) || !aligned(ids, 0, 4) || !aligned(base, 0, 4) ||
+      !aligned(y, 0, 4) || !aligned(workspace, 0, 256))
+    return SMOE_ERR_MISALIGNED;
+  LoraArgs a{};
+  if (workspace_bytes < lora_workspace(s.n_adapters, s.max_rank, n_tokens, &a, (uint8_t*)workspace))
+    return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  if (int rc = use_device(h)) return rc;
+  a.a = (const uint8_t*)s.a;
+  a.b = (const uint8_t*)s.b;
+  a.a_stride = s.a_stride;
+  a.b_stride = s.b_stride;
+  a.scale = s.scale;
+  a.ranks = s.ranks;
+  a.n_adapters = s.n_adapters;
+  a.max_rank = s.max_rank;
+  a.ids = ids;
+  a.x = x;
+  a.base = base;
+  a.y = y;
+  a.n = n_tokens;
+  a.in_dim = in_dim;
+  a.out_dim = out_dim;
+  a.vec = out_dim % 4 == 0 && aligned(base, 0, 16) && aligned(y, 0, 16);
+  a.err = h->err;
+  return hip_status(launch_lora(a, x_is_bf16 != 0, h->stream));
+}
+
 static int check_beam(uint32_t n_requests, uint32_t n_beams, uint32_t vocab, uint32_t n_picks) {
   if (!n_requests || !n_beams || !vocab) return SMOE_ERR_INVALID_ARG;
   if (n_beams > kBeamMaxBeams || vocab > kBeamMaxVocab) return SMOE_ERR_UNSUPPORTED_SHAPE;

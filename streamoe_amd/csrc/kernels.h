@@ -305,6 +305,32 @@ struct NormArgs {
   uint32_t group;         // 0, 32, 64 or 128
 };
 hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
+// Low-rank adapters (lora.hip).
+constexpr uint32_t kLoraMaxRank = 128, kLoraMaxAdapters = 4096, kLoraMaxTokens = 65536, kLoraMaxIn = 65536;
+struct LoraItem {
+  uint32_t adapter, start, count;  // rows perm[start ..] of one adapter (n_adapters: none)
+};
+struct LoraArgs {
+  const uint8_t *a, *b;        // adapter i's bf16 [max_rank, in_dim] at a + i a_stride, [out_dim, max_rank] at b + i b_stride
+  uint64_t a_stride, b_stride;
+  const float* scale;          // [n_adapters]
+  const int32_t* ranks;        // [n_adapters], or null: max_rank
+  uint32_t n_adapters, max_rank;
+  const int32_t* ids;          // [n]
+  const void* x;               // [n, in_dim] f32 or bf16
+  const float* base;           // [n, out_dim], or null; may be y
+  float* y;                    // [n, out_dim]
+  uint32_t n, in_dim, out_dim;
+  uint32_t vec;                // base and y on 16 bytes, out_dim a multiple of 4
+  uint32_t* err;
+  // Workspace (lora_workspace).
+  uint32_t n_items, shares;
+  LoraItem* items;             // [n_items], count 0 past the last
+  uint32_t* perm;              // [n]
+  float* u;                    // [shares, n, max_rank]
+};
+uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, LoraArgs* a, uint8_t* base);
+hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st);
 // Beam search step (beam.hip).
 constexpr uint32_t kBeamMaxBeams = 16, kBeamMaxPicks = 32, kBeamMaxVocab = 1u << 28;
 constexpr uint32_t kBeamMaxSlices = 64;  // of one beam's logits

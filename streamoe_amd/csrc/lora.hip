@@ -1,0 +1,248 @@
+// lora.hip — low-rank adapters of many requests beside a shared projection.
+//
+//   y[t] = base[t] + scale[a] B_a (A_a x[t]),  a = ids[t]
+//
+//   k_lora_plan    rows sorted by adapter, items of up to 16 rows of one
+//   k_lora_down    u = A x of an item's rows on bf16 MFMA, one share of the
+//                  inputs per block, partial sums in f32
+//   k_lora_up      the shares added, scaled, times B on bf16 MFMA, plus base
+//
+// f32 values enter the matrix cores as bf16 pairs, v = hi + lo, each rounded
+// to nearest: off by at most 2^-16 |v| (hi leaves up to 2^-8 |v|, of which lo
+// loses 2^-8). A and B are bf16, so the products are exact and the sums f32. An
+// infinity leaves a NaN in lo, so its row's outputs are NaN.
+#include "common.h"
+#include "kernels.h"
+
+namespace smoe {
+
+typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
+typedef float lf32x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kLoraM = 16;  // rows per item
+
+__device__ __forceinline__ f32x4 mfma_bf16(lbf16x8 a, lbf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// v = hi + lo.
+__device__ __forceinline__ void split_bf16(lf32x8 v, lbf16x8& hi, lbf16x8& lo) {
+  hi = __builtin_convertvector(v, lbf16x8);
+  lo = __builtin_convertvector(v - __builtin_convertvector(hi, lf32x8), lbf16x8);
+}
+
+// The first n of eight bf16, zeros behind (n may be <= 0 or >= 8).
+__device__ __forceinline__ lbf16x8 first_of(lbf16x8 v, int n) {
+  u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = n >= 2 * j + 2 ? w[j] : n == 2 * j + 1 ? w[j] & 0xFFFFu : 0u;
+  return __builtin_bit_cast(lbf16x8, w);
+}
+
+__device__ __forceinline__ uint32_t lora_rank(const LoraArgs& a, uint32_t ad) {
+  if (!a.ranks) return a.max_rank;
+  const int32_t r = a.ranks[ad];
+  return r < 0 ? 0u : min((uint32_t)r, a.max_rank);
+}
+
+// One block: counts per adapter, their items, the rows in adapter order. Rows
+// without an adapter (-1, or an id or rank that does not exist, which is
+// reported) come last, as items of adapter n_adapters.
+__global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
+  extern __shared__ uint32_t sh[];  // [n_adapters + 1] counts, then next positions
+  __shared__ uint32_t wrow[16], witem[16], base_row, base_item;
+  const uint32_t t = threadIdx.x, N = a.n_adapters + 1;
+  for (uint32_t i = t; i < N; i += 1024) sh[i] = 0;
+  if (t == 0) base_row = base_item = 0;
+  __syncthreads();
+  bool bad = false;
+  auto adapter = [&](uint32_t row) {
+    const int32_t id = a.ids[row];
+    bad |= id < -1 || id >= (int32_t)a.n_adapters;
+    return id < 0 || id >= (int32_t)a.n_adapters ? a.n_adapters : (uint32_t)id;
+  };
+  for (uint32_t r = t; r < a.n; r += 1024) atomicAdd(&sh[adapter(r)], 1u);
+  if (a.ranks)
+    for (uint32_t i = t; i < a.n_adapters; i += 1024) bad |= a.ranks[i] < 0 || a.ranks[i] > (int32_t)a.max_rank;
+  if (bad) *a.err = 2u;
+  __syncthreads();
+  for (uint32_t i0 = 0; i0 < N; i0 += 1024) {
+    const uint32_t ad = i0 + t, c = ad < N ? sh[ad] : 0u, it = (c + kLoraM - 1) / kLoraM;
+    uint32_t pr = c, pi = it;  // inclusive sums over the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t r = __shfl_up(pr, o, kWave), q = __shfl_up(pi, o, kWave);
+      if ((t & 63) >= (uint32_t)o) pr += r, pi += q;
+    }
+    if ((t & 63) == 63) wrow[t >> 6] = pr, witem[t >> 6] = pi;
+    __syncthreads();
+    uint32_t row = base_row + pr - c, item = base_item + pi - it;
+    for (uint32_t w = 0; w < (t >> 6); ++w) row += wrow[w], item += witem[w];
+    if (ad < N) {
+      sh[ad] = row;
+      for (uint32_t j = 0; j < it; ++j)
+        a.items[item + j] = LoraItem{ad, row + j * kLoraM, min(kLoraM, c - j * kLoraM)};
+    }
+    __syncthreads();
+    if (t == 1023) base_row = row + c, base_item = item + it;
+    __syncthreads();
+  }
+  for (uint32_t i = base_item + t; i < a.n_items; i += 1024) a.items[i] = LoraItem{0u, 0u, 0u};
+  // Which row of an adapter takes which place does not touch any result.
+  for (uint32_t r = t; r < a.n; r += 1024) a.perm[atomicAdd(&sh[adapter(r)], 1u)] = r;
+}
+
+// u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
+// steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c.
+template <bool XBF16>
+__global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
+  constexpr int MT = kLoraMaxRank / 16;
+  __shared__ f32x4 red[4][64];
+  const LoraItem it = a.items[blockIdx.x];
+  if (it.count == 0 || it.adapter >= a.n_adapters) return;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t K = a.in_dim, share = blockIdx.y;
+  const uint32_t rank = lora_rank(a, it.adapter), nt = (rank + 15) / 16;
+  const uint32_t row = a.perm[it.start + min(c16, it.count - 1)];
+  const uint16_t* const A = (const uint16_t*)(a.a + (uint64_t)it.adapter * a.a_stride);
+  const uint32_t steps = (K + 31) / 32, s0 = steps * share / a.shares, s1 = steps * (share + 1) / a.shares;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t s = s0 + wave; s < s1; s += 4) {
+    const uint32_t k = s * 32 + kb * 8;
+    const bool in = k < K;  // K is a multiple of 8
+    const uint64_t e = (uint64_t)row * K + (in ? k : 0);
+    lbf16x8 hi, lo;
+    if constexpr (XBF16) {
+      hi = *reinterpret_cast<const lbf16x8*>((const uint16_t*)a.x + e);
+    } else {
+      split_bf16(*reinterpret_cast<const lf32x8*>((const float*)a.x + e), hi, lo);
+      lo = first_of(lo, in ? 8 : 0);
+    }
+    hi = first_of(hi, in ? 8 : 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (i >= (int)nt) break;
+      const uint32_t j = i * 16 + c16;
+      const lbf16x8 w = first_of(*reinterpret_cast<const lbf16x8*>(A + (uint64_t)min(j, rank - 1) * K + (in ? k : 0)),
+                                 in && j < rank ? 8 : 0);
+      acc[i] = mfma_bf16(hi, w, acc[i]);
+      if constexpr (!XBF16) acc[i] = mfma_bf16(lo, w, acc[i]);
+    }
+  }
+  for (uint32_t i = 0; i < nt; ++i) {
+    f32x4 v = acc[0];
+#pragma unroll
+    for (int j = 1; j < MT; ++j)
+      if ((int)i == j) v = acc[j];
+    red[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0) {
+      const f32x4 s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+      float* const u = a.u + ((uint64_t)share * a.n + it.start) * a.max_rank + i * 16 + c16;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * kb + r < it.count && i * 16 + c16 < a.max_rank) u[(uint64_t)(4 * kb + r) * a.max_rank] = s[r];
+    }
+    __syncthreads();
+  }
+}
+
+constexpr uint32_t kLoraOut = 256;  // outputs per block of k_lora_up: four waves of four tiles of 16
+
+// D = B (outputs) x u (rows): lane (c, kb) ends with outputs 4 kb .. of row c.
+__global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
+  const LoraItem it = a.items[blockIdx.x];
+  if (it.count == 0) return;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t O = a.out_dim, R = a.max_rank;
+  const uint32_t place = it.start + min(c16, it.count - 1), row = a.perm[place];
+  const bool mine = c16 < it.count;
+  f32x4 acc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t o0 = blockIdx.y * kLoraOut + wave * 64;
+  if (it.adapter < a.n_adapters) {
+    const uint32_t rank = lora_rank(a, it.adapter);
+    const uint16_t* const B = (const uint16_t*)(a.b + (uint64_t)it.adapter * a.b_stride);
+    const float scale = a.scale[it.adapter];
+    for (uint32_t k0 = 0; k0 < rank; k0 += 32) {
+      const uint32_t k = k0 + kb * 8;
+      const uint32_t kc = k < R ? k : 0;  // R is a multiple of 8
+      lf32x8 u = {0, 0, 0, 0, 0, 0, 0, 0};
+      for (uint32_t s = 0; s < a.shares; ++s)
+        u += *reinterpret_cast<const lf32x8*>(a.u + ((uint64_t)s * a.n + place) * R + kc);
+      u *= scale;
+      lbf16x8 hi, lo;
+      split_bf16(u, hi, lo);
+      const int left = k < rank ? (int)(rank - k) : 0;
+      hi = first_of(hi, left);
+      lo = first_of(lo, left);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t o = min(o0 + i * 16 + c16, O - 1);
+        const lbf16x8 w = first_of(*reinterpret_cast<const lbf16x8*>(B + (uint64_t)o * R + kc), left);
+        acc[i] = mfma_bf16(w, hi, acc[i]);
+        acc[i] = mfma_bf16(w, lo, acc[i]);
+      }
+    }
+  } else if (a.base == a.y) {
+    return;
+  }
+  if (!mine) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t o = o0 + i * 16 + 4 * kb;
+    const uint64_t e = (uint64_t)row * O + o;
+    if (a.vec) {
+      if (o >= O) continue;
+      f32x4 v = acc[i];
+      if (a.base) v += *reinterpret_cast<const f32x4*>(a.base + e);
+      *reinterpret_cast<f32x4*>(a.y + e) = v;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (o + r < O) a.y[e + r] = acc[i][r] + (a.base ? a.base[e + r] : 0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+static uint64_t al256(uint64_t n) { return (n + 255) & ~255ull; }
+
+// Shares of the inputs: enough blocks for few rows, none to spare for many.
+static uint32_t lora_shares(uint32_t n) { return n <= 256 ? 16u : n <= 1024 ? 8u : n <= 4096 ? 4u : 1u; }
+
+uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, LoraArgs* a, uint8_t* base) {
+  const uint32_t shares = lora_shares(n);
+  // Every adapter in use leaves at most one item short of 16 rows.
+  const uint32_t items = n / kLoraM + (n < n_adapters + 1 ? n : n_adapters + 1);
+  const uint64_t ib = al256((uint64_t)items * sizeof(LoraItem)), pb = al256((uint64_t)n * 4);
+  if (a) {
+    a->n_items = items;
+    a->shares = shares;
+    a->items = reinterpret_cast<LoraItem*>(base);
+    a->perm = reinterpret_cast<uint32_t*>(base + ib);
+    a->u = reinterpret_cast<float*>(base + ib + pb);
+  }
+  return ib + pb + al256((uint64_t)shares * n * max_rank * 4);
+}
+
+hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
+  hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 4, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (x_bf16)
+    hipLaunchKernelGGL(k_lora_down<true>, dim3(a.n_items, a.shares), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(k_lora_down<false>, dim3(a.n_items, a.shares), dim3(256), 0, st, a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k_lora_up, dim3(a.n_items, (a.out_dim + kLoraOut - 1) / kLoraOut), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace smoe

@@ -92,6 +92,19 @@ pub struct smoe_file_layout {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct smoe_adapters {
+    pub a: *const c_void,
+    pub b: *const c_void,
+    pub a_stride: u64,
+    pub b_stride: u64,
+    pub scale: *const f32,
+    pub ranks: *const i32,
+    pub n_adapters: u32,
+    pub max_rank: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct smoe_beam_state {
     pub src: *const c_void,
     pub dst: *mut c_void,
@@ -171,6 +184,10 @@ extern "C" {
                         norm_w: *const c_void, eps: f32, n_tokens: u32, hidden: u32, sum_out: *mut f32,
                         out: *mut c_void, out_is_bf16: c_int, out_q: *mut int8_t, out_scales: *mut f32,
                         q_group: u32) -> c_int;
+    pub fn smoe_lora_workspace_size(adapters: *const smoe_adapters, n_tokens: u32) -> u64;
+    pub fn smoe_lora(h: *mut smoe_handle, adapters: *const smoe_adapters, ids: *const i32, x: *const c_void,
+                     x_is_bf16: c_int, base: *const f32, y: *mut f32, out_dim: u32, in_dim: u32, n_tokens: u32,
+                     workspace: *mut c_void, workspace_bytes: u64) -> c_int;
     pub fn smoe_beam_select_workspace_size(n_requests: u32, n_beams: u32, vocab: u32, n_picks: u32) -> u64;
     pub fn smoe_beam_select(h: *mut smoe_handle, logits: *const f32, scores: *const f32, done: *const uint8_t,
                             pad_token: u32, n_requests: u32, n_beams: u32, vocab: u32, n_picks: u32,
