@@ -522,6 +522,21 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
                  float eps, uint32_t n_tokens, uint32_t hidden, float* sum_out, void* out, int out_is_bf16,
                  int8_t* out_q, float* out_scales, uint32_t q_group);
 
+/* y[n_tokens, out_dim] = x . dequant(W)^T for rows in 8 bits: x[t, c] stands
+ * for x[t, c] * x_scales[t, c / x_group] (one scale per row with x_group 0:
+ * x_scales[t]), as smoe_rmsnorm writes them; smoe_qmm's product with a quarter
+ * of its matrix work, on int8 MFMA. Group sums of code times code are exact,
+ * everything else f32. x: device int8[n_tokens, in_dim], 16-byte aligned, any
+ * codes; x_scales: device f32[n_tokens, in_dim / x_group] or [n_tokens]; y:
+ * device f32. Weights of bits 4, 3 or 8, group 32, 64 or 128, in_dim a
+ * multiple of the group up to 16384; x_group 0 or the weights' group
+ * (SMOE_ERR_UNSUPPORTED_GROUP). A row with a scale that is infinite or NaN
+ * gives infinities or NaN in that row only. Enqueue-only, allocates nothing,
+ * needs no workspace, capturable in a HIP graph. No counterpart in the
+ * reference, whose activations stay f32. */
+int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const float* x_scales, uint32_t x_group,
+                float* y, uint32_t out_dim, uint32_t in_dim, uint32_t n_tokens);
+
 /* ------------------------------------------------------------------ */
 /* Low-rank adapters beside a shared projection                         */
 /* ------------------------------------------------------------------ */

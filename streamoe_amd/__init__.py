@@ -374,6 +374,16 @@ class Kernels:
                                  _ptr(norm_w), C.c_float(eps), n_tokens, hidden, _ptr(sum_out), _ptr(out),
                                  int(out is not None and out.element_size() == 2), _ptr(out_q), _ptr(out_scales), q_group)
 
+    def qmm_i8(self, w: QuantWeights, x, x_scales, x_group, y, out_dim, in_dim, n_tokens):
+        """y[n, out] = (x codes * x_scales)[n, in] . dequant(W)^T for int8 rows as
+        rmsnorm writes them; x_group 0 (one scale per row) or the weights' group."""
+        if _misfit(self.device, (x, ("int8",), n_tokens * in_dim),
+                   (x_scales, _F32, n_tokens * (in_dim // (x_group or in_dim or 1))), (y, _F32, n_tokens * out_dim)):
+            return _INVALID
+        wc = w.c()
+        return _lib.smoe_qmm_i8(self.h, C.byref(wc), _ptr(x), _ptr(x_scales), x_group, _ptr(y), out_dim, in_dim,
+                                n_tokens)
+
     # -- low-rank adapters ---------------------------------------------------------
     def lora_workspace_size(self, adapters: Adapters, n_tokens):
         ac = adapters.c()

@@ -163,6 +163,7 @@ PROTOTYPES = {
     "smoe_moe_prefill_block": (_I, [_P, C.POINTER(ExpertShape), _P, _U64, _U32, _P, _P, _P, _I, _U32, _U32, _P,
                                     _P, _P, _P, _P, _U64]),
     "smoe_rmsnorm": (_I, [_P, _P, _I, _P, _P, C.c_float, _U32, _U32, _P, _P, _I, _P, _P, _U32]),
+    "smoe_qmm_i8": (_I, [_P, C.POINTER(QWeights), _P, _P, _U32, _P, _U32, _U32, _U32]),
     "smoe_lora_workspace_size": (_U64, [C.POINTER(AdaptersC), _U32]),
     "smoe_lora": (_I, [_P, C.POINTER(AdaptersC), _P, _P, _I, _P, _P, _U32, _U32, _U32, _P, _U64]),
     "smoe_beam_select_workspace_size": (_U64, [_U32, _U32, _U32, _U32]),

@@ -969,6 +969,28 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
   return hip_status(launch_rmsnorm(a, x_is_bf16 != 0, n_tokens, h->stream));
 }
 
+int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const float* x_scales, uint32_t x_group,
+                float* y, uint32_t out_dim, uint32_t in_dim, uint32_t n_tokens) {
+  if (!h || !x || !x_scales || !y || !out_dim || !n_tokens) return SMOE_ERR_INVALID_ARG;
+  QView v;
+  if (int rc = qview(w, in_dim, &v, true)) return rc;
+  if (x_group && x_group != v.group) return SMOE_ERR_UNSUPPORTED_GROUP;
+  if (in_dim > kQ8MaxIn || out_dim > 0x7FFFFF00u || n_tokens > 65535u * 16) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(x, 0, 16) || !aligned(x_scales, 0, 4) || !aligned(y, 0, 4)) return SMOE_ERR_MISALIGNED;
+  if (int rc = use_device(h)) return rc;
+  Q8Args a{};
+  a.w = v.codes;
+  a.s = v.scales;
+  a.b = v.biases;
+  a.x = x;
+  a.sx = x_scales;
+  a.y = y;
+  a.O = out_dim;
+  a.K = in_dim;
+  a.n = n_tokens;
+  return hip_status(launch_qmm_i8(a, v.bits, v.group, x_group != 0, h->stream));
+}
+
 static int check_adapters(const smoe_adapters* s, uint32_t n_tokens) {
   if (!s || !n_tokens || !s->n_adapters || !s->max_rank) return SMOE_ERR_INVALID_ARG;
   if (s->max_rank % 8 || s->max_rank > kLoraMaxRank || s->n_adapters > kLoraMaxAdapters || n_tokens > kLoraMaxTokens)

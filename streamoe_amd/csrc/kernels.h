@@ -305,6 +305,17 @@ struct NormArgs {
   uint32_t group;         // 0, 32, 64 or 128
 };
 hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
+// Quantized products of 8-bit rows (rows8.hip).
+constexpr uint32_t kQ8MaxIn = 16384;
+struct Q8Args {
+  const uint8_t* w;        // codes [O, K]
+  const uint16_t *s, *b;   // bf16 [O, K / group]
+  const int8_t* x;         // [n, K], 16-byte aligned
+  const float* sx;         // [n, K / group], or [n]
+  float* y;                // [n, O]
+  uint32_t O, K, n;
+};
+hipError_t launch_qmm_i8(const Q8Args& a, uint32_t bits, uint32_t group, bool x_grouped, hipStream_t st);
 // Low-rank adapters (lora.hip).
 constexpr uint32_t kLoraMaxRank = 128, kLoraMaxAdapters = 4096, kLoraMaxTokens = 65536, kLoraMaxIn = 65536;
 struct LoraItem {

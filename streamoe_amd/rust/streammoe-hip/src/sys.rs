@@ -184,6 +184,8 @@ extern "C" {
                         norm_w: *const c_void, eps: f32, n_tokens: u32, hidden: u32, sum_out: *mut f32,
                         out: *mut c_void, out_is_bf16: c_int, out_q: *mut int8_t, out_scales: *mut f32,
                         q_group: u32) -> c_int;
+    pub fn smoe_qmm_i8(h: *mut smoe_handle, w: *const smoe_qweights, x: *const int8_t, x_scales: *const f32,
+                       x_group: u32, y: *mut f32, out_dim: u32, in_dim: u32, n_tokens: u32) -> c_int;
     pub fn smoe_lora_workspace_size(adapters: *const smoe_adapters, n_tokens: u32) -> u64;
     pub fn smoe_lora(h: *mut smoe_handle, adapters: *const smoe_adapters, ids: *const i32, x: *const c_void,
                      x_is_bf16: c_int, base: *const f32, y: *mut f32, out_dim: u32, in_dim: u32, n_tokens: u32,
