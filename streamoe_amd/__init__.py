@@ -35,17 +35,33 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
-def _misfit(device, *checks):
-    """Whether a tensor is not what a call reads or writes: checks of (tensor
-    or None, element types, elements it has to hold), dense and on `device`."""
-    return any(t is not None and (str(t.dtype).rpartition(".")[2] not in types or not t.is_contiguous()
-                                  or t.device.type != "cuda" or t.device.index != device or t.numel() < n)
-               for t, types, n in checks)
-
-
-_F32 = ("float32",)
-_BF16 = ("bfloat16", "int16", "uint16")  # bf16 also as its bits
 _INVALID = _abi.CODES["SMOE_ERR_INVALID_ARG"]
+# Element types of the tensors a call takes; bf16 also as its bits.
+_TYPES = {}
+
+
+def _types(name):
+    """Torch's element types that may hold `name` (torch is imported on first use)."""
+    if not _TYPES:
+        import torch as t
+
+        bf16 = frozenset((t.bfloat16, t.int16, t.uint16))
+        _TYPES.update(f32=frozenset((t.float32,)), bf16=bf16, f32_bf16=bf16 | {t.float32}, i8=frozenset((t.int8,)),
+                      i32=frozenset((t.int32,)), flag=frozenset((t.uint8, t.bool)))
+    return _TYPES[name]
+
+
+def _fits(t, types, n, device):
+    """Whether a call may take at least n elements of `types` from t: dense, on `device`."""
+    return t.dtype in types and t.numel() >= n and t.is_contiguous() and t.get_device() == device
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _room(workspace):
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
 
 
 @dataclass(frozen=True)
@@ -114,7 +130,7 @@ class QuantWeights:
                              self.biases_offset, self.group_size, self.bits)
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class Adapters:
     """The low-rank adapters of one projection: a [n, max_rank, in_dim] and b
     [n, out_dim, max_rank] in bf16, scale f32[n], ranks int32[n] or None (all
@@ -126,19 +142,29 @@ class Adapters:
     ranks: object = None
 
     def c(self):
-        a, b = self.a, self.b
-        n, r = a.shape[0], a.shape[1]
-        if (a.dim() != 3 or b.dim() != 3 or b.shape[0] != n or b.shape[2] != r or not a[0].is_contiguous()
-                or not b[0].is_contiguous() or _misfit(a.device.index, (a[0], _BF16, 1), (b[0], _BF16, 1),
-                                                       (self.scale, _F32, n), (self.ranks, ("int32",), n))):
+        """The C struct, checked when it is first asked for and again whenever
+        one of the tensors lies elsewhere than then."""
+        at = (self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), _at(self.ranks))
+        known = self.__dict__.get("_known")
+        if known is None or known[0] != at:
+            known = (at, self._struct(at))
+            object.__setattr__(self, "_known", known)
+        return known[1]
+
+    def _struct(self, at):
+        a, b, bf16 = self.a, self.b, _types("bf16")
+        dev = a.get_device()
+        if (a.dim() != 3 or b.dim() != 3 or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1] or not a.numel()
+                or not b.numel() or not _fits(a[0], bf16, 1, dev) or not _fits(b[0], bf16, 1, dev)
+                or not _fits(self.scale, _types("f32"), a.shape[0], dev)
+                or not (self.ranks is None or _fits(self.ranks, _types("i32"), a.shape[0], dev))):
             raise SmoeError(_INVALID, "Adapters")
         # A lone adapter's stride says nothing: its size.
-        step = lambda t: (t.stride(0) if n > 1 else t[0].numel()) * 2
-        return _abi.AdaptersC(a.data_ptr(), b.data_ptr(), step(a), step(b), self.scale.data_ptr(),
-                              None if self.ranks is None else self.ranks.data_ptr(), n, r)
+        step = lambda t: (t.stride(0) if t.shape[0] > 1 else t[0].numel()) * 2
+        return _abi.AdaptersC(at[0], at[1], step(a), step(b), at[2], at[3], a.shape[0], a.shape[1])
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class BeamState:
     """One state tensor of the beams for Kernels.beam_reorder: rows [n, bytes ..]
     or, with the pieces of a row on axis 1, [n, pieces, room ..]; the first
@@ -150,6 +176,16 @@ class BeamState:
     used: int = None
 
     def c(self):
+        """(the C struct's bytes, rows of src, rows of dst, device), checked when
+        first asked for and again whenever one of the tensors lies elsewhere."""
+        at = (self.src.data_ptr(), self.dst.data_ptr())
+        known = self.__dict__.get("_known")
+        if known is None or known[0] != at:
+            known = (at, self._struct(at))
+            object.__setattr__(self, "_known", known)
+        return known[1]
+
+    def _struct(self, at):
         s, d = self.src, self.dst
         if (s.device != d.device or s.device.type != "cuda" or s.dtype != d.dtype or s.dim() not in (2, 3)
                 or s.shape[1:] != d.shape[1:] or s.stride(-1) != 1 or d.stride(-1) != 1):
@@ -161,8 +197,8 @@ class BeamState:
         if not 0 <= used <= room:
             raise SmoeError(_INVALID, "BeamState: used")
         piece = (lambda t: t.stride(1) * size) if s.dim() == 3 else (lambda t: 0)
-        return _abi.BeamStateC(s.data_ptr(), d.data_ptr(), s.stride(0) * size, d.stride(0) * size, piece(s), piece(d),
-                               used, pieces, 0)
+        raw = _abi.BeamStateC(*at, s.stride(0) * size, d.stride(0) * size, piece(s), piece(d), used, pieces, 0)
+        return bytes(raw), s.shape[0], d.shape[0], s.get_device()
 
 
 @dataclass
@@ -365,23 +401,28 @@ class Kernels:
         """r = x + residual (sum_out), RMSNorm(r) * norm_w as f32 or bf16 (out, by
         its type) and / or in 8 bits with scales (out_q, out_scales; q_group 0:
         one scale per row). x: f32 or bf16 rows."""
-        n = n_tokens * hidden
-        if _misfit(self.device, (x, _F32 + _BF16, n), (residual, _F32, n), (norm_w, _BF16, hidden), (sum_out, _F32, n),
-                   (out, _F32 + _BF16, n), (out_q, ("int8",), n),
-                   (out_scales, _F32, n_tokens * (hidden // (q_group or hidden or 1)))):
+        n, dev, f32 = n_tokens * hidden, self.device, _types("f32")
+        either, bf16 = _types("f32_bf16"), _types("bf16")
+        if not (x is not None and _fits(x, either, n, dev) and (residual is None or _fits(residual, f32, n, dev))
+                and (norm_w is None or _fits(norm_w, bf16, hidden, dev))
+                and (sum_out is None or _fits(sum_out, f32, n, dev)) and (out is None or _fits(out, either, n, dev))
+                and (out_q is None or _fits(out_q, _types("i8"), n, dev))
+                and (out_scales is None
+                     or _fits(out_scales, f32, n_tokens * (hidden // (q_group or hidden or 1)), dev))):
             return _INVALID
-        return _lib.smoe_rmsnorm(self.h, _ptr(x), int(x is not None and x.element_size() == 2), _ptr(residual),
-                                 _ptr(norm_w), C.c_float(eps), n_tokens, hidden, _ptr(sum_out), _ptr(out),
-                                 int(out is not None and out.element_size() == 2), _ptr(out_q), _ptr(out_scales), q_group)
+        return _lib.smoe_rmsnorm(self.h, x.data_ptr(), x.element_size() == 2, _at(residual), _at(norm_w), eps, n_tokens,
+                                 hidden, _at(sum_out), _at(out), out is not None and out.element_size() == 2,
+                                 _at(out_q), _at(out_scales), q_group)
 
     def qmm_i8(self, w: QuantWeights, x, x_scales, x_group, y, out_dim, in_dim, n_tokens):
         """y[n, out] = (x codes * x_scales)[n, in] . dequant(W)^T for int8 rows as
         rmsnorm writes them; x_group 0 (one scale per row) or the weights' group."""
-        if _misfit(self.device, (x, ("int8",), n_tokens * in_dim),
-                   (x_scales, _F32, n_tokens * (in_dim // (x_group or in_dim or 1))), (y, _F32, n_tokens * out_dim)):
+        dev, f32 = self.device, _types("f32")
+        if not (_fits(x, _types("i8"), n_tokens * in_dim, dev) and _fits(y, f32, n_tokens * out_dim, dev)
+                and _fits(x_scales, f32, n_tokens * (in_dim // (x_group or in_dim or 1)), dev)):
             return _INVALID
         wc = w.c()
-        return _lib.smoe_qmm_i8(self.h, C.byref(wc), _ptr(x), _ptr(x_scales), x_group, _ptr(y), out_dim, in_dim,
+        return _lib.smoe_qmm_i8(self.h, wc, x.data_ptr(), x_scales.data_ptr(), x_group, y.data_ptr(), out_dim, in_dim,
                                 n_tokens)
 
     # -- low-rank adapters ---------------------------------------------------------
@@ -392,14 +433,16 @@ class Kernels:
     def lora(self, adapters: Adapters, ids, x, base, y, out_dim, in_dim, n_tokens, workspace):
         """y[t] = base[t] + scale[a] b[a] (a[a] x[t]), a = ids[t] (-1: none); base
         None (zeros) or y itself; x f32 or bf16 rows."""
-        ac = adapters.c()
-        if (adapters.a.device.index != self.device or adapters.a.shape[2] != in_dim or adapters.b.shape[1] != out_dim
-                or _misfit(self.device, (ids, ("int32",), n_tokens), (x, _F32 + _BF16, n_tokens * in_dim),
-                           (base, _F32, n_tokens * out_dim), (y, _F32, n_tokens * out_dim))):
+        ac, dev, f32 = adapters.c(), self.device, _types("f32")
+        a, b = adapters.a, adapters.b
+        if (a.get_device() != dev or a.shape[2] != in_dim or b.shape[1] != out_dim
+                or not _fits(ids, _types("i32"), n_tokens, dev)
+                or not _fits(x, _types("f32_bf16"), n_tokens * in_dim, dev)
+                or not (base is None or _fits(base, f32, n_tokens * out_dim, dev))
+                or not _fits(y, f32, n_tokens * out_dim, dev)):
             return _INVALID
-        return _lib.smoe_lora(self.h, C.byref(ac), _ptr(ids), _ptr(x), int(x is not None and x.element_size() == 2),
-                              _ptr(base), _ptr(y), out_dim, in_dim, n_tokens, _ptr(workspace),
-                              0 if workspace is None else workspace.numel() * workspace.element_size())
+        return _lib.smoe_lora(self.h, ac, ids.data_ptr(), x.data_ptr(), x.element_size() == 2, _at(base), y.data_ptr(),
+                              out_dim, in_dim, n_tokens, _at(workspace), _room(workspace))
 
     # -- beam search --------------------------------------------------------------
     def beam_select_workspace_size(self, n_requests, n_beams, vocab, n_picks):
@@ -409,26 +452,26 @@ class Kernels:
                     out_tokens, workspace):
         """The n_picks best continuations of each request's beams (value, row of
         the logits, token); done: uint8 flags of ended beams, or None."""
-        rows, picks = n_requests * n_beams, n_requests * n_picks
-        if _misfit(self.device, (logits, _F32, rows * vocab), (scores, _F32, rows), (done, ("uint8", "bool"), rows),
-                   (out_scores, _F32, picks), (out_rows, ("int32",), picks), (out_tokens, ("int32",), picks)):
+        rows, picks, dev, f32, i32 = n_requests * n_beams, n_requests * n_picks, self.device, _types("f32"), _types("i32")
+        if not (_fits(logits, f32, rows * vocab, dev) and _fits(scores, f32, rows, dev)
+                and (done is None or _fits(done, _types("flag"), rows, dev)) and _fits(out_scores, f32, picks, dev)
+                and _fits(out_rows, i32, picks, dev) and _fits(out_tokens, i32, picks, dev)):
             return _INVALID
-        return _lib.smoe_beam_select(self.h, _ptr(logits), _ptr(scores), _ptr(done), pad_token, n_requests, n_beams,
-                                     vocab, n_picks, _ptr(out_scores), _ptr(out_rows), _ptr(out_tokens),
-                                     _ptr(workspace),
-                                     0 if workspace is None else workspace.numel() * workspace.element_size())
+        return _lib.smoe_beam_select(self.h, logits.data_ptr(), scores.data_ptr(), _at(done), pad_token, n_requests,
+                                     n_beams, vocab, n_picks, out_scores.data_ptr(), out_rows.data_ptr(),
+                                     out_tokens.data_ptr(), _at(workspace), _room(workspace))
 
     def beam_reorder(self, states, rows):
         """dst row i = src row rows[i] of every BeamState, for the rows of `rows`
         (int32, as beam_select's out_rows)."""
         n = rows.numel()
-        if not states or _misfit(self.device, (rows, ("int32",), 1)):
+        if not states or not _fits(rows, _types("i32"), 1, self.device):
             return _INVALID
-        src_rows = min(s.src.shape[0] for s in states)
-        if any(s.dst.shape[0] < n or s.dst.device.index != self.device for s in states):
+        known = [s.c() for s in states]
+        if any(k[2] < n or k[3] != self.device for k in known):
             return _INVALID
-        arr = (_abi.BeamStateC * len(states))(*[s.c() for s in states])
-        return _lib.smoe_beam_reorder(self.h, arr, len(states), _ptr(rows), n, src_rows)
+        arr = (_abi.BeamStateC * len(known)).from_buffer_copy(b"".join([k[0] for k in known]))
+        return _lib.smoe_beam_reorder(self.h, arr, len(known), rows.data_ptr(), n, min([k[1] for k in known]))
 
     # -- expert files -------------------------------------------------------------
     def load_file(self, path, dst, offset=0, nbytes=0):
