@@ -988,6 +988,7 @@ int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const f
   a.O = out_dim;
   a.K = in_dim;
   a.n = n_tokens;
+  a.vec = out_dim % 4 == 0 && aligned(y, 0, 16);
   return hip_status(launch_qmm_i8(a, v.bits, v.group, x_group != 0, h->stream));
 }
 

@@ -18,6 +18,8 @@
 #include "common.h"
 #include "kernels.h"
 
+#include <type_traits>
+
 namespace smoe {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -200,10 +202,348 @@ __global__ __launch_bounds__(256) void k_q8(Q8Args a) {
 }
 
 // ---------------------------------------------------------------------------
+// Many rows: a block of four waves takes WM MT tiles of 16 rows x WN NT tiles
+// of 16 columns, step after step of 128 inputs. A step's rows and codes go
+// through registers into LDS in operand order (a wave's operand is 1 KB that
+// the lanes read in lane order), the codes unpacked and the rows' bytes put in
+// their order once per block instead of once per wave; the next step's loads
+// are in flight while a step is computed. Weights are the A operand, so a lane
+// ends with four neighbouring columns of one row.
+//
+// The fold of a group's sums is what bounds it: two VALU instructions per
+// value (16 x 16 x 64: 8 per lane, 32 cycles, against 16 on the matrix cores).
+// With scales per group the sums come out of the MFMA as floats, 1.5 2^23 + S,
+// by an accumulator that starts as that number's bits (|S| < 2^22), and
+// fma(f, sx, -1.5 2^23 sx) = sx S in one rounding: the product in the constant
+// is exact for an sx of 22 bits, so sx is rounded to those (by 2^-23 of it).
+// The bias term runs on v_mfma_f32_16x16x4_f32, four groups at a time, over the
+// rows' group sums, which come from the staged bytes.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kMagicBits = 0x4B400000u;  // 1.5 * 2^23
+constexpr float kMagic = 12582912.f;
+
+// sx to 22 significant bits.
+__device__ __forceinline__ float q8_round22(float v) {
+  const uint32_t u = __float_as_uint(v);
+  if ((u & 0x7F800000u) == 0x7F800000u) return v;
+  return __uint_as_float((u + 1u + ((u >> 2) & 1u)) & ~3u);
+}
+
+// Where the e-th eight of piece p (16 inputs) of a row's step lies in operand
+// order: [h][kb][row][e], 8-byte units for rows of 16 (see q8_pos).
+template <int BITS, int G>
+__device__ __forceinline__ uint32_t q8_slot(uint32_t p, uint32_t e, uint32_t row) {
+  uint32_t h, kb, f = e;
+  if (G == 32) {
+    h = p >> 2, kb = (p & 1) * 2 + e, f = (p >> 1) & 1;
+  } else if (BITS == 8) {
+    h = p >> 2, kb = p & 3;
+  } else if (G == 64) {
+    h = p >> 2, kb = ((p & 1) << 1) | ((p >> 1) & 1);
+  } else {
+    h = p & 1, kb = p >> 1;
+  }
+  return ((h * 4 + kb) * 16 + row) * 2 + f;
+}
+
+template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
+struct Q8Tile {
+  static constexpr uint32_t BM = WM * MT * 16, BN = WN * NT * 16, GS = kQ8Step / G;
+  struct Buf {
+    u32x4 x[BM * 8], w[BN * 8];
+    float s[GS][BN];
+    float sx[XG ? 2 * GS : 1][XG ? BM : 1];  // sx, then -1.5 2^23 sx
+  };
+  struct Lds {
+    Buf buf[2];
+    float xs[2][4][BM], b[2][4][BN];  // group sums and biases, by group mod 4
+  };
+};
+
+template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint32_t units) {
+  using T = Q8Tile<BITS, G, XG, WM, WN, MT, NT>;
+  constexpr uint32_t BM = T::BM, BN = T::BN, GS = T::GS;
+  static_assert(WM * WN == 4, "four waves");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+  typename T::Lds& lds = *reinterpret_cast<typename T::Lds*>(lds_raw);
+  const uint32_t tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+  // XCD x = blockIdx % 8 takes a contiguous range of the units (rows fastest),
+  // so the row blocks of some columns share their weights in one L2.
+  const uint32_t per = (units + 7) / 8, u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || u >= units) return;
+  const uint32_t row0 = u % nrb * BM, col0 = u / nrb * BN;
+  const uint32_t K = a.K, O = a.O, gpr = K / G, steps = (K + kQ8Step - 1) / kQ8Step;
+  const uint32_t row_bytes = K / 32 * (BITS * 4);
+
+  // What a thread stages: pieces of 16 inputs of rows, chunks of weight rows
+  // (32 codes; 8 bits: 16), a scale and a bias.
+  constexpr uint32_t XP = BM * 8 / 256;
+  constexpr uint32_t WC = BITS == 8 ? 8 : 4, WP = BN * WC / 256;
+  constexpr uint32_t SP = (GS * BN + 255) / 256;
+  static_assert(BM * 8 % 256 == 0 && BN * WC % 256 == 0, "whole pieces per thread");
+  const int8_t* xp[XP];
+#pragma unroll
+  for (uint32_t i = 0; i < XP; ++i) {
+    const uint32_t id = tid + 256 * i;
+    xp[i] = a.x + (uint64_t)min(row0 + id / 8, a.n - 1) * K;
+  }
+  const uint8_t* wp[WP];
+#pragma unroll
+  for (uint32_t i = 0; i < WP; ++i) {
+    const uint32_t id = tid + 256 * i;
+    wp[i] = a.w + (uint64_t)min(col0 + id / WC, O - 1) * row_bytes;
+  }
+  u32x4 xr[XP], wr[WP];
+  float sr[SP], br[SP], sxr[XP];
+  auto load = [&](uint32_t st) {
+#pragma unroll
+    for (uint32_t i = 0; i < XP; ++i) {
+      const uint32_t at = st * kQ8Step + (tid & 7) * 16;  // 256 is a multiple of 8
+      xr[i] = u32x4{0u, 0u, 0u, 0u};
+      if (at < K) xr[i] = *reinterpret_cast<const u32x4*>(xp[i] + at);
+      if (XG) sxr[i] = a.sx[(uint64_t)min(row0 + (tid + 256 * i) / 8, a.n - 1) * gpr + min(at, K - 1) / G];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < WP; ++i) {
+      const uint32_t c = tid % WC;
+      if constexpr (BITS == 8) {
+        wr[i] = *reinterpret_cast<const u32x4*>(wp[i] + min(st * kQ8Step + c * 16, K - 16));
+      } else {
+        const Raw<BITS> r = load_raw<BITS, false>(wp[i] + min(st * 4 + c, K / 32 - 1) * chunk_bytes<BITS>());
+#pragma unroll
+        for (int j = 0; j < BITS; ++j) wr[i][j] = r.d[j];
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < SP; ++i) {
+      const uint32_t id = tid + 256 * i, col = id % BN, j = min(id / BN, GS - 1);
+      const uint64_t g = (uint64_t)min(col0 + col, O - 1) * gpr + min(st * GS + j, gpr - 1);
+      sr[i] = bf16f(a.s[g]);
+      br[i] = bf16f(a.b[g]);
+    }
+  };
+  auto store = [&](uint32_t st) {
+    typename T::Buf& B = lds.buf[st & 1];
+    uint2* const x8 = reinterpret_cast<uint2*>(B.x);
+    uint2* const w8 = reinterpret_cast<uint2*>(B.w);
+    const bool last = st + 1 == steps;
+#pragma unroll
+    for (uint32_t i = 0; i < XP; ++i) {
+      const uint32_t id = tid + 256 * i, row = id / 8, p = id % 8;
+      int32_t sum = 0;
+      uint2 v[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t lo = xr[i][2 * e], hi = xr[i][2 * e + 1];
+        sum = __builtin_amdgcn_sdot4((int)lo, 0x01010101, sum, false);
+        sum = __builtin_amdgcn_sdot4((int)hi, 0x01010101, sum, false);
+        v[e] = BITS == 8 ? make_uint2(lo, hi)
+                         : make_uint2(__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u));
+      }
+      const uint32_t tile = row / 16 * 256, r16 = row % 16;
+      if constexpr (G == 32) {
+        x8[tile + q8_slot<BITS, G>(p, 0, r16)] = v[0];
+        x8[tile + q8_slot<BITS, G>(p, 1, r16)] = v[1];
+      } else {
+        B.x[(tile + q8_slot<BITS, G>(p, 0, r16)) / 2] = u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
+      }
+      // The group's pieces lie in neighbouring lanes.
+      auto dpp_add = [&](auto ctrl) { return sum + __builtin_amdgcn_update_dpp(0, sum, decltype(ctrl)::value, 0xF, 0xF, false); };
+      sum = dpp_add(std::integral_constant<int, 0xB1>{});
+      if constexpr (G >= 64) sum = dpp_add(std::integral_constant<int, 0x4E>{});
+      if constexpr (G == 128) sum = dpp_add(std::integral_constant<int, 0x141>{});
+      if (p % (G / 16) == 0) {
+        const uint32_t j = p / (G / 16), g = st * GS + j;
+        const float sx = XG ? q8_round22(sxr[i]) : 1.f;
+        lds.xs[(g >> 2) & 1][g & 3][row] = sx * (float)sum;
+        if constexpr (XG) {
+          B.sx[j][row] = sx;
+          B.sx[GS + j][row] = -kMagic * sx;
+        }
+        // Groups behind the last up to a whole four count nothing.
+        if (last && j == GS - 1)
+          for (uint32_t z = g + 1; z & 3; ++z) lds.xs[(z >> 2) & 1][z & 3][row] = 0.f;
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < WP; ++i) {
+      const uint32_t id = tid + 256 * i, col = id / WC, c = id % WC;
+      const uint32_t tile = col / 16 * 256, r16 = col % 16;
+      if constexpr (BITS == 8) {
+        const u32x4 v = wr[i] ^ 0x80808080u;
+        if constexpr (G == 32) {
+          w8[tile + q8_slot<BITS, G>(c, 0, r16)] = make_uint2(v.x, v.y);
+          w8[tile + q8_slot<BITS, G>(c, 1, r16)] = make_uint2(v.z, v.w);
+        } else {
+          B.w[(tile + q8_slot<BITS, G>(c, 0, r16)) / 2] = v;
+        }
+      } else {
+        Raw<BITS> r;
+#pragma unroll
+        for (int j = 0; j < BITS; ++j) r.d[j] = wr[i][j];
+        uint32_t q[8];
+        unpack_bytes(r, q);
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          if constexpr (G == 32) {
+            w8[tile + q8_slot<BITS, G>(2 * c + h, 0, r16)] = make_uint2(q[4 * h], q[4 * h + 1]);
+            w8[tile + q8_slot<BITS, G>(2 * c + h, 1, r16)] = make_uint2(q[4 * h + 2], q[4 * h + 3]);
+          } else {
+            B.w[(tile + q8_slot<BITS, G>(2 * c + h, 0, r16)) / 2] = u32x4{q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]};
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < SP; ++i) {
+      const uint32_t id = tid + 256 * i, col = id % BN, j = id / BN, g = st * GS + j;
+      if (j >= GS) continue;
+      B.s[j][col] = sr[i];
+      lds.b[(g >> 2) & 1][g & 3][col] = BITS == 8 ? __builtin_fmaf(sr[i], 128.f, br[i]) : br[i];
+      if (last && j == GS - 1)
+        for (uint32_t z = g + 1; z & 3; ++z) lds.b[(z >> 2) & 1][z & 3][col] = 0.f;
+    }
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kStart = XG ? (int)kMagicBits : 0;
+  const i32x4 start = {kStart, kStart, kStart, kStart};
+  auto compute = [&](uint32_t st) {
+    const typename T::Buf& B = lds.buf[st & 1];
+    const u32x4* const xo = B.x + wm * MT * 128 + lane;
+    const u32x4* const wo = B.w + wn * NT * 128 + lane;
+#pragma unroll
+    for (uint32_t j = 0; j < GS; ++j) {
+      u32x4 x[MT][2];  // G = 128: both operands
+      float sx[MT], cx[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if constexpr (G == 128) {
+          x[m][0] = xo[m * 128];
+          x[m][1] = xo[m * 128 + 64];
+        } else if constexpr (G == 64) {
+          x[m][0] = xo[m * 128 + j * 64];
+        } else {
+          const uint2 v = reinterpret_cast<const uint2*>(xo + m * 128 + j / 2 * 64)[j % 2];
+          x[m][0].x = v.x;
+          x[m][0].y = v.y;
+        }
+        if constexpr (XG) {
+          sx[m] = B.sx[j][wm * MT * 16 + m * 16 + c16];
+          cx[m] = B.sx[GS + j][wm * MT * 16 + m * 16 + c16];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(&B.s[j][wn * NT * 16 + t * 16 + 4 * kb]);
+        u32x4 w[2];
+        if constexpr (G == 128) {
+          w[0] = wo[t * 128];
+          w[1] = wo[t * 128 + 64];
+        } else if constexpr (G == 64) {
+          w[0] = wo[t * 128 + j * 64];
+        } else {
+          const uint2 v = reinterpret_cast<const uint2*>(wo + t * 128 + j / 2 * 64)[j % 2];
+          w[0].x = v.x;
+          w[0].y = v.y;
+        }
+        i32x4 S[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if constexpr (G == 128)
+            S[m] = q8_mfma(w[1], x[m][1], q8_mfma(w[0], x[m][0], start));
+          else if constexpr (G == 64)
+            S[m] = q8_mfma(w[0], x[m][0], start);
+          else
+            S[m] = q8_mfma32(w[0].x, w[0].y, x[m][0].x, x[m][0].y, start);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f;
+            if constexpr (XG)
+              f = __builtin_fmaf(__int_as_float(S[m][i]), sx[m], cx[m]);
+            else
+              f = (float)S[m][i];
+            acc[m][t][i] = __builtin_fmaf(s[i], f, acc[m][t][i]);
+          }
+      }
+    }
+    const uint32_t g1 = (st + 1) * GS;  // groups staged so far
+    if ((g1 & 3) == 0 || st + 1 == steps) {
+      const uint32_t ring = ((g1 - 1) >> 2) & 1;
+      float b[NT], xs[MT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) b[t] = lds.b[ring][kb][wn * NT * 16 + t * 16 + c16];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xs[m] = lds.xs[ring][kb][wm * MT * 16 + m * 16 + c16];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[t], xs[m], acc[m][t], 0, 0, 0);
+    }
+  };
+
+  load(0);
+  store(0);
+  __syncthreads();
+  for (uint32_t st = 0; st < steps; ++st) {
+    const bool more = st + 1 < steps;
+    if (more) load(st + 1);
+    compute(st);
+    if (more) store(st + 1);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const uint32_t r = row0 + (wm * MT + m) * 16 + c16;
+    if (r >= a.n) continue;
+    const float sx = XG ? 1.f : a.sx[r];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint32_t col = col0 + (wn * NT + t) * 16 + 4 * kb;
+      float* const y = a.y + (uint64_t)r * O + col;
+      const f32x4 v = acc[m][t] * sx;
+      if (a.vec) {
+        if (col < O) *reinterpret_cast<f32x4*>(y) = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + i < O) y[i] = v[i];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
+template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
+static hipError_t q8_tile(const Q8Args& a, hipStream_t st) {
+  using T = Q8Tile<BITS, G, XG, WM, WN, MT, NT>;
+  const uint32_t nrb = (a.n + T::BM - 1) / T::BM, units = nrb * ((a.O + T::BN - 1) / T::BN);
+  constexpr uint32_t lds = sizeof(typename T::Lds);
+  auto fn = k_q8_tile<BITS, G, XG, WM, WN, MT, NT>;
+  if (lds > 64 * 1024) {
+    static std::atomic<uint64_t> raised{0};
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(fn), lds, raised);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(fn, dim3((units + 7) / 8 * 8), dim3(256), lds, st, a, nrb, units);
+  return hipGetLastError();
+}
+
 template <int BITS, int G, bool XG>
 static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
+  if (a.n > 64) return q8_tile<BITS, G, XG, 2, 2, 4, 4>(a, st);
   constexpr int NT = 4;
   const dim3 grid((a.O + NT * 16 - 1) / (NT * 16), (a.n + 15) / 16);
   hipLaunchKernelGGL((k_q8<BITS, G, XG, NT>), grid, dim3(256), 0, st, a);
