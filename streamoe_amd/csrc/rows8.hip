@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void k_q8(Q8Args a) {
 // fma(f, sx, -1.5 2^23 sx) = sx S in one rounding: the product in the constant
 // is exact for an sx of 22 bits, so sx is rounded to those (by 2^-23 of it).
 // The bias term runs on v_mfma_f32_16x16x4_f32, four groups at a time, over the
-// rows' group sums, which come from the staged bytes.
+// rows' group sums, which a product with ones leaves in every lane of a row.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMagicBits = 0x4B400000u;  // 1.5 * 2^23
 constexpr float kMagic = 12582912.f;
@@ -230,7 +230,10 @@ __device__ __forceinline__ float q8_round22(float v) {
 }
 
 // Where the e-th eight of piece p (16 inputs) of a row's step lies in operand
-// order: [h][kb][row][e], 8-byte units for rows of 16 (see q8_pos).
+// order: [h][kb][row][e], 8-byte units for rows of 16 (see q8_pos). The row's
+// place is exchanged by 4 h + kb, so that the pieces of a row, which
+// neighbouring lanes write, fall in different banks (8 writes to one: 33 of
+// 54 % of the LDS cycles were conflicts).
 template <int BITS, int G>
 __device__ __forceinline__ uint32_t q8_slot(uint32_t p, uint32_t e, uint32_t row) {
   uint32_t h, kb, f = e;
@@ -243,7 +246,7 @@ __device__ __forceinline__ uint32_t q8_slot(uint32_t p, uint32_t e, uint32_t row
   } else {
     h = p & 1, kb = p >> 1;
   }
-  return ((h * 4 + kb) * 16 + row) * 2 + f;
+  return ((h * 4 + kb) * 16 + (row ^ (h * 4 + kb))) * 2 + f;
 }
 
 template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
@@ -256,7 +259,7 @@ struct Q8Tile {
   };
   struct Lds {
     Buf buf[2];
-    float xs[2][4][BM], b[2][4][BN];  // group sums and biases, by group mod 4
+    float b[2][4][BN];  // biases, by group mod 4
   };
 };
 
@@ -278,67 +281,94 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
   const uint32_t row_bytes = K / 32 * (BITS * 4);
 
   // What a thread stages: pieces of 16 inputs of rows, chunks of weight rows
-  // (32 codes; 8 bits: 16), a scale and a bias.
+  // (32 codes; 8 bits: 16), scales and biases, rows' scales.
   constexpr uint32_t XP = BM * 8 / 256;
   constexpr uint32_t WC = BITS == 8 ? 8 : 4, WP = BN * WC / 256;
-  constexpr uint32_t SP = (GS * BN + 255) / 256;
+  constexpr uint32_t SP = (GS * BN + 255) / 256, XS = XG ? (GS * BM + 255) / 256 : 1;
   static_assert(BM * 8 % 256 == 0 && BN * WC % 256 == 0, "whole pieces per thread");
-  const int8_t* xp[XP];
+  // A wave's 16 cols x 4 chunks in an order whose eights of lanes write to
+  // different banks (columns c and c + 2 side by side).
+  auto w_col = [](uint32_t id) {
+    const uint32_t c = id / WC;
+    return BITS == 8 ? c : (c & ~3u) | ((c & 1) << 1) | ((c >> 1) & 1);
+  };
+  // Scalar bases of the block and 32-bit offsets of the lane.
+  const int8_t* const xb = a.x + (uint64_t)row0 * K;
+  const uint8_t* const wb = a.w + (uint64_t)col0 * row_bytes;
+  const uint16_t* const sb = a.s + (uint64_t)col0 * gpr;
+  const uint16_t* const bb = a.b + (uint64_t)col0 * gpr;
+  const float* const sxb = a.sx + (uint64_t)row0 * (XG ? gpr : 0);
+  const uint32_t rows = min(BM, a.n - row0), cols = min(BN, O - col0);
+  uint32_t xo[XP], wo[WP], so[SP], sxo[XS];
 #pragma unroll
-  for (uint32_t i = 0; i < XP; ++i) {
-    const uint32_t id = tid + 256 * i;
-    xp[i] = a.x + (uint64_t)min(row0 + id / 8, a.n - 1) * K;
-  }
-  const uint8_t* wp[WP];
+  for (uint32_t i = 0; i < XP; ++i) xo[i] = min((tid + 256 * i) / 8, rows - 1) * K + (tid & 7) * 16;
 #pragma unroll
   for (uint32_t i = 0; i < WP; ++i) {
     const uint32_t id = tid + 256 * i;
-    wp[i] = a.w + (uint64_t)min(col0 + id / WC, O - 1) * row_bytes;
+    wo[i] = min(w_col(id), cols - 1) * row_bytes + id % WC * (BITS == 8 ? 16 : chunk_bytes<BITS>());
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < SP; ++i) {
+    const uint32_t id = tid + 256 * i;
+    so[i] = min(id % BN, cols - 1) * gpr + min(id / BN, GS - 1);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < XS; ++i) {
+    const uint32_t id = tid + 256 * i;
+    sxo[i] = min(id % BM, rows - 1) * gpr + min(id / BM, GS - 1);
   }
   u32x4 xr[XP], wr[WP];
-  float sr[SP], br[SP], sxr[XP];
-  auto load = [&](uint32_t st) {
+  float sr[SP], br[SP], sxr[XS];
+  // TAIL: the step that K ends in. Loads past the end step back into the row
+  // (by as many pieces, chunks or groups as they are past it); inputs there
+  // are zero.
+  auto load = [&](uint32_t st, auto tail) {
+    constexpr bool TAIL = decltype(tail)::value;
+    const uint32_t k0 = st * kQ8Step, g0 = st * GS, ng = TAIL ? gpr - g0 : GS;
+    const int8_t* const x = xb + k0;
+    const uint8_t* const w = wb + k0 / 32 * (BITS * 4);
+    auto back = [&](uint32_t at, uint32_t n) { return TAIL && at >= n ? at - (n - 1) : 0u; };
 #pragma unroll
     for (uint32_t i = 0; i < XP; ++i) {
-      const uint32_t at = st * kQ8Step + (tid & 7) * 16;  // 256 is a multiple of 8
-      xr[i] = u32x4{0u, 0u, 0u, 0u};
-      if (at < K) xr[i] = *reinterpret_cast<const u32x4*>(xp[i] + at);
-      if (XG) sxr[i] = a.sx[(uint64_t)min(row0 + (tid + 256 * i) / 8, a.n - 1) * gpr + min(at, K - 1) / G];
+      const uint32_t p = tid & 7, np = TAIL ? (K - k0) / 16 : 8u;
+      xr[i] = *reinterpret_cast<const u32x4*>(x + lane_off(xo[i] - back(p, np) * 16));
+      if (TAIL && p >= np) xr[i] = u32x4{0u, 0u, 0u, 0u};
     }
 #pragma unroll
     for (uint32_t i = 0; i < WP; ++i) {
-      const uint32_t c = tid % WC;
+      constexpr uint32_t CB = BITS == 8 ? 16 : chunk_bytes<BITS>(), CI = BITS == 8 ? 16 : 32;
+      const uint8_t* const q = w + lane_off(wo[i] - back(tid % WC, TAIL ? (K - k0) / CI : WC) * CB);
       if constexpr (BITS == 8) {
-        wr[i] = *reinterpret_cast<const u32x4*>(wp[i] + min(st * kQ8Step + c * 16, K - 16));
+        wr[i] = *reinterpret_cast<const u32x4*>(q);
       } else {
-        const Raw<BITS> r = load_raw<BITS, false>(wp[i] + min(st * 4 + c, K / 32 - 1) * chunk_bytes<BITS>());
+        const Raw<BITS> r = load_raw<BITS, false>(q);
 #pragma unroll
         for (int j = 0; j < BITS; ++j) wr[i][j] = r.d[j];
       }
     }
 #pragma unroll
     for (uint32_t i = 0; i < SP; ++i) {
-      const uint32_t id = tid + 256 * i, col = id % BN, j = min(id / BN, GS - 1);
-      const uint64_t g = (uint64_t)min(col0 + col, O - 1) * gpr + min(st * GS + j, gpr - 1);
-      sr[i] = bf16f(a.s[g]);
-      br[i] = bf16f(a.b[g]);
+      const uint32_t o = lane_off(so[i] - back(min((tid + 256 * i) / BN, GS - 1), ng));
+      sr[i] = bf16f((sb + g0)[o]);
+      br[i] = bf16f((bb + g0)[o]);
+    }
+    if constexpr (XG) {
+#pragma unroll
+      for (uint32_t i = 0; i < XS; ++i)
+        sxr[i] = (sxb + g0)[lane_off(sxo[i] - back(min((tid + 256 * i) / BM, GS - 1), ng))];
     }
   };
   auto store = [&](uint32_t st) {
     typename T::Buf& B = lds.buf[st & 1];
     uint2* const x8 = reinterpret_cast<uint2*>(B.x);
     uint2* const w8 = reinterpret_cast<uint2*>(B.w);
-    const bool last = st + 1 == steps;
 #pragma unroll
     for (uint32_t i = 0; i < XP; ++i) {
       const uint32_t id = tid + 256 * i, row = id / 8, p = id % 8;
-      int32_t sum = 0;
       uint2 v[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t lo = xr[i][2 * e], hi = xr[i][2 * e + 1];
-        sum = __builtin_amdgcn_sdot4((int)lo, 0x01010101, sum, false);
-        sum = __builtin_amdgcn_sdot4((int)hi, 0x01010101, sum, false);
         v[e] = BITS == 8 ? make_uint2(lo, hi)
                          : make_uint2(__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u));
       }
@@ -349,27 +379,10 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
       } else {
         B.x[(tile + q8_slot<BITS, G>(p, 0, r16)) / 2] = u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
       }
-      // The group's pieces lie in neighbouring lanes.
-      auto dpp_add = [&](auto ctrl) { return sum + __builtin_amdgcn_update_dpp(0, sum, decltype(ctrl)::value, 0xF, 0xF, false); };
-      sum = dpp_add(std::integral_constant<int, 0xB1>{});
-      if constexpr (G >= 64) sum = dpp_add(std::integral_constant<int, 0x4E>{});
-      if constexpr (G == 128) sum = dpp_add(std::integral_constant<int, 0x141>{});
-      if (p % (G / 16) == 0) {
-        const uint32_t j = p / (G / 16), g = st * GS + j;
-        const float sx = XG ? q8_round22(sxr[i]) : 1.f;
-        lds.xs[(g >> 2) & 1][g & 3][row] = sx * (float)sum;
-        if constexpr (XG) {
-          B.sx[j][row] = sx;
-          B.sx[GS + j][row] = -kMagic * sx;
-        }
-        // Groups behind the last up to a whole four count nothing.
-        if (last && j == GS - 1)
-          for (uint32_t z = g + 1; z & 3; ++z) lds.xs[(z >> 2) & 1][z & 3][row] = 0.f;
-      }
     }
 #pragma unroll
     for (uint32_t i = 0; i < WP; ++i) {
-      const uint32_t id = tid + 256 * i, col = id / WC, c = id % WC;
+      const uint32_t id = tid + 256 * i, col = w_col(id), c = id % WC;
       const uint32_t tile = col / 16 * 256, r16 = col % 16;
       if constexpr (BITS == 8) {
         const u32x4 v = wr[i] ^ 0x80808080u;
@@ -399,11 +412,19 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
 #pragma unroll
     for (uint32_t i = 0; i < SP; ++i) {
       const uint32_t id = tid + 256 * i, col = id % BN, j = id / BN, g = st * GS + j;
-      if (j >= GS) continue;
+      if (GS * BN % 256 && j >= GS) continue;
       B.s[j][col] = sr[i];
       lds.b[(g >> 2) & 1][g & 3][col] = BITS == 8 ? __builtin_fmaf(sr[i], 128.f, br[i]) : br[i];
-      if (last && j == GS - 1)
-        for (uint32_t z = g + 1; z & 3; ++z) lds.b[(z >> 2) & 1][z & 3][col] = 0.f;
+    }
+    if constexpr (XG) {
+#pragma unroll
+      for (uint32_t i = 0; i < XS; ++i) {
+        const uint32_t id = tid + 256 * i, row = id % BM, j = id / BM;
+        if (GS * BM % 256 && j >= GS) continue;
+        const float sx = q8_round22(sxr[i]);
+        B.sx[j][row] = sx;
+        B.sx[GS + j][row] = -kMagic * sx;
+      }
     }
   };
 
@@ -414,23 +435,44 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int kStart = XG ? (int)kMagicBits : 0;
   const i32x4 start = {kStart, kStart, kStart, kStart};
+  const u32x4 one = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
+  float xs[MT];  // the row's group sums, lane block kb that of group 4 q + kb
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xs[m] = 0.f;
   auto compute = [&](uint32_t st) {
     const typename T::Buf& B = lds.buf[st & 1];
-    const u32x4* const xo = B.x + wm * MT * 128 + lane;
-    const u32x4* const wo = B.w + wn * NT * 128 + lane;
+    // The lane's place in operand h (q8_slot).
+    const uint32_t at[2] = {kb * 16 + (c16 ^ kb), 64 + kb * 16 + (c16 ^ (4 + kb))};
+    const u32x4* const xt = B.x + wm * MT * 128;
+    const u32x4* const wt = B.w + wn * NT * 128;
 #pragma unroll
     for (uint32_t j = 0; j < GS; ++j) {
       u32x4 x[MT][2];  // G = 128: both operands
       float sx[MT], cx[MT];
+      auto product = [&](const u32x4 (&w)[2], int m) {
+        if constexpr (G == 128)
+          return q8_mfma(w[1], x[m][1], q8_mfma(w[0], x[m][0], start));
+        else if constexpr (G == 64)
+          return q8_mfma(w[0], x[m][0], start);
+        else
+          return q8_mfma32(w[0].x, w[0].y, x[m][0].x, x[m][0].y, start);
+      };
+      // The sum S times the row's scale of this group.
+      auto value = [&](int32_t S, int m) {
+        if constexpr (XG)
+          return __builtin_fmaf(__int_as_float(S), sx[m], cx[m]);
+        else
+          return (float)S;
+      };
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if constexpr (G == 128) {
-          x[m][0] = xo[m * 128];
-          x[m][1] = xo[m * 128 + 64];
+          x[m][0] = xt[m * 128 + at[0]];
+          x[m][1] = xt[m * 128 + at[1]];
         } else if constexpr (G == 64) {
-          x[m][0] = xo[m * 128 + j * 64];
+          x[m][0] = xt[m * 128 + at[j]];
         } else {
-          const uint2 v = reinterpret_cast<const uint2*>(xo + m * 128 + j / 2 * 64)[j % 2];
+          const uint2 v = reinterpret_cast<const uint2*>(xt + m * 128 + at[j / 2])[j % 2];
           x[m][0].x = v.x;
           x[m][0].y = v.y;
         }
@@ -444,61 +486,65 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
         const f32x4 s = *reinterpret_cast<const f32x4*>(&B.s[j][wn * NT * 16 + t * 16 + 4 * kb]);
         u32x4 w[2];
         if constexpr (G == 128) {
-          w[0] = wo[t * 128];
-          w[1] = wo[t * 128 + 64];
+          w[0] = wt[t * 128 + at[0]];
+          w[1] = wt[t * 128 + at[1]];
         } else if constexpr (G == 64) {
-          w[0] = wo[t * 128 + j * 64];
+          w[0] = wt[t * 128 + at[j]];
         } else {
-          const uint2 v = reinterpret_cast<const uint2*>(wo + t * 128 + j / 2 * 64)[j % 2];
+          const uint2 v = reinterpret_cast<const uint2*>(wt + t * 128 + at[j / 2])[j % 2];
           w[0].x = v.x;
           w[0].y = v.y;
         }
         i32x4 S[MT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if constexpr (G == 128)
-            S[m] = q8_mfma(w[1], x[m][1], q8_mfma(w[0], x[m][0], start));
-          else if constexpr (G == 64)
-            S[m] = q8_mfma(w[0], x[m][0], start);
-          else
-            S[m] = q8_mfma32(w[0].x, w[0].y, x[m][0].x, x[m][0].y, start);
-        }
+        for (int m = 0; m < MT; ++m) S[m] = product(w, m);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float f;
-            if constexpr (XG)
-              f = __builtin_fmaf(__int_as_float(S[m][i]), sx[m], cx[m]);
-            else
-              f = (float)S[m][i];
-            acc[m][t][i] = __builtin_fmaf(s[i], f, acc[m][t][i]);
-          }
+          for (int i = 0; i < 4; ++i) acc[m][t][i] = __builtin_fmaf(s[i], value(S[m][i], m), acc[m][t][i]);
+      }
+      const u32x4 ones[2] = {one, one};
+      const bool mine = kb == ((st * GS + j) & 3);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const float v = value(product(ones, m)[0], m);
+        xs[m] = mine ? v : xs[m];
       }
     }
     const uint32_t g1 = (st + 1) * GS;  // groups staged so far
     if ((g1 & 3) == 0 || st + 1 == steps) {
       const uint32_t ring = ((g1 - 1) >> 2) & 1;
-      float b[NT], xs[MT];
+      // In the last four, groups that do not exist count nothing.
+      const bool live = g1 - ((g1 - 1) & 3) - 1 + kb < g1;
+      float b[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) b[t] = lds.b[ring][kb][wn * NT * 16 + t * 16 + c16];
+      for (int t = 0; t < NT; ++t) {
+        b[t] = lds.b[ring][kb][wn * NT * 16 + t * 16 + c16];
+        b[t] = live ? b[t] : 0.f;
+      }
 #pragma unroll
-      for (int m = 0; m < MT; ++m) xs[m] = lds.xs[ring][kb][wm * MT * 16 + m * 16 + c16];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[t], xs[m], acc[m][t], 0, 0, 0);
+        xs[m] = 0.f;
+      }
     }
   };
 
-  load(0);
+  const uint32_t whole = K / kQ8Step;  // steps without a tail
+  auto fetch = [&](uint32_t st) {
+    if (st < whole)
+      load(st, std::false_type{});
+    else if (st < steps)
+      load(st, std::true_type{});
+  };
+  fetch(0);
   store(0);
   __syncthreads();
   for (uint32_t st = 0; st < steps; ++st) {
-    const bool more = st + 1 < steps;
-    if (more) load(st + 1);
+    fetch(st + 1);
     compute(st);
-    if (more) store(st + 1);
+    if (st + 1 < steps) store(st + 1);
     __syncthreads();
   }
 
