@@ -315,6 +315,7 @@ struct Q8Args {
   float* y;                // [n, O]
   uint32_t O, K, n;
   uint32_t vec;            // y on 16 bytes, O a multiple of 4
+  uint32_t svec, xvec;     // s and b (sx) on 16 bytes, K / group a multiple of 8 (4)
 };
 hipError_t launch_qmm_i8(const Q8Args& a, uint32_t bits, uint32_t group, bool x_grouped, hipStream_t st);
 // Low-rank adapters (lora.hip).

@@ -203,24 +203,31 @@ __global__ __launch_bounds__(256) void k_q8(Q8Args a) {
 
 // ---------------------------------------------------------------------------
 // Many rows: a block of four waves takes WM MT tiles of 16 rows x WN NT tiles
-// of 16 columns, step after step of 128 inputs. A step's rows and codes go
-// through registers into LDS in operand order (a wave's operand is 1 KB that
-// the lanes read in lane order), the codes unpacked and the rows' bytes put in
-// their order once per block instead of once per wave; the next step's loads
-// are in flight while a step is computed. Weights are the A operand, so a lane
-// ends with four neighbouring columns of one row.
+// of 16 columns, step after step of 128 inputs. A step's rows go straight into
+// LDS, its codes through registers, where they are unpacked once per block
+// instead of once per wave; the next step's loads are in flight while a step is
+// computed. Weights are the A operand, so a lane ends with four neighbouring
+// columns of one row.
 //
 // The fold of a group's sums is what bounds it: two VALU instructions per
-// value (16 x 16 x 64: 8 per lane, 32 cycles, against 16 on the matrix cores).
-// With scales per group the sums come out of the MFMA as floats, 1.5 2^23 + S,
-// by an accumulator that starts as that number's bits (|S| < 2^22), and
-// fma(f, sx, -1.5 2^23 sx) = sx S in one rounding: the product in the constant
-// is exact for an sx of 22 bits, so sx is rounded to those (by 2^-23 of it).
-// The bias term runs on v_mfma_f32_16x16x4_f32, four groups at a time, over the
-// rows' group sums, which a product with ones leaves in every lane of a row.
+// value, 8 per lane and 16 x 16 x 64 product (34 cycles, and the product keeps
+// the VALU from issuing for 10 of its 16). With scales per group the sums come
+// out of the MFMA as floats, 1.5 2^23 + S, by an accumulator that starts as
+// that number's bits (|S| < 2^22), and fma(f, sx, -1.5 2^23 sx) = sx S in one
+// rounding: the product in the constant is exact for an sx of 22 bits, so sx is
+// rounded to those (by 2^-23 of it).
+//
+// The bias term: a product with ones leaves a group's sum of inputs X in every
+// lane of a row, and eight groups' sums times biases are one bf16 MFMA, lane
+// block kb holding groups 2 kb and 2 kb + 1 as sx X = h + m + l in three bf16
+// (exact: 24 bits) against the bias three times. (v_mfma_f32_16x16x4_f32 on the
+// sums as they are takes 64 cycles for four groups: 9 us of 87 at 1000 rows
+// 4096 -> 7168.)
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMagicBits = 0x4B400000u;  // 1.5 * 2^23
 constexpr float kMagic = 12582912.f;
+
+typedef __bf16 qbf16x8 __attribute__((ext_vector_type(8)));
 
 // sx to 22 significant bits.
 __device__ __forceinline__ float q8_round22(float v) {
@@ -229,45 +236,42 @@ __device__ __forceinline__ float q8_round22(float v) {
   return __uint_as_float((u + 1u + ((u >> 2) & 1u)) & ~3u);
 }
 
-// Where the e-th eight of piece p (16 inputs) of a row's step lies in operand
-// order: [h][kb][row][e], 8-byte units for rows of 16 (see q8_pos). The row's
-// place is exchanged by 4 h + kb, so that the pieces of a row, which
-// neighbouring lanes write, fall in different banks (8 writes to one: 33 of
-// 54 % of the LDS cycles were conflicts).
-template <int BITS, int G>
-__device__ __forceinline__ uint32_t q8_slot(uint32_t p, uint32_t e, uint32_t row) {
-  uint32_t h, kb, f = e;
-  if (G == 32) {
-    h = p >> 2, kb = (p & 1) * 2 + e, f = (p >> 1) & 1;
-  } else if (BITS == 8) {
-    h = p >> 2, kb = p & 3;
-  } else if (G == 64) {
-    h = p >> 2, kb = ((p & 1) << 1) | ((p >> 1) & 1);
-  } else {
-    h = p & 1, kb = p >> 1;
-  }
-  return ((h * 4 + kb) * 16 + (row ^ (h * 4 + kb))) * 2 + f;
+// Three bf16 of a and three of b, each the rest of those before it.
+__device__ __forceinline__ qbf16x8 q8_parts(float a, float b) {
+  auto top = [](float v) { return __float_as_uint(v) & 0xFFFF0000u; };
+  const uint32_t ah = top(a), bh = top(b);
+  const float ar = a - __uint_as_float(ah), br = b - __uint_as_float(bh);
+  const uint32_t am = top(ar), bm = top(br);
+  const uint32_t al = __float_as_uint(ar - __uint_as_float(am)), bl = __float_as_uint(br - __uint_as_float(bm));
+  return __builtin_bit_cast(qbf16x8, u32x4{ah >> 16 | am, al >> 16 | bh, bm >> 16 | (bl & 0xFFFF0000u), 0u});
 }
 
-template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
+// LDS place (16 bytes) of piece p (16 inputs) of a row's step: the eight pieces
+// of a row side by side, exchanged by the row so that eight rows' reads of one
+// piece fall in different banks.
+__device__ __forceinline__ uint32_t q8_place(uint32_t row, uint32_t p) { return row * 8 + (p ^ (row & 7)); }
+
+template <bool XG, int WM, int WN, int MT, int NT>
 struct Q8Tile {
-  static constexpr uint32_t BM = WM * MT * 16, BN = WN * NT * 16, GS = kQ8Step / G;
+  static constexpr uint32_t BM = WM * MT * 16, BN = WN * NT * 16;
   struct Buf {
     u32x4 x[BM * 8], w[BN * 8];
-    float s[GS][BN];
-    float sx[XG ? 2 * GS : 1][XG ? BM : 1];  // sx, then -1.5 2^23 sx
   };
   struct Lds {
     Buf buf[2];
-    float b[2][4][BN];  // biases, by group mod 4
+    // Of two fours of groups, by group mod 8: scales, rows' scales; of eight:
+    // the packed biases and scales (pairs of groups) of a column.
+    float s[2][4][BN], sx[XG ? 2 : 1][XG ? 4 : 1][XG ? BM : 1];
+    uint32_t pair[2][2][4][BN];  // [octet mod 2][bias, scale][pair][column]
   };
 };
 
 template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint32_t units) {
-  using T = Q8Tile<BITS, G, XG, WM, WN, MT, NT>;
-  constexpr uint32_t BM = T::BM, BN = T::BN, GS = T::GS;
+  using T = Q8Tile<XG, WM, WN, MT, NT>;
+  constexpr uint32_t BM = T::BM, BN = T::BN, GS = kQ8Step / G;
   static_assert(WM * WN == 4, "four waves");
+  static_assert(BN % 64 == 0 && BM % 64 == 0, "a wave stages one kind");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
   typename T::Lds& lds = *reinterpret_cast<typename T::Lds*>(lds_raw);
   const uint32_t tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kb = lane >> 4;
@@ -279,64 +283,81 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
   const uint32_t row0 = u % nrb * BM, col0 = u / nrb * BN;
   const uint32_t K = a.K, O = a.O, gpr = K / G, steps = (K + kQ8Step - 1) / kQ8Step;
   const uint32_t row_bytes = K / 32 * (BITS * 4);
+  const uint32_t rows = min(BM, a.n - row0), cols = min(BN, O - col0);
 
   // What a thread stages: pieces of 16 inputs of rows, chunks of weight rows
-  // (32 codes; 8 bits: 16), scales and biases, rows' scales.
+  // (32 codes; 8 bits: 16) and, per eight groups, the scales or biases of a
+  // column and half of a row's scales (read step by step, each of these small
+  // reads would fetch its line again). Scalar bases of the block and 32-bit
+  // offsets of the lane.
   constexpr uint32_t XP = BM * 8 / 256;
   constexpr uint32_t WC = BITS == 8 ? 8 : 4, WP = BN * WC / 256;
-  constexpr uint32_t SP = (GS * BN + 255) / 256, XS = XG ? (GS * BM + 255) / 256 : 1;
-  static_assert(BM * 8 % 256 == 0 && BN * WC % 256 == 0, "whole pieces per thread");
-  // A wave's 16 cols x 4 chunks in an order whose eights of lanes write to
-  // different banks (columns c and c + 2 side by side).
-  auto w_col = [](uint32_t id) {
-    const uint32_t c = id / WC;
-    return BITS == 8 ? c : (c & ~3u) | ((c & 1) << 1) | ((c >> 1) & 1);
-  };
-  // Scalar bases of the block and 32-bit offsets of the lane.
+  constexpr uint32_t CB = BITS == 8 ? 16 : chunk_bytes<BITS>(), CI = BITS == 8 ? 16 : 32;  // bytes, codes of a chunk
+  constexpr uint32_t SP = (2 * BN + 255) / 256, XS = (2 * BM + 255) / 256;
   const int8_t* const xb = a.x + (uint64_t)row0 * K;
   const uint8_t* const wb = a.w + (uint64_t)col0 * row_bytes;
   const uint16_t* const sb = a.s + (uint64_t)col0 * gpr;
   const uint16_t* const bb = a.b + (uint64_t)col0 * gpr;
   const float* const sxb = a.sx + (uint64_t)row0 * (XG ? gpr : 0);
-  const uint32_t rows = min(BM, a.n - row0), cols = min(BN, O - col0);
   uint32_t xo[XP], wo[WP], so[SP], sxo[XS];
+  const uint32_t xp = (tid & 7) ^ ((tid >> 3) & 7);  // the piece whose place is tid mod 8 (256 threads are whole eights of rows)
 #pragma unroll
-  for (uint32_t i = 0; i < XP; ++i) xo[i] = min((tid + 256 * i) / 8, rows - 1) * K + (tid & 7) * 16;
+  for (uint32_t i = 0; i < XP; ++i) xo[i] = min((tid + 256 * i) / 8, rows - 1) * K + xp * 16;
 #pragma unroll
-  for (uint32_t i = 0; i < WP; ++i) {
-    const uint32_t id = tid + 256 * i;
-    wo[i] = min(w_col(id), cols - 1) * row_bytes + id % WC * (BITS == 8 ? 16 : chunk_bytes<BITS>());
-  }
+  for (uint32_t i = 0; i < WP; ++i) wo[i] = min((tid + 256 * i) / WC, cols - 1) * row_bytes + tid % WC * CB;
+  auto s_part = [&](uint32_t i) { return (wave * 64 + 256 * i) / BN; };  // 0: scales, 1: biases
+  auto x_part = [&](uint32_t i) { return (wave * 64 + 256 * i) / BM; };  // half of eight groups
 #pragma unroll
-  for (uint32_t i = 0; i < SP; ++i) {
-    const uint32_t id = tid + 256 * i;
-    so[i] = min(id % BN, cols - 1) * gpr + min(id / BN, GS - 1);
-  }
+  for (uint32_t i = 0; i < SP; ++i) so[i] = min((tid + 256 * i) % BN, cols - 1) * gpr;
 #pragma unroll
-  for (uint32_t i = 0; i < XS; ++i) {
-    const uint32_t id = tid + 256 * i;
-    sxo[i] = min(id % BM, rows - 1) * gpr + min(id / BM, GS - 1);
-  }
-  u32x4 xr[XP], wr[WP];
-  float sr[SP], br[SP], sxr[XS];
+  for (uint32_t i = 0; i < XS; ++i) sxo[i] = min((tid + 256 * i) % BM, rows - 1) * gpr;
+
+  u32x4 wr[WP], sr[SP];
+  f32x4 sxr[XS];
+  auto load_scales = [&](uint32_t g0) {  // of groups g0 .. g0 + 7, the last repeated behind it
+#pragma unroll
+    for (uint32_t i = 0; i < SP; ++i) {
+      if (s_part(i) > 1) continue;
+      const uint16_t* const p = s_part(i) ? bb : sb;
+      if (a.svec) {  // gpr is a multiple of 8
+        sr[i] = *reinterpret_cast<const u32x4*>(p + g0 + lane_off(so[i]));
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          const uint32_t lo = p[lane_off(so[i] + min(g0 + 2 * j, gpr - 1))], hi = p[lane_off(so[i] + min(g0 + 2 * j + 1, gpr - 1))];
+          sr[i][j] = lo | hi << 16;
+        }
+      }
+    }
+    if constexpr (XG) {
+#pragma unroll
+      for (uint32_t i = 0; i < XS; ++i) {
+        if (x_part(i) > 1) continue;
+        const uint32_t g = g0 + 4 * x_part(i);
+        if (a.xvec && g + 4 <= gpr) {
+          sxr[i] = *reinterpret_cast<const f32x4*>(sxb + g + lane_off(sxo[i]));
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) sxr[i][j] = sxb[lane_off(sxo[i] + min(g + j, gpr - 1))];
+        }
+      }
+    }
+  };
   // TAIL: the step that K ends in. Loads past the end step back into the row
-  // (by as many pieces, chunks or groups as they are past it); inputs there
-  // are zero.
+  // (by as many pieces or chunks as they are past it); the codes there become
+  // zero in store.
+  const uint32_t whole = K / kQ8Step;
   auto load = [&](uint32_t st, auto tail) {
     constexpr bool TAIL = decltype(tail)::value;
-    const uint32_t k0 = st * kQ8Step, g0 = st * GS, ng = TAIL ? gpr - g0 : GS;
+    const uint32_t k0 = st * kQ8Step;
     const int8_t* const x = xb + k0;
     const uint8_t* const w = wb + k0 / 32 * (BITS * 4);
     auto back = [&](uint32_t at, uint32_t n) { return TAIL && at >= n ? at - (n - 1) : 0u; };
+    u32x4* const xl = lds.buf[st & 1].x + wave * 64;
 #pragma unroll
-    for (uint32_t i = 0; i < XP; ++i) {
-      const uint32_t p = tid & 7, np = TAIL ? (K - k0) / 16 : 8u;
-      xr[i] = *reinterpret_cast<const u32x4*>(x + lane_off(xo[i] - back(p, np) * 16));
-      if (TAIL && p >= np) xr[i] = u32x4{0u, 0u, 0u, 0u};
-    }
+    for (uint32_t i = 0; i < XP; ++i) dma16(x + lane_off(xo[i] - back(xp, TAIL ? (K - k0) / 16 : 8u) * 16), xl + 256 * i);
 #pragma unroll
     for (uint32_t i = 0; i < WP; ++i) {
-      constexpr uint32_t CB = BITS == 8 ? 16 : chunk_bytes<BITS>(), CI = BITS == 8 ? 16 : 32;
       const uint8_t* const q = w + lane_off(wo[i] - back(tid % WC, TAIL ? (K - k0) / CI : WC) * CB);
       if constexpr (BITS == 8) {
         wr[i] = *reinterpret_cast<const u32x4*>(q);
@@ -346,84 +367,62 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
         for (int j = 0; j < BITS; ++j) wr[i][j] = r.d[j];
       }
     }
-#pragma unroll
-    for (uint32_t i = 0; i < SP; ++i) {
-      const uint32_t o = lane_off(so[i] - back(min((tid + 256 * i) / BN, GS - 1), ng));
-      sr[i] = bf16f((sb + g0)[o]);
-      br[i] = bf16f((bb + g0)[o]);
-    }
-    if constexpr (XG) {
-#pragma unroll
-      for (uint32_t i = 0; i < XS; ++i)
-        sxr[i] = (sxb + g0)[lane_off(sxo[i] - back(min((tid + 256 * i) / BM, GS - 1), ng))];
-    }
+    if (st * GS % 8 == 0) load_scales(st * GS);
+  };
+  auto fetch = [&](uint32_t st) {
+    if (st < whole)
+      load(st, std::false_type{});
+    else if (st < steps)
+      load(st, std::true_type{});
   };
   auto store = [&](uint32_t st) {
-    typename T::Buf& B = lds.buf[st & 1];
-    uint2* const x8 = reinterpret_cast<uint2*>(B.x);
-    uint2* const w8 = reinterpret_cast<uint2*>(B.w);
-#pragma unroll
-    for (uint32_t i = 0; i < XP; ++i) {
-      const uint32_t id = tid + 256 * i, row = id / 8, p = id % 8;
-      uint2 v[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t lo = xr[i][2 * e], hi = xr[i][2 * e + 1];
-        v[e] = BITS == 8 ? make_uint2(lo, hi)
-                         : make_uint2(__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u));
-      }
-      const uint32_t tile = row / 16 * 256, r16 = row % 16;
-      if constexpr (G == 32) {
-        x8[tile + q8_slot<BITS, G>(p, 0, r16)] = v[0];
-        x8[tile + q8_slot<BITS, G>(p, 1, r16)] = v[1];
-      } else {
-        B.x[(tile + q8_slot<BITS, G>(p, 0, r16)) / 2] = u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
-      }
-    }
+    u32x4* const wl = lds.buf[st & 1].w;
+    const bool past = st >= whole && tid % WC >= (K - st * kQ8Step) / CI;
 #pragma unroll
     for (uint32_t i = 0; i < WP; ++i) {
-      const uint32_t id = tid + 256 * i, col = w_col(id), c = id % WC;
-      const uint32_t tile = col / 16 * 256, r16 = col % 16;
+      const uint32_t col = (tid + 256 * i) / WC, c = tid % WC;
       if constexpr (BITS == 8) {
-        const u32x4 v = wr[i] ^ 0x80808080u;
-        if constexpr (G == 32) {
-          w8[tile + q8_slot<BITS, G>(c, 0, r16)] = make_uint2(v.x, v.y);
-          w8[tile + q8_slot<BITS, G>(c, 1, r16)] = make_uint2(v.z, v.w);
-        } else {
-          B.w[(tile + q8_slot<BITS, G>(c, 0, r16)) / 2] = v;
-        }
+        wl[q8_place(col, c)] = past ? u32x4{0u, 0u, 0u, 0u} : wr[i] ^ 0x80808080u;
       } else {
         Raw<BITS> r;
 #pragma unroll
-        for (int j = 0; j < BITS; ++j) r.d[j] = wr[i][j];
-        uint32_t q[8];
+        for (int j = 0; j < BITS; ++j) r.d[j] = past ? 0u : wr[i][j];
+        uint32_t q[8];  // evens and odds of eight codes
         unpack_bytes(r, q);
+        uint32_t v[8];
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-          if constexpr (G == 32) {
-            w8[tile + q8_slot<BITS, G>(2 * c + h, 0, r16)] = make_uint2(q[4 * h], q[4 * h + 1]);
-            w8[tile + q8_slot<BITS, G>(2 * c + h, 1, r16)] = make_uint2(q[4 * h + 2], q[4 * h + 3]);
-          } else {
-            B.w[(tile + q8_slot<BITS, G>(2 * c + h, 0, r16)) / 2] = u32x4{q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]};
-          }
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = __builtin_amdgcn_perm(q[2 * j + 1], q[2 * j], 0x05010400u);
+          v[2 * j + 1] = __builtin_amdgcn_perm(q[2 * j + 1], q[2 * j], 0x07030602u);
         }
+        wl[q8_place(col, 2 * c)] = u32x4{v[0], v[1], v[2], v[3]};
+        wl[q8_place(col, 2 * c + 1)] = u32x4{v[4], v[5], v[6], v[7]};
       }
     }
+    if (st * GS % 4) return;
+    const uint32_t half = st * GS / 4 & 1, octet = st * GS / 8 & 1;
 #pragma unroll
     for (uint32_t i = 0; i < SP; ++i) {
-      const uint32_t id = tid + 256 * i, col = id % BN, j = id / BN, g = st * GS + j;
-      if (GS * BN % 256 && j >= GS) continue;
-      B.s[j][col] = sr[i];
-      lds.b[(g >> 2) & 1][g & 3][col] = BITS == 8 ? __builtin_fmaf(sr[i], 128.f, br[i]) : br[i];
+      if (s_part(i) > 1) continue;
+      const uint32_t col = (tid + 256 * i) % BN;
+      if (s_part(i) == 0) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          const uint32_t v = half ? sr[i][2 + j / 2] : sr[i][j / 2];
+          lds.s[half][j][col] = __uint_as_float(j & 1 ? v & 0xFFFF0000u : v << 16);
+        }
+      }
+      if (half == 0 && (BITS == 8 || s_part(i) == 1)) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) lds.pair[octet][1 - s_part(i)][j][col] = sr[i][j];
+      }
     }
     if constexpr (XG) {
 #pragma unroll
       for (uint32_t i = 0; i < XS; ++i) {
-        const uint32_t id = tid + 256 * i, row = id % BM, j = id / BM;
-        if (GS * BM % 256 && j >= GS) continue;
-        const float sx = q8_round22(sxr[i]);
-        B.sx[j][row] = sx;
-        B.sx[GS + j][row] = -kMagic * sx;
+        if (x_part(i) != half) continue;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) lds.sx[half][j][(tid + 256 * i) % BM] = q8_round22(sxr[i][j]);
       }
     }
   };
@@ -436,115 +435,130 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
   constexpr int kStart = XG ? (int)kMagicBits : 0;
   const i32x4 start = {kStart, kStart, kStart, kStart};
   const u32x4 one = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
-  float xs[MT];  // the row's group sums, lane block kb that of group 4 q + kb
+  float xs[MT][2];  // sx X of groups 2 kb and 2 kb + 1 of the eight
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xs[m] = 0.f;
+  for (int m = 0; m < MT; ++m) xs[m][0] = xs[m][1] = 0.f;
+
   auto compute = [&](uint32_t st) {
     const typename T::Buf& B = lds.buf[st & 1];
-    // The lane's place in operand h (q8_slot).
-    const uint32_t at[2] = {kb * 16 + (c16 ^ kb), 64 + kb * 16 + (c16 ^ (4 + kb))};
-    const u32x4* const xt = B.x + wm * MT * 128;
-    const u32x4* const wt = B.w + wn * NT * 128;
+    const uint32_t half = st * GS / 4 & 1, g0 = st * GS % 4;
+    struct Op {
+      u32x4 v[2];  // groups of 128: both operands; of 32: the group's half of one
+    };
+    // Operand of group j of the step: 16 inputs at 64 h + 16 kb, of groups of 32
+    // eight at 32 j + 8 kb.
+    auto read = [&](const u32x4* rows16, uint32_t j) {
+      Op o;
+      if constexpr (G == 32) {
+        const uint2 v = reinterpret_cast<const uint2*>(rows16 + q8_place(c16, 2 * j + kb / 2))[kb & 1];
+        o.v[0] = u32x4{v.x, v.y, 0u, 0u};
+      } else {
+        o.v[0] = rows16[q8_place(c16, (G == 64 ? 4 * j : 0u) + kb)];
+        if (G == 128) o.v[1] = rows16[q8_place(c16, 4 + kb)];
+      }
+      return o;
+    };
+    auto product = [&](const Op& w, const Op& x) {
+      if constexpr (G == 128)
+        return q8_mfma(w.v[1], x.v[1], q8_mfma(w.v[0], x.v[0], start));
+      else if constexpr (G == 64)
+        return q8_mfma(w.v[0], x.v[0], start);
+      else
+        return q8_mfma32(w.v[0].x, w.v[0].y, x.v[0].x, x.v[0].y, start);
+    };
+    const Op ones{{one, one}};
 #pragma unroll
     for (uint32_t j = 0; j < GS; ++j) {
-      u32x4 x[MT][2];  // G = 128: both operands
+      Op x[MT], w[2];
       float sx[MT], cx[MT];
-      auto product = [&](const u32x4 (&w)[2], int m) {
-        if constexpr (G == 128)
-          return q8_mfma(w[1], x[m][1], q8_mfma(w[0], x[m][0], start));
-        else if constexpr (G == 64)
-          return q8_mfma(w[0], x[m][0], start);
-        else
-          return q8_mfma32(w[0].x, w[0].y, x[m][0].x, x[m][0].y, start);
-      };
+      f32x4 s[2];
+      i32x4 S[2];
       // The sum S times the row's scale of this group.
-      auto value = [&](int32_t S, int m) {
+      auto value = [&](int32_t v, int m) {
         if constexpr (XG)
-          return __builtin_fmaf(__int_as_float(S), sx[m], cx[m]);
+          return __builtin_fmaf(__int_as_float(v), sx[m], cx[m]);
         else
-          return (float)S;
+          return (float)v;
+      };
+      auto read_w = [&](int t) {
+        w[t & 1] = read(B.w + (wn * NT + t) * 128, j);
+        s[t & 1] = *reinterpret_cast<const f32x4*>(&lds.s[half][g0 + j][(wn * NT + t) * 16 + 4 * kb]);
       };
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        if constexpr (G == 128) {
-          x[m][0] = xt[m * 128 + at[0]];
-          x[m][1] = xt[m * 128 + at[1]];
-        } else if constexpr (G == 64) {
-          x[m][0] = xt[m * 128 + at[j]];
-        } else {
-          const uint2 v = reinterpret_cast<const uint2*>(xt + m * 128 + at[j / 2])[j % 2];
-          x[m][0].x = v.x;
-          x[m][0].y = v.y;
-        }
+        x[m] = read(B.x + (wm * MT + m) * 128, j);
         if constexpr (XG) {
-          sx[m] = B.sx[j][wm * MT * 16 + m * 16 + c16];
-          cx[m] = B.sx[GS + j][wm * MT * 16 + m * 16 + c16];
+          sx[m] = lds.sx[half][g0 + j][(wm * MT + m) * 16 + c16];
+          cx[m] = -kMagic * sx[m];
         }
       }
+      read_w(0);
+      // Units (column tile t, row tile m), m fastest, the product with ones
+      // behind them: a unit's product is issued ahead of the fold of the one
+      // before it.
+      constexpr int UNITS = (NT + 1) * MT;
+      auto issue = [&](int u) {
+        const int t = u / MT, m = u % MT;
+        S[u & 1] = product(t < NT ? w[t & 1] : ones, x[m]);
+      };
+      issue(0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(&B.s[j][wn * NT * 16 + t * 16 + 4 * kb]);
-        u32x4 w[2];
-        if constexpr (G == 128) {
-          w[0] = wt[t * 128 + at[0]];
-          w[1] = wt[t * 128 + at[1]];
-        } else if constexpr (G == 64) {
-          w[0] = wt[t * 128 + at[j]];
+      for (int u = 0; u < UNITS; ++u) {
+        const int t = u / MT, m = u % MT;
+        if (m == 0 && t + 1 < NT) read_w(t + 1);
+        if (u + 1 < UNITS) {
+          issue(u + 1);
+          // Holds the product ahead of this fold (it would be placed at its
+          // use, with the fold waiting for it).
+          asm volatile("" : "+v"(S[0]), "+v"(S[1]));
+        }
+        if (t < NT) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][t][i] = __builtin_fmaf(s[t & 1][i], value(S[u & 1][i], m), acc[m][t][i]);
         } else {
-          const uint2 v = reinterpret_cast<const uint2*>(wt + t * 128 + at[j / 2])[j % 2];
-          w[0].x = v.x;
-          w[0].y = v.y;
+          const uint32_t g = st * GS + j;
+          const float v = g < gpr ? value(S[u & 1][0], m) : 0.f;
+          const bool mine = kb == (g / 2 & 3);
+          if (g & 1)
+            xs[m][1] = mine ? v : xs[m][1];
+          else
+            xs[m][0] = mine ? v : xs[m][0];
         }
-        i32x4 S[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) S[m] = product(w, m);
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][t][i] = __builtin_fmaf(s[i], value(S[m][i], m), acc[m][t][i]);
-      }
-      const u32x4 ones[2] = {one, one};
-      const bool mine = kb == ((st * GS + j) & 3);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const float v = value(product(ones, m)[0], m);
-        xs[m] = mine ? v : xs[m];
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    const uint32_t g1 = (st + 1) * GS;  // groups staged so far
-    if ((g1 & 3) == 0 || st + 1 == steps) {
-      const uint32_t ring = ((g1 - 1) >> 2) & 1;
-      // In the last four, groups that do not exist count nothing.
-      const bool live = g1 - ((g1 - 1) & 3) - 1 + kb < g1;
-      float b[NT];
+    const uint32_t g1 = (st + 1) * GS;  // groups done
+    if (g1 % 8 == 0 || st + 1 == steps) {
+      const uint32_t octet = (g1 - 1) / 8 & 1;
+      auto term = [&](uint32_t which, float f) {
+        qbf16x8 xv[MT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        b[t] = lds.b[ring][kb][wn * NT * 16 + t * 16 + c16];
-        b[t] = live ? b[t] : 0.f;
-      }
+        for (int m = 0; m < MT; ++m) xv[m] = q8_parts(xs[m][0] * f, xs[m][1] * f);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t p = lds.pair[octet][which][kb][(wn * NT + t) * 16 + c16];
+          const uint32_t lo = __builtin_amdgcn_perm(p, p, 0x01000100u), hi = __builtin_amdgcn_perm(p, p, 0x03020302u);
+          const qbf16x8 bv = __builtin_bit_cast(qbf16x8, u32x4{lo, p, hi, 0u});
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[t], xs[m], acc[m][t], 0, 0, 0);
-        xs[m] = 0.f;
-      }
+          for (int m = 0; m < MT; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv, xv[m], acc[m][t], 0, 0, 0);
+        }
+      };
+      term(0, 1.f);
+      if (BITS == 8) term(1, 128.f);  // 8-bit codes entered less 128
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xs[m][0] = xs[m][1] = 0.f;
     }
   };
 
-  const uint32_t whole = K / kQ8Step;  // steps without a tail
-  auto fetch = [&](uint32_t st) {
-    if (st < whole)
-      load(st, std::false_type{});
-    else if (st < steps)
-      load(st, std::true_type{});
-  };
   fetch(0);
   store(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows' copies into LDS
   __syncthreads();
   for (uint32_t st = 0; st < steps; ++st) {
     fetch(st + 1);
     compute(st);
     if (st + 1 < steps) store(st + 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
 
@@ -574,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
 // ---------------------------------------------------------------------------
 template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
 static hipError_t q8_tile(const Q8Args& a, hipStream_t st) {
-  using T = Q8Tile<BITS, G, XG, WM, WN, MT, NT>;
+  using T = Q8Tile<XG, WM, WN, MT, NT>;
   const uint32_t nrb = (a.n + T::BM - 1) / T::BM, units = nrb * ((a.O + T::BN - 1) / T::BN);
   constexpr uint32_t lds = sizeof(typename T::Lds);
   auto fn = k_q8_tile<BITS, G, XG, WM, WN, MT, NT>;
