@@ -51,41 +51,16 @@ __device__ __forceinline__ uint32_t q8_pos(uint32_t h, uint32_t e, uint32_t kb) 
   return 32 * kb + 16 * h + 8 * e;
 }
 
-// The rows' operands of a step; inputs from K on are zero.
+// The loaded codes of a step as operands.
 template <int BITS, int G>
-__device__ __forceinline__ void q8_load_x(const int8_t* row, uint32_t k0, uint32_t K, uint32_t kb, u32x4 (&x)[2]) {
-#pragma unroll
-  for (uint32_t h = 0; h < 2; ++h) {
-    uint2 v[2];
-#pragma unroll
-    for (uint32_t e = 0; e < 2; ++e) {
-      const uint32_t at = k0 + q8_pos<BITS, G>(h, e, kb);
-      v[e] = make_uint2(0u, 0u);
-      if (at < K) v[e] = *reinterpret_cast<const uint2*>(row + at);
-      if (BITS != 8) {
-        const uint2 n = v[e];
-        v[e].x = __builtin_amdgcn_perm(n.y, n.x, 0x06040200u);
-        v[e].y = __builtin_amdgcn_perm(n.y, n.x, 0x07050301u);
-      }
-    }
-    x[h] = u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
-  }
-}
-
-// The codes of weight row `row` of a step as operands (past K: any codes).
-template <int BITS, int G>
-__device__ __forceinline__ void q8_load_w(const uint8_t* row, uint32_t k0, uint32_t K, uint32_t kb, u32x4 (&b)[2]) {
+__device__ __forceinline__ void q8_operands(const uint32_t (&d)[BITS == 8 ? 8 : BITS], u32x4 (&b)[2]) {
   if constexpr (BITS == 8) {
-#pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-      uint2 v[2];
-#pragma unroll
-      for (uint32_t e = 0; e < 2; ++e)
-        v[e] = *reinterpret_cast<const uint2*>(row + min(k0 + q8_pos<BITS, G>(h, e, kb), K - 8));
-      b[h] = u32x4{v[0].x, v[0].y, v[1].x, v[1].y} ^ 0x80808080u;
-    }
+    b[0] = u32x4{d[0], d[1], d[2], d[3]} ^ 0x80808080u;
+    b[1] = u32x4{d[4], d[5], d[6], d[7]} ^ 0x80808080u;
   } else {
-    Raw<BITS> w = load_raw<BITS, false>(row + min(k0 / 32 + kb, K / 32 - 1) * chunk_bytes<BITS>());
+    Raw<BITS> w;
+#pragma unroll
+    for (int i = 0; i < BITS; ++i) w.d[i] = d[i];
     if constexpr (G == 64 && BITS == 4) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -128,17 +103,30 @@ __device__ __forceinline__ i32x4 q8_sums(const u32x4 (&x)[2], const u32x4 (&b)[2
   }
 }
 
-// A block: 16 rows x NT tiles of 16 columns, its four waves taking the steps
-// in turn; the sums of the inputs come from a product with ones.
-template <int BITS, int G, bool XG, int NT>
-__global__ __launch_bounds__(256) void k_q8(Q8Args a) {
+// ---------------------------------------------------------------------------
+// Few rows or columns: a block's waves share MT tiles of 16 rows x NT tiles of
+// 16 columns and take the steps of 128 inputs in turn (up to 16 waves: a small
+// call is one round trip to memory). Operands come straight from memory, a step
+// ahead; the sums of inputs come from a product with ones; the waves' parts are
+// added in LDS.
+// ---------------------------------------------------------------------------
+template <int BITS, int G, bool XG, int MT, int NT>
+__global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
   constexpr uint32_t GS = kQ8Step / G;
-  __shared__ f32x4 red[4][NT][64];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
+  extern __shared__ __attribute__((aligned(16))) f32x4 red[];  // [wave][MT * NT][64]
+  const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const uint32_t K = a.K, O = a.O, gpr = K / G, steps = (K + kQ8Step - 1) / kQ8Step;
-  const uint32_t col0 = blockIdx.x * (NT * 16), row0 = blockIdx.y * 16;
+  const uint32_t col0 = blockIdx.x * (NT * 16), row0 = blockIdx.y * (MT * 16);
   const uint32_t row_bytes = K / 32 * (BITS * 4);
-  const int8_t* const xr = a.x + (uint64_t)min(row0 + c16, a.n - 1) * K;
+  const int8_t* xr[MT];
+  const float* sxr[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const uint32_t r = min(row0 + m * 16 + c16, a.n - 1);
+    xr[m] = a.x + (uint64_t)r * K;
+    sxr[m] = a.sx + (uint64_t)r * (XG ? gpr : 1u);
+  }
   const uint8_t* wr[NT];
   const uint16_t *sr[NT], *br[NT];
 #pragma unroll
@@ -148,55 +136,135 @@ __global__ __launch_bounds__(256) void k_q8(Q8Args a) {
     sr[t] = a.s + (uint64_t)c * gpr;
     br[t] = a.b + (uint64_t)c * gpr;
   }
-  const float* sx[4];
+  struct Step {
+    uint2 x[MT][2][2];                       // [operand][eight]
+    uint32_t w[NT][BITS == 8 ? 8 : BITS];
+    uint16_t s[NT][GS], b[NT][GS];
+    float sx[MT][GS];
+  };
+  auto load = [&](uint32_t st, Step& v) {
+    const uint32_t k0 = st * kQ8Step;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sx[i] = a.sx + (uint64_t)min(row0 + 4 * kb + i, a.n - 1) * (XG ? gpr : 1u);
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (BITS == 8) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+          for (uint32_t e = 0; e < 2; ++e) {
+            const uint2 q = *reinterpret_cast<const uint2*>(wr[t] + min(k0 + q8_pos<BITS, G>(h, e, kb), K - 8));
+            v.w[t][4 * h + 2 * e] = q.x;
+            v.w[t][4 * h + 2 * e + 1] = q.y;
+          }
+      } else {
+        const Raw<BITS> r = load_raw<BITS, false>(wr[t] + min(k0 / 32 + kb, K / 32 - 1) * chunk_bytes<BITS>());
+#pragma unroll
+        for (int i = 0; i < BITS; ++i) v.w[t][i] = r.d[i];
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < GS; ++j) {
+        const uint32_t g = min(st * GS + j, gpr - 1);
+        v.s[t][j] = sr[t][g];
+        v.b[t][j] = br[t][g];
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+          const uint32_t at = k0 + q8_pos<BITS, G>(h, e, kb);
+          v.x[m][h][e] = make_uint2(0u, 0u);
+          if (at < K) v.x[m][h][e] = *reinterpret_cast<const uint2*>(xr[m] + at);
+        }
+      if constexpr (XG)
+#pragma unroll
+        for (uint32_t j = 0; j < GS; ++j) v.sx[m][j] = sxr[m][min(st * GS + j, gpr - 1)];
+    }
+  };
   const u32x4 one = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
   const u32x4 ones[2] = {one, one};
-  f32x4 acc[NT];
+  f32x4 acc[MT][NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (uint32_t st = wave; st < steps; st += 4) {
-    const uint32_t k0 = st * kQ8Step;
-    u32x4 x[2], w[NT][2];
-    q8_load_x<BITS, G>(xr, k0, K, kb, x);
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) q8_load_w<BITS, G>(wr[t], k0, K, kb, w[t]);
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto compute = [&](const Step& v) {
+    u32x4 x[MT][2], w[NT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint2 e0 = v.x[m][h][0], e1 = v.x[m][h][1];
+        if (BITS == 8)
+          x[m][h] = u32x4{e0.x, e0.y, e1.x, e1.y};
+        else  // evens before odds, as the codes unpack
+          x[m][h] = u32x4{__builtin_amdgcn_perm(e0.y, e0.x, 0x06040200u), __builtin_amdgcn_perm(e0.y, e0.x, 0x07050301u),
+                          __builtin_amdgcn_perm(e1.y, e1.x, 0x06040200u), __builtin_amdgcn_perm(e1.y, e1.x, 0x07050301u)};
+      }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) q8_operands<BITS, G>(v.w[t], w[t]);
 #pragma unroll
     for (uint32_t j = 0; j < GS; ++j) {
-      const uint32_t g = min(st * GS + j, gpr - 1);
-      const i32x4 X = q8_sums<G>(x, ones, j);
-      f32x4 xf, xs;
+      float xf[MT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xs[i] = XG ? sx[i][g] : 1.f;
-        xf[i] = xs[i] * (float)X[i];
+      for (int m = 0; m < MT; ++m) {
+        xf[m] = (float)q8_sums<G>(ones, x[m], j)[0];
+        if constexpr (XG) xf[m] *= v.sx[m][j];
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float s = bf16f(sr[t][g]);
-        float b = bf16f(br[t][g]);
-        if (BITS == 8) b = __builtin_fmaf(s, 128.f, b);
-        const i32x4 S = q8_sums<G>(x, w[t], j);
+        // Lane (c, kb) of the result holds columns 4 kb .. 4 kb + 3 of row c.
+        const float s1 = bf16f(v.s[t][j]);
+        float b1 = bf16f(v.b[t][j]);
+        if (BITS == 8) b1 = __builtin_fmaf(s1, 128.f, b1);
+        f32x4 s, b;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          acc[t][i] = __builtin_fmaf(s * xs[i], (float)S[i], acc[t][i]);
-          acc[t][i] = __builtin_fmaf(b, xf[i], acc[t][i]);
+          s[i] = __shfl(s1, 4 * (int)kb + i, kWave);
+          b[i] = __shfl(b1, 4 * (int)kb + i, kWave);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const i32x4 S = q8_sums<G>(w[t], x[m], j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f = (float)S[i];
+            if constexpr (XG) f *= v.sx[m][j];
+            acc[m][t][i] = __builtin_fmaf(s[i], f, acc[m][t][i]);
+            acc[m][t][i] = __builtin_fmaf(b[i], xf[m], acc[m][t][i]);
+          }
         }
       }
     }
+  };
+  Step v[2];
+  if (wave < steps) load(wave, v[0]);
+  for (uint32_t st = wave; st < steps; st += 2 * nw) {
+    if (st + nw < steps) load(st + nw, v[1]);
+    compute(v[0]);
+    if (st + nw >= steps) break;
+    if (st + 2 * nw < steps) load(st + 2 * nw, v[0]);
+    compute(v[1]);
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) red[wave][t][lane] = acc[t];
-  __syncthreads();
-  for (uint32_t t = wave; t < NT; t += 4) {
-    const f32x4 v = (red[0][t][lane] + red[1][t][lane]) + (red[2][t][lane] + red[3][t][lane]);
-    const uint32_t col = col0 + t * 16 + c16;
-    if (col >= O) continue;
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t r = row0 + 4 * kb + i;
-      if (r < a.n) a.y[(uint64_t)r * O + col] = XG ? v[i] : v[i] * sx[i][0];
+    for (int t = 0; t < NT; ++t) red[(wave * MT * NT + m * NT + t) * 64 + lane] = acc[m][t];
+  __syncthreads();
+  for (uint32_t mt = wave; mt < MT * NT; mt += nw) {
+    f32x4 sum = red[mt * 64 + lane];
+    for (uint32_t w = 1; w < nw; ++w) sum += red[(w * MT * NT + mt) * 64 + lane];
+    const uint32_t r = row0 + mt / NT * 16 + c16, col = col0 + mt % NT * 16 + 4 * kb;
+    if (r >= a.n) continue;
+    if constexpr (!XG) sum *= a.sx[r];
+    float* const y = a.y + (uint64_t)r * O + col;
+    if (a.vec) {
+      if (col < O) *reinterpret_cast<f32x4*>(y) = sum;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col + i < O) y[i] = sum[i];
     }
   }
 }
@@ -601,13 +669,22 @@ static hipError_t q8_tile(const Q8Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int BITS, int G, bool XG, int MT, int NT>
+static hipError_t q8_few(const Q8Args& a, uint32_t waves, hipStream_t st) {
+  const dim3 grid((a.O + NT * 16 - 1) / (NT * 16), (a.n + MT * 16 - 1) / (MT * 16));
+  hipLaunchKernelGGL((k_q8_few<BITS, G, XG, MT, NT>), grid, dim3(waves * 64), waves * MT * NT * 1024, st, a);
+  return hipGetLastError();
+}
+
 template <int BITS, int G, bool XG>
 static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   if (a.n > 64) return q8_tile<BITS, G, XG, 2, 2, 4, 4>(a, st);
-  constexpr int NT = 4;
-  const dim3 grid((a.O + NT * 16 - 1) / (NT * 16), (a.n + 15) / 16);
-  hipLaunchKernelGGL((k_q8<BITS, G, XG, NT>), grid, dim3(256), 0, st, a);
-  return hipGetLastError();
+#ifdef Q8_FEW
+  return q8_few<BITS, G, XG, Q8_FEW>(a, Q8_WAVES, st);
+#else
+  const uint32_t steps = (a.K + kQ8Step - 1) / kQ8Step;
+  return q8_few<BITS, G, XG, 1, 1>(a, steps < 16 ? steps : 16, st);
+#endif
 }
 
 template <int BITS, bool XG>
