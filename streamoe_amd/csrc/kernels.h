@@ -316,6 +316,7 @@ struct Q8Args {
   uint32_t O, K, n;
   uint32_t vec;            // y on 16 bytes, O a multiple of 4
   uint32_t svec, xvec;     // s and b (sx) on 16 bytes, K / group a multiple of 8 (4)
+  uint32_t even;           // s and b on 4 bytes, K / group even
 };
 hipError_t launch_qmm_i8(const Q8Args& a, uint32_t bits, uint32_t group, bool x_grouped, hipStream_t st);
 // Low-rank adapters (lora.hip).

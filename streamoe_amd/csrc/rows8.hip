@@ -51,28 +51,34 @@ __device__ __forceinline__ uint32_t q8_pos(uint32_t h, uint32_t e, uint32_t kb) 
   return 32 * kb + 16 * h + 8 * e;
 }
 
-// The loaded codes of a step as operands.
-template <int BITS, int G>
+// The loaded codes of a step as operands. CHUNK: 8-bit codes come as chunks of
+// 32 like the others, else as the operands they are.
+template <int BITS, int G, bool CHUNK = false>
 __device__ __forceinline__ void q8_operands(const uint32_t (&d)[BITS == 8 ? 8 : BITS], u32x4 (&b)[2]) {
-  if constexpr (BITS == 8) {
+  if constexpr (BITS == 8 && !CHUNK) {
     b[0] = u32x4{d[0], d[1], d[2], d[3]} ^ 0x80808080u;
     b[1] = u32x4{d[4], d[5], d[6], d[7]} ^ 0x80808080u;
   } else {
-    Raw<BITS> w;
-#pragma unroll
-    for (int i = 0; i < BITS; ++i) w.d[i] = d[i];
-    if constexpr (G == 64 && BITS == 4) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const auto r = __builtin_amdgcn_permlane32_swap(w.d[i], w.d[i + 2], false, false);
-        w.d[i] = r[0];
-        w.d[i + 2] = r[1];
-      }
-    }
-    if constexpr (G == 32 && BITS == 4) q8_transpose4(w.d[0], w.d[1], w.d[2], w.d[3]);
     uint32_t q[8];
-    unpack_bytes(w, q);
-    if constexpr (G == 64 && BITS == 3) {
+    if constexpr (BITS == 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = d[i] ^ 0x80808080u;
+    } else {
+      Raw<BITS> w;
+#pragma unroll
+      for (int i = 0; i < BITS; ++i) w.d[i] = d[i];
+      if constexpr (G == 64 && BITS == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const auto r = __builtin_amdgcn_permlane32_swap(w.d[i], w.d[i + 2], false, false);
+          w.d[i] = r[0];
+          w.d[i + 2] = r[1];
+        }
+      }
+      if constexpr (G == 32 && BITS == 4) q8_transpose4(w.d[0], w.d[1], w.d[2], w.d[3]);
+      unpack_bytes(w, q);
+    }
+    if constexpr (G == 64 && BITS != 4) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const auto r = __builtin_amdgcn_permlane32_swap(q[i], q[i + 4], false, false);
@@ -80,7 +86,7 @@ __device__ __forceinline__ void q8_operands(const uint32_t (&d)[BITS == 8 ? 8 : 
         q[i + 4] = r[1];
       }
     }
-    if constexpr (G == 32 && BITS == 3) {
+    if constexpr (G == 32 && BITS != 4) {
       q8_transpose4(q[0], q[2], q[4], q[6]);
       q8_transpose4(q[1], q[3], q[5], q[7]);
     }
@@ -89,10 +95,9 @@ __device__ __forceinline__ void q8_operands(const uint32_t (&d)[BITS == 8 ? 8 : 
   }
 }
 
-// Sums of group g of a step.
+// Sums of group g of a step, from z on.
 template <int G>
-__device__ __forceinline__ i32x4 q8_sums(const u32x4 (&x)[2], const u32x4 (&b)[2], uint32_t g) {
-  const i32x4 z = {0, 0, 0, 0};
+__device__ __forceinline__ i32x4 q8_sums(const u32x4 (&x)[2], const u32x4 (&b)[2], uint32_t g, i32x4 z = {0, 0, 0, 0}) {
   if constexpr (G == 64) {
     return q8_mfma(x[g], b[g], z);
   } else if constexpr (G == 32) {
@@ -269,6 +274,253 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
   }
 }
 
+constexpr uint32_t kMagicBits = 0x4B400000u;  // 1.5 * 2^23
+constexpr float kMagic = 12582912.f;
+
+typedef __bf16 qbf16x8 __attribute__((ext_vector_type(8)));
+
+// sx to 22 significant bits.
+__device__ __forceinline__ float q8_round22(float v) {
+  const uint32_t u = __float_as_uint(v);
+  if ((u & 0x7F800000u) == 0x7F800000u) return v;
+  return __uint_as_float((u + 1u + ((u >> 2) & 1u)) & ~3u);
+}
+
+// Three bf16 of a and three of b, each the rest of those before it.
+__device__ __forceinline__ qbf16x8 q8_parts(float a, float b) {
+  auto top = [](float v) { return __float_as_uint(v) & 0xFFFF0000u; };
+  const uint32_t ah = top(a), bh = top(b);
+  const float ar = a - __uint_as_float(ah), br = b - __uint_as_float(bh);
+  const uint32_t am = top(ar), bm = top(br);
+  const uint32_t al = __float_as_uint(ar - __uint_as_float(am)), bl = __float_as_uint(br - __uint_as_float(bm));
+  return __builtin_bit_cast(qbf16x8, u32x4{ah >> 16 | am, al >> 16 | bh, bm >> 16 | (bl & 0xFFFF0000u), 0u});
+}
+
+// ---------------------------------------------------------------------------
+// Few rows, many columns: the rows stay in LDS, as operands, and the waves
+// stream the weights, a tile of 16 columns at a time over all inputs, four
+// steps ahead. A wave's load of a step is made in memory order (lane 4 r + p:
+// part p of row r, one cache access per four lanes instead of one per lane) and
+// a lane permute brings the parts to the operand's lanes. Rows are the A
+// operand: lane (c, kb) ends with column c of rows 4 kb .. 4 kb + 3, and needs
+// the scales of one column only.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kWideSteps = 4;  // per round of loads
+
+// Where piece p (16 inputs) of a row's step lies among its operands: place of
+// its e-th eight, in 8-byte units of [h][kb][row][e]; rows are exchanged by
+// 4 h + kb so that the pieces of a row fall in different banks.
+template <int G>
+__device__ __forceinline__ uint32_t q8_slot(uint32_t p, uint32_t e, uint32_t row) {
+  const uint32_t h = G == 128 ? p & 1 : p >> 2;
+  const uint32_t kb = G == 32 ? (p & 1) * 2 + e : G == 64 ? ((p & 1) << 1) | ((p >> 1) & 1) : p >> 1;
+  const uint32_t f = G == 32 ? (p >> 1) & 1 : e;
+  return ((h * 4 + kb) * 16 + (row ^ (h * 4 + kb))) * 2 + f;
+}
+
+__host__ __device__ constexpr uint32_t q8_wide_steps(uint32_t K) {
+  return (K + kWideSteps * kQ8Step - 1) / (kWideSteps * kQ8Step) * kWideSteps;
+}
+// LDS: operands, the bias term's operands per eight groups, the rows' scales.
+__host__ __device__ constexpr uint32_t q8_wide_lds(uint32_t K, uint32_t G, uint32_t mt, bool xg) {
+  const uint32_t steps = q8_wide_steps(K), groups = steps * (kQ8Step / G);
+  return mt * (steps * 2048 + (groups + 7) / 8 * 1024 + (xg ? groups * 64 : 0));
+}
+
+template <int BITS, int G, bool XG, int MT>
+__global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
+  constexpr uint32_t GS = kQ8Step / G, W = BITS == 8 ? 8 : BITS, GC = GS * kWideSteps;  // groups per round
+  constexpr uint32_t PW = GC >= 8 ? GC / 8 : 1;  // pairs of scales a lane loads per round (G = 128: two lanes the same)
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t K = a.K, O = a.O, gpr = K / G, row_bytes = K / 32 * (BITS * 4);
+  const uint32_t steps = q8_wide_steps(K), groups = steps * GS, octets = (groups + 7) / 8, rounds = steps / kWideSteps;
+  u32x4* const xl = reinterpret_cast<u32x4*>(lds_raw);                 // [step][m][h][64]
+  u32x4* const parts = xl + steps * MT * 128;                          // [octet][m][64]
+  float* const sxl = reinterpret_cast<float*>(parts + octets * MT * 64);  // [group][m][16]
+
+  // The loads of a round, in memory order: part lp of row lr of the tile.
+  const uint32_t lr = lane >> 2, lp = lane & 3;
+  struct Round {
+    uint32_t w[kWideSteps][W];
+    uint32_t s[PW], b[PW];
+  };
+  auto load = [&](uint32_t tile, uint32_t rd, Round& v) {
+    const uint32_t row = min(tile * 16 + lr, O - 1), col = min(tile * 16 + c16, O - 1);
+    const uint8_t* const w = a.w + (uint64_t)row * row_bytes;
+#pragma unroll
+    for (uint32_t i = 0; i < kWideSteps; ++i) {
+      const uint8_t* const p = w + min((rd * kWideSteps + i) * 4 + lp, K / 32 - 1) * (BITS * 4);
+      if constexpr (BITS == 8) {
+        const u32x4 lo = ld_w<true>(reinterpret_cast<const u32x4*>(p)), hi = ld_w<true>(reinterpret_cast<const u32x4*>(p + 16));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.w[i][j] = lo[j], v.w[i][4 + j] = hi[j];
+      } else {
+        const Raw<BITS> r = load_raw<BITS, true>(p);
+#pragma unroll
+        for (int j = 0; j < BITS; ++j) v.w[i][j] = r.d[j];
+      }
+    }
+    // Pairs of groups: lane block kb those of pair kb (and 4 + kb); the last
+    // group again past the end.
+#pragma unroll
+    for (uint32_t i = 0; i < PW; ++i) {
+      const uint32_t g = rd * GC + 8 * i + 2 * (GC < 8 ? kb & 1 : kb);
+      const uint64_t at = (uint64_t)col * gpr;
+      if (a.even) {
+        const uint64_t e = at + min(g, gpr - 2);
+        v.s[i] = *reinterpret_cast<const uint32_t*>(a.s + e);
+        v.b[i] = *reinterpret_cast<const uint32_t*>(a.b + e);
+      } else {
+        const uint64_t e0 = at + min(g, gpr - 1), e1 = at + min(g + 1, gpr - 1);
+        v.s[i] = a.s[e0] | (uint32_t)a.s[e1] << 16;
+        v.b[i] = a.b[e0] | (uint32_t)a.b[e1] << 16;
+      }
+    }
+  };
+  const uint32_t stride = gridDim.x * 4;
+  uint32_t tile = blockIdx.x * 4 + wave;
+  Round v[2];
+  if (tile < tiles) load(tile, 0, v[0]);
+
+  // The rows as operands; rows past the last and inputs from K on are zero.
+  for (uint32_t i = tid; i < steps * 8 * MT * 16; i += 256) {
+    const uint32_t p = i % (steps * 8), r = i / (steps * 8);
+    u32x4 q = {0u, 0u, 0u, 0u};
+    if (r < a.n && p * 16 < K) q = *reinterpret_cast<const u32x4*>(a.x + (uint64_t)r * K + p * 16);
+    uint2* const to = reinterpret_cast<uint2*>(xl + ((p / 8) * MT + r / 16) * 128);
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e) {
+      uint2 o = make_uint2(q[2 * e], q[2 * e + 1]);
+      if (BITS != 8) o = make_uint2(__builtin_amdgcn_perm(o.y, o.x, 0x06040200u), __builtin_amdgcn_perm(o.y, o.x, 0x07050301u));
+      to[q8_slot<G>(p % 8, e, r % 16)] = o;
+    }
+  }
+  if constexpr (XG)
+    for (uint32_t i = tid; i < groups * MT * 16; i += 256) {
+      const uint32_t r = i % (MT * 16), g = i / (MT * 16);
+      sxl[i] = r < a.n ? q8_round22(a.sx[(uint64_t)r * gpr + min(g, gpr - 1)]) : 0.f;
+    }
+  __syncthreads();
+  const uint32_t at[2] = {kb * 16 + (c16 ^ kb), 64 + kb * 16 + (c16 ^ (4 + kb))};
+  const u32x4 one = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
+  const u32x4 ones[2] = {one, one};
+  for (uint32_t i = wave; i < octets * MT; i += 4) {
+    const uint32_t o = i / MT, m = i % MT;
+    float xs[2] = {0.f, 0.f};
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      const uint32_t g = o * 8 + j;
+      if (g >= gpr) break;
+      const u32x4* const xo = xl + (g / GS * MT + m) * 128;
+      const u32x4 x[2] = {xo[at[0]], xo[at[1]]};
+      i32x4 S;
+      if constexpr (GS == 1)
+        S = q8_sums<G>(ones, x, 0);
+      else if constexpr (GS == 2)
+        S = j & 1 ? q8_sums<G>(ones, x, 1) : q8_sums<G>(ones, x, 0);
+      else
+        S = j % 4 == 0 ? q8_sums<G>(ones, x, 0) : j % 4 == 1 ? q8_sums<G>(ones, x, 1) : j % 4 == 2 ? q8_sums<G>(ones, x, 2) : q8_sums<G>(ones, x, 3);
+      float f = (float)S[0];
+      if constexpr (XG) f *= sxl[g * MT * 16 + m * 16 + c16];
+      if (kb == j / 2) xs[j & 1] = f;
+    }
+    parts[i * 64 + lane] = __builtin_bit_cast(u32x4, q8_parts(xs[0], xs[1]));
+  }
+  __syncthreads();
+
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kStart = XG ? (int)kMagicBits : 0;
+  const i32x4 start = {kStart, kStart, kStart, kStart};
+  const int psrc = (int)((c16 * 4 + kb) * 4);
+  auto from = [&](int src, uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)x); };
+  auto compute = [&](uint32_t rd, const Round& v) {
+    // The bias term of this round's eights (G = 128: a round is half of one).
+#pragma unroll
+    for (uint32_t i = 0; i < PW; ++i) {
+      const uint32_t o = rd * GC / 8 + i;
+      uint32_t p = v.b[i], q = v.s[i];
+      if (GC < 8 && (kb >> 1) != (rd & 1)) p = q = 0;  // the other half's pairs
+      auto term = [&](uint32_t p, float f) {
+        const u32x4 t = {__builtin_amdgcn_perm(p, p, 0x01000100u), p, __builtin_amdgcn_perm(p, p, 0x03020302u), 0u};
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          f32x4 z = acc[m];
+          if (f != 1.f) z = f32x4{0.f, 0.f, 0.f, 0.f};
+          z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, parts[(o * MT + m) * 64 + lane]),
+                                                      __builtin_bit_cast(qbf16x8, t), z, 0, 0, 0);
+          acc[m] = f != 1.f ? acc[m] + z * f : z;
+        }
+      };
+      term(p, 1.f);
+      if (BITS == 8) term(q, 128.f);  // 8-bit codes enter less 128
+    }
+    uint32_t sw[GC / 2];  // the column's pairs of scales
+#pragma unroll
+    for (uint32_t i = 0; i < GC / 2; ++i) sw[i] = from((int)(((i % 4) * 16 + c16) * 4), v.s[i / 4]);
+#pragma unroll
+    for (uint32_t i = 0; i < kWideSteps; ++i) {
+      uint32_t d[W];
+#pragma unroll
+      for (uint32_t j = 0; j < W; ++j) d[j] = from(psrc, v.w[i][j]);
+      u32x4 w[2];
+      q8_operands<BITS, G, true>(d, w);
+      const uint32_t st = rd * kWideSteps + i;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const u32x4* const xo = xl + (st * MT + m) * 128;
+        const u32x4 x[2] = {xo[at[0]], xo[at[1]]};
+#pragma unroll
+        for (uint32_t j = 0; j < GS; ++j) {
+          const uint32_t g = i * GS + j, p = sw[g / 2];
+          const float s = __uint_as_float(g & 1 ? p & 0xFFFF0000u : p << 16);
+          const i32x4 S = q8_sums<G>(x, w, j, start);
+          f32x4 sx;
+          if constexpr (XG) sx = *reinterpret_cast<const f32x4*>(sxl + (st * GS + j) * MT * 16 + m * 16 + 4 * kb);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float f = XG ? __builtin_fmaf(__int_as_float(S[k]), sx[k], -kMagic * sx[k]) : (float)S[k];
+            acc[m][k] = __builtin_fmaf(s, f, acc[m][k]);
+          }
+        }
+      }
+    }
+  };
+  auto finish = [&](uint32_t tile) {
+    const uint32_t col = tile * 16 + c16;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t r = m * 16 + 4 * kb + k;
+        if (r < a.n && col < O) a.y[(uint64_t)r * O + col] = XG ? acc[m][k] : acc[m][k] * a.sx[r];
+      }
+      acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  // Rounds of all of the wave's tiles in one sequence, two at a time.
+  uint32_t rd = 0;
+  auto next = [&](uint32_t& t, uint32_t& r) {
+    if (++r == rounds) r = 0, t += stride;
+  };
+  while (tile < tiles) {
+    uint32_t t1 = tile, r1 = rd;
+    next(t1, r1);
+    if (t1 < tiles) load(t1, r1, v[1]);
+    compute(rd, v[0]);
+    if (rd + 1 == rounds) finish(tile);
+    if (t1 >= tiles) break;
+    tile = t1, rd = r1;
+    next(tile, rd);
+    if (tile < tiles) load(tile, rd, v[0]);
+    compute(r1, v[1]);
+    if (r1 + 1 == rounds) finish(t1);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Many rows: a block of four waves takes WM MT tiles of 16 rows x WN NT tiles
 // of 16 columns, step after step of 128 inputs. A step's rows go straight into
@@ -292,28 +544,6 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
 // sums as they are takes 64 cycles for four groups: 9 us of 87 at 1000 rows
 // 4096 -> 7168.)
 // ---------------------------------------------------------------------------
-constexpr uint32_t kMagicBits = 0x4B400000u;  // 1.5 * 2^23
-constexpr float kMagic = 12582912.f;
-
-typedef __bf16 qbf16x8 __attribute__((ext_vector_type(8)));
-
-// sx to 22 significant bits.
-__device__ __forceinline__ float q8_round22(float v) {
-  const uint32_t u = __float_as_uint(v);
-  if ((u & 0x7F800000u) == 0x7F800000u) return v;
-  return __uint_as_float((u + 1u + ((u >> 2) & 1u)) & ~3u);
-}
-
-// Three bf16 of a and three of b, each the rest of those before it.
-__device__ __forceinline__ qbf16x8 q8_parts(float a, float b) {
-  auto top = [](float v) { return __float_as_uint(v) & 0xFFFF0000u; };
-  const uint32_t ah = top(a), bh = top(b);
-  const float ar = a - __uint_as_float(ah), br = b - __uint_as_float(bh);
-  const uint32_t am = top(ar), bm = top(br);
-  const uint32_t al = __float_as_uint(ar - __uint_as_float(am)), bl = __float_as_uint(br - __uint_as_float(bm));
-  return __builtin_bit_cast(qbf16x8, u32x4{ah >> 16 | am, al >> 16 | bh, bm >> 16 | (bl & 0xFFFF0000u), 0u});
-}
-
 // LDS place (16 bytes) of piece p (16 inputs) of a row's step: the eight pieces
 // of a row side by side, exchanged by the row so that eight rows' reads of one
 // piece fall in different banks.
@@ -676,8 +906,26 @@ static hipError_t q8_few(const Q8Args& a, uint32_t waves, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int BITS, int G, bool XG, int MT>
+static hipError_t q8_wide(const Q8Args& a, hipStream_t st) {
+  const uint32_t lds = q8_wide_lds(a.K, G, MT, XG), tiles = (a.O + 15) / 16;
+  auto fn = k_q8_wide<BITS, G, XG, MT>;
+  if (lds > 64 * 1024) {
+    static std::atomic<uint64_t> raised{0};
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(fn), 160 * 1024, raised);
+    if (e != hipSuccess) return e;
+  }
+  // Two blocks on each CU (one where the rows fill its LDS), every wave as
+  // many tiles.
+  const uint32_t slots = 256 * (lds > 80 * 1024 ? 1 : 2) * 4, rounds = (tiles + slots - 1) / slots;
+  const uint32_t blocks = (tiles + 4 * rounds - 1) / (4 * rounds);
+  hipLaunchKernelGGL(fn, dim3(blocks), dim3(256), lds, st, a, tiles);
+  return hipGetLastError();
+}
+
 template <int BITS, int G, bool XG>
 static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
+  if (a.n <= 16 && a.O >= 16384 && q8_wide_lds(a.K, G, 1, XG) <= 160 * 1024) return q8_wide<BITS, G, XG, 1>(a, st);
   if (a.n > 64) return q8_tile<BITS, G, XG, 2, 2, 4, 4>(a, st);
 #ifdef Q8_FEW
   return q8_few<BITS, G, XG, Q8_FEW>(a, Q8_WAVES, st);

@@ -104,6 +104,16 @@ def test_sizes(kernels, n, O, K, bits, G, xg):
     _check(kernels, n, O, K, bits, G, xg)
 
 
+@pytest.mark.parametrize("bits", [4, 3, 8])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_many_columns(kernels, bits, G, grouped):
+    """Vocabulary-wide outputs of few rows; groups that end inside a round of
+    loads, odd counts of groups."""
+    for n, O, K in [(1, 16385, 3 * G), (16, 20007, 640), (9, 33000, 9 * G), (5, 16400, 1152)]:
+        _check(kernels, n, O, K, bits, G, G if grouped else 0)
+
+
 def test_largest_codes(kernels):
     """The extreme codes of both sides in whole groups: the integer sums' range."""
     rng = np.random.default_rng(3)
