@@ -301,7 +301,9 @@ __device__ __forceinline__ qbf16x8 q8_parts(float a, float b) {
 // stream the weights, a tile of 16 columns at a time over all inputs, four
 // steps ahead. A wave's load of a step is made in memory order (lane 4 r + p:
 // part p of row r, one cache access per four lanes instead of one per lane) and
-// a lane permute brings the parts to the operand's lanes. Rows are the A
+// a lane permute brings the parts to the operand's lanes. The loads are
+// temporal: a step takes half of a row's line, the next step the other half
+// (non-temporal: 16 rows 2048 -> 151936 in 47 us instead of 35). Rows are the A
 // operand: lane (c, kb) ends with column c of rows 4 kb .. 4 kb + 3, and needs
 // the scales of one column only.
 // ---------------------------------------------------------------------------
@@ -353,11 +355,11 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
     for (uint32_t i = 0; i < kWideSteps; ++i) {
       const uint8_t* const p = w + min((rd * kWideSteps + i) * 4 + lp, K / 32 - 1) * (BITS * 4);
       if constexpr (BITS == 8) {
-        const u32x4 lo = ld_w<true>(reinterpret_cast<const u32x4*>(p)), hi = ld_w<true>(reinterpret_cast<const u32x4*>(p + 16));
+        const u32x4 lo = ld_w<false>(reinterpret_cast<const u32x4*>(p)), hi = ld_w<false>(reinterpret_cast<const u32x4*>(p + 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) v.w[i][j] = lo[j], v.w[i][4 + j] = hi[j];
       } else {
-        const Raw<BITS> r = load_raw<BITS, true>(p);
+        const Raw<BITS> r = load_raw<BITS, false>(p);
 #pragma unroll
         for (int j = 0; j < BITS; ++j) v.w[i][j] = r.d[j];
       }
