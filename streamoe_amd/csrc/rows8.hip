@@ -42,32 +42,39 @@ __device__ __forceinline__ void q8_transpose4(uint32_t& a, uint32_t& b, uint32_t
   a = ab[0], b = ab[1], c = cd[0], d = cd[1];
 }
 
-// First input (of a step) of the e-th eight of operand h at lane block kb.
-template <int BITS, int G>
-__device__ __forceinline__ uint32_t q8_pos(uint32_t h, uint32_t e, uint32_t kb) {
-  if (G == 32) return 64 * h + 8 * kb + 32 * e;
-  if (BITS == 8) return 64 * h + 16 * kb + 8 * e;
-  if (G == 64) return 64 * h + 32 * (kb & 1) + 16 * (kb >> 1) + 8 * e;
-  return 32 * kb + 16 * h + 8 * e;
+// Chunks of 32 bytes, one per lane block, to operands of one group each: the
+// halves of two lanes' chunks exchanged (groups of 64), the four lanes' chunks
+// transposed by their eights (of 32).
+template <int G>
+__device__ __forceinline__ void q8_exchange(uint32_t (&q)[8]) {
+  if constexpr (G == 64) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto r = __builtin_amdgcn_permlane32_swap(q[i], q[i + 4], false, false);
+      q[i] = r[0];
+      q[i + 4] = r[1];
+    }
+  }
+  if constexpr (G == 32) {
+    q8_transpose4(q[0], q[2], q[4], q[6]);
+    q8_transpose4(q[1], q[3], q[5], q[7]);
+  }
 }
 
-// The loaded codes of a step as operands. CHUNK: 8-bit codes come as chunks of
-// 32 like the others, else as the operands they are.
-template <int BITS, int G, bool CHUNK = false>
+// The loaded codes of a step (chunks of 32) as operands.
+template <int BITS, int G>
 __device__ __forceinline__ void q8_operands(const uint32_t (&d)[BITS == 8 ? 8 : BITS], u32x4 (&b)[2]) {
-  if constexpr (BITS == 8 && !CHUNK) {
-    b[0] = u32x4{d[0], d[1], d[2], d[3]} ^ 0x80808080u;
-    b[1] = u32x4{d[4], d[5], d[6], d[7]} ^ 0x80808080u;
+  uint32_t q[8];
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = d[i] ^ 0x80808080u;
+    q8_exchange<G>(q);
   } else {
-    uint32_t q[8];
-    if constexpr (BITS == 8) {
+    Raw<BITS> w;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = d[i] ^ 0x80808080u;
-    } else {
-      Raw<BITS> w;
-#pragma unroll
-      for (int i = 0; i < BITS; ++i) w.d[i] = d[i];
-      if constexpr (G == 64 && BITS == 4) {
+    for (int i = 0; i < BITS; ++i) w.d[i] = d[i];
+    if constexpr (BITS == 4) {  // the same exchange while it is half the words
+      if constexpr (G == 64) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const auto r = __builtin_amdgcn_permlane32_swap(w.d[i], w.d[i + 2], false, false);
@@ -75,24 +82,13 @@ __device__ __forceinline__ void q8_operands(const uint32_t (&d)[BITS == 8 ? 8 : 
           w.d[i + 2] = r[1];
         }
       }
-      if constexpr (G == 32 && BITS == 4) q8_transpose4(w.d[0], w.d[1], w.d[2], w.d[3]);
-      unpack_bytes(w, q);
+      if constexpr (G == 32) q8_transpose4(w.d[0], w.d[1], w.d[2], w.d[3]);
     }
-    if constexpr (G == 64 && BITS != 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const auto r = __builtin_amdgcn_permlane32_swap(q[i], q[i + 4], false, false);
-        q[i] = r[0];
-        q[i + 4] = r[1];
-      }
-    }
-    if constexpr (G == 32 && BITS != 4) {
-      q8_transpose4(q[0], q[2], q[4], q[6]);
-      q8_transpose4(q[1], q[3], q[5], q[7]);
-    }
-    b[0] = u32x4{q[0], q[1], q[2], q[3]};
-    b[1] = u32x4{q[4], q[5], q[6], q[7]};
+    unpack_bytes(w, q);
+    if constexpr (BITS == 3) q8_exchange<G>(q);
   }
+  b[0] = u32x4{q[0], q[1], q[2], q[3]};
+  b[1] = u32x4{q[4], q[5], q[6], q[7]};
 }
 
 // Sums of group g of a step, from z on.
@@ -111,15 +107,19 @@ __device__ __forceinline__ i32x4 q8_sums(const u32x4 (&x)[2], const u32x4 (&b)[2
 // ---------------------------------------------------------------------------
 // Few rows or columns: a block's waves share MT tiles of 16 rows x NT tiles of
 // 16 columns and take the steps of 128 inputs in turn (up to 16 waves: a small
-// call is one round trip to memory). Operands come straight from memory, a step
-// ahead; the sums of inputs come from a product with ones; the waves' parts are
-// added in LDS.
+// call is one round trip to memory), a step ahead. Loads are made in memory
+// order: lane 4 r + p takes part p (32 inputs) of row r, one cache access per
+// four lanes where the operand order would take one per lane, and a lane
+// permute brings the parts to the operand's lanes (4 rows 2048 -> 4096 took
+// 5.9 us in operand order). Rows are the A operand: lane (c, kb) ends with column c of rows 4 kb
+// .. 4 kb + 3. The sums of inputs come from a product with ones; the waves'
+// parts are added in LDS.
 // ---------------------------------------------------------------------------
 template <int BITS, int G, bool XG, int MT, int NT>
-__global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
-  constexpr uint32_t GS = kQ8Step / G;
+__global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_q8_few(Q8Args a) {
+  constexpr uint32_t GS = kQ8Step / G, W = BITS == 8 ? 8 : BITS, SW = (GS + 1) / 2;
   extern __shared__ __attribute__((aligned(16))) f32x4 red[];  // [wave][MT * NT][64]
-  const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, kb = lane >> 4, lr = lane >> 2, lp = lane & 3;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const uint32_t K = a.K, O = a.O, gpr = K / G, steps = (K + kQ8Step - 1) / kQ8Step;
   const uint32_t col0 = blockIdx.x * (NT * 16), row0 = blockIdx.y * (MT * 16);
@@ -128,65 +128,65 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
   const float* sxr[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const uint32_t r = min(row0 + m * 16 + c16, a.n - 1);
-    xr[m] = a.x + (uint64_t)r * K;
-    sxr[m] = a.sx + (uint64_t)r * (XG ? gpr : 1u);
+    xr[m] = a.x + (uint64_t)min(row0 + m * 16 + lr, a.n - 1) * K;
+    sxr[m] = a.sx + (uint64_t)min(row0 + m * 16 + c16, a.n - 1) * (XG ? gpr : 1u);
   }
   const uint8_t* wr[NT];
   const uint16_t *sr[NT], *br[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const uint32_t c = min(col0 + t * 16 + c16, O - 1);
-    wr[t] = a.w + (uint64_t)c * row_bytes;
-    sr[t] = a.s + (uint64_t)c * gpr;
-    br[t] = a.b + (uint64_t)c * gpr;
+    wr[t] = a.w + (uint64_t)min(col0 + t * 16 + lr, O - 1) * row_bytes;
+    const uint64_t c = (uint64_t)min(col0 + t * 16 + c16, O - 1) * gpr;
+    sr[t] = a.s + c;
+    br[t] = a.b + c;
   }
   struct Step {
-    uint2 x[MT][2][2];                       // [operand][eight]
-    uint32_t w[NT][BITS == 8 ? 8 : BITS];
-    uint16_t s[NT][GS], b[NT][GS];
+    u32x4 x[MT][2];
+    uint32_t w[NT][W], s[NT][SW], b[NT][SW];  // pairs of groups
     float sx[MT][GS];
   };
   auto load = [&](uint32_t st, Step& v) {
     const uint32_t k0 = st * kQ8Step;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      const uint8_t* const p = wr[t] + min(k0 / 32 + lp, K / 32 - 1) * (BITS * 4);
       if constexpr (BITS == 8) {
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(p), hi = *reinterpret_cast<const u32x4*>(p + 16);
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-          for (uint32_t e = 0; e < 2; ++e) {
-            const uint2 q = *reinterpret_cast<const uint2*>(wr[t] + min(k0 + q8_pos<BITS, G>(h, e, kb), K - 8));
-            v.w[t][4 * h + 2 * e] = q.x;
-            v.w[t][4 * h + 2 * e + 1] = q.y;
-          }
+        for (int i = 0; i < 4; ++i) v.w[t][i] = lo[i], v.w[t][4 + i] = hi[i];
       } else {
-        const Raw<BITS> r = load_raw<BITS, false>(wr[t] + min(k0 / 32 + kb, K / 32 - 1) * chunk_bytes<BITS>());
+        const Raw<BITS> r = load_raw<BITS, false>(p);
 #pragma unroll
         for (int i = 0; i < BITS; ++i) v.w[t][i] = r.d[i];
       }
 #pragma unroll
-      for (uint32_t j = 0; j < GS; ++j) {
-        const uint32_t g = min(st * GS + j, gpr - 1);
-        v.s[t][j] = sr[t][g];
-        v.b[t][j] = br[t][g];
+      for (uint32_t j = 0; j < SW; ++j) {
+        const uint32_t g = st * GS + 2 * j;
+        if (GS > 1 && a.even) {
+          v.s[t][j] = *reinterpret_cast<const uint32_t*>(sr[t] + min(g, gpr - 2));
+          v.b[t][j] = *reinterpret_cast<const uint32_t*>(br[t] + min(g, gpr - 2));
+        } else {
+          const uint32_t g0 = min(g, gpr - 1), g1 = min(g + 1, gpr - 1);
+          v.s[t][j] = sr[t][g0] | (GS > 1 ? (uint32_t)sr[t][g1] << 16 : 0u);
+          v.b[t][j] = br[t][g0] | (GS > 1 ? (uint32_t)br[t][g1] << 16 : 0u);
+        }
       }
     }
+    const uint32_t at = k0 + lp * 32;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-        for (uint32_t e = 0; e < 2; ++e) {
-          const uint32_t at = k0 + q8_pos<BITS, G>(h, e, kb);
-          v.x[m][h][e] = make_uint2(0u, 0u);
-          if (at < K) v.x[m][h][e] = *reinterpret_cast<const uint2*>(xr[m] + at);
-        }
+      v.x[m][0] = v.x[m][1] = u32x4{0u, 0u, 0u, 0u};
+      if (at < K) {  // K is a multiple of 32
+        v.x[m][0] = *reinterpret_cast<const u32x4*>(xr[m] + at);
+        v.x[m][1] = *reinterpret_cast<const u32x4*>(xr[m] + at + 16);
+      }
       if constexpr (XG)
 #pragma unroll
         for (uint32_t j = 0; j < GS; ++j) v.sx[m][j] = sxr[m][min(st * GS + j, gpr - 1)];
     }
   };
+  const int psrc = (int)((c16 * 4 + kb) * 4);
+  auto from = [&](int src, uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)x); };
   const u32x4 one = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
   const u32x4 ones[2] = {one, one};
   f32x4 acc[MT][NT];
@@ -197,47 +197,55 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
   auto compute = [&](const Step& v) {
     u32x4 x[MT][2], w[NT][2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+      uint32_t d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = from(psrc, v.x[m][i / 4][i % 4]);
+      q8_exchange<G>(d);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint2 e0 = v.x[m][h][0], e1 = v.x[m][h][1];
+        const uint32_t* const e = d + 4 * h;
         if (BITS == 8)
-          x[m][h] = u32x4{e0.x, e0.y, e1.x, e1.y};
+          x[m][h] = u32x4{e[0], e[1], e[2], e[3]};
         else  // evens before odds, as the codes unpack
-          x[m][h] = u32x4{__builtin_amdgcn_perm(e0.y, e0.x, 0x06040200u), __builtin_amdgcn_perm(e0.y, e0.x, 0x07050301u),
-                          __builtin_amdgcn_perm(e1.y, e1.x, 0x06040200u), __builtin_amdgcn_perm(e1.y, e1.x, 0x07050301u)};
+          x[m][h] = u32x4{__builtin_amdgcn_perm(e[1], e[0], 0x06040200u), __builtin_amdgcn_perm(e[1], e[0], 0x07050301u),
+                          __builtin_amdgcn_perm(e[3], e[2], 0x06040200u), __builtin_amdgcn_perm(e[3], e[2], 0x07050301u)};
       }
+    }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) q8_operands<BITS, G>(v.w[t], w[t]);
+    for (int t = 0; t < NT; ++t) {
+      uint32_t d[W];
+#pragma unroll
+      for (uint32_t i = 0; i < W; ++i) d[i] = from(psrc, v.w[t][i]);
+      q8_operands<BITS, G>(d, w[t]);
+    }
 #pragma unroll
     for (uint32_t j = 0; j < GS; ++j) {
-      float xf[MT];
+      f32x4 xf[MT], sx[MT];  // of rows 4 kb ..
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        xf[m] = (float)q8_sums<G>(ones, x[m], j)[0];
-        if constexpr (XG) xf[m] *= v.sx[m][j];
+        const i32x4 X = q8_sums<G>(x[m], ones, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (XG) sx[m][i] = __shfl(v.sx[m][j], 4 * (int)kb + i, kWave);
+          xf[m][i] = XG ? (float)X[i] * sx[m][i] : (float)X[i];
+        }
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        // Lane (c, kb) of the result holds columns 4 kb .. 4 kb + 3 of row c.
-        const float s1 = bf16f(v.s[t][j]);
-        float b1 = bf16f(v.b[t][j]);
-        if (BITS == 8) b1 = __builtin_fmaf(s1, 128.f, b1);
-        f32x4 s, b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[i] = __shfl(s1, 4 * (int)kb + i, kWave);
-          b[i] = __shfl(b1, 4 * (int)kb + i, kWave);
-        }
+        auto half = [&](uint32_t p) { return __uint_as_float(j & 1 ? p & 0xFFFF0000u : p << 16); };
+        const float s = half(v.s[t][j / 2]);
+        float b = half(v.b[t][j / 2]);
+        if (BITS == 8) b = __builtin_fmaf(s, 128.f, b);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const i32x4 S = q8_sums<G>(w[t], x[m], j);
+          const i32x4 S = q8_sums<G>(x[m], w[t], j);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float f = (float)S[i];
-            if constexpr (XG) f *= v.sx[m][j];
-            acc[m][t][i] = __builtin_fmaf(s[i], f, acc[m][t][i]);
-            acc[m][t][i] = __builtin_fmaf(b[i], xf[m], acc[m][t][i]);
+            if constexpr (XG) f *= sx[m][i];
+            acc[m][t][i] = __builtin_fmaf(s, f, acc[m][t][i]);
+            acc[m][t][i] = __builtin_fmaf(b, xf[m][i], acc[m][t][i]);
           }
         }
       }
@@ -260,16 +268,12 @@ __global__ __launch_bounds__(1024) void k_q8_few(Q8Args a) {
   for (uint32_t mt = wave; mt < MT * NT; mt += nw) {
     f32x4 sum = red[mt * 64 + lane];
     for (uint32_t w = 1; w < nw; ++w) sum += red[(w * MT * NT + mt) * 64 + lane];
-    const uint32_t r = row0 + mt / NT * 16 + c16, col = col0 + mt % NT * 16 + 4 * kb;
-    if (r >= a.n) continue;
-    if constexpr (!XG) sum *= a.sx[r];
-    float* const y = a.y + (uint64_t)r * O + col;
-    if (a.vec) {
-      if (col < O) *reinterpret_cast<f32x4*>(y) = sum;
-    } else {
+    const uint32_t col = col0 + mt % NT * 16 + c16;
+    if (col >= O) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col + i < O) y[i] = sum[i];
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = row0 + mt / NT * 16 + 4 * kb + i;
+      if (r < a.n) a.y[(uint64_t)r * O + col] = XG ? sum[i] : sum[i] * a.sx[r];
     }
   }
 }
@@ -469,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
 #pragma unroll
       for (uint32_t j = 0; j < W; ++j) d[j] = from(psrc, v.w[i][j]);
       u32x4 w[2];
-      q8_operands<BITS, G, true>(d, w);
+      q8_operands<BITS, G>(d, w);
       const uint32_t st = rd * kWideSteps + i;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -929,12 +933,8 @@ template <int BITS, int G, bool XG>
 static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   if (a.n <= 16 && a.O >= 16384 && q8_wide_lds(a.K, G, 1, XG) <= 160 * 1024) return q8_wide<BITS, G, XG, 1>(a, st);
   if (a.n > 64) return q8_tile<BITS, G, XG, 2, 2, 4, 4>(a, st);
-#ifdef Q8_FEW
-  return q8_few<BITS, G, XG, Q8_FEW>(a, Q8_WAVES, st);
-#else
   const uint32_t steps = (a.K + kQ8Step - 1) / kQ8Step;
   return q8_few<BITS, G, XG, 1, 1>(a, steps < 16 ? steps : 16, st);
-#endif
 }
 
 template <int BITS, bool XG>
