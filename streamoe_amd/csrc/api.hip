@@ -992,7 +992,8 @@ int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const f
   a.svec = in_dim / v.group % 8 == 0 && aligned(v.scales, 0, 16) && aligned(v.biases, 0, 16);
   a.even = in_dim / v.group % 2 == 0 && aligned(v.scales, 0, 4) && aligned(v.biases, 0, 4);
   a.xvec = in_dim / v.group % 4 == 0 && aligned(x_scales, 0, 16);
-  return hip_status(launch_qmm_i8(a, v.bits, v.group, x_group != 0, h->stream));
+  const auto launch = v.bits == 3 ? launch_qmm_i8_q3 : v.bits == 4 ? launch_qmm_i8_q4 : launch_qmm_i8_q8;
+  return hip_status(launch(a, v.group, x_group != 0, h->stream));
 }
 
 static int check_adapters(const smoe_adapters* s, uint32_t n_tokens) {

@@ -305,7 +305,7 @@ struct NormArgs {
   uint32_t group;         // 0, 32, 64 or 128
 };
 hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
-// Quantized products of 8-bit rows (rows8.hip).
+// Quantized products of 8-bit rows (rows8.h), by the weights' bits.
 constexpr uint32_t kQ8MaxIn = 16384;
 struct Q8Args {
   const uint8_t* w;        // codes [O, K]
@@ -318,7 +318,9 @@ struct Q8Args {
   uint32_t svec, xvec;     // s and b (sx) on 16 bytes, K / group a multiple of 8 (4)
   uint32_t even;           // s and b on 4 bytes, K / group even
 };
-hipError_t launch_qmm_i8(const Q8Args& a, uint32_t bits, uint32_t group, bool x_grouped, hipStream_t st);
+hipError_t launch_qmm_i8_q3(const Q8Args& a, uint32_t group, bool x_grouped, hipStream_t st);
+hipError_t launch_qmm_i8_q4(const Q8Args& a, uint32_t group, bool x_grouped, hipStream_t st);
+hipError_t launch_qmm_i8_q8(const Q8Args& a, uint32_t group, bool x_grouped, hipStream_t st);
 // Low-rank adapters (lora.hip).
 constexpr uint32_t kLoraMaxRank = 128, kLoraMaxAdapters = 4096, kLoraMaxTokens = 65536, kLoraMaxIn = 65536;
 struct LoraItem {

@@ -1,4 +1,6 @@
-// rows8.hip — quantized products of 8-bit rows on the int8 matrix cores.
+// rows8.h — quantized products of 8-bit rows on the int8 matrix cores (one
+// translation unit per weight width includes it: rows8_q4.hip, rows8_q3.hip,
+// rows8_q8.hip).
 //
 //   y[t, o] = sum_g sx[t, g] (s[o, g] sum_{c in g} q[o, c] x[t, c]
 //                             + b[o, g] sum_{c in g} x[t, c])
@@ -15,9 +17,12 @@
 // their words, so that an operand lies in one group (or two halves of it do,
 // in groups of 32). The rows' inputs are loaded from the matching places and
 // put in the codes' byte order, evens before odds of eight.
+#pragma once
+
 #include "common.h"
 #include "kernels.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace smoe {
@@ -528,8 +533,10 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a block of four waves takes WM MT tiles of 16 rows x WN NT tiles
-// of 16 columns, step after step of 128 inputs. A step's rows go straight into
+// Many rows: four waves take WM MT tiles of 16 rows x WN NT tiles of 16 columns,
+// step after step of 128 inputs; a block is KS of them, each over its share of
+// the steps with LDS of its own, for calls of few tiles (one wave per SIMD is
+// the latency of its steps, 0.9 us each). A step's rows go straight into
 // LDS, its codes through registers, where they are unpacked once per block
 // instead of once per wave; the next step's loads are in flight while a step is
 // computed. Weights are the A operand, so a lane ends with four neighbouring
@@ -555,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
 // piece fall in different banks.
 __device__ __forceinline__ uint32_t q8_place(uint32_t row, uint32_t p) { return row * 8 + (p ^ (row & 7)); }
 
-template <bool XG, int WM, int WN, int MT, int NT>
+template <int BITS, bool XG, int WM, int WN, int MT, int NT>
 struct Q8Tile {
   static constexpr uint32_t BM = WM * MT * 16, BN = WN * NT * 16;
   struct Buf {
@@ -566,19 +573,20 @@ struct Q8Tile {
     // Of two fours of groups, by group mod 8: scales, rows' scales; of eight:
     // the packed biases and scales (pairs of groups) of a column.
     float s[2][4][BN], sx[XG ? 2 : 1][XG ? 4 : 1][XG ? BM : 1];
-    uint32_t pair[2][2][4][BN];  // [octet mod 2][bias, scale][pair][column]
+    uint32_t pair[2][BITS == 8 ? 2 : 1][4][BN];  // [octet mod 2][bias, scale][pair][column]
   };
 };
 
-template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
-__global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint32_t units) {
-  using T = Q8Tile<XG, WM, WN, MT, NT>;
+template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT, int KS>
+__global__ __launch_bounds__(256 * KS, KS == 1 ? 2 : KS) void k_q8_tile(Q8Args a, uint32_t nrb, uint32_t units) {
+  using T = Q8Tile<BITS, XG, WM, WN, MT, NT>;
   constexpr uint32_t BM = T::BM, BN = T::BN, GS = kQ8Step / G;
   static_assert(WM * WN == 4, "four waves");
   static_assert(BN % 64 == 0 && BM % 64 == 0, "a wave stages one kind");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-  typename T::Lds& lds = *reinterpret_cast<typename T::Lds*>(lds_raw);
-  const uint32_t tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t share = KS == 1 ? 0u : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  typename T::Lds& lds = reinterpret_cast<typename T::Lds*>(lds_raw)[share];
+  const uint32_t tid = KS == 1 ? threadIdx.x : threadIdx.x & 255, lane = tid & 63, c16 = lane & 15, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
   // XCD x = blockIdx % 8 takes a contiguous range of the units (rows fastest),
   // so the row blocks of some columns share their weights in one L2.
@@ -743,7 +751,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
 #pragma unroll
   for (int m = 0; m < MT; ++m) xs[m][0] = xs[m][1] = 0.f;
 
-  auto compute = [&](uint32_t st) {
+  auto compute = [&](uint32_t st, bool last) {
     const typename T::Buf& B = lds.buf[st & 1];
     const uint32_t half = st * GS / 4 & 1, g0 = st * GS % 4;
     struct Op {
@@ -832,7 +840,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
       }
     }
     const uint32_t g1 = (st + 1) * GS;  // groups done
-    if (g1 % 8 == 0 || st + 1 == steps) {
+    if (g1 % 8 == 0 || last) {
       const uint32_t octet = (g1 - 1) / 8 & 1;
       auto term = [&](uint32_t which, float f) {
         qbf16x8 xv[MT];
@@ -854,16 +862,40 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
     }
   };
 
-  fetch(0);
-  store(0);
+  // A share starts with a whole eight of groups.
+  constexpr uint32_t ALIGN = GS >= 8 ? 1 : 8 / GS;
+  const uint32_t each = KS == 1 ? steps : ((steps + KS - 1) / KS + ALIGN - 1) / ALIGN * ALIGN;
+  const uint32_t first = KS == 1 ? 0u : share * each, end = KS == 1 ? steps : min(first + each, steps);
+  if (KS == 1 || first < end) {
+    fetch(first);
+    store(first);
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows' copies into LDS
   __syncthreads();
-  for (uint32_t st = 0; st < steps; ++st) {
-    fetch(st + 1);
-    compute(st);
-    if (st + 1 < steps) store(st + 1);
+  for (uint32_t i = 0; i < each; ++i) {  // as many barriers in every share
+    const uint32_t st = first + i;
+    if (KS == 1 || st + 1 < end) fetch(st + 1);  // nothing past the last step
+    if (KS == 1 || st < end) compute(st, st + 1 == end);
+    if (st + 1 < end) store(st + 1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+  }
+  if constexpr (KS > 1) {  // the shares' parts, over their LDS
+    f32x4* const part = reinterpret_cast<f32x4*>(lds_raw);
+    if (share) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) part[((share - 1) * MT * NT + m * NT + t) * 256 + tid] = acc[m][t];
+    }
+    __syncthreads();
+    if (share) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < KS - 1; ++k) acc[m][t] += part[(k * MT * NT + m * NT + t) * 256 + tid];
   }
 
 #pragma unroll
@@ -890,18 +922,19 @@ __global__ __launch_bounds__(256, 2) void k_q8_tile(Q8Args a, uint32_t nrb, uint
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT>
+template <int BITS, int G, bool XG, int WM, int WN, int MT, int NT, int KS>
 static hipError_t q8_tile(const Q8Args& a, hipStream_t st) {
-  using T = Q8Tile<XG, WM, WN, MT, NT>;
+  using T = Q8Tile<BITS, XG, WM, WN, MT, NT>;
   const uint32_t nrb = (a.n + T::BM - 1) / T::BM, units = nrb * ((a.O + T::BN - 1) / T::BN);
-  constexpr uint32_t lds = sizeof(typename T::Lds);
-  auto fn = k_q8_tile<BITS, G, XG, WM, WN, MT, NT>;
+  constexpr uint32_t lds = KS * sizeof(typename T::Lds);
+  static_assert(lds <= 160 * 1024 && (KS - 1) * MT * NT * 4096 <= lds, "the shares' LDS");
+  auto fn = k_q8_tile<BITS, G, XG, WM, WN, MT, NT, KS>;
   if (lds > 64 * 1024) {
     static std::atomic<uint64_t> raised{0};
     const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(fn), lds, raised);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(fn, dim3((units + 7) / 8 * 8), dim3(256), lds, st, a, nrb, units);
+  hipLaunchKernelGGL(fn, dim3((units + 7) / 8 * 8), dim3(256 * KS), lds, st, a, nrb, units);
   return hipGetLastError();
 }
 
@@ -929,23 +962,58 @@ static hipError_t q8_wide(const Q8Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Which kernel, by how many blocks there are for the 256 CUs. Times in us, 4
+// bits, groups of 64, row scales, graph replays; n rows K -> O. Over 630 calls
+// of all bits and groups drawn from 1 to 1000 rows, 150 to 60000 columns, 512
+// to 7168 inputs the chosen kernel took 1.03 times the fastest one's time.
 template <int BITS, int G, bool XG>
 static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
-  if (a.n <= 16 && a.O >= 16384 && q8_wide_lds(a.K, G, 1, XG) <= 160 * 1024) return q8_wide<BITS, G, XG, 1>(a, st);
-  if (a.n > 64) return q8_tile<BITS, G, XG, 2, 2, 4, 4>(a, st);
   const uint32_t steps = (a.K + kQ8Step - 1) / kQ8Step;
-  return q8_few<BITS, G, XG, 1, 1>(a, steps < 16 ? steps : 16, st);
+  const uint64_t rt = (a.n + 15) / 16, ct = (a.O + 15) / 16;  // row and column tiles
+  auto units = [&](uint32_t m, uint32_t n) { return (uint64_t)((a.n + m - 1) / m) * ((a.O + n - 1) / n); };
+  const uint64_t u64 = units(64, 64), u128 = units(128, 128);
+  // Whether s shares of the steps all have some (they start on eight groups).
+  auto shares = [&](uint32_t s) { return steps >= s * (8 * G / kQ8Step); };
+  // One tile a block, all steps at once (16 rows 2048 -> 4096: 5.1, two column
+  // tiles a block 6.3; 32 rows: 7.2 and, two row tiles a block, 6.1).
+  if (rt * ct <= 256) return q8_few<BITS, G, XG, 1, 1>(a, std::min(steps, 16u), st);
+  if (rt == 1) {
+    // 16 rows 2048 -> 16384: 8.6, rows in LDS 10.3; -> 50000: 39 and 18.
+    if (ct <= 1024 || q8_wide_lds(a.K, G, 1, XG) > 160 * 1024)
+      return q8_few<BITS, G, XG, 1, 2>(a, std::min(steps, 8u), st);
+    return q8_wide<BITS, G, XG, 1>(a, st);
+  }
+  // Two tiles a block, side by side where that wastes less (64 rows 7168 ->
+  // 2048: 11.0, four tiles 14.3; 45 rows 2048 -> 2560: 6.5 and 8.1), or four
+  // (64 rows 2048 -> 4096: 7.8, two tiles 8.3).
+  const uint64_t b21 = (rt + 1) / 2 * ct, b12 = rt * ((ct + 1) / 2), b22 = (rt + 1) / 2 * ((ct + 1) / 2);
+  if (b21 <= 256 && b21 <= b12) return q8_few<BITS, G, XG, 2, 1>(a, std::min(steps, 8u), st);
+  if (b12 <= 256) return q8_few<BITS, G, XG, 1, 2>(a, std::min(steps, 8u), st);
+  if (b22 <= 256) return q8_few<BITS, G, XG, 2, 2>(a, std::min(steps, 8u), st);
+  // Fewer waves each for somewhat more blocks, while 64 x 64 tiles would leave
+  // CUs idle (200 rows 7168 -> 2048, 448 blocks: 24.3, staged 27.7), and for
+  // short sums, which have no steps to share (200 rows 512 -> 2048: 5.4, staged
+  // 7.1; 400 rows: 7.6 and 7.1).
+  if (b22 <= (steps < 8 ? 640u : 448u)) return q8_few<BITS, G, XG, 2, 2>(a, std::min(steps, 4u), st);
+  // 64 x 64 tiles, four shares while their blocks fit the chip at once, then
+  // two (200 rows 2048 -> 4096, 256 tiles: 11.1, two shares 12.7, one 17.5; 400
+  // rows, 448: 19.5, 17.2, 20.4).
+  if (u64 <= 256 && shares(4)) return q8_tile<BITS, G, XG, 2, 2, 2, 2, 4>(a, st);
+  if (u64 <= 512 && shares(2)) return q8_tile<BITS, G, XG, 2, 2, 2, 2, 2>(a, st);
+  // 128 x 128 where they fill the chip with two shares each (1000 rows 2048 ->
+  // 4096, 256 tiles: 27.0, 64 x 64 29.9) or two blocks on most CUs (1000 rows
+  // 4096 -> 7168, 448: 78 and 89; 600 rows 4096 -> 8192, 320: 70 and 64), but
+  // for short sums (140 rows 512 -> 43682: 32 and 25).
+  if (u128 > 192 && u128 <= 256 && shares(2)) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 2>(a, st);
+  if (u128 > 384 && steps >= 8) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 1>(a, st);
+  return q8_tile<BITS, G, XG, 2, 2, 2, 2, 1>(a, st);
 }
 
-template <int BITS, bool XG>
-static hipError_t q8_group(const Q8Args& a, uint32_t group, hipStream_t st) {
-  return group == 32 ? q8_go<BITS, 32, XG>(a, st) : group == 64 ? q8_go<BITS, 64, XG>(a, st) : q8_go<BITS, 128, XG>(a, st);
-}
-
-hipError_t launch_qmm_i8(const Q8Args& a, uint32_t bits, uint32_t group, bool x_grouped, hipStream_t st) {
-  if (bits == 8) return x_grouped ? q8_group<8, true>(a, group, st) : q8_group<8, false>(a, group, st);
-  if (bits == 4) return x_grouped ? q8_group<4, true>(a, group, st) : q8_group<4, false>(a, group, st);
-  return x_grouped ? q8_group<3, true>(a, group, st) : q8_group<3, false>(a, group, st);
+template <int BITS>
+hipError_t q8_launch(const Q8Args& a, uint32_t group, bool x_grouped, hipStream_t st) {
+  if (x_grouped)
+    return group == 32 ? q8_go<BITS, 32, true>(a, st) : group == 64 ? q8_go<BITS, 64, true>(a, st) : q8_go<BITS, 128, true>(a, st);
+  return group == 32 ? q8_go<BITS, 32, false>(a, st) : group == 64 ? q8_go<BITS, 64, false>(a, st) : q8_go<BITS, 128, false>(a, st);
 }
 
 }  // namespace smoe

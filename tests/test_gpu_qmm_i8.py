@@ -104,6 +104,27 @@ def test_sizes(kernels, n, O, K, bits, G, xg):
     _check(kernels, n, O, K, bits, G, xg)
 
 
+@pytest.mark.parametrize("bits,G,grouped", [(4, 64, False), (3, 64, True), (8, 128, False), (4, 32, True), (8, 32, False),
+                                            (3, 128, True)])
+@pytest.mark.parametrize("n,O,steps", [
+    (31, 2090, 5),     # two row tiles a block
+    (45, 2563, 4),     # two column tiles a block
+    (64, 2600, 11),    # four tiles a block
+    (100, 2560, 3),    # four tiles a block, four waves
+    (130, 4100, 33),   # 64 x 64 tiles, four shares of the steps
+    (129, 4096, 8),    # .. or fewer where the groups do not divide
+    (390, 4100, 17),   # .. two shares
+    (400, 4100, 4),    # .. one
+    (500, 7001, 17),   # 128 x 128 tiles, two shares
+    (1000, 6404, 9),   # .. one
+])
+def test_every_kernel(kernels, n, O, steps, bits, G, grouped):
+    """Sizes that every kernel and tile takes, the last step short of 128 inputs
+    where the group allows."""
+    K = steps * 128 - (128 - G)
+    _check(kernels, n, O, K, bits, G, G if grouped else 0)
+
+
 @pytest.mark.parametrize("bits", [4, 3, 8])
 @pytest.mark.parametrize("G", [32, 64, 128])
 @pytest.mark.parametrize("grouped", [False, True])
