@@ -351,7 +351,7 @@ hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st);
 constexpr uint32_t kBeamMaxBeams = 16, kBeamMaxPicks = 32, kBeamMaxVocab = 1u << 28;
 constexpr uint32_t kBeamMaxSlices = 64;  // of one beam's logits
 struct BeamStat {
-  double sum;  // of exp(logit - max) over a slice
+  double sum;  // of exp(logit - max) over a wave's part of a slice
   float max;
   uint32_t pad;
 };
@@ -364,7 +364,7 @@ struct BeamArgs {
   int32_t *out_rows, *out_tokens;
   // Workspace (beam_workspace): per row and slice, of `tiles` tiles each.
   uint32_t slices, tiles;
-  BeamStat* stats;
+  BeamStat* stats;           // four, one per wave
   unsigned long long* cand;  // picks keys each, in falling order, 0 past the last
 };
 uint64_t beam_workspace(uint32_t requests, uint32_t beams, uint32_t vocab, uint32_t picks, BeamArgs* a, uint8_t* base);

@@ -1,14 +1,16 @@
 """smoe_beam_select and smoe_beam_reorder.
 
 Picks are compared with the definition in 64 bits on the host; a pick may
-differ only where its value lies within the error of the sums: the log-sum-exp
-adds exponentials of relative error 2 u each (u = 2^-24, expf's last place, of
-either sign) and rounds partial sums of 16 by 16 u, so a value is off by at
-most 20 u, and its f32 score by u |score| more. Within a row the log-sum-exp is
+differ only where its value lies within the error of the sums. With u = 2^-24:
+a term exp(l - m) is off by 2 u (the exponential's last place), by u |l - m|
+(the difference's rounding) and 0.25 u |l - m| (log2 e in 24 bits); weighted as
+in the sum, |l - m| is at most the entropy, ln V <= 13.4 for the sizes here, so
+that is 19 u; partial sums of 16 terms round by up to 16 u. A value is off by at
+most 36 u, its f32 score by u |score| more. Within a row the log-sum-exp is
 one number, so there the order is exact; and so it is between rows of the same
 logits. Rows whose log-sum-exps are equal only as real numbers (one row another
 one's permutation) may come in either order, each value being off by up to
-20 u: two picks of different rows whose 64-bit values are within 40 u."""
+36 u: two picks of different rows whose 64-bit values are within 72 u."""
 import numpy as np
 import pytest
 
@@ -67,7 +69,7 @@ def _either_order(logits, scores, done, pad, R, W, V, P, rows, tok, wv, wr):
         value = {(r, t): v for v, r, t in zip(av[q], ar[q], at[q])}
         for j in range(P):
             if (rows[q, j], tok[q, j]) != (ar[q, j], at[q, j]):
-                assert rows[q, j] != wr[q, j] and abs(value[rows[q, j], tok[q, j]] - wv[q, j]) <= 40 * U
+                assert rows[q, j] != wr[q, j] and abs(value[rows[q, j], tok[q, j]] - wv[q, j]) <= 72 * U
         for r in set(rows[q]):  # a row's own picks: the first of its order
             own = tok[q][rows[q] == r]
             assert np.array_equal(own, at[q][ar[q] == r][:len(own)])
@@ -83,7 +85,7 @@ def _check(kernels, logits, scores, done, pad, R, W, V, P):
         _either_order(host, scores, done, pad, R, W, V, P, rows, tok, wv, wr)
     fin = np.isfinite(wv)
     assert np.array_equal(v[~fin], wv[~fin])
-    assert np.all(np.abs(v - wv)[fin] <= 20 * U + U * np.abs(wv[fin]))
+    assert np.all(np.abs(v - wv)[fin] <= 36 * U + U * np.abs(wv[fin]))
 
 
 @pytest.mark.parametrize("R,W,V,P", [
