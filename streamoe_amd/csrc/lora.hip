@@ -2,7 +2,8 @@
 //
 //   y[t] = base[t] + scale[a] B_a (A_a x[t]),  a = ids[t]
 //
-//   k_lora_plan    rows sorted by adapter, items of up to 16 rows of one
+//   k_lora_plan    rows sorted by adapter, items of up to 16 rows of one (up to
+//                  64 rows the blocks below find their item by themselves)
 //   k_lora_down    u = A x of an item's rows on bf16 MFMA, one share of the
 //                  inputs per block, partial sums in f32
 //   k_lora_up      the shares added, scaled, times B on bf16 MFMA, plus base
@@ -92,18 +93,57 @@ __global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
   for (uint32_t r = t; r < a.n; r += 1024) a.perm[atomicAdd(&sh[adapter(r)], 1u)] = r;
 }
 
+constexpr uint32_t kLoraSmall = 64;  // rows whose items need no plan: one per lane
+
+// Item blockIdx.x of a call of up to 64 rows, by every wave for itself: the
+// rows' ids, one per lane, taken group by group in the order of their first
+// rows; `rows` receives the item's rows (kLoraM per wave).
+__device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t lane, uint32_t* rows) {
+  const int32_t id = lane < a.n ? a.ids[lane] : -2;
+  const bool bad = lane < a.n && (id < -1 || id >= (int32_t)a.n_adapters);
+  const uint32_t ad = bad || id < 0 ? a.n_adapters : (uint32_t)id;
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    bool wrong = bad;
+    if (a.ranks)
+      for (uint32_t i = lane; i < a.n_adapters; i += 64) wrong |= a.ranks[i] < 0 || a.ranks[i] > (int32_t)a.max_rank;
+    if (wrong) *a.err = 2u;
+  }
+  uint64_t left = __ballot(lane < a.n);
+  uint32_t item = blockIdx.x, start = 0;
+  LoraItem it{0u, 0u, 0u};
+  while (left) {
+    const uint32_t leader = (uint32_t)__ffsll((long long)left) - 1;
+    const uint32_t mine = (uint32_t)__builtin_amdgcn_readlane((int)ad, (int)leader);
+    const uint64_t group = __ballot(lane < a.n && ad == mine);
+    const uint32_t c = (uint32_t)__popcll(group), items = (c + kLoraM - 1) / kLoraM;
+    if (item < items) {
+      const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(group >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)group, 0u));
+      if ((group >> lane & 1) && at / kLoraM == item) rows[at % kLoraM] = lane;
+      it = LoraItem{mine, start + item * kLoraM, min(kLoraM, c - item * kLoraM)};
+      break;
+    }
+    item -= items;
+    start += c;
+    left &= ~group;
+  }
+  // The rows are in LDS: no other wave writes or reads this part.
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  return it;
+}
+
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c.
-template <bool XBF16>
+template <bool XBF16, bool SMALL>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   constexpr int MT = kLoraMaxRank / 16;
   __shared__ f32x4 red[4][64];
-  const LoraItem it = a.items[blockIdx.x];
-  if (it.count == 0 || it.adapter >= a.n_adapters) return;
+  __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
+  const LoraItem it = SMALL ? lora_small_item(a, lane, rows[wave]) : a.items[blockIdx.x];
+  if (it.count == 0 || it.adapter >= a.n_adapters) return;
   const uint32_t K = a.in_dim, share = blockIdx.y;
   const uint32_t rank = lora_rank(a, it.adapter), nt = (rank + 15) / 16;
-  const uint32_t row = a.perm[it.start + min(c16, it.count - 1)];
+  const uint32_t row = SMALL ? rows[wave][min(c16, it.count - 1)] : a.perm[it.start + min(c16, it.count - 1)];
   const uint16_t* const A = (const uint16_t*)(a.a + (uint64_t)it.adapter * a.a_stride);
   const uint32_t steps = (K + 31) / 32, s0 = steps * share / a.shares, s1 = steps * (share + 1) / a.shares;
   f32x4 acc[MT];
@@ -149,61 +189,102 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   }
 }
 
-constexpr uint32_t kLoraOut = 256;  // outputs per block of k_lora_up: four waves of four tiles of 16
-
 // D = B (outputs) x u (rows): lane (c, kb) ends with outputs 4 kb .. of row c.
+// A block takes 64 NT outputs of an item; it adds the shares once, into LDS, as
+// the bf16 pairs that its waves read as operands (added by every wave for
+// itself the shares were 22 of 33 us: 200 rows, 40 adapters of rank 64, 4096 ->
+// 4096). B's and base's loads go out ahead of that.
+template <bool SMALL, int KT, int NT>
 __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
-  const LoraItem it = a.items[blockIdx.x];
-  if (it.count == 0) return;
+  constexpr uint32_t RP = KT * 32 + 8;  // bf16 per row in LDS: rows apart by 16 bytes of banks
+  __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
+  __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
+  const LoraItem it = SMALL ? lora_small_item(a, lane, rows[wave]) : a.items[blockIdx.x];
+  if (it.count == 0) return;
   const uint32_t O = a.out_dim, R = a.max_rank;
-  const uint32_t place = it.start + min(c16, it.count - 1), row = a.perm[place];
-  const bool mine = c16 < it.count;
-  f32x4 acc[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const uint32_t o0 = blockIdx.y * kLoraOut + wave * 64;
-  if (it.adapter < a.n_adapters) {
-    const uint32_t rank = lora_rank(a, it.adapter);
+  const uint32_t row = SMALL ? rows[wave][min(c16, it.count - 1)] : a.perm[it.start + min(c16, it.count - 1)];
+  const uint32_t o0 = (blockIdx.y * 4 + wave) * NT * 16;
+  const bool none = it.adapter >= a.n_adapters;
+  if (none && a.base == a.y) return;
+  const uint32_t rank = none ? 0u : lora_rank(a, it.adapter);
+  lbf16x8 w[KT][NT];
+  if (rank) {
     const uint16_t* const B = (const uint16_t*)(a.b + (uint64_t)it.adapter * a.b_stride);
-    const float scale = a.scale[it.adapter];
-    for (uint32_t k0 = 0; k0 < rank; k0 += 32) {
-      const uint32_t k = k0 + kb * 8;
-      const uint32_t kc = k < R ? k : 0;  // R is a multiple of 8
-      lf32x8 u = {0, 0, 0, 0, 0, 0, 0, 0};
-      for (uint32_t s = 0; s < a.shares; ++s)
-        u += *reinterpret_cast<const lf32x8*>(a.u + ((uint64_t)s * a.n + place) * R + kc);
-      u *= scale;
-      lbf16x8 hi, lo;
-      split_bf16(u, hi, lo);
-      const int left = k < rank ? (int)(rank - k) : 0;
-      hi = first_of(hi, left);
-      lo = first_of(lo, left);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t o = min(o0 + i * 16 + c16, O - 1);
-        const lbf16x8 w = first_of(*reinterpret_cast<const lbf16x8*>(B + (uint64_t)o * R + kc), left);
-        acc[i] = mfma_bf16(w, hi, acc[i]);
-        acc[i] = mfma_bf16(w, lo, acc[i]);
-      }
+    for (int s = 0; s < KT; ++s) {
+      const uint32_t k = s * 32 + kb * 8;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (s * 32 < (int)rank)
+          w[s][i] = *reinterpret_cast<const lbf16x8*>(B + (uint64_t)min(o0 + i * 16 + c16, O - 1) * R + (k < R ? k : 0));  // R is a multiple of 8
     }
-  } else if (a.base == a.y) {
-    return;
   }
-  if (!mine) return;
+  f32x4 acc[NT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NT; ++i) {
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     const uint32_t o = o0 + i * 16 + 4 * kb;
     const uint64_t e = (uint64_t)row * O + o;
+    if (!a.base || c16 >= it.count) continue;
     if (a.vec) {
-      if (o >= O) continue;
-      f32x4 v = acc[i];
-      if (a.base) v += *reinterpret_cast<const f32x4*>(a.base + e);
-      *reinterpret_cast<f32x4*>(a.y + e) = v;
+      if (o < O) acc[i] = *reinterpret_cast<const f32x4*>(a.base + e);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (o + r < O) a.y[e + r] = acc[i][r] + (a.base ? a.base[e + r] : 0.f);
+        if (o + r < O) acc[i][r] = a.base[e + r];
+    }
+  }
+  f32x4 low[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) low[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (rank) {  // the same for the whole block
+    const float scale = a.scale[it.adapter];
+    const uint32_t q = R / 4;  // quarters of eights: a thread adds four values
+    for (uint32_t i = threadIdx.x; i < kLoraM * KT * 8; i += 256) {
+      const uint32_t r = i / (KT * 8), k = i % (KT * 8) * 4;
+      f32x4 u = {0.f, 0.f, 0.f, 0.f};
+      if (r < it.count && k < R)
+        for (uint32_t s = 0; s < a.shares; ++s)
+          u += reinterpret_cast<const f32x4*>(a.u)[((uint64_t)s * a.n + it.start + r) * q + k / 4];
+      uint16_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v = k + j < rank ? u[j] * scale : 0.f;  // nothing was written behind the rank
+        const __bf16 hi = (__bf16)v;
+        h[j] = __builtin_bit_cast(uint16_t, hi);
+        l[j] = __builtin_bit_cast(uint16_t, (__bf16)(v - (float)hi));
+      }
+      *reinterpret_cast<uint2*>(uh + r * RP + k) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+      *reinterpret_cast<uint2*>(ul + r * RP + k) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      const uint32_t k = s * 32 + kb * 8;
+      if (s * 32 >= (int)rank) break;
+      const int left = k < rank ? (int)(rank - k) : 0;
+      const lbf16x8 hi = *reinterpret_cast<const lbf16x8*>(uh + c16 * RP + k), lo = *reinterpret_cast<const lbf16x8*>(ul + c16 * RP + k);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const lbf16x8 b = first_of(w[s][i], left);
+        low[i] = mfma_bf16(b, hi, low[i]);
+        low[i] = mfma_bf16(b, lo, low[i]);
+      }
+    }
+  }
+  if (c16 >= it.count) return;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const uint32_t o = o0 + i * 16 + 4 * kb;
+    const uint64_t e = (uint64_t)row * O + o;
+    const f32x4 v = acc[i] + low[i];
+    if (a.vec) {
+      if (o < O) *reinterpret_cast<f32x4*>(a.y + e) = v;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (o + r < O) a.y[e + r] = v[r];
     }
   }
 }
@@ -231,18 +312,31 @@ uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, Lora
   return ib + pb + al256((uint64_t)shares * n * max_rank * 4);
 }
 
-hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
-  hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 4, st, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+template <bool SMALL>
+static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
+  const dim3 grid(a.n_items, a.shares);
   if (x_bf16)
-    hipLaunchKernelGGL(k_lora_down<true>, dim3(a.n_items, a.shares), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_lora_down<true, SMALL>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL(k_lora_down<false>, dim3(a.n_items, a.shares), dim3(256), 0, st, a);
-  e = hipGetLastError();
+    hipLaunchKernelGGL((k_lora_down<false, SMALL>), grid, dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k_lora_up, dim3(a.n_items, (a.out_dim + kLoraOut - 1) / kLoraOut), dim3(256), 0, st, a);
-  return hipGetLastError();
+  // Outputs per block: as many as leave two blocks for every CU.
+  auto up = [&](auto fn, uint32_t nt) {
+    hipLaunchKernelGGL(fn, dim3(a.n_items, (a.out_dim + 64 * nt - 1) / (64 * nt)), dim3(256), 0, st, a);
+    return hipGetLastError();
+  };
+  const bool wide = (uint64_t)a.n_items * ((a.out_dim + 255) / 256) >= 512;
+  if (a.max_rank <= 32) return wide ? up(k_lora_up<SMALL, 1, 4>, 4) : up(k_lora_up<SMALL, 1, 1>, 1);
+  if (a.max_rank <= 64) return wide ? up(k_lora_up<SMALL, 2, 4>, 4) : up(k_lora_up<SMALL, 2, 1>, 1);
+  return wide ? up(k_lora_up<SMALL, 4, 4>, 4) : up(k_lora_up<SMALL, 4, 1>, 1);
+}
+
+hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
+  if (a.n <= kLoraSmall) return lora_go<true>(a, x_bf16, st);
+  hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 4, st, a);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : lora_go<false>(a, x_bf16, st);
 }
 
 }  // namespace smoe
