@@ -15,6 +15,8 @@
 #include "common.h"
 #include "kernels.h"
 
+#include <type_traits>
+
 namespace smoe {
 
 typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
@@ -46,6 +48,21 @@ __device__ __forceinline__ uint32_t lora_rank(const LoraArgs& a, uint32_t ad) {
   return r < 0 ? 0u : min((uint32_t)r, a.max_rank);
 }
 
+// Inclusive sums over the wave: DPP row shifts, then row broadcasts.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lora_dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t lora_scan(uint32_t v) {
+  v += lora_dpp<0x111, 0xF>(v);
+  v += lora_dpp<0x112, 0xF>(v);
+  v += lora_dpp<0x114, 0xF>(v);
+  v += lora_dpp<0x118, 0xF>(v);
+  v += lora_dpp<0x142, 0xA>(v);
+  v += lora_dpp<0x143, 0xC>(v);
+  return v;
+}
+
 // One block: counts per adapter, their items, the rows in adapter order. Rows
 // without an adapter (-1, or an id or rank that does not exist, which is
 // reported) come last, as items of adapter n_adapters.
@@ -53,12 +70,13 @@ __global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
   extern __shared__ uint32_t sh[];  // [n_adapters + 1] counts, then next positions
   __shared__ uint32_t wrow[16], witem[16], base_row, base_item;
   const uint32_t t = threadIdx.x, N = a.n_adapters + 1;
+  const int32_t id0 = t < a.n ? a.ids[t] : -1;  // the first 1024 rows' stay in registers
   for (uint32_t i = t; i < N; i += 1024) sh[i] = 0;
   if (t == 0) base_row = base_item = 0;
   __syncthreads();
   bool bad = false;
   auto adapter = [&](uint32_t row) {
-    const int32_t id = a.ids[row];
+    const int32_t id = row < 1024 ? id0 : a.ids[row];
     bad |= id < -1 || id >= (int32_t)a.n_adapters;
     return id < 0 || id >= (int32_t)a.n_adapters ? a.n_adapters : (uint32_t)id;
   };
@@ -69,12 +87,7 @@ __global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
   __syncthreads();
   for (uint32_t i0 = 0; i0 < N; i0 += 1024) {
     const uint32_t ad = i0 + t, c = ad < N ? sh[ad] : 0u, it = (c + kLoraM - 1) / kLoraM;
-    uint32_t pr = c, pi = it;  // inclusive sums over the wave
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t r = __shfl_up(pr, o, kWave), q = __shfl_up(pi, o, kWave);
-      if ((t & 63) >= (uint32_t)o) pr += r, pi += q;
-    }
+    const uint32_t pr = lora_scan(c), pi = lora_scan(it);
     if ((t & 63) == 63) wrow[t >> 6] = pr, witem[t >> 6] = pi;
     __syncthreads();
     uint32_t row = base_row + pr - c, item = base_item + pi - it;
@@ -133,9 +146,8 @@ __device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t 
 
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c.
-template <bool XBF16, bool SMALL>
+template <bool XBF16, bool SMALL, int MT>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
-  constexpr int MT = kLoraMaxRank / 16;
   __shared__ f32x4 red[4][64];
   __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
@@ -149,27 +161,43 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (uint32_t s = s0 + wave; s < s1; s += 4) {
-    const uint32_t k = s * 32 + kb * 8;
-    const bool in = k < K;  // K is a multiple of 8
-    const uint64_t e = (uint64_t)row * K + (in ? k : 0);
+  // Two steps' loads at once.
+  using X = std::conditional_t<XBF16, lbf16x8, lf32x8>;
+  struct Step {
+    X x;
+    lbf16x8 w[MT];
+  };
+  auto load = [&](uint32_t s, Step& v) {
+    const uint32_t k = s * 32 + kb * 8, kc = k < K ? k : 0;  // K is a multiple of 8
+    v.x = *reinterpret_cast<const X*>(reinterpret_cast<const uint8_t*>(a.x) + ((uint64_t)row * K + kc) * (sizeof(X) / 8));
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      if (i < (int)nt) v.w[i] = *reinterpret_cast<const lbf16x8*>(A + (uint64_t)min(i * 16 + c16, rank - 1) * K + kc);
+  };
+  auto compute = [&](uint32_t s, const Step& v) {
+    const bool in = s * 32 + kb * 8 < K;
     lbf16x8 hi, lo;
     if constexpr (XBF16) {
-      hi = *reinterpret_cast<const lbf16x8*>((const uint16_t*)a.x + e);
+      hi = first_of(v.x, in ? 8 : 0);
     } else {
-      split_bf16(*reinterpret_cast<const lf32x8*>((const float*)a.x + e), hi, lo);
+      split_bf16(v.x, hi, lo);
+      hi = first_of(hi, in ? 8 : 0);
       lo = first_of(lo, in ? 8 : 0);
     }
-    hi = first_of(hi, in ? 8 : 0);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       if (i >= (int)nt) break;
-      const uint32_t j = i * 16 + c16;
-      const lbf16x8 w = first_of(*reinterpret_cast<const lbf16x8*>(A + (uint64_t)min(j, rank - 1) * K + (in ? k : 0)),
-                                 in && j < rank ? 8 : 0);
+      const lbf16x8 w = first_of(v.w[i], in && i * 16 + c16 < rank ? 8 : 0);
       acc[i] = mfma_bf16(hi, w, acc[i]);
       if constexpr (!XBF16) acc[i] = mfma_bf16(lo, w, acc[i]);
     }
+  };
+  for (uint32_t s = s0 + wave; s < s1; s += 8) {
+    Step v[2];
+    load(s, v[0]);
+    if (s + 4 < s1) load(s + 4, v[1]);
+    compute(s, v[0]);
+    if (s + 4 < s1) compute(s + 4, v[1]);
   }
   for (uint32_t i = 0; i < nt; ++i) {
     f32x4 v = acc[0];
@@ -244,9 +272,26 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
     for (uint32_t i = threadIdx.x; i < kLoraM * KT * 8; i += 256) {
       const uint32_t r = i / (KT * 8), k = i % (KT * 8) * 4;
       f32x4 u = {0.f, 0.f, 0.f, 0.f};
-      if (r < it.count && k < R)
-        for (uint32_t s = 0; s < a.shares; ++s)
-          u += reinterpret_cast<const f32x4*>(a.u)[((uint64_t)s * a.n + it.start + r) * q + k / 4];
+      if (r < it.count && k < R) {
+        const f32x4* const p = reinterpret_cast<const f32x4*>(a.u) + ((uint64_t)it.start + r) * q + k / 4;
+        const uint64_t apart = (uint64_t)a.n * q;
+        // Loads of up to eight shares at once, added in order.
+        auto add = [&](uint32_t s0, auto count) {
+          constexpr int C = decltype(count)::value;
+          f32x4 v[C];
+#pragma unroll
+          for (int s = 0; s < C; ++s) v[s] = p[(s0 + s) * apart];
+#pragma unroll
+          for (int s = 0; s < C; ++s) u += v[s];
+        };
+        if (a.shares >= 8) {
+          for (uint32_t s = 0; s < a.shares; s += 8) add(s, std::integral_constant<int, 8>{});
+        } else if (a.shares == 4) {
+          add(0, std::integral_constant<int, 4>{});
+        } else {
+          add(0, std::integral_constant<int, 1>{});
+        }
+      }
       uint16_t h[4], l[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -294,7 +339,8 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
 // ---------------------------------------------------------------------------
 static uint64_t al256(uint64_t n) { return (n + 255) & ~255ull; }
 
-// Shares of the inputs: enough blocks for few rows, none to spare for many.
+// Shares of the inputs: enough blocks for few rows, none to spare for many
+// (k_lora_up adds 16, 8, 4 or 1).
 static uint32_t lora_shares(uint32_t n) { return n <= 256 ? 16u : n <= 1024 ? 8u : n <= 4096 ? 4u : 1u; }
 
 uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, LoraArgs* a, uint8_t* base) {
@@ -314,12 +360,19 @@ uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, Lora
 
 template <bool SMALL>
 static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
-  const dim3 grid(a.n_items, a.shares);
-  if (x_bf16)
-    hipLaunchKernelGGL((k_lora_down<true, SMALL>), grid, dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_lora_down<false, SMALL>), grid, dim3(256), 0, st, a);
-  const hipError_t e = hipGetLastError();
+  auto down = [&](auto fn) {
+    hipLaunchKernelGGL(fn, dim3(a.n_items, a.shares), dim3(256), 0, st, a);
+    return hipGetLastError();
+  };
+  const uint32_t mt = (a.max_rank + 15) / 16;  // tiles of 16 ranks
+  const hipError_t e = x_bf16 ? (mt <= 1   ? down(k_lora_down<true, SMALL, 1>)
+                                 : mt <= 2 ? down(k_lora_down<true, SMALL, 2>)
+                                 : mt <= 4 ? down(k_lora_down<true, SMALL, 4>)
+                                           : down(k_lora_down<true, SMALL, 8>))
+                              : (mt <= 1   ? down(k_lora_down<false, SMALL, 1>)
+                                 : mt <= 2 ? down(k_lora_down<false, SMALL, 2>)
+                                 : mt <= 4 ? down(k_lora_down<false, SMALL, 4>)
+                                           : down(k_lora_down<false, SMALL, 8>));
   if (e != hipSuccess) return e;
   // Outputs per block: as many as leave two blocks for every CU.
   auto up = [&](auto fn, uint32_t nt) {
