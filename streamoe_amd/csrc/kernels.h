@@ -324,7 +324,8 @@ hipError_t launch_qmm_i8_q8(const Q8Args& a, uint32_t group, bool x_grouped, hip
 // Low-rank adapters (lora.hip).
 constexpr uint32_t kLoraMaxRank = 128, kLoraMaxAdapters = 4096, kLoraMaxTokens = 65536, kLoraMaxIn = 65536;
 struct LoraItem {
-  uint32_t adapter, start, count;  // rows perm[start ..] of one adapter (n_adapters: none)
+  uint32_t adapter, start, count, rank;  // up to 16 rows of one adapter (n_adapters: none); start: rows before them
+  float scale;
 };
 struct LoraArgs {
   const uint8_t *a, *b;        // adapter i's bf16 [max_rank, in_dim] at a + i a_stride, [out_dim, max_rank] at b + i b_stride
@@ -342,7 +343,7 @@ struct LoraArgs {
   // Workspace (lora_workspace).
   uint32_t n_items, shares;
   LoraItem* items;             // [n_items], count 0 past the last
-  uint32_t* perm;              // [n]
+  uint32_t* rows;              // [n_items, 16], unset past the count
   float* u;                    // [shares, n, max_rank]
 };
 uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, LoraArgs* a, uint8_t* base);

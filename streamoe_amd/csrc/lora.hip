@@ -63,13 +63,15 @@ __device__ __forceinline__ uint32_t lora_scan(uint32_t v) {
   return v;
 }
 
-// One block: counts per adapter, their items, the rows in adapter order. Rows
-// without an adapter (-1, or an id or rank that does not exist, which is
-// reported) come last, as items of adapter n_adapters.
+// One block: counts per adapter, their items, each item's rows. Rows without
+// an adapter (-1, or an id that does not exist, which is reported as a rank out
+// of range is) come last, as items of adapter n_adapters. An item holds all
+// that the other kernels need to know of its adapter.
 __global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
-  extern __shared__ uint32_t sh[];  // [n_adapters + 1] counts, then next positions
+  extern __shared__ uint32_t sh[];  // [n_adapters + 1] counts, then taken; [n_adapters + 1] first items
   __shared__ uint32_t wrow[16], witem[16], base_row, base_item;
   const uint32_t t = threadIdx.x, N = a.n_adapters + 1;
+  uint32_t* const first = sh + N;
   const int32_t id0 = t < a.n ? a.ids[t] : -1;  // the first 1024 rows' stay in registers
   for (uint32_t i = t; i < N; i += 1024) sh[i] = 0;
   if (t == 0) base_row = base_item = 0;
@@ -81,29 +83,39 @@ __global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
     return id < 0 || id >= (int32_t)a.n_adapters ? a.n_adapters : (uint32_t)id;
   };
   for (uint32_t r = t; r < a.n; r += 1024) atomicAdd(&sh[adapter(r)], 1u);
-  if (a.ranks)
-    for (uint32_t i = t; i < a.n_adapters; i += 1024) bad |= a.ranks[i] < 0 || a.ranks[i] > (int32_t)a.max_rank;
-  if (bad) *a.err = 2u;
-  __syncthreads();
   for (uint32_t i0 = 0; i0 < N; i0 += 1024) {
-    const uint32_t ad = i0 + t, c = ad < N ? sh[ad] : 0u, it = (c + kLoraM - 1) / kLoraM;
+    const uint32_t ad = i0 + t;
+    uint32_t rank = 0;
+    float scale = 0.f;
+    if (ad < a.n_adapters) {
+      rank = lora_rank(a, ad);
+      scale = a.scale[ad];
+      if (a.ranks) bad |= a.ranks[ad] < 0 || a.ranks[ad] > (int32_t)a.max_rank;
+    }
+    __syncthreads();  // the counts; the bases of the 1024 before
+    const uint32_t c = ad < N ? sh[ad] : 0u, it = (c + kLoraM - 1) / kLoraM;
     const uint32_t pr = lora_scan(c), pi = lora_scan(it);
     if ((t & 63) == 63) wrow[t >> 6] = pr, witem[t >> 6] = pi;
     __syncthreads();
     uint32_t row = base_row + pr - c, item = base_item + pi - it;
     for (uint32_t w = 0; w < (t >> 6); ++w) row += wrow[w], item += witem[w];
     if (ad < N) {
-      sh[ad] = row;
+      sh[ad] = 0;
+      first[ad] = item;
       for (uint32_t j = 0; j < it; ++j)
-        a.items[item + j] = LoraItem{ad, row + j * kLoraM, min(kLoraM, c - j * kLoraM)};
+        a.items[item + j] = LoraItem{ad, row + j * kLoraM, min(kLoraM, c - j * kLoraM), rank, scale};
     }
     __syncthreads();
     if (t == 1023) base_row = row + c, base_item = item + it;
-    __syncthreads();
   }
-  for (uint32_t i = base_item + t; i < a.n_items; i += 1024) a.items[i] = LoraItem{0u, 0u, 0u};
+  __syncthreads();
+  if (bad) *a.err = 2u;
+  for (uint32_t i = base_item + t; i < a.n_items; i += 1024) a.items[i] = LoraItem{0u, 0u, 0u, 0u, 0.f};
   // Which row of an adapter takes which place does not touch any result.
-  for (uint32_t r = t; r < a.n; r += 1024) a.perm[atomicAdd(&sh[adapter(r)], 1u)] = r;
+  for (uint32_t r = t; r < a.n; r += 1024) {
+    const uint32_t ad = adapter(r);
+    a.rows[first[ad] * kLoraM + atomicAdd(&sh[ad], 1u)] = r;
+  }
 }
 
 constexpr uint32_t kLoraSmall = 64;  // rows whose items need no plan: one per lane
@@ -115,6 +127,9 @@ __device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t 
   const int32_t id = lane < a.n ? a.ids[lane] : -2;
   const bool bad = lane < a.n && (id < -1 || id >= (int32_t)a.n_adapters);
   const uint32_t ad = bad || id < 0 ? a.n_adapters : (uint32_t)id;
+  uint32_t rank = 0;  // of the lane's adapter
+  float scale = 0.f;
+  if (ad < a.n_adapters) rank = lora_rank(a, ad), scale = a.scale[ad];
   if (blockIdx.x == 0 && blockIdx.y == 0) {
     bool wrong = bad;
     if (a.ranks)
@@ -123,7 +138,7 @@ __device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t 
   }
   uint64_t left = __ballot(lane < a.n);
   uint32_t item = blockIdx.x, start = 0;
-  LoraItem it{0u, 0u, 0u};
+  LoraItem it{0u, 0u, 0u, 0u, 0.f};
   while (left) {
     const uint32_t leader = (uint32_t)__ffsll((long long)left) - 1;
     const uint32_t mine = (uint32_t)__builtin_amdgcn_readlane((int)ad, (int)leader);
@@ -132,7 +147,8 @@ __device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t 
     if (item < items) {
       const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(group >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)group, 0u));
       if ((group >> lane & 1) && at / kLoraM == item) rows[at % kLoraM] = lane;
-      it = LoraItem{mine, start + item * kLoraM, min(kLoraM, c - item * kLoraM)};
+      it = LoraItem{mine, start + item * kLoraM, min(kLoraM, c - item * kLoraM),
+                    (uint32_t)__builtin_amdgcn_readlane((int)rank, (int)leader), readlane_f(scale, (int)leader)};
       break;
     }
     item -= items;
@@ -144,6 +160,22 @@ __device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t 
   return it;
 }
 
+// The item of this block and row min(c, count - 1) of it.
+template <bool SMALL>
+__device__ __forceinline__ LoraItem lora_item(const LoraArgs& a, uint32_t lane, uint32_t* rows, uint32_t& row) {
+  if constexpr (SMALL) {
+    const LoraItem it = lora_small_item(a, lane, rows);
+    row = it.count ? rows[min(lane & 15, it.count - 1)] : 0u;
+    return it;
+  } else {
+    const LoraItem it = a.items[blockIdx.x];
+    const uint32_t r = a.rows[blockIdx.x * kLoraM + (lane & 15)];  // unset past the count: replaced
+    const uint32_t last = (uint32_t)__shfl((int)r, (int)(it.count ? it.count - 1 : 0u), kWave);
+    row = (lane & 15) < it.count ? r : last;
+    return it;
+  }
+}
+
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c.
 template <bool XBF16, bool SMALL, int MT>
@@ -151,11 +183,11 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   __shared__ f32x4 red[4][64];
   __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
-  const LoraItem it = SMALL ? lora_small_item(a, lane, rows[wave]) : a.items[blockIdx.x];
+  uint32_t row;
+  const LoraItem it = lora_item<SMALL>(a, lane, rows[wave], row);
   if (it.count == 0 || it.adapter >= a.n_adapters) return;
   const uint32_t K = a.in_dim, share = blockIdx.y;
-  const uint32_t rank = lora_rank(a, it.adapter), nt = (rank + 15) / 16;
-  const uint32_t row = SMALL ? rows[wave][min(c16, it.count - 1)] : a.perm[it.start + min(c16, it.count - 1)];
+  const uint32_t rank = it.rank, nt = (rank + 15) / 16;
   const uint16_t* const A = (const uint16_t*)(a.a + (uint64_t)it.adapter * a.a_stride);
   const uint32_t steps = (K + 31) / 32, s0 = steps * share / a.shares, s1 = steps * (share + 1) / a.shares;
   f32x4 acc[MT];
@@ -228,14 +260,14 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
   __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
-  const LoraItem it = SMALL ? lora_small_item(a, lane, rows[wave]) : a.items[blockIdx.x];
+  uint32_t row;
+  const LoraItem it = lora_item<SMALL>(a, lane, rows[wave], row);
   if (it.count == 0) return;
   const uint32_t O = a.out_dim, R = a.max_rank;
-  const uint32_t row = SMALL ? rows[wave][min(c16, it.count - 1)] : a.perm[it.start + min(c16, it.count - 1)];
   const uint32_t o0 = (blockIdx.y * 4 + wave) * NT * 16;
   const bool none = it.adapter >= a.n_adapters;
   if (none && a.base == a.y) return;
-  const uint32_t rank = none ? 0u : lora_rank(a, it.adapter);
+  const uint32_t rank = none ? 0u : it.rank;
   lbf16x8 w[KT][NT];
   if (rank) {
     const uint16_t* const B = (const uint16_t*)(a.b + (uint64_t)it.adapter * a.b_stride);
@@ -267,7 +299,7 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) low[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (rank) {  // the same for the whole block
-    const float scale = a.scale[it.adapter];
+    const float scale = it.scale;
     const uint32_t q = R / 4;  // quarters of eights: a thread adds four values
     for (uint32_t i = threadIdx.x; i < kLoraM * KT * 8; i += 256) {
       const uint32_t r = i / (KT * 8), k = i % (KT * 8) * 4;
@@ -347,12 +379,12 @@ uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, Lora
   const uint32_t shares = lora_shares(n);
   // Every adapter in use leaves at most one item short of 16 rows.
   const uint32_t items = n / kLoraM + (n < n_adapters + 1 ? n : n_adapters + 1);
-  const uint64_t ib = al256((uint64_t)items * sizeof(LoraItem)), pb = al256((uint64_t)n * 4);
+  const uint64_t ib = al256((uint64_t)items * sizeof(LoraItem)), pb = al256((uint64_t)items * kLoraM * 4);
   if (a) {
     a->n_items = items;
     a->shares = shares;
     a->items = reinterpret_cast<LoraItem*>(base);
-    a->perm = reinterpret_cast<uint32_t*>(base + ib);
+    a->rows = reinterpret_cast<uint32_t*>(base + ib);
     a->u = reinterpret_cast<float*>(base + ib + pb);
   }
   return ib + pb + al256((uint64_t)shares * n * max_rank * 4);
@@ -387,7 +419,7 @@ static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
 
 hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
   if (a.n <= kLoraSmall) return lora_go<true>(a, x_bf16, st);
-  hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 4, st, a);
+  hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 8, st, a);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess ? e : lora_go<false>(a, x_bf16, st);
 }
