@@ -253,11 +253,15 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
 // A block takes 64 NT outputs of an item; it adds the shares once, into LDS, as
 // the bf16 pairs that its waves read as operands (added by every wave for
 // itself the shares were 22 of 33 us: 200 rows, 40 adapters of rank 64, 4096 ->
-// 4096). B's and base's loads go out ahead of that.
+// 4096). The products go through LDS too, so that base and y move in whole rows
+// of the block (in the products' order each lane touches a line of its own).
+// B's and base's loads go out ahead of everything.
 template <bool SMALL, int KT, int NT>
 __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   constexpr uint32_t RP = KT * 32 + 8;  // bf16 per row in LDS: rows apart by 16 bytes of banks
+  constexpr uint32_t OB = 64 * NT, OP = OB + 4;  // outputs of the block; floats per row in LDS, apart by 16 bytes of banks
   __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
+  __shared__ __attribute__((aligned(16))) float prod[kLoraM * OP];
   __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
   uint32_t row;
@@ -280,19 +284,27 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
           w[s][i] = *reinterpret_cast<const lbf16x8*>(B + (uint64_t)min(o0 + i * 16 + c16, O - 1) * R + (k < R ? k : 0));  // R is a multiple of 8
     }
   }
+  // Fours of outputs of whole rows: thread i's are i, i + 256, ..
+  const uint32_t ob = blockIdx.y * OB;
+  auto place = [&](int i, uint32_t& r, uint32_t& o) {
+    const uint32_t f = threadIdx.x + 256 * i;
+    r = f / (OB / 4);
+    o = f % (OB / 4) * 4;
+    return (uint64_t)(uint32_t)__shfl((int)row, (int)r, kWave) * O + ob + o;
+  };
   f32x4 acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint32_t o = o0 + i * 16 + 4 * kb;
-    const uint64_t e = (uint64_t)row * O + o;
-    if (!a.base || c16 >= it.count) continue;
+    uint32_t r, o;
+    const uint64_t e = place(i, r, o);
+    if (!a.base || r >= it.count) continue;
     if (a.vec) {
-      if (o < O) acc[i] = *reinterpret_cast<const f32x4*>(a.base + e);
+      if (ob + o < O) acc[i] = *reinterpret_cast<const f32x4*>(a.base + e);
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (o + r < O) acc[i][r] = a.base[e + r];
+      for (int c = 0; c < 4; ++c)
+        if (ob + o + c < O) acc[i][c] = a.base[e + c];
     }
   }
   f32x4 low[NT];
@@ -350,18 +362,24 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
       }
     }
   }
-  if (c16 >= it.count) return;
+  if (rank) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4*>(prod + c16 * OP + (wave * NT + i) * 16 + 4 * kb) = low[i];
+    __syncthreads();
+  }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    const uint32_t o = o0 + i * 16 + 4 * kb;
-    const uint64_t e = (uint64_t)row * O + o;
-    const f32x4 v = acc[i] + low[i];
+    uint32_t r, o;
+    const uint64_t e = place(i, r, o);
+    if (r >= it.count) continue;
+    f32x4 v = acc[i];
+    if (rank) v += *reinterpret_cast<const f32x4*>(prod + r * OP + o);
     if (a.vec) {
-      if (o < O) *reinterpret_cast<f32x4*>(a.y + e) = v;
+      if (ob + o < O) *reinterpret_cast<f32x4*>(a.y + e) = v;
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (o + r < O) a.y[e + r] = v[r];
+      for (int c = 0; c < 4; ++c)
+        if (ob + o + c < O) a.y[e + c] = v[c];
     }
   }
 }
