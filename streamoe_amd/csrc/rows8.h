@@ -308,13 +308,14 @@ __device__ __forceinline__ qbf16x8 q8_parts(float a, float b) {
 // ---------------------------------------------------------------------------
 // Few rows, many columns: the rows stay in LDS, as operands, and the waves
 // stream the weights, a tile of 16 columns at a time over all inputs, four
-// steps ahead. A wave's load of a step is made in memory order (lane 4 r + p:
-// part p of row r, one cache access per four lanes instead of one per lane) and
-// a lane permute brings the parts to the operand's lanes. The loads are
-// temporal: a step takes half of a row's line, the next step the other half
-// (non-temporal: 16 rows 2048 -> 151936 in 47 us instead of 35). Rows are the A
-// operand: lane (c, kb) ends with column c of rows 4 kb .. 4 kb + 3, and needs
-// the scales of one column only.
+// steps ahead. A wave's load takes four rows' codes of those steps, whole lines
+// (256 bytes a row with 4 bits), and its own part of LDS hands them to the
+// operands' lanes. The loads are non-temporal: weights that a step reads once
+// come from HBM (16 rows 2048 -> 151936, three sets of weights in turn: 42 us,
+// 4.4 TB/s, temporal 45; the same set again and again 41 and, from the
+// memory-side cache, 35); without the arithmetic, temporal, 43.5. Rows
+// are the A operand: lane (c, kb) ends with column c of rows 4 kb .. 4 kb + 3,
+// and needs the scales of one column only.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kWideSteps = 4;  // per round of loads
 
@@ -332,10 +333,19 @@ __device__ __forceinline__ uint32_t q8_slot(uint32_t p, uint32_t e, uint32_t row
 __host__ __device__ constexpr uint32_t q8_wide_steps(uint32_t K) {
   return (K + kWideSteps * kQ8Step - 1) / (kWideSteps * kQ8Step) * kWideSteps;
 }
-// LDS: operands, the bias term's operands per eight groups, the rows' scales.
-__host__ __device__ constexpr uint32_t q8_wide_lds(uint32_t K, uint32_t G, uint32_t mt, bool xg) {
+// LDS: operands, the bias term's operands per eight groups, the rows' scales,
+// each wave's 16 x 16 chunks of a round.
+__host__ __device__ constexpr uint32_t q8_wide_lds(uint32_t bits, uint32_t K, uint32_t G, uint32_t mt, bool xg) {
   const uint32_t steps = q8_wide_steps(K), groups = steps * (kQ8Step / G);
-  return mt * (steps * 2048 + (groups + 7) / 8 * 1024 + (xg ? groups * 64 : 0));
+  return mt * (steps * 2048 + (groups + 7) / 8 * 1024 + (xg ? groups * 64 : 0)) + 4 * 256 * (bits == 8 ? 32 : 16);
+}
+
+// Orders a wave's own LDS traffic (which the hardware runs in order) for the
+// compiler.
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 template <int BITS, int G, bool XG, int MT>
@@ -350,25 +360,29 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
   u32x4* const xl = reinterpret_cast<u32x4*>(lds_raw);                 // [step][m][h][64]
   u32x4* const parts = xl + steps * MT * 128;                          // [octet][m][64]
   float* const sxl = reinterpret_cast<float*>(parts + octets * MT * 64);  // [group][m][16]
+  // The wave's chunks of a round: chunk p of row r at place 16 r + (p ^ r), so
+  // that the rows' reads of one chunk fall in different banks.
+  constexpr uint32_t CW = BITS == 8 ? 2 : 1;  // 16-byte words per chunk
+  u32x4* const mine = reinterpret_cast<u32x4*>(sxl + (XG ? groups * MT * 16 : 0)) + wave * 256 * CW;
 
-  // The loads of a round, in memory order: part lp of row lr of the tile.
-  const uint32_t lr = lane >> 2, lp = lane & 3;
+  // The loads of a round: chunk lp of rows lr, lr + 4, .. of the tile.
+  const uint32_t lr = lane >> 4, lp = lane & 15;
   struct Round {
     uint32_t w[kWideSteps][W];
     uint32_t s[PW], b[PW];
   };
   auto load = [&](uint32_t tile, uint32_t rd, Round& v) {
-    const uint32_t row = min(tile * 16 + lr, O - 1), col = min(tile * 16 + c16, O - 1);
-    const uint8_t* const w = a.w + (uint64_t)row * row_bytes;
+    const uint32_t col = min(tile * 16 + c16, O - 1);
+    const uint32_t chunk = min(rd * kWideSteps * 4 + lp, K / 32 - 1) * (BITS * 4);
 #pragma unroll
     for (uint32_t i = 0; i < kWideSteps; ++i) {
-      const uint8_t* const p = w + min((rd * kWideSteps + i) * 4 + lp, K / 32 - 1) * (BITS * 4);
+      const uint8_t* const p = a.w + (uint64_t)min(tile * 16 + 4 * i + lr, O - 1) * row_bytes + chunk;
       if constexpr (BITS == 8) {
-        const u32x4 lo = ld_w<false>(reinterpret_cast<const u32x4*>(p)), hi = ld_w<false>(reinterpret_cast<const u32x4*>(p + 16));
+        const u32x4 lo = ld_w<true>(reinterpret_cast<const u32x4*>(p)), hi = ld_w<true>(reinterpret_cast<const u32x4*>(p + 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) v.w[i][j] = lo[j], v.w[i][4 + j] = hi[j];
       } else {
-        const Raw<BITS> r = load_raw<BITS, false>(p);
+        const Raw<BITS> r = load_raw<BITS, true>(p);
 #pragma unroll
         for (int j = 0; j < BITS; ++j) v.w[i][j] = r.d[j];
       }
@@ -446,9 +460,21 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
   for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int kStart = XG ? (int)kMagicBits : 0;
   const i32x4 start = {kStart, kStart, kStart, kStart};
-  const int psrc = (int)((c16 * 4 + kb) * 4);
   auto from = [&](int src, uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)x); };
   auto compute = [&](uint32_t rd, const Round& v) {
+    static_assert(kWideSteps == 4, "16 chunks of a row, four rows per load");
+    wave_lds();  // the last round's reads come first
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t r = 4 * i + lr;
+#pragma unroll
+      for (uint32_t c = 0; c < CW; ++c) {
+        u32x4 q = {v.w[i][4 * c], v.w[i][4 * c + 1], v.w[i][4 * c + 2], 0u};
+        if (BITS != 3) q.w = v.w[i][(4 * c + 3) % W];
+        mine[(r * 16 + (lp ^ r)) * CW + c] = q;
+      }
+    }
+    wave_lds();
     // The bias term of this round's eights (G = 128: a round is half of one).
 #pragma unroll
     for (uint32_t i = 0; i < PW; ++i) {
@@ -476,7 +502,12 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
     for (uint32_t i = 0; i < kWideSteps; ++i) {
       uint32_t d[W];
 #pragma unroll
-      for (uint32_t j = 0; j < W; ++j) d[j] = from(psrc, v.w[i][j]);
+      for (uint32_t c = 0; c < CW; ++c) {
+        const u32x4 q = mine[(c16 * 16 + ((i * 4 + kb) ^ c16)) * CW + c];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          if (4 * c + j < W) d[4 * c + j] = q[j];
+      }
       u32x4 w[2];
       q8_operands<BITS, G>(d, w);
       const uint32_t st = rd * kWideSteps + i;
@@ -947,7 +978,7 @@ static hipError_t q8_few(const Q8Args& a, uint32_t waves, hipStream_t st) {
 
 template <int BITS, int G, bool XG, int MT>
 static hipError_t q8_wide(const Q8Args& a, hipStream_t st) {
-  const uint32_t lds = q8_wide_lds(a.K, G, MT, XG), tiles = (a.O + 15) / 16;
+  const uint32_t lds = q8_wide_lds(BITS, a.K, G, MT, XG), tiles = (a.O + 15) / 16;
   auto fn = k_q8_wide<BITS, G, XG, MT>;
   if (lds > 64 * 1024) {
     static std::atomic<uint64_t> raised{0};
@@ -979,7 +1010,7 @@ static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   if (rt * ct <= 256) return q8_few<BITS, G, XG, 1, 1>(a, std::min(steps, 16u), st);
   if (rt == 1) {
     // 16 rows 2048 -> 16384: 8.6, rows in LDS 10.3; -> 50000: 39 and 18.
-    if (ct <= 1024 || q8_wide_lds(a.K, G, 1, XG) > 160 * 1024)
+    if (ct <= 1024 || q8_wide_lds(BITS, a.K, G, 1, XG) > 160 * 1024)
       return q8_few<BITS, G, XG, 1, 2>(a, std::min(steps, 8u), st);
     return q8_wide<BITS, G, XG, 1>(a, st);
   }
