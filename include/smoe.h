@@ -516,7 +516,8 @@ int smoe_moe_prefill_block(smoe_handle* h, const smoe_expert_shape* shape, const
  * out_scales: device f32[n_tokens, hidden / q_group], with out_q. All 16-byte
  * aligned. sum_out or out may be the buffer of x or residual where the types
  * are the same; else outputs overlap nothing. hidden 1..16384 (a multiple of
- * q_group), else SMOE_ERR_UNSUPPORTED_SHAPE (SMOE_ERR_IN_DIM_NOT_MULTIPLE).
+ * q_group), n_tokens below 2^24, else SMOE_ERR_UNSUPPORTED_SHAPE
+ * (SMOE_ERR_IN_DIM_NOT_MULTIPLE).
  * Enqueue-only, allocates nothing, capturable in a HIP graph. */
 int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* residual, const void* norm_w,
                  float eps, uint32_t n_tokens, uint32_t hidden, float* sum_out, void* out, int out_is_bf16,
@@ -526,11 +527,13 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
  * for x[t, c] * x_scales[t, c / x_group] (one scale per row with x_group 0:
  * x_scales[t]), as smoe_rmsnorm writes them; smoe_qmm's product with a quarter
  * of its matrix work, on int8 MFMA. Group sums of code times code are exact,
- * everything else f32. x: device int8[n_tokens, in_dim], 16-byte aligned, any
+ * everything else f32 (products of many rows round x_scales per group to 22
+ * bits, by 2^-23; a row's last bits may depend on n_tokens). x: device int8[n_tokens, in_dim], 16-byte aligned, any
  * codes; x_scales: device f32[n_tokens, in_dim / x_group] or [n_tokens]; y:
  * device f32. Weights of bits 4, 3 or 8, group 32, 64 or 128, in_dim a
- * multiple of the group up to 16384; x_group 0 or the weights' group
- * (SMOE_ERR_UNSUPPORTED_GROUP). A row with a scale that is infinite or NaN
+ * multiple of the group up to 16384, out_dim up to 2^28, n_tokens up to
+ * 1048560 (SMOE_ERR_UNSUPPORTED_SHAPE); x_group 0 or the weights' group
+ * (SMOE_ERR_UNSUPPORTED_GROUP). y overlaps nothing. A row with a scale that is infinite or NaN
  * gives infinities or NaN in that row only. Enqueue-only, allocates nothing,
  * needs no workspace, capturable in a HIP graph. No counterpart in the
  * reference, whose activations stay f32. */
@@ -564,10 +567,11 @@ uint64_t smoe_lora_workspace_size(const smoe_adapters* adapters, uint32_t n_toke
  * ids: device int32[n_tokens], in any order; x: device [n_tokens, in_dim],
  * bf16 when x_is_bf16 else f32; base: device f32[n_tokens, out_dim] or NULL
  * (zeros), may be y; y: device f32[n_tokens, out_dim]. x, a, b 16-byte
- * aligned, in_dim a multiple of 8; out_dim any (multiples of 4 with y and base
- * on 16 bytes are the fast case). On bf16 MFMA with f32 sums; f32 x and the
+ * aligned, in_dim a multiple of 8; out_dim up to 4194240 (multiples of 4 with y
+ * and base on 16 bytes are the fast case); y overlaps nothing but base. On bf16 MFMA with f32 sums; f32 x and the
  * low-rank values between the products enter as bf16 pairs (off by at most
- * 2^-16 of each value); a row with an infinity or NaN gives NaN. An id or a
+ * 2^-16 of each value); a row with an infinity, a NaN or an f32 that bf16
+ * rounds to infinity gives NaN. An id or a
  * rank out of range is found on the device: the next smoe_sync returns
  * SMOE_ERR_INVALID_ARG, the row's y is base (the rank is clamped). n_tokens up
  * to 65536, in_dim up to 65536, else SMOE_ERR_UNSUPPORTED_SHAPE. workspace:
@@ -602,7 +606,8 @@ uint64_t smoe_beam_select_workspace_size(uint32_t n_requests, uint32_t n_beams, 
  * smoe_beam_reorder takes); out_tokens: device int32. out_scores may be
  * scores when n_picks == n_beams; nothing else overlaps. workspace: device, of
  * smoe_beam_select_workspace_size bytes, 256-byte aligned, one call's at a
- * time. n_beams 1..16, vocab up to 2^28 (SMOE_ERR_UNSUPPORTED_SHAPE); n_picks
+ * time. n_beams 1..16, vocab up to 2^28, n_requests * n_beams up to 262143
+ * (SMOE_ERR_UNSUPPORTED_SHAPE); n_picks
  * 1..32 and at most n_beams * vocab (SMOE_ERR_BAD_K). No counterpart in the
  * reference, whose sampling is greedy (io/gpu_lm_head.rs:130-193). The same
  * bits on every run. Enqueue-only, allocates nothing, capturable in a HIP
@@ -635,7 +640,8 @@ typedef struct {
  * SMOE_ERR_INVALID_ARG. src and dst of a state must not overlap, nor rows or
  * pieces of dst (SMOE_ERR_INVALID_ARG); a state's dst must not overlap
  * another state. Addresses and strides of any alignment (16 bytes are the
- * fast case). Enqueue-only, allocates nothing, capturable in a HIP graph. */
+ * fast case). Pieces of all rows below 2^24 in a state, longer pieces counted
+ * per 16 KiB (SMOE_ERR_UNSUPPORTED_SHAPE). Enqueue-only, allocates nothing, capturable in a HIP graph. */
 int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_states, const int32_t* rows,
                       uint32_t n_rows, uint32_t src_rows);
 

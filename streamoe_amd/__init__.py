@@ -53,7 +53,12 @@ def _types(name):
 
 def _fits(t, types, n, device):
     """Whether a call may take at least n elements of `types` from t: dense, on `device`."""
-    return t.dtype in types and t.numel() >= n and t.is_contiguous() and t.get_device() == device
+    return t is not None and t.dtype in types and t.numel() >= n and t.is_contiguous() and t.get_device() == device
+
+
+def _view(t):
+    """What a checked struct of a tensor holds for."""
+    return None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype)
 
 
 def _at(t):
@@ -143,15 +148,15 @@ class Adapters:
 
     def c(self):
         """The C struct, checked when it is first asked for and again whenever
-        one of the tensors lies elsewhere than then."""
-        at = (self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), _at(self.ranks))
+        one of the tensors lies elsewhere or in another way than then."""
+        views = (_view(self.a), _view(self.b), _view(self.scale), _view(self.ranks))
         known = self.__dict__.get("_known")
-        if known is None or known[0] != at:
-            known = (at, self._struct(at))
+        if known is None or known[0] != views:
+            known = (views, self._struct())
             object.__setattr__(self, "_known", known)
         return known[1]
 
-    def _struct(self, at):
+    def _struct(self):
         a, b, bf16 = self.a, self.b, _types("bf16")
         dev = a.get_device()
         if (a.dim() != 3 or b.dim() != 3 or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1] or not a.numel()
@@ -161,7 +166,8 @@ class Adapters:
             raise SmoeError(_INVALID, "Adapters")
         # A lone adapter's stride says nothing: its size.
         step = lambda t: (t.stride(0) if t.shape[0] > 1 else t[0].numel()) * 2
-        return _abi.AdaptersC(at[0], at[1], step(a), step(b), at[2], at[3], a.shape[0], a.shape[1])
+        return _abi.AdaptersC(a.data_ptr(), b.data_ptr(), step(a), step(b), self.scale.data_ptr(), _at(self.ranks),
+                              a.shape[0], a.shape[1])
 
 
 @dataclass(frozen=True, eq=False)
@@ -177,15 +183,16 @@ class BeamState:
 
     def c(self):
         """(the C struct's bytes, rows of src, rows of dst, device), checked when
-        first asked for and again whenever one of the tensors lies elsewhere."""
-        at = (self.src.data_ptr(), self.dst.data_ptr())
+        first asked for and again whenever one of the tensors lies elsewhere or
+        in another way."""
+        views = (_view(self.src), _view(self.dst))
         known = self.__dict__.get("_known")
-        if known is None or known[0] != at:
-            known = (at, self._struct(at))
+        if known is None or known[0] != views:
+            known = (views, self._struct())
             object.__setattr__(self, "_known", known)
         return known[1]
 
-    def _struct(self, at):
+    def _struct(self):
         s, d = self.src, self.dst
         if (s.device != d.device or s.device.type != "cuda" or s.dtype != d.dtype or s.dim() not in (2, 3)
                 or s.shape[1:] != d.shape[1:] or s.stride(-1) != 1 or d.stride(-1) != 1):
@@ -197,7 +204,7 @@ class BeamState:
         if not 0 <= used <= room:
             raise SmoeError(_INVALID, "BeamState: used")
         piece = (lambda t: t.stride(1) * size) if s.dim() == 3 else (lambda t: 0)
-        raw = _abi.BeamStateC(*at, s.stride(0) * size, d.stride(0) * size, piece(s), piece(d), used, pieces, 0)
+        raw = _abi.BeamStateC(s.data_ptr(), d.data_ptr(), s.stride(0) * size, d.stride(0) * size, piece(s), piece(d), used, pieces, 0)
         return bytes(raw), s.shape[0], d.shape[0], s.get_device()
 
 
@@ -403,7 +410,7 @@ class Kernels:
         one scale per row). x: f32 or bf16 rows."""
         n, dev, f32 = n_tokens * hidden, self.device, _types("f32")
         either, bf16 = _types("f32_bf16"), _types("bf16")
-        if not (x is not None and _fits(x, either, n, dev) and (residual is None or _fits(residual, f32, n, dev))
+        if not (_fits(x, either, n, dev) and (residual is None or _fits(residual, f32, n, dev))
                 and (norm_w is None or _fits(norm_w, bf16, hidden, dev))
                 and (sum_out is None or _fits(sum_out, f32, n, dev)) and (out is None or _fits(out, either, n, dev))
                 and (out_q is None or _fits(out_q, _types("i8"), n, dev))

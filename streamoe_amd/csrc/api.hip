@@ -949,7 +949,7 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
     if (int rc = check_group(q_group)) return rc;
     if (hidden % q_group) return SMOE_ERR_IN_DIM_NOT_MULTIPLE;
   }
-  if (hidden > kNormMaxHidden || n_tokens > 0x7FFFFFFFu) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (hidden > kNormMaxHidden || n_tokens > kMaxBlocks) return SMOE_ERR_UNSUPPORTED_SHAPE;
   for (const void* p : {x, (const void*)residual, norm_w, (const void*)sum_out, (const void*)out, (const void*)out_q,
                         (const void*)out_scales})
     if (!aligned(p, 0, 16)) return SMOE_ERR_MISALIGNED;
@@ -975,7 +975,7 @@ int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const f
   QView v;
   if (int rc = qview(w, in_dim, &v, true)) return rc;
   if (x_group && x_group != v.group) return SMOE_ERR_UNSUPPORTED_GROUP;
-  if (in_dim > kQ8MaxIn || out_dim > 0x7FFFFF00u || n_tokens > 65535u * 16) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (in_dim > kQ8MaxIn || out_dim > kQ8MaxOut || n_tokens > 65535u * 16) return SMOE_ERR_UNSUPPORTED_SHAPE;
   if (!aligned(x, 0, 16) || !aligned(x_scales, 0, 4) || !aligned(y, 0, 4)) return SMOE_ERR_MISALIGNED;
   if (int rc = use_device(h)) return rc;
   Q8Args a{};
@@ -1015,7 +1015,7 @@ int smoe_lora(smoe_handle* h, const smoe_adapters* adapters, const int32_t* ids,
   if (int rc = check_adapters(adapters, n_tokens)) return rc;
   const smoe_adapters& s = *adapters;
   if (!s.a || !s.b || !s.scale) return SMOE_ERR_INVALID_ARG;
-  if (in_dim % 8 || in_dim > kLoraMaxIn || out_dim > 0x7FFFFF00u) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (in_dim % 8 || in_dim > kLoraMaxIn || out_dim > kLoraMaxOut) return SMOE_ERR_UNSUPPORTED_SHAPE;
   if (s.a_stride < (uint64_t)s.max_rank * in_dim * 2 || s.b_stride < (uint64_t)s.max_rank * out_dim * 2)
     return SMOE_ERR_INVALID_ARG;
   if (!aligned(s.a, 0, 16) || !aligned(s.b, 0, 16) || s.a_stride % 16 || s.b_stride % 16 || !aligned(x, 0, 16) ||
@@ -1051,7 +1051,7 @@ static int check_beam(uint32_t n_requests, uint32_t n_beams, uint32_t vocab, uin
   if (n_beams > kBeamMaxBeams || vocab > kBeamMaxVocab) return SMOE_ERR_UNSUPPORTED_SHAPE;
   if (n_picks < 1 || n_picks > kBeamMaxPicks || n_picks > (uint64_t)n_beams * vocab) return SMOE_ERR_BAD_K;
   // One block per row and slice.
-  if ((uint64_t)n_requests * n_beams * kBeamMaxSlices > 0x7FFFFFFFull) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if ((uint64_t)n_requests * n_beams > kMaxBlocks / kBeamMaxSlices) return SMOE_ERR_UNSUPPORTED_SHAPE;
   return SMOE_OK;
 }
 
@@ -1134,7 +1134,7 @@ int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_
         const bool by_piece = (s.n_pieces == 1 || s.dst_piece_stride >= col) &&
                               (n_rows == 1 || s.dst_row_stride >= s.piece_bytes);
         if (!by_row && !by_piece) return SMOE_ERR_INVALID_ARG;
-        if ((unsigned __int128)((s.piece_bytes >> 14) + 1) * s.n_pieces * n_rows > kBeamCopyMaxBlocks)
+        if ((unsigned __int128)((s.piece_bytes >> 14) + 1) * s.n_pieces * n_rows > kMaxBlocks)
           return SMOE_ERR_UNSUPPORTED_SHAPE;
       }
       if (pass) {

@@ -442,7 +442,7 @@ hipError_t launch_beam_copy(const BeamCopy* states, uint32_t n, const int32_t* r
     for (; i < n && a.n < kCopyStates; ++i) {
       const uint64_t b = beam_copy_blocks(states[i], n_rows);
       if (b == 0) continue;
-      if (a.n && blocks + b > kBeamCopyMaxBlocks) break;
+      if (a.n && blocks + b > kMaxBlocks) break;
       a.s[a.n] = states[i];
       a.end[a.n++] = blocks += b;
     }

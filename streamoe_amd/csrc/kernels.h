@@ -290,6 +290,8 @@ hipError_t launch_ph_down(const BlobGeom& routed, const BlobGeom& shared, const 
                           const float* shared_out, float* hidden_out, hipStream_t st, bool ordered = false,
                           uint32_t n_tokens = 1, uint32_t astride = 0);
 // Residual addition + RMSNorm + 8-bit rows (norm.hip); row t at + t hidden.
+// A launch holds fewer than 2^32 threads in x: blocks of 256 in one.
+constexpr uint64_t kMaxBlocks = (1u << 24) - 1;
 constexpr uint32_t kNormMaxHidden = 16384;  // 64 values per thread
 struct NormArgs {
   const void* x;          // [n, hidden] f32 or bf16
@@ -306,7 +308,7 @@ struct NormArgs {
 };
 hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
 // Quantized products of 8-bit rows (rows8.h), by the weights' bits.
-constexpr uint32_t kQ8MaxIn = 16384;
+constexpr uint32_t kQ8MaxIn = 16384, kQ8MaxOut = 1u << 28;
 struct Q8Args {
   const uint8_t* w;        // codes [O, K]
   const uint16_t *s, *b;   // bf16 [O, K / group]
@@ -323,6 +325,7 @@ hipError_t launch_qmm_i8_q4(const Q8Args& a, uint32_t group, bool x_grouped, hip
 hipError_t launch_qmm_i8_q8(const Q8Args& a, uint32_t group, bool x_grouped, hipStream_t st);
 // Low-rank adapters (lora.hip).
 constexpr uint32_t kLoraMaxRank = 128, kLoraMaxAdapters = 4096, kLoraMaxTokens = 65536, kLoraMaxIn = 65536;
+constexpr uint32_t kLoraMaxOut = 65535 * 64;  // blocks in y
 struct LoraItem {
   uint32_t adapter, start, count, rank;  // up to 16 rows of one adapter (n_adapters: none); start: rows before them
   float scale;
@@ -377,7 +380,6 @@ struct BeamCopy {
   uint64_t src_row, dst_row, src_piece, dst_piece, bytes;  // strides in bytes
   uint32_t pieces, unit;                                   // unit: 16, 4 or 1, what addresses and strides divide by
 };
-constexpr uint64_t kBeamCopyMaxBlocks = 1u << 30;  // per launch
 uint64_t beam_copy_blocks(const BeamCopy& s, uint32_t n_rows);
 hipError_t launch_beam_copy(const BeamCopy* states, uint32_t n, const int32_t* rows, uint32_t n_rows,
                             uint32_t src_rows, uint32_t* err, hipStream_t st);

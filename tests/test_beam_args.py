@@ -30,6 +30,7 @@ def _select(**kw):
     (dict(n_picks=33), "BAD_K"),
     (dict(n_picks=9, vocab=2), "BAD_K"),               # more than there are continuations
     (dict(n_requests=1 << 26), "UNSUPPORTED_SHAPE"),
+    (dict(n_requests=262144), "UNSUPPORTED_SHAPE"),
     (dict(done=24576, pad_token=100), "INVALID_ARG"),
     (dict(out_scores=8192), "INVALID_ARG"),            # in place with more picks than beams
     (dict(logits=4100), "MISALIGNED"),
@@ -79,6 +80,8 @@ def _reorder(each=None, n=None, **kw):
     ([dict(dst_piece_stride=99)], {}, "INVALID_ARG"),
     ([dict(src_row_stride=1 << 63)], {}, "INVALID_ARG"),
     ([dict(piece_bytes=1 << 46, dst=1 << 60, n_pieces=1, dst_row_stride=1 << 46)], {}, "UNSUPPORTED_SHAPE"),
+    ([dict(n_pieces=1 << 24, piece_bytes=1, src_piece_stride=1, dst_piece_stride=1, dst_row_stride=1 << 24, dst=1 << 60)], {},
+     "UNSUPPORTED_SHAPE"),
     ([{}] * 70 + [dict(n_pieces=0)], {}, "INVALID_ARG"),                  # past the first batch of states
 ])
 def test_reorder_refusals(states, kw, code):

@@ -43,6 +43,7 @@ def _call(over=None, **kw):
     ({}, dict(n_tokens=65537), "UNSUPPORTED_SHAPE"),
     ({}, dict(in_dim=252), "UNSUPPORTED_SHAPE"),
     ({}, dict(in_dim=65544), "UNSUPPORTED_SHAPE"),
+    (dict(b_stride=4194304 * 32), dict(out_dim=4194304), "UNSUPPORTED_SHAPE"),
     (dict(a=(1 << 20) + 8), {}, "MISALIGNED"),
     (dict(b=(1 << 24) + 2), {}, "MISALIGNED"),
     (dict(a_stride=16 * 256 * 2 + 2), {}, "MISALIGNED"),
@@ -64,3 +65,20 @@ def test_workspace_size():
     size = lambda n, **kw: _abi.load().smoe_lora_workspace_size(C.byref(_abi.AdaptersC(*dict(SET, **kw).values())), n)
     assert size(5) > 0 and size(1000) > size(5)
     assert size(0) == 0 and size(5, max_rank=12) == 0 and size(65537) == 0
+
+
+def test_struct_follows_its_tensors():
+    """Tensors that change in place, at the same address, are checked again."""
+    import torch
+
+    import streamoe_amd as sa
+
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    s = sa.Adapters(z(3, 16, 32), z(3, 48, 16), torch.ones(3))
+    assert (s.c().max_rank, s.c().a_stride, s.c().b_stride) == (16, 1024, 1536)
+    s.a.resize_(3, 8, 32)
+    s.b.resize_(3, 48, 8)
+    assert (s.c().max_rank, s.c().a_stride, s.c().b_stride) == (8, 512, 768)
+    s.a.resize_(3, 16, 16)
+    with pytest.raises(sa.SmoeError):
+        s.c()

@@ -27,6 +27,7 @@ def _call(**kw):
     (dict(out_q=16384, out_scales=32768, q_group=16), "UNSUPPORTED_GROUP"),
     (dict(out_q=16384, out_scales=32768, q_group=64, hidden=96), "IN_DIM_NOT_MULTIPLE"),
     (dict(hidden=16385), "UNSUPPORTED_SHAPE"),
+    (dict(n_tokens=1 << 24), "UNSUPPORTED_SHAPE"),
     (dict(x=4100), "MISALIGNED"),
     (dict(residual=8200), "MISALIGNED"),
     (dict(norm_w=8194), "MISALIGNED"),

@@ -34,6 +34,7 @@ def _call(over=None, **kw):
     ({}, dict(in_dim=288), "IN_DIM_NOT_MULTIPLE"),
     ({}, dict(in_dim=16448), "UNSUPPORTED_SHAPE"),
     ({}, dict(n_tokens=65535 * 16 + 1), "UNSUPPORTED_SHAPE"),
+    ({}, dict(out_dim=(1 << 28) + 1), "UNSUPPORTED_SHAPE"),
     (dict(packed_offset=8), {}, "MISALIGNED"),
     (dict(scales_offset=1), {}, "MISALIGNED"),
     ({}, dict(x=(1 << 24) + 8), "MISALIGNED"),
