@@ -13,6 +13,11 @@ follow the reference:
 * ``ExpertFiles``, ``layout_and_stride``, ``declared_stride``
                         crates/streammoe/src/riir/io/expert_io.rs:229-420 (resident layers)
 
+Beside that path, the operators of a serving step over many requests:
+``Kernels.rmsnorm`` (with 8-bit rows), ``Kernels.qmm_i8`` (products of
+those), ``Adapters`` and ``Kernels.lora``, ``Kernels.beam_select``,
+``BeamState`` and ``Kernels.beam_reorder``.
+
 Device buffers are torch tensors on ``cuda`` (PyTorch is only the
 allocator and stream provider here). Every call goes through libsmoe;
 nothing falls back to a CPU path: importing this package without the

@@ -180,6 +180,17 @@ impl Kernels {
         unsafe { sys::smoe_moe_prefill_block_workspace_size(&s, n_tokens, n_experts, k, has_shared as c_int) }
     }
 
+    /// Device workspace bytes a [`LoraCall`] needs (0: sizes it does not take).
+    pub fn lora_workspace_size(adapters: &Adapters, n_tokens: u32) -> u64 {
+        unsafe { sys::smoe_lora_workspace_size(&adapters.view(), n_tokens) }
+    }
+
+    /// Device workspace bytes a [`BeamSelectCall`] needs (0: sizes it does
+    /// not take).
+    pub fn beam_select_workspace_size(n_requests: u32, n_beams: u32, vocab: u32, n_picks: u32) -> u64 {
+        unsafe { sys::smoe_beam_select_workspace_size(n_requests, n_beams, vocab, n_picks) }
+    }
+
     /// Copy a byte range of a layer file into device memory (the resident
     /// part of `ExpertFiles::open` + `attach_to_device`,
     /// io/expert_io.rs:300-420); returns the bytes copied.
@@ -590,6 +601,253 @@ impl KernelCall for SoftmaxCall<'_> {
         let l = self.logits.f32_span(0, m, what)?;
         let p = self.probs.f32_span(0, m, what)?;
         check(unsafe { sys::smoe_softmax(k.h, l, self.n_tokens, self.n, p) }, what)
+    }
+}
+
+/// Residual addition, RMSNorm and 8-bit rows for a batch or a prompt
+/// (`rms_norm_bf16_n_tokens_cpu`, backend/cpu/mod.rs:406-430, after the
+/// residual's addition): `sum = input + residual`, `output = sum /
+/// sqrt(mean(sum^2) + eps) * norm_w`, `codes` and `scales` the same in 8 bits
+/// with a scale per `q_group` values (0: per row). At least one of `output`
+/// and `codes`; `codes` and `scales` together.
+pub struct RmsNormCall<'a> {
+    pub input: &'a BufferRef,
+    pub input_is_bf16: bool,
+    pub residual: Option<&'a BufferRef>,
+    pub norm_w: Option<&'a BufferRef>,
+    pub eps: f32,
+    pub n_tokens: u32,
+    pub hidden: u32,
+    pub sum: Option<&'a BufferRef>,
+    pub output: Option<&'a BufferRef>,
+    pub output_is_bf16: bool,
+    pub codes: Option<&'a BufferRef>,
+    pub scales: Option<&'a BufferRef>,
+    pub q_group: u32,
+}
+
+/// The span of an optional buffer, null without one.
+fn opt_span(b: Option<&BufferRef>, n: u64, size: u64, what: &'static str) -> Result<*mut c_void, SmoeError> {
+    match b {
+        Some(b) => b.span(0, n.checked_mul(size).unwrap_or(u64::MAX), what),
+        None => Ok(ptr::null_mut()),
+    }
+}
+
+impl KernelCall for RmsNormCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_rmsnorm";
+        let n = self.n_tokens as u64 * self.hidden as u64;
+        let per = if self.q_group == 0 { self.hidden } else { self.q_group }.max(1) as u64;
+        let x = opt_span(Some(self.input), n, if self.input_is_bf16 { 2 } else { 4 }, what)?;
+        let r = opt_span(self.residual, n, 4, what)?;
+        let w = opt_span(self.norm_w, self.hidden as u64, 2, what)?;
+        let s = opt_span(self.sum, n, 4, what)?;
+        let o = opt_span(self.output, n, if self.output_is_bf16 { 2 } else { 4 }, what)?;
+        let q = opt_span(self.codes, n, 1, what)?;
+        let qs = opt_span(self.scales, self.n_tokens as u64 * (self.hidden as u64 / per), 4, what)?;
+        check(unsafe {
+            sys::smoe_rmsnorm(k.h, x, self.input_is_bf16 as c_int, r as *const f32, w, self.eps, self.n_tokens,
+                              self.hidden, s as *mut f32, o, self.output_is_bf16 as c_int, q as *mut i8,
+                              qs as *mut f32, self.q_group)
+        }, what)
+    }
+}
+
+/// [`QmmCall`] for rows in 8 bits, as [`RmsNormCall`] writes them; `x_group`
+/// 0 (a scale per row) or the weights' group. Needs no workspace.
+pub struct QmmI8Call<'a> {
+    pub weights: QuantWeights<'a>,
+    pub codes: &'a BufferRef,
+    pub scales: &'a BufferRef,
+    pub x_group: u32,
+    pub output: &'a BufferRef,
+    pub output_offset: u64,
+    pub in_dim: u32,
+    pub out_dim: u32,
+    pub n_tokens: u32,
+}
+
+impl KernelCall for QmmI8Call<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_qmm_i8";
+        let w = self.weights.raw(self.out_dim, self.in_dim, what)?;
+        let n = self.n_tokens as u64;
+        let per = if self.x_group == 0 { self.in_dim } else { self.x_group }.max(1) as u64;
+        let x = self.codes.span(0, n * self.in_dim as u64, what)?;
+        let sx = self.scales.f32_span(0, n * (self.in_dim as u64 / per), what)?;
+        let y = self.output.f32_span(self.output_offset, n * self.out_dim as u64, what)?;
+        check(unsafe {
+            sys::smoe_qmm_i8(k.h, &w, x as *const i8, sx, self.x_group, y, self.out_dim, self.in_dim, self.n_tokens)
+        }, what)
+    }
+}
+
+/// The low-rank adapters of one projection: `a` `[n, max_rank, in_dim]` and
+/// `b` `[n, out_dim, max_rank]` in bf16, one behind the other, `scale` f32 and
+/// `ranks` int32 per adapter (`None`: all `max_rank`).
+#[derive(Clone, Copy, Debug)]
+pub struct Adapters<'a> {
+    pub a: &'a BufferRef,
+    pub b: &'a BufferRef,
+    pub scale: &'a BufferRef,
+    pub ranks: Option<&'a BufferRef>,
+    pub n_adapters: u32,
+    pub max_rank: u32,
+    pub in_dim: u32,
+    pub out_dim: u32,
+}
+
+impl Adapters<'_> {
+    fn view(&self) -> sys::smoe_adapters {
+        sys::smoe_adapters {
+            a: self.a.ptr,
+            b: self.b.ptr,
+            a_stride: self.max_rank as u64 * self.in_dim as u64 * 2,
+            b_stride: self.max_rank as u64 * self.out_dim as u64 * 2,
+            scale: self.scale.ptr as *const f32,
+            ranks: self.ranks.map_or(ptr::null(), |r| r.ptr as *const i32),
+            n_adapters: self.n_adapters,
+            max_rank: self.max_rank,
+        }
+    }
+
+    /// The C view, after checking that the buffers hold the adapters.
+    fn raw(&self, what: &'static str) -> Result<sys::smoe_adapters, SmoeError> {
+        let n = self.n_adapters as u64;
+        let v = self.view();
+        self.a.span(0, n.checked_mul(v.a_stride).unwrap_or(u64::MAX), what)?;
+        self.b.span(0, n.checked_mul(v.b_stride).unwrap_or(u64::MAX), what)?;
+        self.scale.f32_span(0, n, what)?;
+        opt_span(self.ranks, n, 4, what)?;
+        Ok(v)
+    }
+}
+
+/// Many requests' adapters beside a projection: `output[t] = base[t] +
+/// scale[a] B_a (A_a input[t])`, `a = ids[t]` (-1: none); `base` `None`
+/// (zeros) or `output` itself. Workspace: [`Kernels::lora_workspace_size`]
+/// bytes. An id out of range is reported by the next [`Kernels::sync`].
+pub struct LoraCall<'a> {
+    pub adapters: Adapters<'a>,
+    pub ids: &'a BufferRef,
+    pub input: &'a BufferRef,
+    pub input_is_bf16: bool,
+    pub base: Option<&'a BufferRef>,
+    pub output: &'a BufferRef,
+    pub n_tokens: u32,
+    pub workspace: &'a BufferRef,
+}
+
+impl KernelCall for LoraCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_lora";
+        let set = self.adapters.raw(what)?;
+        let (n, i, o) = (self.n_tokens as u64, self.adapters.in_dim as u64, self.adapters.out_dim as u64);
+        let ids = opt_span(Some(self.ids), n, 4, what)?;
+        let x = opt_span(Some(self.input), n * i, if self.input_is_bf16 { 2 } else { 4 }, what)?;
+        let base = opt_span(self.base, n * o, 4, what)?;
+        let y = self.output.f32_span(0, n * o, what)?;
+        check(unsafe {
+            sys::smoe_lora(k.h, &set, ids as *const i32, x, self.input_is_bf16 as c_int, base as *const f32, y,
+                           self.adapters.out_dim, self.adapters.in_dim, self.n_tokens, self.workspace.ptr,
+                           self.workspace.len)
+        }, what)
+    }
+}
+
+/// One step of `n_requests` beam searches behind the LM head (the reference
+/// samples greedily, io/gpu_lm_head.rs:130-193): the `n_picks` best
+/// continuations of each request's `n_beams` rows of logits, as scores, rows of
+/// the logits and tokens. `done`: a byte per beam, those that have ended keep
+/// their score with `pad_token`. Workspace:
+/// [`Kernels::beam_select_workspace_size`] bytes.
+pub struct BeamSelectCall<'a> {
+    pub logits: &'a BufferRef,
+    pub scores: &'a BufferRef,
+    pub done: Option<&'a BufferRef>,
+    pub pad_token: u32,
+    pub n_requests: u32,
+    pub n_beams: u32,
+    pub vocab: u32,
+    pub n_picks: u32,
+    pub out_scores: &'a BufferRef,
+    pub out_rows: &'a BufferRef,
+    pub out_tokens: &'a BufferRef,
+    pub workspace: &'a BufferRef,
+}
+
+impl KernelCall for BeamSelectCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_beam_select";
+        let rows = self.n_requests as u64 * self.n_beams as u64;
+        let picks = self.n_requests as u64 * self.n_picks as u64;
+        let logits = self.logits.f32_span(0, rows.checked_mul(self.vocab as u64).unwrap_or(u64::MAX), what)?;
+        let scores = self.scores.f32_span(0, rows, what)?;
+        let done = opt_span(self.done, rows, 1, what)?;
+        let v = self.out_scores.f32_span(0, picks, what)?;
+        let r = self.out_rows.f32_span(0, picks, what)?;
+        let t = self.out_tokens.f32_span(0, picks, what)?;
+        check(unsafe {
+            sys::smoe_beam_select(k.h, logits, scores, done as *const u8, self.pad_token, self.n_requests,
+                                  self.n_beams, self.vocab, self.n_picks, v, r as *mut i32, t as *mut i32,
+                                  self.workspace.ptr, self.workspace.len)
+        }, what)
+    }
+}
+
+/// One state tensor of the beams, in bytes: row `r` holds `n_pieces` pieces of
+/// `piece_bytes`, piece `p` at `r * row_stride + p * piece_stride` (the used
+/// part of a cache of several heads; one piece for a dense row).
+#[derive(Clone, Copy, Debug)]
+pub struct BeamState<'a> {
+    pub src: &'a BufferRef,
+    pub dst: &'a BufferRef,
+    pub src_row_stride: u64,
+    pub dst_row_stride: u64,
+    pub src_piece_stride: u64,
+    pub dst_piece_stride: u64,
+    pub piece_bytes: u64,
+    pub n_pieces: u32,
+}
+
+/// `dst` row `i` = `src` row `rows[i]` of every state, for `rows` as
+/// [`BeamSelectCall`] writes them. A row out of range is reported by the next
+/// [`Kernels::sync`].
+pub struct BeamReorderCall<'a> {
+    pub states: &'a [BeamState<'a>],
+    pub rows: &'a BufferRef,
+    pub n_rows: u32,
+    pub src_rows: u32,
+}
+
+impl KernelCall for BeamReorderCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_beam_reorder";
+        let rows = self.rows.f32_span(0, self.n_rows as u64, what)? as *const i32;
+        let extent = |n: u32, row: u64, pieces: u32, piece: u64, bytes: u64| {
+            let last = |n: u32, stride: u64| (n as u64).saturating_sub(1).checked_mul(stride);
+            last(n, row)?.checked_add(last(pieces, piece)?)?.checked_add(bytes)
+        };
+        let mut raw = Vec::with_capacity(self.states.len());
+        for s in self.states {
+            let from = extent(self.src_rows, s.src_row_stride, s.n_pieces, s.src_piece_stride, s.piece_bytes);
+            let to = extent(self.n_rows, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes);
+            raw.push(sys::smoe_beam_state {
+                src: s.src.span(0, from.unwrap_or(u64::MAX), what)?,
+                dst: s.dst.span(0, to.unwrap_or(u64::MAX), what)?,
+                src_row_stride: s.src_row_stride,
+                dst_row_stride: s.dst_row_stride,
+                src_piece_stride: s.src_piece_stride,
+                dst_piece_stride: s.dst_piece_stride,
+                piece_bytes: s.piece_bytes,
+                n_pieces: s.n_pieces,
+                reserved: 0,
+            });
+        }
+        check(unsafe {
+            sys::smoe_beam_reorder(k.h, raw.as_ptr(), raw.len() as u32, rows, self.n_rows, self.src_rows)
+        }, what)
     }
 }
 
