@@ -2,10 +2,10 @@
 //
 //   y[t] = base[t] + scale[a] B_a (A_a x[t]),  a = ids[t]
 //
-//   k_lora_plan    rows sorted by adapter, items of up to 16 rows of one (up to
-//                  64 rows the blocks below find their item by themselves)
+//   k_lora_plan    rows sorted by adapter, items of up to 16 rows of one, for
+//                  more rows or adapters than the next kernel sorts by itself
 //   k_lora_down    u = A x of an item's rows on bf16 MFMA, one share of the
-//                  inputs per block, partial sums in f32
+//                  inputs per block, partial sums in f32; leaves the items
 //   k_lora_up      the shares added, scaled, times B on bf16 MFMA, plus base
 //
 // f32 values enter the matrix cores as bf16 pairs, v = hi + lo, each rounded
@@ -123,7 +123,7 @@ constexpr uint32_t kLoraSmall = 64;  // rows whose items need no plan: one per l
 // Item blockIdx.x of a call of up to 64 rows, by every wave for itself: the
 // rows' ids, one per lane, taken group by group in the order of their first
 // rows; `rows` receives the item's rows (kLoraM per wave).
-__device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t lane, uint32_t* rows) {
+__device__ __forceinline__ LoraItem lora_wave_item(const LoraArgs& a, uint32_t lane, uint32_t* rows) {
   const int32_t id = lane < a.n ? a.ids[lane] : -2;
   const bool bad = lane < a.n && (id < -1 || id >= (int32_t)a.n_adapters);
   const uint32_t ad = bad || id < 0 ? a.n_adapters : (uint32_t)id;
@@ -160,31 +160,156 @@ __device__ __forceinline__ LoraItem lora_small_item(const LoraArgs& a, uint32_t 
   return it;
 }
 
-// The item of this block and row min(c, count - 1) of it.
-template <bool SMALL>
-__device__ __forceinline__ LoraItem lora_item(const LoraArgs& a, uint32_t lane, uint32_t* rows, uint32_t& row) {
-  if constexpr (SMALL) {
-    const LoraItem it = lora_small_item(a, lane, rows);
-    row = it.count ? rows[min(lane & 15, it.count - 1)] : 0u;
-    return it;
-  } else {
-    const LoraItem it = a.items[blockIdx.x];
-    const uint32_t r = a.rows[blockIdx.x * kLoraM + (lane & 15)];  // unset past the count: replaced
-    const uint32_t last = (uint32_t)__shfl((int)r, (int)(it.count ? it.count - 1 : 0u), kWave);
-    row = (lane & 15) < it.count ? r : last;
-    return it;
+constexpr uint32_t kLoraMid = 1024;  // rows, and adapters and one: four of each per thread
+
+struct LoraFind {
+  uint32_t count[kLoraMid];
+  uint32_t sums[4], of[4][4];
+  LoraItem item;
+  uint32_t nth;  // of the adapter's items
+  uint32_t rows[kLoraM];
+};
+
+// Item blockIdx.x of a call of up to 1024 rows and 1023 adapters, by the block:
+// counts per adapter, their items (the adapters t, t + 256, .. of thread 0, of
+// thread 1, ..), then the places of the item's adapter's rows in the rows'
+// order.
+__device__ __forceinline__ LoraItem lora_block_item(const LoraArgs& a, LoraFind& f) {
+  const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), N = a.n_adapters;
+  int32_t id[4], rk[4];
+  float sc[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    const uint32_t row = 256 * j + t;
+    id[j] = -1;
+    if (256 * j < a.n) id[j] = a.ids[min(row, a.n - 1)];
   }
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    rk[j] = (int32_t)a.max_rank;
+    sc[j] = 0.f;
+    if (256 * j < N) {
+      sc[j] = a.scale[min(256 * j + t, N - 1)];
+      if (a.ranks) rk[j] = a.ranks[min(256 * j + t, N - 1)];
+    }
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j)
+    if (256 * j <= N) f.count[256 * j + t] = 0;
+  if (t == 0) f.item = LoraItem{0u, 0u, 0u, 0u, 0.f};
+  __syncthreads();
+  uint32_t ad[4];  // ~0: no row
+  bool bad = false;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    ad[j] = ~0u;
+    if (256 * j >= a.n) continue;
+    const bool in = 256 * j + t < a.n, is = id[j] >= 0 && id[j] < (int32_t)N;
+    bad |= in && !is && id[j] != -1;
+    if (in) ad[j] = is ? (uint32_t)id[j] : N;
+    // Those of the first lane's adapter in one, the others one by one (64 adds
+    // to one address are 64 turns).
+    const uint32_t lead = (uint32_t)__builtin_amdgcn_readfirstlane((int)ad[j]);
+    const uint64_t same = __ballot(ad[j] == lead);
+    if (ad[j] != lead || lane == 0)
+      if (ad[j] != ~0u) atomicAdd(&f.count[ad[j]], lane == 0 ? (uint32_t)__popcll(same) : 1u);
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) bad |= rk[j] < 0 || rk[j] > (int32_t)a.max_rank;
+  if (bad && blockIdx.x == 0 && blockIdx.y == 0) *a.err = 2u;
+  __syncthreads();
+  // Items in the upper half, rows in the lower.
+  uint32_t own[4], sum = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    own[j] = 0;
+    if (256 * j > N) continue;
+    const uint32_t c = f.count[256 * j + t];
+    own[j] = (c + kLoraM - 1) / kLoraM << 16 | c;
+    sum += own[j];
+  }
+  uint32_t before = lora_scan(sum);
+  if (lane == 63) f.sums[wave] = before;
+  __syncthreads();
+  before -= sum;
+  for (uint32_t w = 0; w < wave; ++w) before += f.sums[w];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    const uint32_t nth = blockIdx.x - (before >> 16), i = 256 * j + t;
+    if (nth < own[j] >> 16) {
+      const uint32_t rank = i < N ? (uint32_t)min(max(rk[j], 0), (int32_t)a.max_rank) : 0u;
+      f.item = LoraItem{i, (before & 0xFFFFu) + nth * kLoraM, min(kLoraM, (own[j] & 0xFFFFu) - nth * kLoraM), rank,
+                        i < N ? sc[j] : 0.f};
+      f.nth = nth;
+    }
+    before += own[j];
+  }
+  __syncthreads();
+  const LoraItem it = f.item;
+  if (it.count == 0) return it;  // the whole block
+  uint64_t of[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    of[j] = __ballot(ad[j] == it.adapter);
+    if (lane == 0) f.of[j][wave] = (uint32_t)__popcll(of[j]);
+  }
+  __syncthreads();
+  uint32_t at = 0u - f.nth * kLoraM;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    uint32_t place = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(of[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)of[j], 0u));
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const uint32_t c = f.of[j][w];
+      at += c;
+      if (w < wave) place += c;
+    }
+    if (ad[j] == it.adapter && place < kLoraM) f.rows[place] = 256 * j + t;
+  }
+  __syncthreads();
+  return it;
 }
+
+// The item of this block as k_lora_plan or k_lora_down left it, and row
+// min(c, count - 1) of it.
+__device__ __forceinline__ LoraItem lora_item(const LoraArgs& a, uint32_t lane, uint32_t& row) {
+  const LoraItem it = a.items[blockIdx.x];
+  const uint32_t r = a.rows[blockIdx.x * kLoraM + (lane & 15)];  // unset past the count: replaced
+  const uint32_t last = (uint32_t)__shfl((int)r, (int)(it.count ? it.count - 1 : 0u), kWave);
+  row = (lane & 15) < it.count ? r : last;
+  return it;
+}
+
+// Who finds the items: k_lora_plan, k_lora_down's waves, its blocks.
+enum LoraBy { kByPlan, kByWave, kByBlock };
 
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c.
-template <bool XBF16, bool SMALL, int MT>
+template <bool XBF16, LoraBy BY, int MT>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   __shared__ f32x4 red[4][64];
-  __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
   uint32_t row;
-  const LoraItem it = lora_item<SMALL>(a, lane, rows[wave], row);
+  LoraItem it;
+  if constexpr (BY == kByPlan) {
+    it = lora_item(a, lane, row);
+  } else {
+    const uint32_t* rows;
+    if constexpr (BY == kByWave) {
+      __shared__ uint32_t of_wave[4][kLoraM];
+      it = lora_wave_item(a, lane, of_wave[wave]);
+      rows = of_wave[wave];
+    } else {
+      __shared__ LoraFind f;
+      it = lora_block_item(a, f);
+      rows = f.rows;
+    }
+    row = it.count ? rows[min(c16, it.count - 1)] : 0u;
+    if (blockIdx.y == 0 && threadIdx.x < kLoraM) {
+      a.rows[blockIdx.x * kLoraM + threadIdx.x] = row;
+      if (threadIdx.x == 0) a.items[blockIdx.x] = it;
+    }
+  }
   if (it.count == 0 || it.adapter >= a.n_adapters) return;
   const uint32_t K = a.in_dim, share = blockIdx.y;
   const uint32_t rank = it.rank, nt = (rank + 15) / 16;
@@ -256,16 +381,15 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
 // 4096). The products go through LDS too, so that base and y move in whole rows
 // of the block (in the products' order each lane touches a line of its own).
 // B's and base's loads go out ahead of everything.
-template <bool SMALL, int KT, int NT>
+template <int KT, int NT>
 __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   constexpr uint32_t RP = KT * 32 + 8;  // bf16 per row in LDS: rows apart by 16 bytes of banks
   constexpr uint32_t OB = 64 * NT, OP = OB + 4;  // outputs of the block; floats per row in LDS, apart by 16 bytes of banks
   __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
   __shared__ __attribute__((aligned(16))) float prod[kLoraM * OP];
-  __shared__ uint32_t rows[4][kLoraM];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
   uint32_t row;
-  const LoraItem it = lora_item<SMALL>(a, lane, rows[wave], row);
+  const LoraItem it = lora_item(a, lane, row);
   if (it.count == 0) return;
   const uint32_t O = a.out_dim, R = a.max_rank;
   const uint32_t o0 = (blockIdx.y * 4 + wave) * NT * 16;
@@ -408,21 +532,21 @@ uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, Lora
   return ib + pb + al256((uint64_t)shares * n * max_rank * 4);
 }
 
-template <bool SMALL>
+template <LoraBy BY>
 static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
   auto down = [&](auto fn) {
     hipLaunchKernelGGL(fn, dim3(a.n_items, a.shares), dim3(256), 0, st, a);
     return hipGetLastError();
   };
   const uint32_t mt = (a.max_rank + 15) / 16;  // tiles of 16 ranks
-  const hipError_t e = x_bf16 ? (mt <= 1   ? down(k_lora_down<true, SMALL, 1>)
-                                 : mt <= 2 ? down(k_lora_down<true, SMALL, 2>)
-                                 : mt <= 4 ? down(k_lora_down<true, SMALL, 4>)
-                                           : down(k_lora_down<true, SMALL, 8>))
-                              : (mt <= 1   ? down(k_lora_down<false, SMALL, 1>)
-                                 : mt <= 2 ? down(k_lora_down<false, SMALL, 2>)
-                                 : mt <= 4 ? down(k_lora_down<false, SMALL, 4>)
-                                           : down(k_lora_down<false, SMALL, 8>));
+  const hipError_t e = x_bf16 ? (mt <= 1   ? down(k_lora_down<true, BY, 1>)
+                                 : mt <= 2 ? down(k_lora_down<true, BY, 2>)
+                                 : mt <= 4 ? down(k_lora_down<true, BY, 4>)
+                                           : down(k_lora_down<true, BY, 8>))
+                              : (mt <= 1   ? down(k_lora_down<false, BY, 1>)
+                                 : mt <= 2 ? down(k_lora_down<false, BY, 2>)
+                                 : mt <= 4 ? down(k_lora_down<false, BY, 4>)
+                                           : down(k_lora_down<false, BY, 8>));
   if (e != hipSuccess) return e;
   // Outputs per block: as many as leave two blocks for every CU.
   auto up = [&](auto fn, uint32_t nt) {
@@ -430,16 +554,17 @@ static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
     return hipGetLastError();
   };
   const bool wide = (uint64_t)a.n_items * ((a.out_dim + 255) / 256) >= 512;
-  if (a.max_rank <= 32) return wide ? up(k_lora_up<SMALL, 1, 4>, 4) : up(k_lora_up<SMALL, 1, 1>, 1);
-  if (a.max_rank <= 64) return wide ? up(k_lora_up<SMALL, 2, 4>, 4) : up(k_lora_up<SMALL, 2, 1>, 1);
-  return wide ? up(k_lora_up<SMALL, 4, 4>, 4) : up(k_lora_up<SMALL, 4, 1>, 1);
+  if (a.max_rank <= 32) return wide ? up(k_lora_up<1, 4>, 4) : up(k_lora_up<1, 1>, 1);
+  if (a.max_rank <= 64) return wide ? up(k_lora_up<2, 4>, 4) : up(k_lora_up<2, 1>, 1);
+  return wide ? up(k_lora_up<4, 4>, 4) : up(k_lora_up<4, 1>, 1);
 }
 
 hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
-  if (a.n <= kLoraSmall) return lora_go<true>(a, x_bf16, st);
+  if (a.n <= kLoraSmall) return lora_go<kByWave>(a, x_bf16, st);
+  if (a.n <= kLoraMid && a.n_adapters < kLoraMid) return lora_go<kByBlock>(a, x_bf16, st);
   hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 8, st, a);
   const hipError_t e = hipGetLastError();
-  return e != hipSuccess ? e : lora_go<false>(a, x_bf16, st);
+  return e != hipSuccess ? e : lora_go<kByPlan>(a, x_bf16, st);
 }
 
 }  // namespace smoe
