@@ -61,11 +61,6 @@ def _fits(t, types, n, device):
     return t is not None and t.dtype in types and t.numel() >= n and t.is_contiguous() and t.get_device() == device
 
 
-def _view(t):
-    """What a checked struct of a tensor holds for."""
-    return None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype)
-
-
 def _at(t):
     return None if t is None else t.data_ptr()
 
@@ -151,28 +146,32 @@ class Adapters:
     scale: object
     ranks: object = None
 
-    def c(self):
-        """The C struct, checked when it is first asked for and again whenever
-        one of the tensors lies elsewhere or in another way than then."""
-        views = (_view(self.a), _view(self.b), _view(self.scale), _view(self.ranks))
-        known = self.__dict__.get("_known")
-        if known is None or known[0] != views:
-            known = (views, self._struct())
-            object.__setattr__(self, "_known", known)
-        return known[1]
+    def __post_init__(self):
+        # Views of its own: what becomes of the caller's shapes does not matter.
+        held = tuple(None if t is None else t.detach() for t in (self.a, self.b, self.scale, self.ranks))
+        object.__setattr__(self, "_held", held)
+        object.__setattr__(self, "_known", (None, None))
 
-    def _struct(self):
-        a, b, bf16 = self.a, self.b, _types("bf16")
-        dev = a.get_device()
+    def c(self):
+        """The C struct, checked when first asked for (and again should a
+        storage have moved)."""
+        a, b, scale, ranks = self._held
+        at = (a.data_ptr(), b.data_ptr(), scale.data_ptr(), _at(ranks))
+        if self._known[0] != at:
+            object.__setattr__(self, "_known", (at, self._struct(at)))
+        return self._known[1]
+
+    def _struct(self, at):
+        a, b, scale, ranks = self._held
+        bf16, dev = _types("bf16"), a.get_device()
         if (a.dim() != 3 or b.dim() != 3 or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1] or not a.numel()
                 or not b.numel() or not _fits(a[0], bf16, 1, dev) or not _fits(b[0], bf16, 1, dev)
-                or not _fits(self.scale, _types("f32"), a.shape[0], dev)
-                or not (self.ranks is None or _fits(self.ranks, _types("i32"), a.shape[0], dev))):
+                or not _fits(scale, _types("f32"), a.shape[0], dev)
+                or not (ranks is None or _fits(ranks, _types("i32"), a.shape[0], dev))):
             raise SmoeError(_INVALID, "Adapters")
         # A lone adapter's stride says nothing: its size.
         step = lambda t: (t.stride(0) if t.shape[0] > 1 else t[0].numel()) * 2
-        return _abi.AdaptersC(a.data_ptr(), b.data_ptr(), step(a), step(b), self.scale.data_ptr(), _at(self.ranks),
-                              a.shape[0], a.shape[1])
+        return _abi.AdaptersC(at[0], at[1], step(a), step(b), at[2], at[3], a.shape[0], a.shape[1])
 
 
 @dataclass(frozen=True, eq=False)
@@ -186,19 +185,21 @@ class BeamState:
     dst: object
     used: int = None
 
+    def __post_init__(self):
+        object.__setattr__(self, "_held", (self.src.detach(), self.dst.detach()))
+        object.__setattr__(self, "_known", (None, None))
+
     def c(self):
         """(the C struct's bytes, rows of src, rows of dst, device), checked when
-        first asked for and again whenever one of the tensors lies elsewhere or
-        in another way."""
-        views = (_view(self.src), _view(self.dst))
-        known = self.__dict__.get("_known")
-        if known is None or known[0] != views:
-            known = (views, self._struct())
-            object.__setattr__(self, "_known", known)
-        return known[1]
+        first asked for (and again should a storage have moved)."""
+        s, d = self._held
+        at = (s.data_ptr(), d.data_ptr())
+        if self._known[0] != at:
+            object.__setattr__(self, "_known", (at, self._struct(at)))
+        return self._known[1]
 
-    def _struct(self):
-        s, d = self.src, self.dst
+    def _struct(self, at):
+        s, d = self._held
         if (s.device != d.device or s.device.type != "cuda" or s.dtype != d.dtype or s.dim() not in (2, 3)
                 or s.shape[1:] != d.shape[1:] or s.stride(-1) != 1 or d.stride(-1) != 1):
             raise SmoeError(_INVALID, "BeamState")
@@ -209,7 +210,7 @@ class BeamState:
         if not 0 <= used <= room:
             raise SmoeError(_INVALID, "BeamState: used")
         piece = (lambda t: t.stride(1) * size) if s.dim() == 3 else (lambda t: 0)
-        raw = _abi.BeamStateC(s.data_ptr(), d.data_ptr(), s.stride(0) * size, d.stride(0) * size, piece(s), piece(d), used, pieces, 0)
+        raw = _abi.BeamStateC(*at, s.stride(0) * size, d.stride(0) * size, piece(s), piece(d), used, pieces, 0)
         return bytes(raw), s.shape[0], d.shape[0], s.get_device()
 
 
@@ -446,7 +447,7 @@ class Kernels:
         """y[t] = base[t] + scale[a] b[a] (a[a] x[t]), a = ids[t] (-1: none); base
         None (zeros) or y itself; x f32 or bf16 rows."""
         ac, dev, f32 = adapters.c(), self.device, _types("f32")
-        a, b = adapters.a, adapters.b
+        a, b = adapters._held[:2]
         if (a.get_device() != dev or a.shape[2] != in_dim or b.shape[1] != out_dim
                 or not _fits(ids, _types("i32"), n_tokens, dev)
                 or not _fits(x, _types("f32_bf16"), n_tokens * in_dim, dev)

@@ -515,7 +515,7 @@ static uint64_t al256(uint64_t n) { return (n + 255) & ~255ull; }
 
 // Shares of the inputs: enough blocks for few rows, none to spare for many
 // (k_lora_up adds 16, 8, 4 or 1).
-static uint32_t lora_shares(uint32_t n) { return n <= 256 ? 16u : n <= 1024 ? 8u : n <= 4096 ? 4u : 1u; }
+static uint32_t lora_shares(uint32_t n) { return n <= 64 ? 16u : n <= 1024 ? 8u : n <= 4096 ? 4u : 1u; }
 
 uint64_t lora_workspace(uint32_t n_adapters, uint32_t max_rank, uint32_t n, LoraArgs* a, uint8_t* base) {
   const uint32_t shares = lora_shares(n);
