@@ -12,12 +12,14 @@
 #include "common.h"
 #include "kernels.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace smoe {
 
 typedef unsigned long long u64;
 
+constexpr uint32_t kBeamBlocks = 512;         // two per CU, if rows and tiles allow
 constexpr uint32_t kBeamTile = 4096;          // logits per block and round: 16 per thread
 constexpr uint32_t kOrdNegInf = 0x007FFFFFu;  // beam_ord(-inf)
 
@@ -30,8 +32,8 @@ __device__ __forceinline__ float beam_value(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
 
-// e^x for x <= 0, from below -87 on 2^-126 (nothing beside a sum of at least
-// one): 2^p with p = x log2 e rounded, times 1 + r ln 2 for what the rounding
+// e^x for x <= 0, from below -87 on (and for a NaN) 2^-126 (nothing beside a
+// sum of at least one): 2^p with p = x log2 e rounded, times 1 + r ln 2 for what the rounding
 // left, r = x log2 e - p; off by two ulp and |x| 1.4e-8 (log2 e in 24 bits).
 __device__ __forceinline__ float beam_exp(float x) {
   constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147182f;
@@ -85,70 +87,82 @@ __device__ __forceinline__ bool beam_open(const BeamArgs& a, uint32_t row) {
   return a.scores[row] > -INFINITY && !(a.done && a.done[row]);
 }
 
-// Each wave collects what of its 1024 logits can be among the P largest: with
-// T the P-th largest of the largest logits of some groups of lanes, at least P
-// logits are >= T. Groups of four or two lanes do where there are twice P of
-// them (16 lane reads instead of 64), with little more than P logits >= T as a
-// rule. Where those are over 17 P, T is the P-th largest of single lanes: those
-// above it lie in fewer than P lanes, and of those equal to it the P of lowest
-// tokens suffice. The block's list is ranked by counting.
+// Keys that a wave may hold: its P largest and what one tile can add, 17 P.
+__host__ __device__ constexpr uint32_t beam_held(uint32_t picks) { return 18 * picks; }
+
+// Each wave goes through its 1024 logits of every tile by itself and keeps what
+// can be among the P largest: with T the least of the largest logits of at
+// least P groups of lanes (over all tiles so far), or the P-th largest of more
+// groups, at least P logits are >= T, and few more as a rule. Where a tile has
+// more of them than there is room for, the wave's list is cut to its P largest
+// and T becomes the P-th largest of the tile's single lanes: those above it lie
+// in fewer than P lanes, and of those equal to it the P of lowest tokens
+// suffice. In the end the block ranks what is >= the waves' largest T by
+// counting.
 __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
-  extern __shared__ __attribute__((aligned(16))) u64 list[];  // [68 P], then twice [P] of the tiles before
+  extern __shared__ __attribute__((aligned(16))) u64 lists[];  // per wave [19 P]; all waves' [72 P]
+  __shared__ __attribute__((aligned(16))) float held[256 * 16];  // logits of threads that have one for the list
+  __shared__ float least_of[4];
   __shared__ uint32_t count;
   const uint32_t t = threadIdx.x, lane = t & 63, P = a.picks;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-  u64* const top = list + 4 * 17 * P;
+  u64* const list = lists + wave * (beam_held(P) + P);
   const uint64_t first = (uint64_t)row * a.vocab, total = (uint64_t)a.rows * a.vocab;
   const uint32_t shift = (uint32_t)(first & 3);  // tiles start on 16 bytes, up to three logits ahead of the row
-  float m = -INFINITY;
-  double sum = 0.0;
-  if (t < P) top[t] = 0;
-  const uint32_t tile0 = slice * a.tiles;
-  for (uint32_t tile = tile0; tile < tile0 + a.tiles; ++tile) {
-    const int64_t tok0 = (int64_t)tile * kBeamTile - shift;
-    if (tok0 >= (int64_t)a.vocab) break;
-    // Value 4 j + c is token tok + 1024 j + c. A NaN counts as -inf, and so do
-    // places outside the row, which must not be taken.
-    const int64_t tok = tok0 + t * 4;
-    const bool whole = tok0 >= 0 && tok0 + kBeamTile <= (int64_t)a.vocab;
-    float v[16];
-    if (whole) {
+  // Thread t's fours j of a tile: tokens tok0 + 1024 j + 4 t on.
+  auto start = [&](uint32_t tile) { return (int64_t)tile * kBeamTile - shift; };
+  auto load = [&](uint32_t tile, f32x4 (&q)[4]) {
+    const int64_t tok0 = start(tile), tok = tok0 + t * 4;
+    if (tok0 >= 0 && tok0 + kBeamTile <= (int64_t)a.vocab) {
       const float* const p = a.logits + first + tok;
-      f32x4 q[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const f32x4*>(p + 1024 * j);
-      if (tile == tile0 && !beam_open(a, row)) return;  // under the loads
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = fmaxf(q[i / 4][i % 4], -INFINITY);
-    } else {
-      if (tile == tile0 && !beam_open(a, row)) return;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t k = tok + 1024 * j, e = (int64_t)first + k;
-        f32x4 q = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (k < (int64_t)a.vocab) {
-          if (e + 4 <= (int64_t)total) {
-            q = *reinterpret_cast<const f32x4*>(a.logits + e);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (e + c < (int64_t)total) q[c] = a.logits[e + c];
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[4 * j + c] = k + c >= 0 && k + c < (int64_t)a.vocab ? fmaxf(q[c], -INFINITY) : -INFINITY;
-      }
+      return;
     }
-    float tm = v[0];
+    // Places outside the row are -inf.
 #pragma unroll
-    for (int i = 1; i < 16; ++i) tm = fmaxf(tm, v[i]);
+    for (int j = 0; j < 4; ++j) {
+      const int64_t k = tok + 1024 * j, e = (int64_t)first + k;
+      q[j] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (k < (int64_t)a.vocab) {
+        if (e + 4 <= (int64_t)total) {
+          q[j] = *reinterpret_cast<const f32x4*>(a.logits + e);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (e + c < (int64_t)total) q[j][c] = a.logits[e + c];
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) q[j][c] = k + c >= 0 && k + c < (int64_t)a.vocab ? q[j][c] : -INFINITY;
+    }
+  };
+  const uint32_t tile0 = slice * a.tiles;
+  uint32_t tiles = a.tiles;
+  while (tiles && start(tile0 + tiles - 1) >= (int64_t)a.vocab) --tiles;
+  f32x4 q[4], ahead[4];
+  if (tiles) load(tile0, q);
+  if (!beam_open(a, row)) return;  // under the loads
+  float m = -INFINITY, least = -INFINITY, most = -INFINITY;
+  double sum = 0.0;
+  uint32_t used = 0;
+  for (uint32_t i = 0; i < tiles; ++i) {
+    if (i + 1 < tiles) load(tile0 + i + 1, ahead);
+    const uint32_t tok0 = (uint32_t)start(tile0 + i);
+    // A NaN counts as -inf: maxima pass it over, and so does beam_exp.
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = __builtin_canonicalizef(q[e / 4][e % 4]);
+    float tm = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) tm = fmaxf(tm, v[e]);
     // Sum of exponentials below the thread's running maximum.
     const float nm = fmaxf(m, tm);
     if (nm > -INFINITY) {
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s += beam_exp(v[i] - nm);
+      for (int e = 0; e < 16; ++e) s += beam_exp(v[e] - nm);
       sum = sum * (double)(m > -INFINITY ? beam_exp(m - nm) : 0.f) + (double)s;
       m = nm;
     }
@@ -156,24 +170,22 @@ __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
     // than P are above.
     auto threshold = [&](float g, auto lanes) {
       uint32_t higher = 0;
-#pragma unroll
+#pragma unroll 16
       for (int l = 0; l < 64; l += decltype(lanes)::value) higher += readlane_f(g, l) > g ? 1u : 0u;
       return -wave_max_f32(higher < P ? -g : -INFINITY);
     };
-    const float two = fmaxf(tm, dpp_f<0xB1>(tm, tm)), four = fmaxf(two, dpp_f<0x4E>(two, two));
-    // What is not above the P-th largest of the tiles before has no place.
-    const float floor = tile == tile0 ? -INFINITY : beam_value((uint32_t)(top[P - 1] >> 32));
-    float least = fmaxf(floor, P <= 8    ? threshold(four, std::integral_constant<int, 4>{})
-                               : P <= 16 ? threshold(two, std::integral_constant<int, 2>{})
-                                         : threshold(tm, std::integral_constant<int, 1>{}));
-    auto key = [&](int i) { return (u64)beam_ord(v[i]) << 32 | (uint32_t)~(uint32_t)(tok + 1024 * (i / 4) + i % 4); };
-    u64* const out = top + P;  // beside the tops, which are still read
-    if (t == 0) count = 0;
-    if (t < P) out[t] = 0;
-    __syncthreads();
-    uint32_t mine = 0;
+    most = fmaxf(most, tm);
+    const float two = fmaxf(most, dpp_f<0xB1>(most, most)), four = fmaxf(two, dpp_f<0x4E>(two, two));
+    least = P <= 8    ? threshold(four, std::integral_constant<int, 4>{})
+            : P <= 16 ? threshold(two, std::integral_constant<int, 2>{})
+                      : threshold(most, std::integral_constant<int, 1>{});
+    // Bit 15 - e: v[e] >= least, as the sign of what is next below least minus v.
+    const uint32_t lb = __float_as_uint(least + 0.f);
+    const float below = least > -INFINITY ? __uint_as_float(lb == 0u ? 0x80000001u : (int32_t)lb > 0 ? lb - 1 : lb + 1) : least;
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mine += v[i] >= least ? 1u : 0u;
+    for (int e = 0; e < 16; ++e) bits = __builtin_amdgcn_alignbit(bits, __float_as_uint(below - v[e]), 31);
+    const uint32_t mine = (uint32_t)__popc(bits);
     uint32_t upto = mine;
     upto += dpp_u32<0x111, 0xF>(upto);
     upto += dpp_u32<0x112, 0xF>(upto);
@@ -182,80 +194,101 @@ __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
     upto += dpp_u32<0x142, 0xA>(upto);
     upto += dpp_u32<0x143, 0xC>(upto);
     const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-    // Few enough, and none of them a place outside the row.
-    if (n <= 17 * P && (whole || least > -INFINITY)) {
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(&count, n);
-      uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)base) + upto - mine;
-      if (mine) {
+    auto key = [&](float x, uint32_t token) { return (u64)beam_ord(x) << 32 | ~token; };
+    auto hold = [&]() {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (v[i] >= least) list[at++] = key(i);
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(held + t * 16 + 4 * j) = f32x4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
+    };
+    if (used + n <= beam_held(P) && least > -INFINITY) {
+      if (bits) {
+        hold();
+        uint32_t at = used + upto - mine;
+        do {
+          const uint32_t e = (uint32_t)__clz((int)bits) - 16;
+          list[at++] = key(held[t * 16 + e], tok0 + t * 4 + 1024 * (e / 4) + e % 4);
+          bits &= ~(0x8000u >> e);
+        } while (bits);
       }
+      used += n;
     } else {
-      // Those above the single lanes' threshold, then the first P of the equal
-      // ones.
-      least = fmaxf(floor, threshold(tm, std::integral_constant<int, 1>{}));
-      uint32_t above = 0, met = 0;
-      u64 mask[16];
-      bool same[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int64_t k = tok + 1024 * (i / 4) + i % 4;
-        above += (uint32_t)__popcll(__ballot(v[i] > least));
-        same[i] = v[i] == least && k >= 0 && k < (int64_t)a.vocab;
-        mask[i] = __ballot(same[i]);
-        met += (uint32_t)__popcll(mask[i]);
-      }
-      met = min(met, P);
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(&count, above + met);
-      base = (uint32_t)__builtin_amdgcn_readfirstlane((int)base);
-      uint32_t seen = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {  // tokens ascend over j, then the lanes, then c
-        uint32_t at = seen;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) at += count_below(mask[4 * j + c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (same[4 * j + c]) {
-            if (at < P) list[base + at] = key(4 * j + c);
-            ++at;
-          }
-          seen += (uint32_t)__popcll(mask[4 * j + c]);
+      if (used > P) {  // the P largest, by way of the places behind the list
+        wave_lds();
+        u64* const best = list + beam_held(P);
+        for (uint32_t e = lane; e < used; e += 64) {
+          const u64 k = list[e];
+          uint32_t r = 0;
+          for (uint32_t o = 0; o < used; ++o) r += list[o] > k ? 1u : 0u;
+          if (r < P) best[r] = k;
         }
+        wave_lds();
+        if (lane < P) list[lane] = best[lane];
+        used = P;
       }
-      base += met;
+      // 64 logits at a time in token order: the fours 0 of all lanes, the fours
+      // 1, ..
+      const float edge = fmaxf(least, threshold(tm, std::integral_constant<int, 1>{}));
+      hold();
+      wave_lds();
+      auto look = [&](uint32_t r, uint32_t& token) {
+        const uint32_t from = wave * 64 + r % 4 * 16 + lane / 4;
+        token = tok0 + from * 4 + 1024 * (r / 4) + lane % 4;
+        return fmaxf(held[from * 16 + 4 * (r / 4) + lane % 4], -INFINITY);
+      };
+      uint32_t token, met = 0;
+      for (uint32_t r = 0; r < 16; ++r) {
+        const float x = look(r, token);
+        const bool same = x == edge && token < a.vocab;
+        const u64 m1 = __ballot(x > edge), m2 = __ballot(same);
+        if (x > edge) list[used + count_below(m1)] = key(x, token);
+        used += (uint32_t)__popcll(m1);
+        const uint32_t at = met + count_below(m2);
+        if (same && at < P) list[used + at - met] = key(x, token);
+        const uint32_t more = min((uint32_t)__popcll(m2), P - met);
+        used += more;
+        met += more;
+      }
+      wave_lds();
+    }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const u64 m1 = __ballot(v[i] > least);
-        if (v[i] > least) list[base + count_below(m1)] = key(i);
-        base += (uint32_t)__popcll(m1);
-      }
-    }
-    __syncthreads();
-    const uint32_t all = count, before = tile > tile0 ? P : 0u;
-    for (uint32_t e = t; e < all + before; e += 256) {
-      const u64 k = e < all ? list[e] : top[e - all];
-      if (!k) continue;
-      uint32_t r = 0, i = 0;
-      for (; i + 4 <= all; i += 4) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + i), y = *reinterpret_cast<const ulonglong2*>(list + i + 2);
-        r += (x.x > k ? 1u : 0u) + (x.y > k ? 1u : 0u) + (y.x > k ? 1u : 0u) + (y.y > k ? 1u : 0u);
-      }
-      for (; i < all; ++i) r += list[i] > k ? 1u : 0u;
-      for (i = 0; i < before; ++i) r += top[i] > k ? 1u : 0u;
-      if (r < P) out[r] = k;
-    }
-    __syncthreads();
-    if (t < P) top[t] = out[t];
-    if (a.tiles > 1) __syncthreads();
+    for (int j = 0; j < 4; ++j) q[j] = ahead[j];
   }
+  // What is >= the waves' largest T, then ranks by counting, a quarter of those
+  // per lane of a quad.
+  u64* const all = lists + 4 * (beam_held(P) + P);
+  if (lane == 0) least_of[wave] = least;
+  if (t == 0) count = 0;
+  __syncthreads();
+  const float floor = fmaxf(fmaxf(least_of[0], least_of[1]), fmaxf(least_of[2], least_of[3]));
+  const u64 from = (u64)beam_ord(floor) << 32;
+  for (uint32_t e = lane; e < used + lane; e += 64) {
+    const u64 k = e < used ? list[e] : 0;
+    const u64 mask = __ballot(k >= from && k);
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&count, (uint32_t)__popcll(mask));
+    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+    if (k >= from && k) all[at + count_below(mask)] = k;
+  }
+  __syncthreads();
+  u64* const out = a.cand + (uint64_t)blockIdx.x * P;
+  const uint32_t n = count, part = t & 3, per = (n + 15) / 16 * 4;
+  for (uint32_t e = t / 4; e < (n + 15) / 16 * 16; e += 64) {
+    const u64 k = e < n ? all[e] : 0;
+    uint32_t r = 0, i = part * per;
+    const uint32_t last = min(i + per, n);
+    for (; i + 4 <= last; i += 4) {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(all + i), y = *reinterpret_cast<const ulonglong2*>(all + i + 2);
+      r += (x.x > k ? 1u : 0u) + (x.y > k ? 1u : 0u) + (y.x > k ? 1u : 0u) + (y.y > k ? 1u : 0u);
+    }
+    for (; i < last; ++i) r += all[i] > k ? 1u : 0u;
+    r += dpp_u32<0xB1, 0xF>(r);
+    r += dpp_u32<0x4E, 0xF>(r);
+    if (part == 0 && k && r < P) out[r] = k;
+  }
+  if (t >= n && t < P) out[t] = 0;
   const float wm = wave_max_f32(m);
   const double ws = wave_sum_f64(m > -INFINITY ? sum * (double)beam_exp(m - wm) : 0.0);
   if (lane == 0) a.stats[(uint64_t)blockIdx.x * 4 + wave] = BeamStat{ws, wm, 0u};
-  if (t < P) a.cand[(uint64_t)blockIdx.x * P + t] = top[t];
 }
 
 struct BeamKey {
@@ -403,7 +436,10 @@ static uint64_t al256(uint64_t n) { return (n + 255) & ~255ull; }
 uint64_t beam_workspace(uint32_t requests, uint32_t beams, uint32_t vocab, uint32_t picks, BeamArgs* a, uint8_t* base) {
   // Tiles of a row start up to three logits ahead of it.
   const uint32_t tiles = (vocab + 3 + kBeamTile - 1) / kBeamTile;
-  const uint32_t per = (tiles + kBeamMaxSlices - 1) / kBeamMaxSlices, slices = (tiles + per - 1) / per;
+  const uint64_t rows = (uint64_t)requests * beams;
+  const uint32_t per = (uint32_t)std::max<uint64_t>((tiles + kBeamMaxSlices - 1) / kBeamMaxSlices,
+                                                    std::min<uint64_t>((rows * tiles + kBeamBlocks - 1) / kBeamBlocks, tiles));
+  const uint32_t slices = (tiles + per - 1) / per;
   const uint64_t lists = (uint64_t)requests * beams * slices;
   const uint64_t sb = al256(lists * 4 * sizeof(BeamStat));
   if (a) {
@@ -416,7 +452,7 @@ uint64_t beam_workspace(uint32_t requests, uint32_t beams, uint32_t vocab, uint3
 }
 
 hipError_t launch_beam_select(const BeamArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(k_beam_slice, dim3(a.rows * a.slices), dim3(256), (4 * 17 + 2) * a.picks * 8, st, a);
+  hipLaunchKernelGGL(k_beam_slice, dim3(a.rows * a.slices), dim3(256), (4 * (beam_held(a.picks) + a.picks) + 4 * beam_held(a.picks)) * 8, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t lds = a.beams * a.picks * sizeof(BeamKey) + 4 * a.picks * 64 * 8;

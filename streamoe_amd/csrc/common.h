@@ -507,4 +507,12 @@ inline hipError_t raise_lds_limit(const void* fn, int bytes, std::atomic<uint64_
   return e;
 }
 
+// Orders a wave's own LDS traffic (which the hardware runs in order) for the
+// compiler.
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 }  // namespace smoe

@@ -340,14 +340,6 @@ __host__ __device__ constexpr uint32_t q8_wide_lds(uint32_t bits, uint32_t K, ui
   return mt * (steps * 2048 + (groups + 7) / 8 * 1024 + (xg ? groups * 64 : 0)) + 4 * 256 * (bits == 8 ? 32 : 16);
 }
 
-// Orders a wave's own LDS traffic (which the hardware runs in order) for the
-// compiler.
-__device__ __forceinline__ void wave_lds() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 template <int BITS, int G, bool XG, int MT>
 __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
   constexpr uint32_t GS = kQ8Step / G, W = BITS == 8 ? 8 : BITS, GC = GS * kWideSteps;  // groups per round
