@@ -10,7 +10,11 @@ most 36 u, its f32 score by u |score| more. Within a row the log-sum-exp is
 one number, so there the order is exact; and so it is between rows of the same
 logits. Rows whose log-sum-exps are equal only as real numbers (one row another
 one's permutation) may come in either order, each value being off by up to
-36 u: two picks of different rows whose 64-bit values are within 72 u."""
+36 u: two picks of different rows whose 64-bit values are within 72 u.
+
+Of many rows a wave takes several tiles of 4096 in turn; a tile with a larger
+logit scales the sum before it by one more exponential, 2 u per tile (what the
+differences' rounding adds is in the 19 u: they add up to |l - m|)."""
 import numpy as np
 import pytest
 
@@ -75,7 +79,7 @@ def _either_order(logits, scores, done, pad, R, W, V, P, rows, tok, wv, wr):
             assert np.array_equal(own, at[q][ar[q] == r][:len(own)])
 
 
-def _check(kernels, logits, scores, done, pad, R, W, V, P):
+def _check(kernels, logits, scores, done, pad, R, W, V, P, tiles=1):
     import torch
 
     host = logits.cpu().numpy() if isinstance(logits, torch.Tensor) else logits
@@ -85,7 +89,7 @@ def _check(kernels, logits, scores, done, pad, R, W, V, P):
         _either_order(host, scores, done, pad, R, W, V, P, rows, tok, wv, wr)
     fin = np.isfinite(wv)
     assert np.array_equal(v[~fin], wv[~fin])
-    assert np.all(np.abs(v - wv)[fin] <= 36 * U + U * np.abs(wv[fin]))
+    assert np.all(np.abs(v - wv)[fin] <= (34 + 2 * tiles) * U + U * np.abs(wv[fin]))
 
 
 @pytest.mark.parametrize("R,W,V,P", [
@@ -106,6 +110,31 @@ def test_all_logits_equal(kernels):
     # Every thread holds the same values: only the token decides.
     for V in (40, 5000, 20000):
         _check(kernels, np.full((3, V), 1.5, np.float32), np.zeros(3, np.float32), None, 0, 1, 3, V, 32)
+
+
+@pytest.mark.parametrize("R,W,V,P", [(64, 16, 5000, 32), (40, 4, 30000, 8), (300, 2, 12289, 4), (70, 2, 40001, 15)])
+@pytest.mark.parametrize("kind", ["random", "rising", "falling", "steps", "late", "nan"])
+def test_several_tiles_in_turn(kernels, R, W, V, P, kind):
+    rng = np.random.default_rng(R + P)
+    l = (rng.standard_normal((R * W, V)) * 2.5).astype(np.float32)
+    if kind == "rising":      # every tile has more than the list holds
+        l = np.broadcast_to(np.arange(V, dtype=np.float32) / 64, (R * W, V)).copy()
+    elif kind == "falling":
+        l = np.broadcast_to(-np.arange(V, dtype=np.float32) / 64, (R * W, V)).copy()
+    elif kind == "steps":     # ties everywhere, larger ones later
+        l = np.broadcast_to(np.floor(np.arange(V) / 1500).astype(np.float32), (R * W, V)).copy()
+    elif kind == "late":      # nothing in the first tiles, ties of few values behind
+        l = np.round(l)
+        l[:, : V // 2] = -np.inf
+    elif kind == "nan":       # of both signs and kinds
+        bits = l.view(np.uint32)
+        at = rng.random(l.shape)
+        bits[at < 0.4] = 0x7FC00000
+        bits[at < 0.3] = 0xFFC00001
+        bits[at < 0.2] = 0x7F800001
+        bits[at < 0.1] = 0xFF8FFFFF
+    sc = (-10 * rng.random(R * W)).astype(np.float32)
+    _check(kernels, l, sc, None, 0, R, W, V, P, tiles=10)
 
 
 def test_ties_across_rows_and_zeros_of_both_signs(kernels):
