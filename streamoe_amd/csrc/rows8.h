@@ -307,13 +307,14 @@ __device__ __forceinline__ qbf16x8 q8_parts(float a, float b) {
 
 // ---------------------------------------------------------------------------
 // Few rows, many columns: the rows stay in LDS, as operands, and the waves
-// stream the weights, a tile of 16 columns at a time over all inputs, four
-// steps ahead. A wave's load takes four rows' codes of those steps, whole lines
+// stream the weights, a tile of 16 columns after another, four steps (a round)
+// at a time. A wave's load takes four rows' codes of those steps, whole lines
 // (256 bytes a row with 4 bits), and its own part of LDS hands them to the
 // operands' lanes. The loads are non-temporal: weights that a step reads once
-// come from HBM (16 rows 2048 -> 151936, three sets of weights in turn: 42 us,
-// 4.4 TB/s, temporal 45; the same set again and again 41 and, from the
-// memory-side cache, 35); without the arithmetic, temporal, 43.5. Rows
+// come from HBM (16 rows 2048 -> 151936, three sets of weights in turn: 40 us,
+// 4.6 TB/s, temporal 42.5; the same set again and again 39 and, from the
+// memory-side cache, 34). Two rounds are in flight while one is computed (one:
+// 43, three: 41, five: 42), for which nothing between them may branch. Rows
 // are the A operand: lane (c, kb) ends with column c of rows 4 kb .. 4 kb + 3,
 // and needs the scales of one column only.
 // ---------------------------------------------------------------------------
@@ -363,6 +364,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
     uint32_t w[kWideSteps][W];
     uint32_t s[PW], b[PW];
   };
+  auto group_of = [&](uint32_t rd, uint32_t i) { return rd * GC + 8 * i + 2 * (GC < 8 ? kb & 1 : kb); };
   auto load = [&](uint32_t tile, uint32_t rd, Round& v) {
     const uint32_t col = min(tile * 16 + c16, O - 1);
     const uint32_t chunk = min(rd * kWideSteps * 4 + lp, K / 32 - 1) * (BITS * 4);
@@ -380,26 +382,31 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
       }
     }
     // Pairs of groups: lane block kb those of pair kb (and 4 + kb); the last
-    // group again past the end.
+    // two again past the end.
 #pragma unroll
     for (uint32_t i = 0; i < PW; ++i) {
-      const uint32_t g = rd * GC + 8 * i + 2 * (GC < 8 ? kb & 1 : kb);
-      const uint64_t at = (uint64_t)col * gpr;
-      if (a.even) {
-        const uint64_t e = at + min(g, gpr - 2);
-        v.s[i] = *reinterpret_cast<const uint32_t*>(a.s + e);
-        v.b[i] = *reinterpret_cast<const uint32_t*>(a.b + e);
-      } else {
-        const uint64_t e0 = at + min(g, gpr - 1), e1 = at + min(g + 1, gpr - 1);
-        v.s[i] = a.s[e0] | (uint32_t)a.s[e1] << 16;
-        v.b[i] = a.b[e0] | (uint32_t)a.b[e1] << 16;
-      }
+      const uint32_t g = group_of(rd, i);
+      const uint64_t e = (uint64_t)col * gpr + min(g, gpr - 2);
+      __builtin_memcpy(&v.s[i], a.s + e, 4);  // on two bytes
+      __builtin_memcpy(&v.b[i], a.b + e, 4);
     }
   };
   const uint32_t stride = gridDim.x * 4;
   uint32_t tile = blockIdx.x * 4 + wave;
-  Round v[2];
-  if (tile < tiles) load(tile, 0, v[0]);
+  uint32_t rd = 0, lt = tile, ld = 0;  // computed next, loaded next
+  auto next = [&](uint32_t& t, uint32_t& r) {
+    if (++r == rounds) r = 0, t += stride;
+  };
+  // Without a branch, or the waits for a round would be for all of them; past
+  // the last tile the first again.
+  constexpr int D = BITS == 8 ? 2 : 3;
+  Round v[D];
+  auto ahead = [&](Round& v) {
+    load(lt < tiles ? lt : min(tile, tiles - 1), ld, v);
+    next(lt, ld);
+  };
+#pragma unroll
+  for (int k = 0; k < D - 1; ++k) ahead(v[k]);
 
   // The rows as operands; rows past the last and inputs from K on are zero.
   for (uint32_t i = tid; i < steps * 8 * MT * 16; i += 256) {
@@ -453,7 +460,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
   constexpr int kStart = XG ? (int)kMagicBits : 0;
   const i32x4 start = {kStart, kStart, kStart, kStart};
   auto from = [&](int src, uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)x); };
-  auto compute = [&](uint32_t rd, const Round& v) {
+  auto compute = [&](uint32_t rd, Round& v) {
     static_assert(kWideSteps == 4, "16 chunks of a row, four rows per load");
     wave_lds();  // the last round's reads come first
 #pragma unroll
@@ -467,6 +474,11 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
       }
     }
     wave_lds();
+    if (gpr & 1) {  // the last group alone, loaded behind the one before
+#pragma unroll
+      for (uint32_t i = 0; i < PW; ++i)
+        if (group_of(rd, i) == gpr - 1) v.s[i] >>= 16, v.b[i] >>= 16;
+    }
     // The bias term of this round's eights (G = 128: a round is half of one).
 #pragma unroll
     for (uint32_t i = 0; i < PW; ++i) {
@@ -523,6 +535,13 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
       }
     }
   };
+  f32x4 sxr[MT];  // the rows' scales
+  if constexpr (!XG) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sxr[m][k] = a.sx[min((uint32_t)(m * 16 + 4 * kb + k), a.n - 1)];
+  }
   auto finish = [&](uint32_t tile) {
     const uint32_t col = tile * 16 + c16;
 #pragma unroll
@@ -530,28 +549,21 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t r = m * 16 + 4 * kb + k;
-        if (r < a.n && col < O) a.y[(uint64_t)r * O + col] = XG ? acc[m][k] : acc[m][k] * a.sx[r];
+        if (r < a.n && col < O) a.y[(uint64_t)r * O + col] = XG ? acc[m][k] : acc[m][k] * sxr[m][k];
       }
       acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   };
-  // Rounds of all of the wave's tiles in one sequence, two at a time.
-  uint32_t rd = 0;
-  auto next = [&](uint32_t& t, uint32_t& r) {
-    if (++r == rounds) r = 0, t += stride;
-  };
+  // Rounds of all of the wave's tiles in one sequence.
   while (tile < tiles) {
-    uint32_t t1 = tile, r1 = rd;
-    next(t1, r1);
-    if (t1 < tiles) load(t1, r1, v[1]);
-    compute(rd, v[0]);
-    if (rd + 1 == rounds) finish(tile);
-    if (t1 >= tiles) break;
-    tile = t1, rd = r1;
-    next(tile, rd);
-    if (tile < tiles) load(tile, rd, v[0]);
-    compute(r1, v[1]);
-    if (r1 + 1 == rounds) finish(t1);
+#pragma unroll
+    for (int k = 0; k < D; ++k) {
+      ahead(v[(k + D - 1) % D]);
+      compute(rd, v[k]);
+      if (rd + 1 == rounds) finish(tile);
+      next(tile, rd);
+      if (tile >= tiles) return;
+    }
   }
 }
 
@@ -1001,8 +1013,9 @@ static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   // tiles a block 6.3; 32 rows: 7.2 and, two row tiles a block, 6.1).
   if (rt * ct <= 256) return q8_few<BITS, G, XG, 1, 1>(a, std::min(steps, 16u), st);
   if (rt == 1) {
-    // 16 rows 2048 -> 16384: 8.6, rows in LDS 10.3; -> 50000: 39 and 18.
-    if (ct <= 1024 || q8_wide_lds(BITS, a.K, G, 1, XG) > 160 * 1024)
+    // 16 rows 2048 -> 16384, weights from HBM: 10.0, rows in LDS 10.1; -> 24576:
+    // 13.7 and 12.6; -> 32768: 16.8 and 13.5.
+    if (ct <= 1024 || a.K < 2 * G || q8_wide_lds(BITS, a.K, G, 1, XG) > 160 * 1024)
       return q8_few<BITS, G, XG, 1, 2>(a, std::min(steps, 8u), st);
     return q8_wide<BITS, G, XG, 1>(a, st);
   }
