@@ -116,8 +116,8 @@ __device__ __forceinline__ i32x4 q8_sums(const u32x4 (&x)[2], const u32x4 (&b)[2
 // order: lane 4 r + p takes part p (32 inputs) of row r, one cache access per
 // four lanes where the operand order would take one per lane, and a lane
 // permute brings the parts to the operand's lanes (4 rows 2048 -> 4096 took
-// 5.9 us in operand order). Rows are the A operand: lane (c, kb) ends with column c of rows 4 kb
-// .. 4 kb + 3. The sums of inputs come from a product with ones; the waves'
+// 5.9 us in operand order). Rows are the A operand: lane (c, kb) ends with
+// column c of rows 4 kb .. 4 kb + 3. The sums of inputs come from a product with ones; the waves'
 // parts are added in LDS.
 // ---------------------------------------------------------------------------
 template <int BITS, int G, bool XG, int MT, int NT>
@@ -177,14 +177,11 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_q8_few(Q8Args a) 
         }
       }
     }
-    const uint32_t at = k0 + lp * 32;
+    const uint32_t at = min(k0 + lp * 32, K - 32);  // K is a multiple of 32
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      v.x[m][0] = v.x[m][1] = u32x4{0u, 0u, 0u, 0u};
-      if (at < K) {  // K is a multiple of 32
-        v.x[m][0] = *reinterpret_cast<const u32x4*>(xr[m] + at);
-        v.x[m][1] = *reinterpret_cast<const u32x4*>(xr[m] + at + 16);
-      }
+      v.x[m][0] = *reinterpret_cast<const u32x4*>(xr[m] + at);
+      v.x[m][1] = *reinterpret_cast<const u32x4*>(xr[m] + at + 16);
       if constexpr (XG)
 #pragma unroll
         for (uint32_t j = 0; j < GS; ++j) v.sx[m][j] = sxr[m][min(st * GS + j, gpr - 1)];
@@ -199,13 +196,14 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_q8_few(Q8Args a) 
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](const Step& v) {
+  auto compute = [&](uint32_t st, const Step& v) {
+    const bool in = st * kQ8Step + lp * 32 < K;
     u32x4 x[MT][2], w[NT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       uint32_t d[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = from(psrc, v.x[m][i / 4][i % 4]);
+      for (int i = 0; i < 8; ++i) d[i] = from(psrc, in ? v.x[m][i / 4][i % 4] : 0u);
       q8_exchange<G>(d);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -256,29 +254,48 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_q8_few(Q8Args a) 
       }
     }
   };
-  Step v[2];
-  if (wave < steps) load(wave, v[0]);
-  for (uint32_t st = wave; st < steps; st += 2 * nw) {
-    if (st + nw < steps) load(st + nw, v[1]);
-    compute(v[0]);
-    if (st + nw >= steps) break;
-    if (st + 2 * nw < steps) load(st + 2 * nw, v[0]);
-    compute(v[1]);
+  f32x4 scale[MT];  // of the rows that the wave ends
+  if (!XG && wave < MT * NT) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) scale[m][i] = a.sx[min(row0 + m * 16 + 4 * kb + i, a.n - 1)];
   }
+  // Every path to a use of a step has the same loads behind it, or the wait
+  // would be for all of them.
+  Step v[2];
+  uint32_t st = wave;  // there are no more waves than steps
+  load(st, v[0]);
+  while (st + nw < steps) {
+    load(st + nw, v[1]);
+    compute(st, v[0]);
+    st += nw;
+    if (st + nw >= steps) {
+      v[0] = v[1];
+      break;
+    }
+    load(st + nw, v[0]);
+    compute(st, v[1]);
+    st += nw;
+  }
+  compute(st, v[0]);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) red[(wave * MT * NT + m * NT + t) * 64 + lane] = acc[m][t];
   __syncthreads();
   for (uint32_t mt = wave; mt < MT * NT; mt += nw) {
-    f32x4 sum = red[mt * 64 + lane];
+    f32x4 sum = red[mt * 64 + lane], by = scale[0];
+#pragma unroll
+    for (uint32_t m = 1; m < MT; ++m)
+      if (mt / NT == m) by = scale[m];
     for (uint32_t w = 1; w < nw; ++w) sum += red[(w * MT * NT + mt) * 64 + lane];
     const uint32_t col = col0 + mt % NT * 16 + c16;
     if (col >= O) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = row0 + mt / NT * 16 + 4 * kb + i;
-      if (r < a.n) a.y[(uint64_t)r * O + col] = XG ? sum[i] : sum[i] * a.sx[r];
+      if (r < a.n) a.y[(uint64_t)r * O + col] = XG ? sum[i] : sum[i] * by[i];
     }
   }
 }
