@@ -950,16 +950,18 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 2 : KS) void k_q8_tile(Q8Args a
         for (int k = 0; k < KS - 1; ++k) acc[m][t] += part[(k * MT * NT + m * NT + t) * 256 + tid];
   }
 
+  float scale[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) scale[m] = XG ? 1.f : a.sx[min(row0 + (wm * MT + m) * 16 + c16, a.n - 1)];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const uint32_t r = row0 + (wm * MT + m) * 16 + c16;
     if (r >= a.n) continue;
-    const float sx = XG ? 1.f : a.sx[r];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const uint32_t col = col0 + (wn * NT + t) * 16 + 4 * kb;
       float* const y = a.y + (uint64_t)r * O + col;
-      const f32x4 v = acc[m][t] * sx;
+      const f32x4 v = acc[m][t] * scale[m];
       if (a.vec) {
         if (col < O) *reinterpret_cast<f32x4*>(y) = v;
       } else {
