@@ -284,7 +284,11 @@ __device__ __forceinline__ LoraItem lora_item(const LoraArgs& a, uint32_t lane, 
 enum LoraBy { kByPlan, kByWave, kByBlock };
 
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
-// steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c.
+// steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c. A
+// share per block makes blocks of few rows: 8 rows, 4 adapters of rank 16, 2048
+// inputs 2.6 us (one round trip each for the ids, the rows and the shares' sum);
+// 200 rows, 40 adapters of rank 64, 4096 inputs 8.9 us for 24 MB, of which
+// finding the items is about 3.
 template <bool XBF16, LoraBy BY, int MT>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   __shared__ f32x4 red[4][64];
@@ -380,7 +384,10 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
 // itself the shares were 22 of 33 us: 200 rows, 40 adapters of rank 64, 4096 ->
 // 4096). The products go through LDS too, so that base and y move in whole rows
 // of the block (in the products' order each lane touches a line of its own).
-// B's and base's loads go out ahead of everything.
+// B's and base's loads go out ahead of everything. 8 rows -> 2048 3.2 us, the
+// 200 rows -> 4096 8.6 us for 28 MB, 1000 rows of rank 32 -> 4096 11.3 us for
+// 33 MB of base and y: all blocks run at once, so the loads of items, shares
+// and base come one after another for each of them.
 template <int KT, int NT>
 __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   constexpr uint32_t RP = KT * 32 + 8;  // bf16 per row in LDS: rows apart by 16 bytes of banks
