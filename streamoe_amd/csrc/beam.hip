@@ -100,11 +100,13 @@ __host__ __device__ constexpr uint32_t beam_held(uint32_t picks) { return 18 * p
 // suffice. In the end the block ranks what is >= the waves' largest T by
 // counting.
 //
-// Four rows of 151936 (one tile a block) take 6.3 us, the latency of loads,
-// threshold, list and ranks one after another; 64 rows 11.9 us for 39 MB, of
-// which the loads alone are 5.7 and the exponentials 2: a wave runs some 350
-// VALU instructions per tile. One tile a block took 14 us there (each with a
-// threshold, a list to rank and its reductions).
+// Four rows of 151936 (one tile a block) take 5 to 6 us, of which the loads are
+// 2.0, threshold 0.7, list and ranks 1.7; 64 rows 11.9 us for 39 MB: loads 5.2,
+// the exponentials 2.5, thresholds 2.4, lists 1.5, most of it VALU time (some
+// 350 instructions of a wave per tile). One tile a block took 14 us there (each
+// with a threshold, a list to rank and its reductions). Peeling the last tile
+// off, so that no branch stands between a tile's loads and its use, gained
+// nothing.
 __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
   extern __shared__ __attribute__((aligned(16))) u64 lists[];  // per wave [19 P]; all waves' [72 P]
   __shared__ __attribute__((aligned(16))) float held[256 * 16];  // logits of threads that have one for the list
