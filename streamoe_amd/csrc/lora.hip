@@ -7,6 +7,7 @@
 //   k_lora_down    u = A x of an item's rows on bf16 MFMA, one share of the
 //                  inputs per block, partial sums in f32; leaves the items
 //   k_lora_up      the shares added, scaled, times B on bf16 MFMA, plus base
+//   k_lora_one     the last two for few rows and little of A
 //
 // f32 values enter the matrix cores as bf16 pairs, v = hi + lo, each rounded
 // to nearest: off by at most 2^-16 |v| (hi leaves up to 2^-8 |v|, of which lo
@@ -121,11 +122,14 @@ __global__ __launch_bounds__(1024) void k_lora_plan(LoraArgs a) {
 constexpr uint32_t kLoraSmall = 64;  // rows whose items need no plan: one per lane
 
 // Item blockIdx.x of a call of up to 64 rows, by every wave for itself: the
-// rows' ids, one per lane, taken group by group in the order of their first
-// rows; `rows` receives the item's rows (kLoraM per wave).
+// rows' ids, one per lane, the lanes of the same id from ballots of its bits;
+// every 16th of them starts an item, items are in the order of those lanes.
+// `rows` receives the item's rows (kLoraM per wave). (Adapter after adapter in a
+// loop a call of 64 rows of 64 adapters took 18 us, 9.5 so.)
 __device__ __forceinline__ LoraItem lora_wave_item(const LoraArgs& a, uint32_t lane, uint32_t* rows) {
-  const int32_t id = lane < a.n ? a.ids[lane] : -2;
-  const bool bad = lane < a.n && (id < -1 || id >= (int32_t)a.n_adapters);
+  const bool there = lane < a.n;
+  const int32_t id = a.ids[min(lane, a.n - 1)];
+  const bool bad = there && (id < -1 || id >= (int32_t)a.n_adapters);
   const uint32_t ad = bad || id < 0 ? a.n_adapters : (uint32_t)id;
   uint32_t rank = 0;  // of the lane's adapter
   float scale = 0.f;
@@ -136,27 +140,28 @@ __device__ __forceinline__ LoraItem lora_wave_item(const LoraArgs& a, uint32_t l
       for (uint32_t i = lane; i < a.n_adapters; i += 64) wrong |= a.ranks[i] < 0 || a.ranks[i] > (int32_t)a.max_rank;
     if (wrong) *a.err = 2u;
   }
-  uint64_t left = __ballot(lane < a.n);
-  uint32_t item = blockIdx.x, start = 0;
+  uint64_t same = __ballot(there);
+  for (uint32_t bit = 0; a.n_adapters >> bit; ++bit) {
+    const bool set = ad >> bit & 1;
+    const uint64_t m = __ballot(set);
+    same &= set ? m : ~m;
+  }
+  auto below = [](uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
+  const uint32_t place = below(same), all = (uint32_t)__popcll(same);
+  const bool first = there && place % kLoraM == 0;
+  const uint64_t firsts = __ballot(first);
+  const uint32_t count = first ? min(kLoraM, all - place) : 0u, upto = lora_scan(count);
+  const uint64_t which = __ballot(first && below(firsts) == blockIdx.x);
   LoraItem it{0u, 0u, 0u, 0u, 0.f};
-  while (left) {
-    const uint32_t leader = (uint32_t)__ffsll((long long)left) - 1;
-    const uint32_t mine = (uint32_t)__builtin_amdgcn_readlane((int)ad, (int)leader);
-    const uint64_t group = __ballot(lane < a.n && ad == mine);
-    const uint32_t c = (uint32_t)__popcll(group), items = (c + kLoraM - 1) / kLoraM;
-    if (item < items) {
-      const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(group >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)group, 0u));
-      if ((group >> lane & 1) && at / kLoraM == item) rows[at % kLoraM] = lane;
-      it = LoraItem{mine, start + item * kLoraM, min(kLoraM, c - item * kLoraM),
-                    (uint32_t)__builtin_amdgcn_readlane((int)rank, (int)leader), readlane_f(scale, (int)leader)};
-      break;
-    }
-    item -= items;
-    start += c;
-    left &= ~group;
+  if (which) {
+    const int lead = __ffsll((long long)which) - 1;
+    auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lead); };
+    it = LoraItem{of(ad), of(upto - count), of(count), of(rank), readlane_f(scale, lead)};
+    const uint32_t at = place - of(place);
+    if (there && ad == it.adapter && at < kLoraM) rows[at] = lane;
   }
   // The rows are in LDS: no other wave writes or reads this part.
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  wave_lds();
   return it;
 }
 
@@ -515,6 +520,131 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   }
 }
 
+// Both products of a small item in one launch: sixteen waves share the inputs
+// (step s is wave s mod 16's), their parts are added in LDS, and each wave takes
+// 16 outputs. Every block of 256 outputs forms u for itself, from the caches (8
+// rows, 4 adapters of rank 16, 2048 -> 2048: 6.1 us, the two kernels 5.8 and a second launch): what a
+// CU can load bounds it, 64 bytes a cycle.
+template <bool XBF16, int MT>
+__global__ __launch_bounds__(1024) void k_lora_one(LoraArgs a) {
+  constexpr int KT = (MT + 1) / 2, U = MT <= 2 ? 4 : 2;  // steps of 32 ranks; steps of inputs in flight
+  constexpr uint32_t RP = KT * 32 + 8;                   // as in k_lora_up
+  __shared__ __attribute__((aligned(16))) float red[16][256];
+  __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
+  __shared__ uint32_t of_wave[16][kLoraM];
+  const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, kb = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const LoraItem it = lora_wave_item(a, lane, of_wave[wave]);
+  if (it.count == 0) return;
+  const bool none = it.adapter >= a.n_adapters;
+  if (none && a.base == a.y) return;
+  const uint32_t row = of_wave[wave][min(c16, it.count - 1)];
+  const uint32_t K = a.in_dim, O = a.out_dim, R = a.max_rank, rank = none ? 0u : it.rank, steps = (K + 31) / 32;
+  const uint32_t o0 = (blockIdx.y * 16 + wave) * 16, o = o0 + 4 * kb;
+  // B's rows and base first: they are needed last.
+  lbf16x8 b[KT];
+  if (rank) {
+    const uint16_t* const B = (const uint16_t*)(a.b + (uint64_t)it.adapter * a.b_stride) + (uint64_t)min(o0 + c16, O - 1) * R;
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      const uint32_t k = s * 32 + kb * 8;
+      b[s] = *reinterpret_cast<const lbf16x8*>(B + (k < R ? k : 0));  // R is a multiple of 8
+    }
+  }
+  const bool mine = c16 < it.count;
+  const uint64_t e = (uint64_t)row * O + o;
+  f32x4 base = {0.f, 0.f, 0.f, 0.f};
+  if (a.base && mine) {
+    if (a.vec) {
+      if (o < O) base = *reinterpret_cast<const f32x4*>(a.base + e);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (o + c < O) base[c] = a.base[e + c];
+    }
+  }
+  f32x4 low = {0.f, 0.f, 0.f, 0.f};
+  if (rank) {  // the same for the whole block
+    const uint32_t nt = (rank + 15) / 16;
+    const uint16_t* const A = (const uint16_t*)(a.a + (uint64_t)it.adapter * a.a_stride);
+    using X = std::conditional_t<XBF16, lbf16x8, lf32x8>;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s0 = wave; s0 < steps; s0 += 16 * U) {
+      X x[U];
+      lbf16x8 w[U][MT];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const uint32_t k = (s0 + 16 * j) * 32 + kb * 8, kc = k < K ? k : 0;  // K is a multiple of 8
+        if (s0 + 16 * j >= steps) continue;
+        x[j] = X{};
+        if (mine) x[j] = *reinterpret_cast<const X*>(reinterpret_cast<const uint8_t*>(a.x) + ((uint64_t)row * K + kc) * (sizeof(X) / 8));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          if (i < (int)nt) w[j][i] = *reinterpret_cast<const lbf16x8*>(A + (uint64_t)min(i * 16 + c16, rank - 1) * K + kc);
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (s0 + 16 * j >= steps) break;
+        const bool in = (s0 + 16 * j) * 32 + kb * 8 < K;
+        lbf16x8 hi, lo;
+        if constexpr (XBF16) {
+          hi = first_of(x[j], in ? 8 : 0);
+        } else {
+          split_bf16(x[j], hi, lo);
+          hi = first_of(hi, in ? 8 : 0);
+          lo = first_of(lo, in ? 8 : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (i >= (int)nt) break;
+          const lbf16x8 v = first_of(w[j][i], in && i * 16 + c16 < rank ? 8 : 0);
+          acc[i] = mfma_bf16(hi, v, acc[i]);
+          if constexpr (!XBF16) acc[i] = mfma_bf16(lo, v, acc[i]);
+        }
+      }
+    }
+    const uint32_t t = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2 * KT; ++i) {  // tiles behind the rank leave zeros
+      const f32x4 v = i < MT ? acc[i < MT ? i : 0] : f32x4{0.f, 0.f, 0.f, 0.f};
+      if (i) __syncthreads();
+      *reinterpret_cast<f32x4*>(&red[wave][lane * 4]) = v;
+      __syncthreads();
+      // Value 4 l + r: row 4 (l / 16) + r, rank 16 i + l % 16.
+      if (t < 256) {
+        float sum = red[0][t];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) sum += red[w][t];
+        const uint32_t j = i * 16 + (t >> 2 & 15), at = ((t >> 6) * 4 + (t & 3)) * RP + j;
+        const float f = j < rank ? sum * it.scale : 0.f;
+        const __bf16 hi = (__bf16)f;
+        uh[at] = __builtin_bit_cast(uint16_t, hi);
+        ul[at] = __builtin_bit_cast(uint16_t, (__bf16)(f - (float)hi));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      const uint32_t k = s * 32 + kb * 8;
+      const lbf16x8 hi = *reinterpret_cast<const lbf16x8*>(uh + c16 * RP + k), lo = *reinterpret_cast<const lbf16x8*>(ul + c16 * RP + k);
+      const lbf16x8 v = first_of(b[s], k < rank ? (int)(rank - k) : 0);
+      low = mfma_bf16(v, hi, low);
+      low = mfma_bf16(v, lo, low);
+    }
+  }
+  if (!mine) return;
+  const f32x4 y = base + low;
+  if (a.vec) {
+    if (o < O) *reinterpret_cast<f32x4*>(a.y + e) = y;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (o + c < O) a.y[e + c] = y[c];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
@@ -566,7 +696,26 @@ static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
   return wide ? up(k_lora_up<4, 4>, 4) : up(k_lora_up<4, 1>, 1);
 }
 
+// One launch where a block's part of A and x is little: us on the device, f32
+// rows, 8 rows of 4 adapters, one launch and two: 512 -> 512 rank 16 6.0 and 8.5,
+// rank 64 8.4 and 9.4; 2048 -> 2048 rank 16 (196 KB) 8.3 and 8.4 (16 rows 9.3
+// and 8.2), rank 32 10.0 and 8.8; 4096 -> 512 rank 16 11.0 and 8.6. A caller
+// without a graph pays 2.5 for the second launch.
+constexpr uint64_t kOneBlocks = 512, kOneBytes = 200 * 1000;
+
 hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
+  const uint64_t blocks = (uint64_t)a.n_items * ((a.out_dim + 255) / 256);
+  const uint32_t mt = (a.max_rank + 15) / 16;  // tiles of 16 ranks
+  if (a.n <= kLoraSmall && mt <= 4 && blocks <= kOneBlocks &&
+      (uint64_t)a.in_dim * kLoraM * (2 * mt + (x_bf16 ? 2 : 4)) <= kOneBytes) {
+    auto one = [&](auto fn) {
+      hipLaunchKernelGGL(fn, dim3(a.n_items, (a.out_dim + 255) / 256), dim3(1024), 0, st, a);
+      return hipGetLastError();
+    };
+    if (mt <= 1) return x_bf16 ? one(k_lora_one<true, 1>) : one(k_lora_one<false, 1>);
+    if (mt <= 2) return x_bf16 ? one(k_lora_one<true, 2>) : one(k_lora_one<false, 2>);
+    return x_bf16 ? one(k_lora_one<true, 4>) : one(k_lora_one<false, 4>);
+  }
   if (a.n <= kLoraSmall) return lora_go<kByWave>(a, x_bf16, st);
   if (a.n <= kLoraMid && a.n_adapters < kLoraMid) return lora_go<kByBlock>(a, x_bf16, st);
   hipLaunchKernelGGL(k_lora_plan, dim3(1), dim3(1024), (a.n_adapters + 1) * 8, st, a);

@@ -86,6 +86,16 @@ def test_lora(kernels, n, K, O, N, r, xb):
     _check(kernels, _case(n, K, O, N, r, seed=n + K, xb=xb))
 
 
+@pytest.mark.parametrize("n,K,O,N,r", [
+    (8, 4096, 260, 4, 16), (64, 2048, 300, 64, 64), (5, 2048, 513, 3, 128), (33, 8192, 64, 2, 8), (40, 512, 5000, 37, 24),
+])
+@pytest.mark.parametrize("xb", [False, True])
+def test_few_rows_of_much_work(kernels, n, K, O, N, r, xb):
+    _check(kernels, _case(n, K, O, N, r, seed=n + K, xb=xb))
+    case = _case(n, K, O, N, r, seed=n, xb=xb, ranks=[(5 * i) % (r + 1) for i in range(N)])
+    _check(kernels, case, inplace=True)
+
+
 @pytest.mark.parametrize("n", [3, 70, 300])
 def test_ranks_of_their_own_and_garbage_behind_them(kernels, n):
     ranks = [0, 1, 7, 8, 16, 31, 32, 33, 40]
