@@ -290,9 +290,7 @@ enum LoraBy { kByPlan, kByWave, kByBlock };
 
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c. A
-// share per block makes blocks of few rows: 8 rows, 4 adapters of rank 16, 2048
-// inputs 2.6 us (one round trip each for the ids, the rows and the shares' sum);
-// 200 rows, 40 adapters of rank 64, 4096 inputs 8.9 us for 24 MB, of which
+// share per block makes blocks of few rows: 200 rows, 40 adapters of rank 64, 4096 inputs 8.9 us for 24 MB, of which
 // finding the items is about 3.
 template <bool XBF16, LoraBy BY, int MT>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
@@ -389,8 +387,8 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
 // itself the shares were 22 of 33 us: 200 rows, 40 adapters of rank 64, 4096 ->
 // 4096). The products go through LDS too, so that base and y move in whole rows
 // of the block (in the products' order each lane touches a line of its own).
-// B's and base's loads go out ahead of everything. 8 rows -> 2048 3.2 us, the
-// 200 rows -> 4096 8.6 us for 28 MB, 1000 rows of rank 32 -> 4096 11.3 us for
+// B's and base's loads go out ahead of everything. 200 rows of rank 64 -> 4096
+// 8.6 us for 28 MB, 1000 rows of rank 32 -> 4096 11.3 us for
 // 33 MB of base and y: all blocks run at once, so the loads of items, shares
 // and base come one after another for each of them.
 template <int KT, int NT>
