@@ -290,8 +290,8 @@ enum LoraBy { kByPlan, kByWave, kByBlock };
 
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c. A
-// share per block makes blocks of few rows: 200 rows, 40 adapters of rank 64, 4096 inputs 8.9 us for 24 MB, of which
-// finding the items is about 3.
+// share per block makes blocks of few rows: 200 rows, 40 adapters of rank 64,
+// 4096 inputs 8.9 us for 24 MB, of which finding the items is about 3.
 template <bool XBF16, LoraBy BY, int MT>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   __shared__ f32x4 red[4][64];

@@ -131,8 +131,17 @@ def test_every_kernel(kernels, n, O, steps, bits, G, grouped):
 def test_many_columns(kernels, bits, G, grouped):
     """Vocabulary-wide outputs of few rows; groups that end inside a round of
     loads, odd counts of groups."""
-    for n, O, K in [(1, 16385, 3 * G), (16, 20007, 640), (9, 33000, 9 * G), (5, 16400, 1152)]:
+    for n, O, K in [(1, 16385, 3 * G), (16, 20007, 640), (9, 33000, 9 * G), (5, 16400, 1152), (7, 17000, G),
+                    (2, 16399, 2 * G)]:
         _check(kernels, n, O, K, bits, G, G if grouped else 0)
+
+
+@pytest.mark.parametrize("n,O,K,bits,G,xg", [
+    (3, 16500, 8192, 4, 64, 0), (16, 16500, 7168, 8, 128, 128), (13, 16500, 7168, 3, 32, 32), (4, 16500, 8192, 8, 64, 64),
+])
+def test_many_columns_of_long_rows(kernels, n, O, K, bits, G, xg):
+    """Rows that take most of a CU's LDS, or do not fit it."""
+    _check(kernels, n, O, K, bits, G, xg)
 
 
 def test_largest_codes(kernels):
@@ -152,14 +161,14 @@ def test_largest_codes(kernels):
 
 def test_nan_and_infinite_scales_stay_in_their_row(kernels):
     rng = np.random.default_rng(4)
-    W = _weights(rng, 200, 512, 4, 64)
-    for n in (8, 200):
+    for n, O in ((8, 200), (200, 200), (11, 17000)):
+        W = _weights(rng, O, 512, 4, 64)
         for xg in (0, 64):
             x, sx = _rows(rng, n, 512, xg)
-            clean = _run(kernels, W, 4, 64, x, sx, xg, 200)
+            clean = _run(kernels, W, 4, 64, x, sx, xg, O)
             sx[3, -1] = np.nan
             sx[5, 0] = np.inf
-            y = _run(kernels, W, 4, 64, x, sx, xg, 200)
+            y = _run(kernels, W, 4, 64, x, sx, xg, O)
             assert np.all(np.isnan(y[3])) and not np.any(np.isfinite(y[5]))
             keep = [i for i in range(n) if i not in (3, 5)]
             assert np.array_equal(y[keep], clean[keep])
