@@ -18,8 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libsmoe.so")
-SOURCES = ["api.hip", "beam.hip", "decode.hip", "fused.hip", "limb.hip", "loader.hip", "lora.hip", "norm.hip", "phase.hip", "prefill.hip", "router.hip", "rows8_q3.hip", "rows8_q4.hip",
-           "rows8_q8.hip", "synth.hip"]
+SOURCES = ["api.hip", "beam.hip", "decode.hip", "fused.hip", "limb.hip", "loader.hip", "lora.hip", "norm.hip",
+           "phase.hip", "prefill.hip", "router.hip", "rows8_q3.hip", "rows8_q4.hip", "rows8_q8.hip", "synth.hip"]
 HEADERS = ["common.h", "handle.h", "kernels.h", "rows8.h", os.path.join("..", "..", "include", "smoe.h")]
 ARCH = "gfx950"
 
