@@ -3,10 +3,10 @@
 //
 //   r = x + residual,  inv = 1 / sqrt(sum r^2 / hidden + eps),  y = r inv w
 //   8 bits: over each group (or the row) top = max |y|, scale = top / 127,
-//   code = rint(y 127 / top)
+//   code = rint(y / scale)
 //
-// The sum, the norm and the codes' quotient are f32; only the outputs round
-// (bf16 and int8 to nearest even).
+// The sum, the norm and both quotients are f32; only the outputs round (bf16
+// and int8 to nearest even).
 #include "common.h"
 #include "kernels.h"
 
@@ -161,12 +161,26 @@ __global__ __launch_bounds__(kNormThreads) void k_rmsnorm(NormArgs a) {
   for (int i = 0; i < V; ++i) {
     // An infinity or NaN in the group: scale NaN, codes 0.
     const bool ok = top[i] >= kQuantFloor && top[i] < INFINITY;
-    const float f = ok ? 127.f / top[i] : 0.f;
     const float s = top[i] < INFINITY ? (ok ? top[i] / 127.f : 0.f) : __builtin_nanf("");
+    // y / s rounded to an integer, by way of y (127 / top): the two quotients
+    // differ by less than 4 2^-24 of at most 127.5, so only a product within
+    // 2^-14 of a tie needs the division itself (one thread in a thousand; with
+    // all values divided the 1000 rows above take 0.4 us more).
+    const float f = ok ? 127.f / top[i] : 0.f;
+    float k[8], off = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = ok ? r[i][j] * f : 0.f;
+      k[j] = __builtin_rintf(v);
+      off = fmaxf(off, fabsf(v - k[j]));
+    }
+    if (off > 0.5f - 0x1p-14f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j] = __builtin_rintf(r[i][j] / s);
+    }
     int32_t c[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      c[j] = ok ? (int32_t)__builtin_rintf(fminf(fmaxf(r[i][j] * f, -127.f), 127.f)) : 0;
+    for (int j = 0; j < 8; ++j) c[j] = (int32_t)k[j];
     if constexpr (VEC) {
       const uint32_t e = at(i, 0);
       if (e < H) {
