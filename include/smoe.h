@@ -508,8 +508,9 @@ int smoe_moe_prefill_block(smoe_handle* h, const smoe_expert_shape* shape, const
  * per q_group values (32, 64 or 128; 0: one per row), the rows smoe_qmm_i8
  * takes: scale = max|y| / 127, code = y / scale rounded to nearest even; a
  * group with an infinity or NaN has scale NaN and codes 0, one whose largest
- * magnitude is below 2^-119 scale 0 and codes 0. The sum of squares is f32:
- * a row whose r^2 add up past its range gives zeros.
+ * magnitude is below 2^-119 scale 0 and codes 0. The mean and its root are
+ * f64, so any row of finite r has its norm; one with an infinity gives zeros
+ * beside it, as the formula does.
  * x: device [n_tokens, hidden], bf16 when x_is_bf16 else f32; residual:
  * device f32 or NULL (r = x); norm_w: device bf16[hidden] or NULL (ones);
  * sum_out: device f32, out: device bf16 when out_is_bf16 else f32, out_q:

@@ -960,6 +960,7 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
   a.w = (const uint16_t*)norm_w;
   a.eps = eps;
   a.hidden = hidden;
+  a.inv_hidden = 1.0 / hidden;
   a.sum = sum_out;
   a.out = out;
   a.out_bf16 = out_is_bf16;

@@ -46,10 +46,6 @@ __device__ __forceinline__ float beam_exp(float x) {
 
 // Wave reductions on DPP (row shifts, then row broadcasts: complete in lane
 // 63), the result in every lane. A shuffle is an LDS permute, 100 cycles each.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   v = max(v, dpp_u32<0x111, 0xF>(v));
   v = max(v, dpp_u32<0x112, 0xF>(v));
@@ -58,23 +54,6 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   v = max(v, dpp_u32<0x142, 0xA>(v));
   v = max(v, dpp_u32<0x143, 0xC>(v));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_add_f64(double v) {
-  const u64 b = (u64)__double_as_longlong(v);
-  const u64 o = (u64)dpp_u32<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp_u32<CTRL, ROWS>((uint32_t)b);
-  return v + __longlong_as_double((long long)o);
-}
-__device__ __forceinline__ double wave_sum_f64(double v) {
-  v = dpp_add_f64<0x111, 0xF>(v);
-  v = dpp_add_f64<0x112, 0xF>(v);
-  v = dpp_add_f64<0x114, 0xF>(v);
-  v = dpp_add_f64<0x118, 0xF>(v);
-  v = dpp_add_f64<0x142, 0xA>(v);
-  v = dpp_add_f64<0x143, 0xC>(v);
-  const u64 b = (u64)__double_as_longlong(v);
-  const u64 hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63), lo = (uint32_t)__builtin_amdgcn_readlane((int)b, 63);
-  return __longlong_as_double((long long)(hi << 32 | lo));
 }
 __device__ __forceinline__ float wave_max_f32(float v) { return readlane_f(wave_max_last(v), 63); }
 

@@ -276,6 +276,30 @@ __device__ __forceinline__ float group_sum_last(float v) {
   return v;
 }
 
+// Sums of doubles over the wave on DPP (row shifts, then row broadcasts:
+// complete in lane 63), the result in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add_f64(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t o = (uint64_t)dpp_u32<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp_u32<CTRL, ROWS>((uint32_t)b);
+  return v + __longlong_as_double((long long)o);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v = dpp_add_f64<0x111, 0xF>(v);
+  v = dpp_add_f64<0x112, 0xF>(v);
+  v = dpp_add_f64<0x114, 0xF>(v);
+  v = dpp_add_f64<0x118, 0xF>(v);
+  v = dpp_add_f64<0x142, 0xA>(v);
+  v = dpp_add_f64<0x143, 0xC>(v);
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63), lo = (uint32_t)__builtin_amdgcn_readlane((int)b, 63);
+  return __longlong_as_double((long long)(hi << 32 | lo));
+}
+
 // Transposed reductions: several per-lane partial sums reduced at once, each
 // exchange halving the values per lane while every lane stays busy.
 // swap32_add(a, b): lanes 0-31 hold a's partial over lanes {l, l + 32},

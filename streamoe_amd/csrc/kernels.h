@@ -299,6 +299,7 @@ struct NormArgs {
   const uint16_t* w;      // bf16 [hidden], or null
   float eps;
   uint32_t hidden;
+  double inv_hidden;      // 1 / hidden
   float* sum;             // x + residual, or null
   void* out;              // f32 or bf16, or null
   int out_bf16;

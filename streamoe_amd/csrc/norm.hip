@@ -5,8 +5,9 @@
 //   8 bits: over each group (or the row) top = max |y|, scale = top / 127,
 //   code = rint(y / scale)
 //
-// The sum, the norm and both quotients are f32; only the outputs round (bf16
-// and int8 to nearest even).
+// The sum and its root are f64 (an f32 r^2 leaves the range from 2^64 on),
+// 1 / sqrt and both quotients round to f32; only the outputs round further
+// (bf16 and int8 to nearest even).
 #include "common.h"
 #include "kernels.h"
 
@@ -27,9 +28,17 @@ constexpr uint32_t kNormThreads = 256;
 // rows (1000 of 4096, bf16 in and out, codes in groups of 64, 53 MB: 11.8 us,
 // 4.5 TB/s, of the 5.0 of a large copy), one round trip a single one (2048: 1.8
 // us). The weight's loads go out with the row's.
+// 1 / sqrt(m) by one Newton step on the hardware's estimate (good to 2^-23):
+// to 2^-45; 0 for an infinity.
+__device__ __forceinline__ float norm_rsqrt(double m) {
+  const double y = __builtin_amdgcn_rsq(m), e = __builtin_fma(-m * y, y, 1.0);
+  return m == (double)INFINITY ? 0.f : (float)__builtin_fma(0.5 * y, e, y);
+}
+
 template <bool XBF16, int V, bool VEC>
 __global__ __launch_bounds__(kNormThreads) void k_rmsnorm(NormArgs a) {
-  __shared__ float red[2][kNormThreads / 64];
+  __shared__ double sums[kNormThreads / 64];
+  __shared__ float tops[kNormThreads / 64];
   const uint32_t t = threadIdx.x, H = a.hidden;
   const uint64_t row = (uint64_t)blockIdx.x * H;
   auto at = [&](int i, int j) { return VEC ? (i * kNormThreads + t) * 8 + j : t + kNormThreads * (i * 8 + j); };
@@ -64,15 +73,15 @@ __global__ __launch_bounds__(kNormThreads) void k_rmsnorm(NormArgs a) {
       }
     }
   }
-  float ss = 0.f;
+  double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(r[i][j], r[i][j], ss);
-  ss = group_sum<64>(ss);
-  if ((t & 63) == 0) red[0][t >> 6] = ss;
+    for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)r[i][j], (double)r[i][j], ss);
+  ss = wave_sum_f64(ss);
+  if ((t & 63) == 0) sums[t >> 6] = ss;
   __syncthreads();
-  const float inv = 1.0f / sqrtf(((red[0][0] + red[0][1]) + (red[0][2] + red[0][3])) / (float)H + a.eps);
+  const float inv = norm_rsqrt(((sums[0] + sums[1]) + (sums[2] + sums[3])) * a.inv_hidden + (double)a.eps);
   if (a.sum) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -140,9 +149,9 @@ __global__ __launch_bounds__(kNormThreads) void k_rmsnorm(NormArgs a) {
 #pragma unroll
     for (int i = 1; i < V; ++i) m = fmaxf(m, top[i]);
     m = wave_max(m);
-    if ((t & 63) == 0) red[1][t >> 6] = m;
+    if ((t & 63) == 0) tops[t >> 6] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 #pragma unroll
     for (int i = 0; i < V; ++i) top[i] = m;
   } else {  // 4, 8 or 16 neighbouring threads hold a group
