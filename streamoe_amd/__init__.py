@@ -61,12 +61,17 @@ def _fits(t, types, n, device):
     return t is not None and t.dtype in types and t.numel() >= n and t.is_contiguous() and t.get_device() == device
 
 
+def _dense(t, device):
+    """Whether t is one dense piece of `device`'s memory: what a workspace has to be."""
+    return t is not None and t.is_contiguous() and t.get_device() == device
+
+
 def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _room(workspace):
-    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+def _room(t):
+    return t.numel() * t.element_size()
 
 
 @dataclass(frozen=True)
@@ -452,7 +457,7 @@ class Kernels:
                 or not _fits(ids, _types("i32"), n_tokens, dev)
                 or not _fits(x, _types("f32_bf16"), n_tokens * in_dim, dev)
                 or not (base is None or _fits(base, f32, n_tokens * out_dim, dev))
-                or not _fits(y, f32, n_tokens * out_dim, dev)):
+                or not _fits(y, f32, n_tokens * out_dim, dev) or not _dense(workspace, dev)):
             return _INVALID
         return _lib.smoe_lora(self.h, ac, ids.data_ptr(), x.data_ptr(), x.element_size() == 2, _at(base), y.data_ptr(),
                               out_dim, in_dim, n_tokens, _at(workspace), _room(workspace))
@@ -468,7 +473,8 @@ class Kernels:
         rows, picks, dev, f32, i32 = n_requests * n_beams, n_requests * n_picks, self.device, _types("f32"), _types("i32")
         if not (_fits(logits, f32, rows * vocab, dev) and _fits(scores, f32, rows, dev)
                 and (done is None or _fits(done, _types("flag"), rows, dev)) and _fits(out_scores, f32, picks, dev)
-                and _fits(out_rows, i32, picks, dev) and _fits(out_tokens, i32, picks, dev)):
+                and _fits(out_rows, i32, picks, dev) and _fits(out_tokens, i32, picks, dev)
+                and _dense(workspace, dev)):
             return _INVALID
         return _lib.smoe_beam_select(self.h, logits.data_ptr(), scores.data_ptr(), _at(done), pad_token, n_requests,
                                      n_beams, vocab, n_picks, out_scores.data_ptr(), out_rows.data_ptr(),
