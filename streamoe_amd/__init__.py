@@ -139,6 +139,14 @@ class QuantWeights:
         return _abi.QWeights(self.buffer.data_ptr(), self.packed_offset, self.scales_offset,
                              self.biases_offset, self.group_size, self.bits)
 
+    def holds(self, out_dim, in_dim, device):
+        """Whether the buffer, dense on `device`, has all of an [out_dim, in_dim] matrix."""
+        if not _dense(self.buffer, device):
+            return False
+        room, at, per_group = _room(self.buffer), self.packed_offset, out_dim * (in_dim // (self.group_size or 1)) * 2
+        return (min(at, self.scales_offset, self.biases_offset) >= 0 and at + out_dim * in_dim * self.bits // 8 <= room
+                and max(self.scales_offset, self.biases_offset) + per_group <= room)
+
 
 @dataclass(frozen=True, eq=False)
 class Adapters:
@@ -437,7 +445,8 @@ class Kernels:
         rmsnorm writes them; x_group 0 (one scale per row) or the weights' group."""
         dev, f32 = self.device, _types("f32")
         if not (_fits(x, _types("i8"), n_tokens * in_dim, dev) and _fits(y, f32, n_tokens * out_dim, dev)
-                and _fits(x_scales, f32, n_tokens * (in_dim // (x_group or in_dim or 1)), dev)):
+                and _fits(x_scales, f32, n_tokens * (in_dim // (x_group or in_dim or 1)), dev)
+                and w.holds(out_dim, in_dim, dev)):
             return _INVALID
         wc = w.c()
         return _lib.smoe_qmm_i8(self.h, wc, x.data_ptr(), x_scales.data_ptr(), x_group, y.data_ptr(), out_dim, in_dim,

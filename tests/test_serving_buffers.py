@@ -83,3 +83,38 @@ def test_workspace_of_beam_select(k):
     assert go(On(1 << 16, dtype=torch.uint8)) == 0 and k.lib.calls == 1
     for w in WRONG:
         _refused(k, lambda: go(On(1 << 16, dtype=torch.uint8, **w)))
+
+
+# 64 x 256 codes of 4 bits, groups of 64: 8192 bytes, then 512 and 512.
+AT = (0, 8192, 8704)
+
+
+def _qmm(k, buf, at=AT, out_dim=64, in_dim=256, n=5, **kw):
+    w = sa.QuantWeights(buf, *at, kw.get("group", 64), kw.get("bits", 4))
+    return k.qmm_i8(w, On(n, in_dim, dtype=torch.int8), On(n), 0, On(n, out_dim), out_dim, in_dim, n)
+
+
+def test_weights_of_qmm_i8(k):
+    u8 = torch.uint8
+    assert _qmm(k, On(9216, dtype=u8)) == 0 and k.lib.calls == 1
+    assert _qmm(k, On(96, 48, dtype=torch.int16)) == 0           # any type and shape that holds the bytes
+    assert _qmm(k, On(9216, dtype=u8), at=(1024, 0, 512)) == 0   # any order
+    assert _qmm(k, On(9216, dtype=u8), in_dim=384, out_dim=42, at=(0, 8064, 8568), bits=4) == 0
+    for w in WRONG:
+        _refused(k, lambda: _qmm(k, On(9216, dtype=u8, **w)))
+    _refused(k, lambda: _qmm(k, On(9215, dtype=u8)))                            # the biases end behind it
+    _refused(k, lambda: _qmm(k, On(9216, dtype=u8), out_dim=65))
+    _refused(k, lambda: _qmm(k, On(9216, dtype=u8), bits=8))                    # the codes do
+    _refused(k, lambda: _qmm(k, On(9216, dtype=u8), at=(0, 8706, 8192)))        # the scales do
+    _refused(k, lambda: _qmm(k, On(9216, dtype=u8), at=(-16, 8192, 8704)))
+    _refused(k, lambda: _qmm(k, On(9216, dtype=u8), group=32))
+    _refused(k, lambda: _qmm(k, None))
+
+
+def test_weights_the_library_refuses_reach_it(k):
+    """Widths and groups that do not exist are the library's to name."""
+    buf = On(1 << 16, dtype=torch.uint8)
+    before = k.lib.calls
+    for kw in (dict(bits=5), dict(group=0), dict(group=48), dict(bits=0)):
+        assert _qmm(k, buf, **kw) == 0
+    assert k.lib.calls == before + 4
