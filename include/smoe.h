@@ -517,7 +517,7 @@ int smoe_moe_prefill_block(smoe_handle* h, const smoe_expert_shape* shape, const
  * device int8, each [n_tokens, hidden] or NULL, out and out_q not both;
  * out_scales: device f32[n_tokens, hidden / q_group], with out_q. All 16-byte
  * aligned. sum_out or out may be the buffer of x or residual where the types
- * are the same; else outputs overlap nothing. hidden 1..16384 (a multiple of
+ * are the same; else outputs overlap nothing (SMOE_ERR_INVALID_ARG). hidden 1..16384 (a multiple of
  * q_group), n_tokens below 2^24, else SMOE_ERR_UNSUPPORTED_SHAPE
  * (SMOE_ERR_IN_DIM_NOT_MULTIPLE).
  * Enqueue-only, allocates nothing, capturable in a HIP graph. */

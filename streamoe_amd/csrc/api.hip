@@ -23,6 +23,15 @@ bool aligned(const void* p, uint64_t off, uint64_t a) {
   return (((uintptr_t)p + off) % a) == 0;
 }
 
+struct Span {
+  const void* at;  // or null
+  uint64_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t p = (uintptr_t)a.at, q = (uintptr_t)b.at;
+  return p && q && p < q + b.bytes && q < p + a.bytes;
+}
+
 int check_group(uint32_t group) {
   return (group == 32 || group == 64 || group == 128) ? SMOE_OK : SMOE_ERR_UNSUPPORTED_GROUP;
 }
@@ -953,6 +962,22 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
   for (const void* p : {x, (const void*)residual, norm_w, (const void*)sum_out, (const void*)out, (const void*)out_q,
                         (const void*)out_scales})
     if (!aligned(p, 0, 16)) return SMOE_ERR_MISALIGNED;
+  // A block reads its row before it writes it: an output may be an input's rows
+  // of the same type, and else overlaps nothing.
+  const uint64_t values = (uint64_t)n_tokens * hidden, xb = values * (x_is_bf16 ? 2 : 4);
+  const Span in[] = {{x, xb}, {residual, values * 4}, {norm_w, (uint64_t)hidden * 2}};
+  const Span to[] = {{sum_out, values * 4},
+                     {out, values * (out_is_bf16 ? 2 : 4)},
+                     {out_q, values},
+                     {out_scales, (uint64_t)n_tokens * (q_group ? hidden / q_group : 1) * 4}};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < 3; ++j) {
+      const bool in_place = i < 2 && j < 2 && to[i].at == in[j].at && to[i].bytes == in[j].bytes;
+      if (!in_place && overlap(to[i], in[j])) return SMOE_ERR_INVALID_ARG;
+    }
+    for (int j = 0; j < i; ++j)
+      if (overlap(to[i], to[j])) return SMOE_ERR_INVALID_ARG;
+  }
   if (int rc = use_device(h)) return rc;
   NormArgs a{};
   a.x = x;
