@@ -70,10 +70,6 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _room(t):
-    return t.numel() * t.element_size()
-
-
 @dataclass(frozen=True)
 class ExpertLayout:
     """Packed-expert layout `[gate | up | down]`, each block
@@ -141,11 +137,11 @@ class QuantWeights:
 
     def holds(self, out_dim, in_dim, device):
         """Whether the buffer, dense on `device`, has all of an [out_dim, in_dim] matrix."""
-        if not _dense(self.buffer, device):
+        b, group = self.buffer, self.group_size or 1
+        if not _dense(b, device):
             return False
-        room, at, per_group = _room(self.buffer), self.packed_offset, out_dim * (in_dim // (self.group_size or 1)) * 2
-        return (min(at, self.scales_offset, self.biases_offset) >= 0 and at + out_dim * in_dim * self.bits // 8 <= room
-                and max(self.scales_offset, self.biases_offset) + per_group <= room)
+        codes, last = b.nbytes - out_dim * in_dim * self.bits // 8, b.nbytes - out_dim * (in_dim // group) * 2
+        return 0 <= self.packed_offset <= codes and 0 <= self.scales_offset <= last and 0 <= self.biases_offset <= last
 
 
 @dataclass(frozen=True, eq=False)
@@ -469,7 +465,7 @@ class Kernels:
                 or not _fits(y, f32, n_tokens * out_dim, dev) or not _dense(workspace, dev)):
             return _INVALID
         return _lib.smoe_lora(self.h, ac, ids.data_ptr(), x.data_ptr(), x.element_size() == 2, _at(base), y.data_ptr(),
-                              out_dim, in_dim, n_tokens, _at(workspace), _room(workspace))
+                              out_dim, in_dim, n_tokens, _at(workspace), workspace.nbytes)
 
     # -- beam search --------------------------------------------------------------
     def beam_select_workspace_size(self, n_requests, n_beams, vocab, n_picks):
@@ -487,7 +483,7 @@ class Kernels:
             return _INVALID
         return _lib.smoe_beam_select(self.h, logits.data_ptr(), scores.data_ptr(), _at(done), pad_token, n_requests,
                                      n_beams, vocab, n_picks, out_scores.data_ptr(), out_rows.data_ptr(),
-                                     out_tokens.data_ptr(), _at(workspace), _room(workspace))
+                                     out_tokens.data_ptr(), _at(workspace), workspace.nbytes)
 
     def beam_reorder(self, states, rows):
         """dst row i = src row rows[i] of every BeamState, for the rows of `rows`
