@@ -535,8 +535,10 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
  * device f32. Weights of bits 4, 3 or 8, group 32, 64 or 128, in_dim a
  * multiple of the group up to 16384, out_dim up to 2^28, n_tokens up to
  * 1048560 (SMOE_ERR_UNSUPPORTED_SHAPE); x_group 0 or the weights' group
- * (SMOE_ERR_UNSUPPORTED_GROUP). y overlaps nothing. A row with a scale that is infinite or NaN
- * gives infinities or NaN in that row only. Enqueue-only, allocates nothing,
+ * (SMOE_ERR_UNSUPPORTED_GROUP). y overlaps nothing. A row with a scale that is
+ * infinite or NaN gives infinities or NaN in that row only; any other scale
+ * may be as large as f32 holds (per group, one below 2^-102 is taken to within
+ * 2^-124). Enqueue-only, allocates nothing,
  * needs no workspace, capturable in a HIP graph. No counterpart in the
  * reference, whose activations stay f32. */
 int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const float* x_scales, uint32_t x_group,

@@ -31,6 +31,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kQ8Step = 128;
 
+// Rows' scales per group enter times 2^-24 and the finished sums leave times
+// 2^24: a group's sum (up to 2^21, and 1.5 2^23 in the kernels that read it from
+// a float's bits) times the largest scale then stays in f32's range. Both are
+// exact but for scales below 2^-102.
+constexpr float kQ8Down = 0x1p-24f, kQ8Up = 0x1p24f;
+
 __device__ __forceinline__ i32x4 q8_mfma(u32x4 a, u32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
@@ -230,7 +236,7 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_q8_few(Q8Args a) 
         const i32x4 X = q8_sums<G>(x[m], ones, j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (XG) sx[m][i] = __shfl(v.sx[m][j], 4 * (int)kb + i, kWave);
+          if constexpr (XG) sx[m][i] = __shfl(v.sx[m][j], 4 * (int)kb + i, kWave) * kQ8Down;
           xf[m][i] = XG ? (float)X[i] * sx[m][i] : (float)X[i];
         }
       }
@@ -295,7 +301,7 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_q8_few(Q8Args a) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = row0 + mt / NT * 16 + 4 * kb + i;
-      if (r < a.n) a.y[(uint64_t)r * O + col] = XG ? sum[i] : sum[i] * by[i];
+      if (r < a.n) a.y[(uint64_t)r * O + col] = sum[i] * (XG ? kQ8Up : by[i]);
     }
   }
 }
@@ -441,7 +447,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
   if constexpr (XG)
     for (uint32_t i = tid; i < groups * MT * 16; i += 256) {
       const uint32_t r = i % (MT * 16), g = i / (MT * 16);
-      sxl[i] = r < a.n ? q8_round22(a.sx[(uint64_t)r * gpr + min(g, gpr - 1)]) : 0.f;
+      sxl[i] = r < a.n ? q8_round22(a.sx[(uint64_t)r * gpr + min(g, gpr - 1)] * kQ8Down) : 0.f;
     }
   __syncthreads();
   const uint32_t at[2] = {kb * 16 + (c16 ^ kb), 64 + kb * 16 + (c16 ^ (4 + kb))};
@@ -566,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t r = m * 16 + 4 * kb + k;
-        if (r < a.n && col < O) a.y[(uint64_t)r * O + col] = XG ? acc[m][k] : acc[m][k] * sxr[m][k];
+        if (r < a.n && col < O) a.y[(uint64_t)r * O + col] = acc[m][k] * (XG ? kQ8Up : sxr[m][k]);
       }
       acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -786,7 +792,7 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 2 : KS) void k_q8_tile(Q8Args a
       for (uint32_t i = 0; i < XS; ++i) {
         if (x_part(i) != half) continue;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) lds.sx[half][j][(tid + 256 * i) % BM] = q8_round22(sxr[i][j]);
+        for (uint32_t j = 0; j < 4; ++j) lds.sx[half][j][(tid + 256 * i) % BM] = q8_round22(sxr[i][j] * kQ8Down);
       }
     }
   };
@@ -952,7 +958,7 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 2 : KS) void k_q8_tile(Q8Args a
 
   float scale[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) scale[m] = XG ? 1.f : a.sx[min(row0 + (wm * MT + m) * 16 + c16, a.n - 1)];
+  for (int m = 0; m < MT; ++m) scale[m] = XG ? kQ8Up : a.sx[min(row0 + (wm * MT + m) * 16 + c16, a.n - 1)];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const uint32_t r = row0 + (wm * MT + m) * 16 + c16;
