@@ -573,9 +573,9 @@ uint64_t smoe_lora_workspace_size(const smoe_adapters* adapters, uint32_t n_toke
  * (zeros), may be y; y: device f32[n_tokens, out_dim]. x, a, b 16-byte
  * aligned, in_dim a multiple of 8; out_dim up to 4194240 (multiples of 4 with y
  * and base on 16 bytes are the fast case); y overlaps nothing but base. On bf16 MFMA with f32 sums; f32 x and the
- * low-rank values between the products enter as bf16 pairs (off by at most
- * 2^-16 of each value); a row with an infinity, a NaN or an f32 that bf16
- * rounds to infinity gives NaN. An id or a
+ * low-rank values between the products enter as three bf16 that add up to the
+ * f32. A row with an infinity or a NaN (in x, or where scale A x leaves f32's
+ * range) gives NaN. An id or a
  * rank out of range is found on the device: the next smoe_sync returns
  * SMOE_ERR_INVALID_ARG, the row's y is base (the rank is clamped). n_tokens up
  * to 65536, in_dim up to 65536, else SMOE_ERR_UNSUPPORTED_SHAPE. workspace:

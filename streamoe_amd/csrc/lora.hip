@@ -9,10 +9,9 @@
 //   k_lora_up      the shares added, scaled, times B on bf16 MFMA, plus base
 //   k_lora_one     the last two for few rows and little of A
 //
-// f32 values enter the matrix cores as bf16 pairs, v = hi + lo, each rounded
-// to nearest: off by at most 2^-16 |v| (hi leaves up to 2^-8 |v|, of which lo
-// loses 2^-8). A and B are bf16, so the products are exact and the sums f32. An
-// infinity leaves a NaN in lo, so its row's outputs are NaN.
+// f32 values enter the matrix cores as three bf16, eight bits of the value each:
+// nothing is lost. A and B are bf16, so the products are exact and the sums f32.
+// An infinity leaves a NaN in the second part, so its row's outputs are NaN.
 #include "common.h"
 #include "kernels.h"
 
@@ -29,10 +28,26 @@ __device__ __forceinline__ f32x4 mfma_bf16(lbf16x8 a, lbf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// v = hi + lo.
-__device__ __forceinline__ void split_bf16(lf32x8 v, lbf16x8& hi, lbf16x8& lo) {
-  hi = __builtin_convertvector(v, lbf16x8);
-  lo = __builtin_convertvector(v - __builtin_convertvector(hi, lf32x8), lbf16x8);
+// v = p[0] + p[1] + p[2], each the rest's upper half.
+__device__ __forceinline__ void split_bf16(lf32x8 v, lbf16x8 (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = __builtin_amdgcn_perm(__float_as_uint(v[2 * j + 1]), __float_as_uint(v[2 * j]), 0x07060302u);
+    p[i] = __builtin_bit_cast(lbf16x8, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] -= __uint_as_float(__float_as_uint(v[j]) & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void split_bf16(float v, uint16_t (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t top = __float_as_uint(v) & 0xFFFF0000u;
+    p[i] = (uint16_t)(top >> 16);
+    v -= __uint_as_float(top);
+  }
 }
 
 // The first n of eight bf16, zeros behind (n may be <= 0 or >= 8).
@@ -340,20 +355,17 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   };
   auto compute = [&](uint32_t s, const Step& v) {
     const bool in = s * 32 + kb * 8 < K;
-    lbf16x8 hi, lo;
-    if constexpr (XBF16) {
-      hi = first_of(v.x, in ? 8 : 0);
-    } else {
-      split_bf16(v.x, hi, lo);
-      hi = first_of(hi, in ? 8 : 0);
-      lo = first_of(lo, in ? 8 : 0);
-    }
+    lbf16x8 x[3];
+    if constexpr (XBF16)
+      x[0] = first_of(v.x, in ? 8 : 0);
+    else
+      split_bf16(in ? v.x : lf32x8{0, 0, 0, 0, 0, 0, 0, 0}, x);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       if (i >= (int)nt) break;
       const lbf16x8 w = first_of(v.w[i], in && i * 16 + c16 < rank ? 8 : 0);
-      acc[i] = mfma_bf16(hi, w, acc[i]);
-      if constexpr (!XBF16) acc[i] = mfma_bf16(lo, w, acc[i]);
+#pragma unroll
+      for (int k = 0; k < (XBF16 ? 1 : 3); ++k) acc[i] = mfma_bf16(x[k], w, acc[i]);
     }
   };
   for (uint32_t s = s0 + wave; s < s1; s += 8) {
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
 
 // D = B (outputs) x u (rows): lane (c, kb) ends with outputs 4 kb .. of row c.
 // A block takes 64 NT outputs of an item; it adds the shares once, into LDS, as
-// the bf16 pairs that its waves read as operands (added by every wave for
+// the bf16 parts that its waves read as operands (added by every wave for
 // itself the shares were 22 of 33 us: 200 rows, 40 adapters of rank 64, 4096 ->
 // 4096). The products go through LDS too, so that base and y move in whole rows
 // of the block (in the products' order each lane touches a line of its own).
@@ -395,7 +407,7 @@ template <int KT, int NT>
 __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   constexpr uint32_t RP = KT * 32 + 8;  // bf16 per row in LDS: rows apart by 16 bytes of banks
   constexpr uint32_t OB = 64 * NT, OP = OB + 4;  // outputs of the block; floats per row in LDS, apart by 16 bytes of banks
-  __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
+  __shared__ __attribute__((aligned(16))) uint16_t up[3][kLoraM * RP];
   __shared__ __attribute__((aligned(16))) float prod[kLoraM * OP];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, kb = lane >> 4;
   uint32_t row;
@@ -470,16 +482,13 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
           add(0, std::integral_constant<int, 1>{});
         }
       }
-      uint16_t h[4], l[4];
+      uint16_t p[4][3];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float v = k + j < rank ? u[j] * scale : 0.f;  // nothing was written behind the rank
-        const __bf16 hi = (__bf16)v;
-        h[j] = __builtin_bit_cast(uint16_t, hi);
-        l[j] = __builtin_bit_cast(uint16_t, (__bf16)(v - (float)hi));
-      }
-      *reinterpret_cast<uint2*>(uh + r * RP + k) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-      *reinterpret_cast<uint2*>(ul + r * RP + k) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
+      for (int j = 0; j < 4; ++j) split_bf16(k + j < rank ? u[j] * scale : 0.f, p[j]);  // nothing was written behind the rank
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        *reinterpret_cast<uint2*>(up[j] + r * RP + k) =
+            make_uint2(p[0][j] | (uint32_t)p[1][j] << 16, p[2][j] | (uint32_t)p[3][j] << 16);
     }
     __syncthreads();
 #pragma unroll
@@ -487,12 +496,14 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
       const uint32_t k = s * 32 + kb * 8;
       if (s * 32 >= (int)rank) break;
       const int left = k < rank ? (int)(rank - k) : 0;
-      const lbf16x8 hi = *reinterpret_cast<const lbf16x8*>(uh + c16 * RP + k), lo = *reinterpret_cast<const lbf16x8*>(ul + c16 * RP + k);
+      lbf16x8 v[3];
+#pragma unroll
+      for (int j = 0; j < 3; ++j) v[j] = *reinterpret_cast<const lbf16x8*>(up[j] + c16 * RP + k);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const lbf16x8 b = first_of(w[s][i], left);
-        low[i] = mfma_bf16(b, hi, low[i]);
-        low[i] = mfma_bf16(b, lo, low[i]);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) low[i] = mfma_bf16(b, v[j], low[i]);
       }
     }
   }
@@ -528,7 +539,7 @@ __global__ __launch_bounds__(1024) void k_lora_one(LoraArgs a) {
   constexpr int KT = (MT + 1) / 2, U = MT <= 2 ? 4 : 2;  // steps of 32 ranks; steps of inputs in flight
   constexpr uint32_t RP = KT * 32 + 8;                   // as in k_lora_up
   __shared__ __attribute__((aligned(16))) float red[16][256];
-  __shared__ __attribute__((aligned(16))) uint16_t uh[kLoraM * RP], ul[kLoraM * RP];
+  __shared__ __attribute__((aligned(16))) uint16_t up[3][kLoraM * RP];
   __shared__ uint32_t of_wave[16][kLoraM];
   const uint32_t lane = threadIdx.x & 63, c16 = lane & 15, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -586,20 +597,17 @@ __global__ __launch_bounds__(1024) void k_lora_one(LoraArgs a) {
       for (int j = 0; j < U; ++j) {
         if (s0 + 16 * j >= steps) break;
         const bool in = (s0 + 16 * j) * 32 + kb * 8 < K;
-        lbf16x8 hi, lo;
-        if constexpr (XBF16) {
-          hi = first_of(x[j], in ? 8 : 0);
-        } else {
-          split_bf16(x[j], hi, lo);
-          hi = first_of(hi, in ? 8 : 0);
-          lo = first_of(lo, in ? 8 : 0);
-        }
+        lbf16x8 p[3];
+        if constexpr (XBF16)
+          p[0] = first_of(x[j], in ? 8 : 0);
+        else
+          split_bf16(in ? x[j] : lf32x8{0, 0, 0, 0, 0, 0, 0, 0}, p);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if (i >= (int)nt) break;
           const lbf16x8 v = first_of(w[j][i], in && i * 16 + c16 < rank ? 8 : 0);
-          acc[i] = mfma_bf16(hi, v, acc[i]);
-          if constexpr (!XBF16) acc[i] = mfma_bf16(lo, v, acc[i]);
+#pragma unroll
+          for (int k = 0; k < (XBF16 ? 1 : 3); ++k) acc[i] = mfma_bf16(p[k], v, acc[i]);
         }
       }
     }
@@ -616,20 +624,19 @@ __global__ __launch_bounds__(1024) void k_lora_one(LoraArgs a) {
 #pragma unroll
         for (int w = 1; w < 16; ++w) sum += red[w][t];
         const uint32_t j = i * 16 + (t >> 2 & 15), at = ((t >> 6) * 4 + (t & 3)) * RP + j;
-        const float f = j < rank ? sum * it.scale : 0.f;
-        const __bf16 hi = (__bf16)f;
-        uh[at] = __builtin_bit_cast(uint16_t, hi);
-        ul[at] = __builtin_bit_cast(uint16_t, (__bf16)(f - (float)hi));
+        uint16_t p[3];
+        split_bf16(j < rank ? sum * it.scale : 0.f, p);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) up[k][at] = p[k];
       }
     }
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < KT; ++s) {
       const uint32_t k = s * 32 + kb * 8;
-      const lbf16x8 hi = *reinterpret_cast<const lbf16x8*>(uh + c16 * RP + k), lo = *reinterpret_cast<const lbf16x8*>(ul + c16 * RP + k);
       const lbf16x8 v = first_of(b[s], k < rank ? (int)(rank - k) : 0);
-      low = mfma_bf16(v, hi, low);
-      low = mfma_bf16(v, lo, low);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) low = mfma_bf16(v, *reinterpret_cast<const lbf16x8*>(up[j] + c16 * RP + k), low);
     }
   }
   if (!mine) return;
