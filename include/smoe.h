@@ -534,7 +534,8 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
  * codes; x_scales: device f32[n_tokens, in_dim / x_group] or [n_tokens]; y:
  * device f32. Weights of bits 4, 3 or 8, group 32, 64 or 128, in_dim a
  * multiple of the group up to 16384, out_dim up to 2^28, n_tokens up to
- * 1048560 (SMOE_ERR_UNSUPPORTED_SHAPE); x_group 0 or the weights' group
+ * 1048560, fewer than 2^24 - 7 tiles of 128 x 128 outputs
+ * (SMOE_ERR_UNSUPPORTED_SHAPE); x_group 0 or the weights' group
  * (SMOE_ERR_UNSUPPORTED_GROUP). y overlaps nothing. A row with a scale that is
  * infinite or NaN gives infinities or NaN in that row only; any other scale
  * may be as large as f32 holds (per group, one below 2^-102 is taken to within

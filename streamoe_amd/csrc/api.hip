@@ -1002,6 +1002,7 @@ int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const f
   if (int rc = qview(w, in_dim, &v, true)) return rc;
   if (x_group && x_group != v.group) return SMOE_ERR_UNSUPPORTED_GROUP;
   if (in_dim > kQ8MaxIn || out_dim > kQ8MaxOut || n_tokens > 65535u * 16) return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (((uint64_t)n_tokens + 127) / 128 * (((uint64_t)out_dim + 127) / 128) > kQ8MaxBlocks) return SMOE_ERR_UNSUPPORTED_SHAPE;
   if (!aligned(x, 0, 16) || !aligned(x_scales, 0, 4) || !aligned(y, 0, 4)) return SMOE_ERR_MISALIGNED;
   if (int rc = use_device(h)) return rc;
   Q8Args a{};

@@ -310,6 +310,7 @@ struct NormArgs {
 hipError_t launch_rmsnorm(const NormArgs& a, bool x_bf16, uint32_t n, hipStream_t st);
 // Quantized products of 8-bit rows (rows8.h), by the weights' bits.
 constexpr uint32_t kQ8MaxIn = 16384, kQ8MaxOut = 1u << 28;
+constexpr uint64_t kQ8MaxBlocks = kMaxBlocks - 7;  // a launch's are a multiple of 8
 struct Q8Args {
   const uint8_t* w;        // codes [O, K]
   const uint16_t *s, *b;   // bf16 [O, K / group]

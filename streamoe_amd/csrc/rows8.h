@@ -1064,9 +1064,10 @@ static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   // 128 x 128 where they fill the chip with two shares each (1000 rows 2048 ->
   // 4096, 256 tiles: 27.0, 64 x 64 29.9) or two blocks on most CUs (1000 rows
   // 4096 -> 7168, 448: 78 and 89; 600 rows 4096 -> 8192, 320: 70 and 64), but
-  // for short sums (140 rows 512 -> 43682: 32 and 25).
+  // for short sums (140 rows 512 -> 43682: 32 and 25) that 64 x 64 tiles have
+  // blocks for.
   if (u128 > 192 && u128 <= 256 && shares(2)) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 2>(a, st);
-  if (u128 > 384 && steps >= 8) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 1>(a, st);
+  if (u128 > 384 && (steps >= 8 || u64 > kQ8MaxBlocks)) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 1>(a, st);
   return q8_tile<BITS, G, XG, 2, 2, 2, 2, 1>(a, st);
 }
 
