@@ -701,18 +701,21 @@ static hipError_t lora_go(const LoraArgs& a, bool x_bf16, hipStream_t st) {
   return wide ? up(k_lora_up<4, 4>, 4) : up(k_lora_up<4, 1>, 1);
 }
 
-// One launch where a block's part of A and x is little: us on the device, f32
-// rows, 8 rows of 4 adapters, one launch and two: 512 -> 512 rank 16 6.0 and 8.5,
-// rank 64 8.4 and 9.4; 2048 -> 2048 rank 16 (196 KB) 8.3 and 8.4 (16 rows 9.3
-// and 8.2), rank 32 10.0 and 8.8; 4096 -> 512 rank 16 11.0 and 8.6. A caller
-// without a graph pays 2.5 for the second launch.
-constexpr uint64_t kOneBlocks = 512, kOneBytes = 200 * 1000;
+// One launch where what a block reads of A and x is little: us on the device,
+// f32 rows, 4 adapters, one launch and two: 8 rows 512 -> 512 rank 16 4.0 and
+// 6.3, rank 64 7.0 and 7.4; 2048 -> 2048 rank 16 6.7 and 6.2 (131 KB), 16 rows
+// 7.1 and 6.4 (197 KB), 64 rows 9.6 and 6.7; rank 32 8.6 and 6.6; 4096 -> 512
+// rank 16 9.8 and 6.5. Over 1500 calls of 1 to 64 rows and as many adapters, 256
+// to 4096 inputs, 64 to 4096 outputs, ranks 8 to 64 the chosen took 1.007 times
+// the faster one's time (135 or 165 KB: 1.008). A caller without a graph pays
+// 2.5 for the second launch.
+constexpr uint64_t kOneBlocks = 512, kOneBytes = 150 * 1000;
 
 hipError_t launch_lora(const LoraArgs& a, bool x_bf16, hipStream_t st) {
   const uint64_t blocks = (uint64_t)a.n_items * ((a.out_dim + 255) / 256);
   const uint32_t mt = (a.max_rank + 15) / 16;  // tiles of 16 ranks
   if (a.n <= kLoraSmall && mt <= 4 && blocks <= kOneBlocks &&
-      (uint64_t)a.in_dim * kLoraM * (2 * mt + (x_bf16 ? 2 : 4)) <= kOneBytes) {
+      (uint64_t)a.in_dim * (kLoraM * 2 * mt + (a.n < kLoraM ? a.n : kLoraM) * (x_bf16 ? 2 : 4)) <= kOneBytes) {
     auto one = [&](auto fn) {
       hipLaunchKernelGGL(fn, dim3(a.n_items, (a.out_dim + 255) / 256), dim3(1024), 0, st, a);
       return hipGetLastError();
