@@ -1025,7 +1025,9 @@ static hipError_t q8_wide(const Q8Args& a, hipStream_t st) {
 // Which kernel, by how many blocks there are for the 256 CUs. Times in us, 4
 // bits, groups of 64, row scales, graph replays; n rows K -> O. Over 630 calls
 // of all bits and groups drawn from 1 to 1000 rows, 150 to 60000 columns, 512
-// to 7168 inputs the chosen kernel took 1.03 times the fastest one's time.
+// to 7168 inputs the chosen kernel took 1.03 times the fastest one's time; of the
+// two tiles of 64 and 128, over 235 calls of 17 to 1000 rows and 4000 to 152000
+// columns, 1.01 times.
 template <int BITS, int G, bool XG>
 static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   const uint32_t steps = (a.K + kQ8Step - 1) / kQ8Step;
@@ -1065,9 +1067,11 @@ static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   // 4096, 256 tiles: 27.0, 64 x 64 29.9) or two blocks on most CUs (1000 rows
   // 4096 -> 7168, 448: 78 and 89; 600 rows 4096 -> 8192, 320: 70 and 64), but
   // for short sums (140 rows 512 -> 43682: 32 and 25) that 64 x 64 tiles have
-  // blocks for.
+  // blocks for, and where they hold fewer rows or columns than they have room
+  // for: a tile of 128 takes 3.4 times one of 64 (64 rows 2048 -> 151936: 88 and
+  // 64; 65 rows: 89 and 110; 130 rows: 169 and 153).
   if (u128 > 192 && u128 <= 256 && shares(2)) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 2>(a, st);
-  if (u128 > 384 && (steps >= 8 || u64 > kQ8MaxBlocks)) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 1>(a, st);
+  if (u128 > 384 && ((steps >= 8 && 10 * u64 >= 34 * u128) || u64 > kQ8MaxBlocks)) return q8_tile<BITS, G, XG, 2, 2, 4, 4, 1>(a, st);
   return q8_tile<BITS, G, XG, 2, 2, 2, 2, 1>(a, st);
 }
 
