@@ -536,7 +536,7 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
  * multiple of the group up to 16384, out_dim up to 2^28, n_tokens up to
  * 1048560, fewer than 2^24 - 7 tiles of 128 x 128 outputs
  * (SMOE_ERR_UNSUPPORTED_SHAPE); x_group 0 or the weights' group
- * (SMOE_ERR_UNSUPPORTED_GROUP). y overlaps nothing. A row with a scale that is
+ * (SMOE_ERR_UNSUPPORTED_GROUP). y overlaps nothing (SMOE_ERR_INVALID_ARG). A row with a scale that is
  * infinite or NaN gives infinities or NaN in that row only; any other scale
  * may be as large as f32 holds (per group, one below 2^-102 is taken to within
  * 2^-124). Enqueue-only, allocates nothing,
@@ -573,7 +573,8 @@ uint64_t smoe_lora_workspace_size(const smoe_adapters* adapters, uint32_t n_toke
  * bf16 when x_is_bf16 else f32; base: device f32[n_tokens, out_dim] or NULL
  * (zeros), may be y; y: device f32[n_tokens, out_dim]. x, a, b 16-byte
  * aligned, in_dim a multiple of 8; out_dim up to 4194240 (multiples of 4 with y
- * and base on 16 bytes are the fast case); y overlaps nothing but base. On bf16 MFMA with f32 sums; f32 x and the
+ * and base on 16 bytes are the fast case); y and the workspace overlap nothing,
+ * but for y as base (SMOE_ERR_INVALID_ARG). On bf16 MFMA with f32 sums; f32 x and the
  * low-rank values between the products enter as three bf16 that add up to the
  * f32. A row with an infinity or a NaN (in x, or where scale A x leaves f32's
  * range) gives NaN. An id or a
@@ -609,7 +610,8 @@ uint64_t smoe_beam_select_workspace_size(uint32_t n_requests, uint32_t n_beams, 
  * or NULL. out_scores: device f32[n_requests, n_picks]; out_rows: device int32,
  * the logits' row a pick continues (request * n_beams + beam, what
  * smoe_beam_reorder takes); out_tokens: device int32. out_scores may be
- * scores when n_picks == n_beams; nothing else overlaps. workspace: device, of
+ * scores when n_picks == n_beams; else outputs and workspace overlap nothing
+ * (SMOE_ERR_INVALID_ARG). workspace: device, of
  * smoe_beam_select_workspace_size bytes, 256-byte aligned, one call's at a
  * time. n_beams 1..16, vocab up to 2^28, n_requests * n_beams up to 262143
  * (SMOE_ERR_UNSUPPORTED_SHAPE); n_picks

@@ -3,6 +3,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <new>
 
@@ -30,6 +31,17 @@ struct Span {
 bool overlap(const Span& a, const Span& b) {
   const uintptr_t p = (uintptr_t)a.at, q = (uintptr_t)b.at;
   return p && q && p < q + b.bytes && q < p + a.bytes;
+}
+
+// Whether one of `to` overlaps one of `in` or another of `to`.
+bool collide(std::initializer_list<Span> to, std::initializer_list<Span> in) {
+  for (const Span* a = to.begin(); a != to.end(); ++a) {
+    for (const Span& b : in)
+      if (overlap(*a, b)) return true;
+    for (const Span* b = to.begin(); b != a; ++b)
+      if (overlap(*a, *b)) return true;
+  }
+  return false;
 }
 
 int check_group(uint32_t group) {
@@ -1004,6 +1016,11 @@ int smoe_qmm_i8(smoe_handle* h, const smoe_qweights* w, const int8_t* x, const f
   if (in_dim > kQ8MaxIn || out_dim > kQ8MaxOut || n_tokens > 65535u * 16) return SMOE_ERR_UNSUPPORTED_SHAPE;
   if (((uint64_t)n_tokens + 127) / 128 * (((uint64_t)out_dim + 127) / 128) > kQ8MaxBlocks) return SMOE_ERR_UNSUPPORTED_SHAPE;
   if (!aligned(x, 0, 16) || !aligned(x_scales, 0, 4) || !aligned(y, 0, 4)) return SMOE_ERR_MISALIGNED;
+  const uint64_t groups = in_dim / v.group, per_weights = out_dim * groups * 2;
+  if (collide({{y, (uint64_t)n_tokens * out_dim * 4}},
+              {{x, (uint64_t)n_tokens * in_dim}, {x_scales, n_tokens * (x_group ? groups : 1) * 4},
+               {v.codes, (uint64_t)out_dim * in_dim * v.bits / 8}, {v.scales, per_weights}, {v.biases, per_weights}}))
+    return SMOE_ERR_INVALID_ARG;
   if (int rc = use_device(h)) return rc;
   Q8Args a{};
   a.w = v.codes;
@@ -1050,8 +1067,15 @@ int smoe_lora(smoe_handle* h, const smoe_adapters* adapters, const int32_t* ids,
       !aligned(y, 0, 4) || !aligned(workspace, 0, 256))
     return SMOE_ERR_MISALIGNED;
   LoraArgs a{};
-  if (workspace_bytes < lora_workspace(s.n_adapters, s.max_rank, n_tokens, &a, (uint8_t*)workspace))
-    return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  const uint64_t need = lora_workspace(s.n_adapters, s.max_rank, n_tokens, &a, (uint8_t*)workspace);
+  if (workspace_bytes < need) return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  const uint64_t rows = n_tokens, out_bytes = rows * out_dim * 4, last = s.n_adapters - 1;
+  if (collide({{y, out_bytes}, {workspace, need}},
+              {{base == y ? nullptr : base, out_bytes}, {x, rows * in_dim * (x_is_bf16 ? 2 : 4)}, {ids, rows * 4},
+               {s.a, last * s.a_stride + (uint64_t)s.max_rank * in_dim * 2},
+               {s.b, last * s.b_stride + (uint64_t)s.max_rank * out_dim * 2}, {s.scale, (last + 1) * 4},
+               {s.ranks, (last + 1) * 4}}))
+    return SMOE_ERR_INVALID_ARG;
   if (int rc = use_device(h)) return rc;
   a.a = (const uint8_t*)s.a;
   a.b = (const uint8_t*)s.b;
@@ -1099,8 +1123,14 @@ int smoe_beam_select(smoe_handle* h, const float* logits, const float* scores, c
       !aligned(out_tokens, 0, 4) || !aligned(workspace, 0, 256))
     return SMOE_ERR_MISALIGNED;
   BeamArgs a{};
-  if (workspace_bytes < beam_workspace(n_requests, n_beams, vocab, n_picks, &a, (uint8_t*)workspace))
-    return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  const uint64_t need = beam_workspace(n_requests, n_beams, vocab, n_picks, &a, (uint8_t*)workspace);
+  if (workspace_bytes < need) return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  const uint64_t rows = (uint64_t)n_requests * n_beams, out_bytes = (uint64_t)n_requests * n_picks * 4;
+  if (collide({{out_scores, out_bytes}, {out_rows, out_bytes}, {out_tokens, out_bytes}, {workspace, need}},
+              {{logits, rows * vocab * 4}, {done, rows}}) ||
+      collide({{out_rows, out_bytes}, {out_tokens, out_bytes}, {workspace, need}, {out_scores == scores ? nullptr : out_scores, out_bytes}},
+              {{scores, rows * 4}}))
+    return SMOE_ERR_INVALID_ARG;
   if (int rc = use_device(h)) return rc;
   a.logits = logits;
   a.scores = scores;
