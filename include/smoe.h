@@ -529,9 +529,10 @@ int smoe_rmsnorm(smoe_handle* h, const void* x, int x_is_bf16, const float* resi
  * for x[t, c] * x_scales[t, c / x_group] (one scale per row with x_group 0:
  * x_scales[t]), as smoe_rmsnorm writes them; smoe_qmm's product with a quarter
  * of its matrix work, on int8 MFMA. Group sums of code times code are exact,
- * everything else f32 (products of many rows round x_scales per group to 22
- * bits, by 2^-23; a row's last bits may depend on n_tokens). x: device int8[n_tokens, in_dim], 16-byte aligned, any
- * codes; x_scales: device f32[n_tokens, in_dim / x_group] or [n_tokens]; y:
+ * everything else f32 (products of many rows, and of few rows with more than
+ * 16384 columns, round x_scales per group to 22 bits, by 2^-23; a row's last
+ * bits may depend on n_tokens). x: device int8[n_tokens, in_dim], 16-byte
+ * aligned, any codes; x_scales: device f32[n_tokens, in_dim / x_group] or [n_tokens]; y:
  * device f32. Weights of bits 4, 3 or 8, group 32, 64 or 128, in_dim a
  * multiple of the group up to 16384, out_dim up to 2^28, n_tokens up to
  * 1048560, fewer than 2^24 - 7 tiles of 128 x 128 outputs
@@ -644,7 +645,8 @@ typedef struct {
  * in [0, src_rows)). A source row may be taken any number of times; bytes of
  * dst outside the pieces stay. A row index out of range is found on the
  * device: its rows stay as they were and the next smoe_sync returns
- * SMOE_ERR_INVALID_ARG. src and dst of a state must not overlap, nor rows or
+ * SMOE_ERR_INVALID_ARG. src and dst of a state must not overlap (each
+ * from its first byte to its last, whatever lies between), nor rows or
  * pieces of dst (SMOE_ERR_INVALID_ARG); a state's dst must not overlap
  * another state. Addresses and strides of any alignment (16 bytes are the
  * fast case). Pieces of all rows below 2^24 in a state, longer pieces counted

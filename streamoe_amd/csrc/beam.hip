@@ -79,10 +79,10 @@ __host__ __device__ constexpr uint32_t beam_held(uint32_t picks) { return 18 * p
 // suffice. In the end the block ranks what is >= the waves' largest T by
 // counting.
 //
-// Four rows of 151936 (one tile a block) take 5 to 6 us, of which the loads are
-// 2.0, threshold 0.7, list and ranks 1.7; 64 rows 11.9 us for 39 MB: loads 5.2,
-// the exponentials 2.5, thresholds 2.4, lists 1.5, most of it VALU time (some
-// 350 instructions of a wave per tile). One tile a block took 14 us there (each
+// Four rows of 151936 (one tile a block) take 7.2 us, of which the loads are
+// 2.0, threshold 0.7, list and ranks 1.7; 64 rows 13.4 us for 39 MB: loads 5.2,
+// the exponentials 2.5, thresholds 2.4, lists 1.5, one after another (two blocks
+// per CU are two waves per SIMD; the VALU is busy a quarter of the time). One tile a block took 14 us there (each
 // with a threshold, a list to rank and its reductions). Peeling the last tile
 // off, so that no branch stands between a tile's loads and its use, gained
 // nothing.
@@ -296,7 +296,7 @@ __device__ __forceinline__ BeamKey beam_key(double v, uint32_t beam, uint32_t or
 // A wave per beam: lane s holds the head of slice s's list (at most 64 slices);
 // the largest head, of equal ones the lowest lane's (slices are in token
 // order), is taken P times. The beams' P each are ranked by counting, each by eight
-// lanes. 3.1 us for one request of four beams and 8 picks, 4.4 for 16: a chain
+// lanes. 4.4 us for one request of four beams and 8 picks, 4.8 for 16: a chain
 // of one load, P rounds of a wave's maximum (0.1 us each) and the ranks (one
 // lane per pick: 0.8 us more).
 __global__ __launch_bounds__(256) void k_beam_pick(BeamArgs a) {
@@ -377,7 +377,9 @@ __global__ __launch_bounds__(256) void k_beam_pick(BeamArgs a) {
 // Reordering: a block per 16 KiB of a piece; a launch takes up to 32 states, so
 // a cache of many layers needs few. 2.3 GB (40 states of 64 rows, four pieces
 // of 150 KB, each source row taken twice) in 457 us, 5.0 TB/s, a large copy's
-// rate; eight states of four rows of 64 KiB in 3.0 us.
+// rate; eight states of four rows of 64 KiB in 4.1 us. Addresses or strides that 4
+// does not divide go byte by byte (16 rows of 4 MiB, from the caches: 44 us, 18 on 16
+// bytes and 20 on 4).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kCopyChunk = 16384;  // bytes per block
 constexpr uint32_t kCopyStates = 32;    // states per launch (by value: 2.5 KB of arguments)

@@ -306,7 +306,7 @@ enum LoraBy { kByPlan, kByWave, kByBlock };
 // u[share][place][j] = sum over the share's inputs of A[j] x. Four waves take
 // steps of 32 inputs in turn; lane (c, kb) holds eight inputs kb of row c. A
 // share per block makes blocks of few rows: 200 rows, 40 adapters of rank 64,
-// 4096 inputs 8.9 us for 24 MB, of which finding the items is about 3.
+// 4096 inputs 10.5 us for 24 MB, of which finding the items is about 3.
 template <bool XBF16, LoraBy BY, int MT>
 __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
   __shared__ f32x4 red[4][64];
@@ -400,9 +400,10 @@ __global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
 // 4096). The products go through LDS too, so that base and y move in whole rows
 // of the block (in the products' order each lane touches a line of its own).
 // B's and base's loads go out ahead of everything. 200 rows of rank 64 -> 4096
-// 8.6 us for 28 MB, 1000 rows of rank 32 -> 4096 11.3 us for
-// 33 MB of base and y: all blocks run at once, so the loads of items, shares
-// and base come one after another for each of them.
+// 10.1 us for 28 MB, 1000 rows of rank 32 -> 4096 12.6 us for 33 MB of base and
+// y. With NT = 4 the 162 to 198 registers and 16 accumulators leave two blocks
+// per CU, so these 848 and 1056 blocks run in two to three rounds, each the
+// chain of its loads: items, shares and base, products, stores.
 template <int KT, int NT>
 __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
   constexpr uint32_t RP = KT * 32 + 8;  // bf16 per row in LDS: rows apart by 16 bytes of banks
@@ -532,8 +533,9 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
 // Both products of a small item in one launch: sixteen waves share the inputs
 // (step s is wave s mod 16's), their parts are added in LDS, and each wave takes
 // 16 outputs. Every block of 256 outputs forms u for itself, from the caches (8
-// rows, 4 adapters of rank 16, 2048 -> 2048: 6.1 us, the two kernels 5.8 and a second launch): what a
-// CU can load bounds it, 64 bytes a cycle.
+// rows, 4 adapters of rank 16, 2048 -> 2048: 6.7 us, the two kernels 6.2). A CU
+// loads a block's 64 KB of A and 16 KB of x in some 0.6 us; the rest is one wave's chain (ids,
+// rows, loads, the joins' barriers, the second product), not taken apart.
 template <bool XBF16, int MT>
 __global__ __launch_bounds__(1024) void k_lora_one(LoraArgs a) {
   constexpr int KT = (MT + 1) / 2, U = MT <= 2 ? 4 : 2;  // steps of 32 ranks; steps of inputs in flight

@@ -25,9 +25,10 @@ constexpr uint32_t kNormThreads = 256;
 // One block per row, the row in registers between its two uses, so it is read
 // once: thread t holds the eights t, t + 256, ... (VEC), or the elements t,
 // t + 256, ... where rows are no whole number of eights. Memory bounds many
-// rows (1000 of 4096, bf16 in and out, codes in groups of 64, 53 MB: 11.8 us,
-// 4.5 TB/s, of the 5.0 of a large copy), one round trip a single one (2048: 1.8
-// us). The weight's loads go out with the row's.
+// rows (1000 of 4096, bf16 in and out, codes in groups of 64, 53 MB: 13.2 us,
+// 4.0 TB/s, of the 5.0 of a large copy), one round trip a single one (2048: 2.0
+// us). The weight's loads go out with the row's. Rows of less than 2048 leave
+// threads without values (65536 rows of 256: 3.4 TB/s, of 128: 1.7).
 // 1 / sqrt(m) by one Newton step on the hardware's estimate (good to 2^-23):
 // to 2^-45; 0 for an infinity.
 __device__ __forceinline__ float norm_rsqrt(double m) {

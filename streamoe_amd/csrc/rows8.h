@@ -600,9 +600,13 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
 // wave; the next step's loads are in flight while a step is computed. Weights
 // are the A operand, so a lane ends with four neighbouring columns of one row.
 //
-// The fold of a group's sums is what bounds it: two VALU instructions per
-// value, 8 per lane and 16 x 16 x 64 product (34 cycles, and the product keeps
-// the VALU from issuing for 10 of its 16). With scales per group the sums come
+// The fold of a group's sums is the largest part of it: two VALU instructions
+// per value, 8 per lane and 16 x 16 x 64 product (34 cycles, and the product
+// keeps the VALU from issuing for 10 of its 16), 36 of the 76 us. Matrix cores
+// are busy 20 % and the VALU 52 % of the time; what the two waves of a SIMD
+// wait for beside that (a step's end waits for all its copies and the barrier)
+// has not been taken apart. Groups of 128, half the folds, take 67 us, groups of
+// 32 126. With scales per group the sums come
 // out of the MFMA as floats, 1.5 2^23 + S, by an accumulator that starts as
 // that number's bits (|S| < 2^22), and fma(f, sx, -1.5 2^23 sx) = sx S in one
 // rounding: the product in the constant is exact for an sx of 22 bits, so sx is
@@ -1041,7 +1045,9 @@ static hipError_t q8_go(const Q8Args& a, hipStream_t st) {
   if (rt * ct <= 256) return q8_few<BITS, G, XG, 1, 1>(a, std::min(steps, 16u), st);
   if (rt == 1) {
     // 16 rows 2048 -> 16384, weights from HBM: 10.0, rows in LDS 10.1; -> 24576:
-    // 13.7 and 12.6; -> 32768: 16.8 and 13.5.
+    // 13.7 and 12.6; -> 32768: 16.8 and 13.5. Rows that do not fit a CU's LDS
+    // fall back (8192 -> 151936: 277 with scales per group, which do not, 154
+    // with scales per row, which do).
     if (ct <= 1024 || a.K < 2 * G || q8_wide_lds(BITS, a.K, G, 1, XG) > 160 * 1024)
       return q8_few<BITS, G, XG, 1, 2>(a, std::min(steps, 8u), st);
     return q8_wide<BITS, G, XG, 1>(a, st);
