@@ -509,8 +509,9 @@ int smoe_moe_prefill_block(smoe_handle* h, const smoe_expert_shape* shape, const
  * takes: scale = max|y| / 127, code = y / scale rounded to nearest even; a
  * group with an infinity or NaN has scale NaN and codes 0, one whose largest
  * magnitude is below 2^-119 scale 0 and codes 0. The mean and its root are
- * f64, so any row of finite r has its norm; one with an infinity gives zeros
- * beside it, as the formula does.
+ * f64, so a row of any finite r has its norm (but where mean(r^2) + eps is
+ * below 2^-256: 1 / sqrt is an f32); one with an infinity gives zeros beside
+ * it, as the formula does.
  * x: device [n_tokens, hidden], bf16 when x_is_bf16 else f32; residual:
  * device f32 or NULL (r = x); norm_w: device bf16[hidden] or NULL (ones);
  * sum_out: device f32, out: device bf16 when out_is_bf16 else f32, out_q:
