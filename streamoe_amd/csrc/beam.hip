@@ -18,6 +18,7 @@
 namespace smoe {
 
 typedef unsigned long long u64;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr uint32_t kBeamBlocks = 512;         // two per CU, if rows and tiles allow
 constexpr uint32_t kBeamTile = 4096;          // logits per block and round: 16 per thread
@@ -95,39 +96,35 @@ __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
   u64* const list = lists + wave * (beam_held(P) + P);
-  const uint64_t first = (uint64_t)row * a.vocab, total = (uint64_t)a.rows * a.vocab;
-  const uint32_t shift = (uint32_t)(first & 3);  // tiles start on 16 bytes, up to three logits ahead of the row
-  // Thread t's fours j of a tile: tokens tok0 + 1024 j + 4 t on.
-  auto start = [&](uint32_t tile) { return (int64_t)tile * kBeamTile - shift; };
+  const uint64_t first = (uint64_t)row * a.vocab;
+  // Thread t's fours j of a tile: tokens start + 1024 j + 4 t on, counted from
+  // the row's first, whatever its address: rows of the same logits are added up
+  // the same way, so they tie. Fours lie on 4 bytes.
   auto load = [&](uint32_t tile, f32x4 (&q)[4]) {
-    const int64_t tok0 = start(tile), tok = tok0 + t * 4;
-    if (tok0 >= 0 && tok0 + kBeamTile <= (int64_t)a.vocab) {
-      const float* const p = a.logits + first + tok;
+    const uint32_t tok0 = tile * kBeamTile, tok = tok0 + t * 4;
+    const float* const p = a.logits + first + tok;
+    if (tok0 + kBeamTile <= a.vocab) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const f32x4*>(p + 1024 * j);
+      for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const f32x4u*>(p + 1024 * j);
       return;
     }
-    // Places outside the row are -inf.
+    // Places behind the row are -inf.
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t k = tok + 1024 * j, e = (int64_t)first + k;
+      const uint32_t k = tok + 1024 * j;
       q[j] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (k < (int64_t)a.vocab) {
-        if (e + 4 <= (int64_t)total) {
-          q[j] = *reinterpret_cast<const f32x4*>(a.logits + e);
-        } else {
+      if (k + 4 <= a.vocab) {
+        q[j] = *reinterpret_cast<const f32x4u*>(p + 1024 * j);
+      } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (e + c < (int64_t)total) q[j][c] = a.logits[e + c];
-        }
+        for (int c = 0; c < 4; ++c)
+          if (k + c < a.vocab) q[j][c] = p[1024 * j + c];
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) q[j][c] = k + c >= 0 && k + c < (int64_t)a.vocab ? q[j][c] : -INFINITY;
     }
   };
   const uint32_t tile0 = slice * a.tiles;
   uint32_t tiles = a.tiles;
-  while (tiles && start(tile0 + tiles - 1) >= (int64_t)a.vocab) --tiles;
+  while (tiles && (tile0 + tiles - 1) * kBeamTile >= a.vocab) --tiles;
   f32x4 q[4], ahead[4];
   if (tiles) load(tile0, q);
   if (!beam_open(a, row)) return;  // under the loads
@@ -136,7 +133,7 @@ __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
   uint32_t used = 0;
   for (uint32_t i = 0; i < tiles; ++i) {
     if (i + 1 < tiles) load(tile0 + i + 1, ahead);
-    const uint32_t tok0 = (uint32_t)start(tile0 + i);
+    const uint32_t tok0 = (tile0 + i) * kBeamTile;
     // A NaN counts as -inf: maxima pass it over, and so does beam_exp.
     float v[16];
 #pragma unroll
@@ -433,8 +430,7 @@ __global__ __launch_bounds__(256) void k_beam_copy(CopyArgs a) {
 static uint64_t al256(uint64_t n) { return (n + 255) & ~255ull; }
 
 uint64_t beam_workspace(uint32_t requests, uint32_t beams, uint32_t vocab, uint32_t picks, BeamArgs* a, uint8_t* base) {
-  // Tiles of a row start up to three logits ahead of it.
-  const uint32_t tiles = (vocab + 3 + kBeamTile - 1) / kBeamTile;
+  const uint32_t tiles = (vocab + kBeamTile - 1) / kBeamTile;
   const uint64_t rows = (uint64_t)requests * beams;
   const uint32_t per = (uint32_t)std::max<uint64_t>((tiles + kBeamMaxSlices - 1) / kBeamMaxSlices,
                                                     std::min<uint64_t>((rows * tiles + kBeamBlocks - 1) / kBeamBlocks, tiles));
