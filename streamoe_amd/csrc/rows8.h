@@ -456,10 +456,13 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
   for (uint32_t i = wave; i < octets * MT; i += 4) {
     const uint32_t o = i / MT, m = i % MT;
     float xs[2] = {0.f, 0.f};
+    // All eight, the last group in the place of those behind it (no branch: out
+    // of the middle of these the compiler (7.2.0) read the last product's result
+    // one instruction after it, where the matrix cores need eight).
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
-      const uint32_t g = o * 8 + j;
-      if (g >= gpr) break;
+      const bool in = o * 8 + j < gpr;
+      const uint32_t g = in ? o * 8 + j : gpr - 1;
       const u32x4* const xo = xl + (g / GS * MT + m) * 128;
       const u32x4 x[2] = {xo[at[0]], xo[at[1]]};
       i32x4 S;
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(256, 2) void k_q8_wide(Q8Args a, uint32_t tiles) {
         S = j % 4 == 0 ? q8_sums<G>(ones, x, 0) : j % 4 == 1 ? q8_sums<G>(ones, x, 1) : j % 4 == 2 ? q8_sums<G>(ones, x, 2) : q8_sums<G>(ones, x, 3);
       float f = (float)S[0];
       if constexpr (XG) f *= sxl[g * MT * 16 + m * 16 + c16];
-      if (kb == j / 2) xs[j & 1] = f;
+      xs[j & 1] = in && kb == j / 2 ? f : xs[j & 1];
     }
     parts[i * 64 + lane] = __builtin_bit_cast(u32x4, q8_parts(xs[0], xs[1]));
   }
