@@ -83,10 +83,10 @@ __host__ __device__ constexpr uint32_t beam_held(uint32_t picks) { return 18 * p
 // Four rows of 151936 (one tile a block) take 7.2 us, of which the loads are
 // 2.0, threshold 0.7, list and ranks 1.7; 64 rows 13.4 us for 39 MB: loads 5.2,
 // the exponentials 2.5, thresholds 2.4, lists 1.5, one after another (two blocks
-// per CU are two waves per SIMD; the VALU is busy a quarter of the time). One tile a block took 14 us there (each
-// with a threshold, a list to rank and its reductions). Peeling the last tile
-// off, so that no branch stands between a tile's loads and its use, gained
-// nothing.
+// per CU are two waves per SIMD; the VALU is busy a quarter of the time). One
+// tile a block took 14 us there (each with a threshold, a list to rank and its
+// reductions). Peeling the last tile off, so that no branch stands between a
+// tile's loads and its use, gained nothing.
 __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
   extern __shared__ __attribute__((aligned(16))) u64 lists[];  // per wave [19 P]; all waves' [72 P]
   __shared__ __attribute__((aligned(16))) float held[256 * 16];  // logits of threads that have one for the list
@@ -374,9 +374,9 @@ __global__ __launch_bounds__(256) void k_beam_pick(BeamArgs a) {
 // Reordering: a block per 16 KiB of a piece; a launch takes up to 32 states, so
 // a cache of many layers needs few. 2.3 GB (40 states of 64 rows, four pieces
 // of 150 KB, each source row taken twice) in 457 us, 5.0 TB/s, a large copy's
-// rate; eight states of four rows of 64 KiB in 4.1 us. Addresses or strides that 4
-// does not divide go byte by byte (16 rows of 4 MiB, from the caches: 44 us, 18 on 16
-// bytes and 20 on 4).
+// rate; eight states of four rows of 64 KiB in 4.1 us. Addresses or strides that
+// 4 does not divide go byte by byte (16 rows of 4 MiB, from the caches: 44 us, 18
+// on 16 bytes and 20 on 4).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kCopyChunk = 16384;  // bytes per block
 constexpr uint32_t kCopyStates = 32;    // states per launch (by value: 2.5 KB of arguments)

@@ -534,8 +534,9 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
 // (step s is wave s mod 16's), their parts are added in LDS, and each wave takes
 // 16 outputs. Every block of 256 outputs forms u for itself, from the caches (8
 // rows, 4 adapters of rank 16, 2048 -> 2048: 6.7 us, the two kernels 6.2). A CU
-// loads a block's 64 KB of A and 16 KB of x in some 0.6 us; the rest is one wave's chain (ids,
-// rows, loads, the joins' barriers, the second product), not taken apart.
+// loads a block's 64 KB of A and 16 KB of x in some 0.6 us; the rest is one
+// wave's chain (ids, rows, loads, the joins' barriers, the second product), not
+// taken apart.
 template <bool XBF16, int MT>
 __global__ __launch_bounds__(1024) void k_lora_one(LoraArgs a) {
   constexpr int KT = (MT + 1) / 2, U = MT <= 2 ? 4 : 2;  // steps of 32 ranks; steps of inputs in flight
