@@ -80,8 +80,8 @@ __host__ __device__ constexpr uint32_t beam_held(uint32_t picks) { return 18 * p
 // suffice. In the end the block ranks what is >= the waves' largest T by
 // counting.
 //
-// Four rows of 151936 (one tile a block) take 7.2 us, of which the loads are
-// 2.0, threshold 0.7, list and ranks 1.7; 64 rows 13.4 us for 39 MB: loads 5.2,
+// Four rows of 151936 (one tile a block) take 7.5 us, of which the loads are
+// 2.0, threshold 0.7, list and ranks 1.7; 64 rows 13.1 us for 39 MB: loads 5.2,
 // the exponentials 2.5, thresholds 2.4, lists 1.5, one after another (two blocks
 // per CU are two waves per SIMD; the VALU is busy a quarter of the time). One
 // tile a block took 14 us there (each with a threshold, a list to rank and its
