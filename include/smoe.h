@@ -656,6 +656,137 @@ int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_
                       uint32_t n_rows, uint32_t src_rows);
 
 /* ------------------------------------------------------------------ */
+/* Paged key / value caches and the attention over them                 */
+/* ------------------------------------------------------------------ */
+
+/* One layer's keys and values in pages of page_size slots: the row of head h
+ * at slot i of page p lies at k (v) + p * page_stride + h * head_stride +
+ * i * slot_stride, head_dim values in bf16 (bits 16), or in 8 bits (bits 8):
+ * int8 codes with one f32 scale per row, value = code * scale, scales in
+ * k_scales (v_scales) [n_pages, n_heads, page_size]. Pages, heads and slots may
+ * lie in any order, keys and values in one buffer or two; no two rows overlap.
+ * A cache that is no pool of pages is one page per sequence. */
+typedef struct {
+  void* k;              /* device, 16-byte aligned */
+  void* v;              /* device, 16-byte aligned */
+  float* k_scales;      /* device f32, 16-byte aligned, with bits 8; else NULL */
+  float* v_scales;      /* device f32, 16-byte aligned, with bits 8; else NULL */
+  uint64_t page_stride; /* bytes, multiples of 16, of k and of v */
+  uint64_t head_stride;
+  uint64_t slot_stride; /* below 2^27 */
+  uint32_t n_pages;
+  uint32_t page_size; /* slots, a multiple of 16 */
+  uint32_t n_heads;   /* of keys and values, up to 256 */
+  uint32_t head_dim;  /* a multiple of 16, up to 256 */
+  uint32_t bits;      /* 16 or 8 */
+  uint32_t reserved;  /* 0 */
+} smoe_kv_cache;
+
+/* The tokens of a call: token t is position pos[t] of sequence seq[t], or a
+ * padding row where seq[t] is -1. Position p of sequence s lies in page
+ * table[s * table_width + p / page_size], slot p % page_size. Table entries that
+ * no position of the call needs may hold anything. */
+typedef struct {
+  const int32_t* table; /* device int32[n_seqs, table_width] */
+  const int32_t* seq;   /* device int32[n_tokens] */
+  const int32_t* pos;   /* device int32[n_tokens] */
+  uint32_t n_seqs;
+  uint32_t table_width; /* table_width * page_size up to 2^30 */
+  uint32_t n_tokens;    /* up to 16384 */
+  uint32_t reserved;    /* 0 */
+} smoe_kv_tokens;
+
+/* The cache's rows of every token = k[t], v[t]: k, v device rows of n_heads *
+ * head_dim values, bf16 when x_is_bf16 else f32, x_stride elements from one
+ * token's to the next (16-byte aligned rows; side by side in one buffer, as a
+ * projection leaves them, or apart). bf16 rounds to nearest even; 8 bits: scale =
+ * max|x| / 127 of the row, code = x / scale rounded to nearest even; a row with
+ * an infinity or NaN has scale NaN and codes 0, one whose largest magnitude is
+ * below 2^-119 scale 0 and codes 0. A position that several tokens of the call
+ * name gets the last of them. Two sequences' positions that the call writes
+ * must not share a slot. Slots that no token names, and what lies between rows,
+ * stay as they were. k, v, table, seq and pos overlap neither the cache nor its
+ * scales (SMOE_ERR_INVALID_ARG). A sequence, position or page out of range is
+ * found on the device: the token is left out and the next smoe_sync returns
+ * SMOE_ERR_INVALID_ARG. Enqueue-only, allocates nothing, capturable in a HIP
+ * graph. */
+int smoe_kv_append(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_tokens* tokens, const void* k,
+                   const void* v, int x_is_bf16, uint64_t x_stride);
+
+/* k[t], v[t] = the cache's rows of every token, as bf16 (out_is_bf16) or f32:
+ * rows of n_heads * head_dim values, out_stride elements from one token's to the
+ * next, 16-byte aligned. 8 bits: code * scale in f32, rounded once. Padding rows,
+ * and tokens whose sequence, position or page is out of range (the next
+ * smoe_sync returns SMOE_ERR_INVALID_ARG), become zeros. Any token may come any
+ * number of times. The outputs overlap nothing (SMOE_ERR_INVALID_ARG).
+ * Enqueue-only, allocates nothing, capturable in a HIP graph. */
+int smoe_kv_gather(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_tokens* tokens, void* k, void* v,
+                   int out_is_bf16, uint64_t out_stride);
+
+/* Device workspace bytes smoe_attn_decode needs (0 for sizes it does not take). */
+uint64_t smoe_attn_decode_workspace_size(const smoe_kv_cache* cache, uint32_t n_heads, uint32_t n_tokens);
+
+/* Attention of every token's n_heads queries over its sequence's cache, its own
+ * position included:
+ *   out[t, h] = sum_p w_p v[p, h / g] / sum_p w_p,  w_p = exp(scale * q[t, h] . k[p, h / g])
+ * over pos[t] - window < p <= pos[t] (window 0: from 0 on), g = n_heads /
+ * cache->n_heads. Tokens of one sequence at positions that follow one
+ * another share reads of the cache; each sees its own positions only, whatever the others' hold.
+ * q: device rows of n_heads * head_dim values, bf16 when q_is_bf16 else f32,
+ * q_stride elements from one token's to the next, 16-byte aligned; out: device
+ * [n_tokens, n_heads, head_dim], bf16 when out_is_bf16 else f32, 16-byte aligned.
+ * Products on bf16 MFMA with f32 sums: bf16 values and codes enter as they are,
+ * f32 queries and the weights as three bf16 that add up to them; maxima and sums
+ * are f32. A padding row gives zeros; so do a row whose scores are all -inf and
+ * a token whose sequence or position is out of range; a page out of range is
+ * left out (the next smoe_sync returns SMOE_ERR_INVALID_ARG for these two). What
+ * an infinity or NaN in a query, key or value makes shows in the rows that see
+ * it only. n_heads a multiple of cache->n_heads, up to
+ * 4096. The last bits of a row depend on the lengths of the call's other rows.
+ * out and the workspace overlap nothing (SMOE_ERR_INVALID_ARG); workspace:
+ * device, 256-byte aligned, one call's at a time. Enqueue-only, allocates
+ * nothing, capturable in a HIP graph. */
+int smoe_attn_decode(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_tokens* tokens, const void* q,
+                     int q_is_bf16, uint64_t q_stride, uint32_t n_heads, float scale, uint32_t window, void* out,
+                     int out_is_bf16, void* workspace, uint64_t workspace_bytes);
+
+/* ------------------------------------------------------------------ */
+/* Sampling behind the LM head                                          */
+/* ------------------------------------------------------------------ */
+
+/* Device workspace bytes smoe_sample needs (0 for sizes it does not take). */
+uint64_t smoe_sample_workspace_size(uint32_t n_rows, uint32_t vocab);
+
+/* One token per row of logits, drawn with the row's number u from the filtered
+ * distribution. In the order of falling logits, equal ones by rising token, and
+ * with e_v = exp((logit_v - max) / temperature), the tokens kept are the first
+ *   top_k (0 or less: all), of these the fewest whose e add up to at least top_p
+ *   of all of theirs (one at least; top_p >= 1: all), of these the ones with
+ *   e_v >= min_p;
+ * the token is the first, by rising token, at which the kept e's running sum
+ * exceeds u times their sum. Temperature 0: the first of the order. A logit of
+ * -inf or NaN is never kept; a row with +inf has e = 1 there and 0 elsewhere.
+ * e is computed in f64 and held as an integer of 2^-s, s = 62 - bits of vocab (44
+ * for 2^18 tokens), so sums do not depend on their order and borders within
+ * 2^-s of the sum are told by the rounded values.
+ * logits: device f32[n_rows, vocab], 16-byte aligned; temperature, top_p, min_p,
+ * u: device f32[n_rows], top_k: device int32[n_rows]; temperature NULL: 1, top_k
+ * NULL: 0, top_p NULL: 1, min_p NULL: 0. out_tokens: device int32[n_rows];
+ * out_logprobs: device f32[n_rows] or NULL, the natural logarithm of the token's
+ * share of the kept sum. A row without a logit above -inf, and one with a
+ * temperature or min_p that is negative, infinite or NaN, min_p above 1, a
+ * top_p that is negative or NaN or a u outside [0, 1) gets token -1 and NaN; for
+ * the latter the next smoe_sync returns SMOE_ERR_INVALID_ARG. n_rows up to 65535, vocab
+ * up to 2^24 (SMOE_ERR_UNSUPPORTED_SHAPE). Outputs and workspace overlap nothing
+ * (SMOE_ERR_INVALID_ARG); workspace: device, 256-byte aligned, one call's at a
+ * time. The same bits on every run. Enqueue-only, allocates nothing, capturable
+ * in a HIP graph. No counterpart in the reference, whose sampling is greedy
+ * (io/gpu_lm_head.rs:130-193). */
+int smoe_sample(smoe_handle* h, const float* logits, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, const float* u, uint32_t n_rows, uint32_t vocab,
+                int32_t* out_tokens, float* out_logprobs, void* workspace, uint64_t workspace_bytes);
+
+/* ------------------------------------------------------------------ */
 /* Expert arena loader: packed_experts/layer_NN.bin -> device memory    */
 /* ------------------------------------------------------------------ */
 

@@ -16,7 +16,9 @@ follow the reference:
 Beside that path, the operators of a serving step over many requests:
 ``Kernels.rmsnorm`` (with 8-bit rows), ``Kernels.qmm_i8`` (products of
 those), ``Adapters`` and ``Kernels.lora``, ``Kernels.beam_select``,
-``BeamState`` and ``Kernels.beam_reorder``.
+``BeamState`` and ``Kernels.beam_reorder``; ``KvCache`` with
+``Kernels.kv_append``, ``Kernels.kv_gather`` and ``Kernels.attn_decode``, and
+``Kernels.sample``.
 
 Device buffers are torch tensors on ``cuda`` (PyTorch is only the
 allocator and stream provider here). Every call goes through libsmoe;
@@ -221,6 +223,65 @@ class BeamState:
         piece = (lambda t: t.stride(1) * size) if s.dim() == 3 else (lambda t: 0)
         raw = _abi.BeamStateC(*at, s.stride(0) * size, d.stride(0) * size, piece(s), piece(d), used, pieces, 0)
         return bytes(raw), s.shape[0], d.shape[0], s.get_device()
+
+
+@dataclass(frozen=True, eq=False)
+class KvCache:
+    """One layer's paged keys and values: k and v [n_pages, n_heads, page_size,
+    head_dim] in bf16, or int8 with k_scales and v_scales f32 [n_pages, n_heads,
+    page_size]. Rows (the last axis) are dense, the other axes may have any
+    strides, the same for k and v: heads behind slots, k and v in one buffer."""
+
+    k: object
+    v: object
+    k_scales: object = None
+    v_scales: object = None
+
+    def __post_init__(self):
+        held = tuple(None if t is None else t.detach() for t in (self.k, self.v, self.k_scales, self.v_scales))
+        object.__setattr__(self, "_held", held)
+        object.__setattr__(self, "_known", (None, None))
+
+    def c(self):
+        """The C struct, checked when first asked for (and again should a
+        storage have moved)."""
+        k, v, ks, vs = self._held
+        at = (k.data_ptr(), v.data_ptr(), _at(ks), _at(vs))
+        if self._known[0] != at:
+            object.__setattr__(self, "_known", (at, self._struct(at)))
+        return self._known[1]
+
+    @property
+    def device(self):
+        return self._held[0].get_device()
+
+    def _struct(self, at):
+        k, v, ks, vs = self._held
+        dev, codes = k.get_device(), k.dtype in _types("i8")
+        if (dev < 0 or v.get_device() != dev or k.dtype != v.dtype or not (codes or k.dtype in _types("bf16"))
+                or k.dim() != 4 or k.shape != v.shape or not k.numel() or k.stride(3) != 1
+                or any(a != b for a, b, n in zip(k.stride(), v.stride(), k.shape) if n > 1)):
+            raise SmoeError(_INVALID, "KvCache")
+        pages, heads, slots, dim = k.shape
+        for t in (ks, vs):
+            if codes != (t is not None) or (codes and (t.shape != k.shape[:3] or not _fits(t, _types("f32"), 1, dev))):
+                raise SmoeError(_INVALID, "KvCache: scales")
+        size = k.element_size()
+        # The stride of an axis of one says nothing.
+        step = [k.stride(i) * size if k.shape[i] > 1 else 0 for i in range(3)]
+        return _abi.KvCacheC(*at, *step, pages, slots, heads, dim, 8 * size, 0)
+
+
+def _row_stride(t, types, n, width, device):
+    """Elements from a row of t to the next, if t holds n rows of `width` dense
+    elements of `types` on `device` ([n, width] or [n, heads, dim]); else None."""
+    if t is None or t.dtype not in types or t.get_device() != device or t.dim() not in (2, 3) or t.shape[0] < n:
+        return None
+    if t.dim() == 2:
+        dense = t.shape[1] == width and (t.stride(1) == 1 or width == 1)
+    else:
+        dense = t.shape[1] * t.shape[2] == width and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2])
+    return None if not dense else t.stride(0) if n > 1 else width
 
 
 @dataclass
@@ -496,6 +557,77 @@ class Kernels:
             return _INVALID
         arr = (_abi.BeamStateC * len(known)).from_buffer_copy(b"".join([k[0] for k in known]))
         return _lib.smoe_beam_reorder(self.h, arr, len(known), rows.data_ptr(), n, min([k[1] for k in known]))
+
+    # -- paged caches and the attention over them -----------------------------------
+    def _kv_tokens(self, cache, table, seq, pos, n_tokens):
+        """The tokens' C struct, or None for tensors that a call may not take."""
+        i32, dev = _types("i32"), self.device
+        if (cache.device != dev or not _fits(table, i32, 1, dev) or table.dim() != 2
+                or not _fits(seq, i32, n_tokens, dev) or not _fits(pos, i32, n_tokens, dev)):
+            return None
+        n_seqs, width = table.shape
+        return _abi.KvTokensC(table.data_ptr(), seq.data_ptr(), pos.data_ptr(), n_seqs, width, n_tokens, 0)
+
+    def _kv_rows(self, cc, k, v, n_tokens):
+        """Row stride of k and v, or None where they are no rows of one kind."""
+        width = cc.n_heads * cc.head_dim
+        step = _row_stride(k, _types("f32_bf16"), n_tokens, width, self.device)
+        if step is None or k.dtype != v.dtype or _row_stride(v, _types("f32_bf16"), n_tokens, width, self.device) != step:
+            return None
+        return step
+
+    def kv_append(self, cache: KvCache, table, seq, pos, k, v, n_tokens):
+        """The cache's rows of tokens (seq[t], pos[t]) = k[t], v[t] (f32 or bf16
+        rows [n, heads, dim], any stride of axis 0); table int32 [sequences,
+        pages]; seq -1: a padding row."""
+        cc = cache.c()
+        tc = self._kv_tokens(cache, table, seq, pos, n_tokens)
+        step = self._kv_rows(cc, k, v, n_tokens)
+        if tc is None or step is None:
+            return _INVALID
+        return _lib.smoe_kv_append(self.h, cc, tc, k.data_ptr(), v.data_ptr(), k.element_size() == 2, step)
+
+    def kv_gather(self, cache: KvCache, table, seq, pos, k, v, n_tokens):
+        """k[t], v[t] = the cache's rows of the tokens, as f32 or bf16 by their type."""
+        cc = cache.c()
+        tc = self._kv_tokens(cache, table, seq, pos, n_tokens)
+        step = self._kv_rows(cc, k, v, n_tokens)
+        if tc is None or step is None:
+            return _INVALID
+        return _lib.smoe_kv_gather(self.h, cc, tc, k.data_ptr(), v.data_ptr(), k.element_size() == 2, step)
+
+    def attn_decode_workspace_size(self, cache: KvCache, n_heads, n_tokens):
+        return _lib.smoe_attn_decode_workspace_size(cache.c(), n_heads, n_tokens)
+
+    def attn_decode(self, cache: KvCache, table, seq, pos, q, scale, window, out, n_heads, n_tokens, workspace):
+        """out[t] = attention of q[t] (f32 or bf16 rows [n, heads, dim], any stride
+        of axis 0) over its sequence's positions up to pos[t], the last `window`
+        of them (0: all); out: f32 or bf16 [n, heads, dim]."""
+        cc, dev, either = cache.c(), self.device, _types("f32_bf16")
+        tc = self._kv_tokens(cache, table, seq, pos, n_tokens)
+        step = _row_stride(q, either, n_tokens, n_heads * cc.head_dim, dev)
+        if tc is None or step is None or not _fits(out, either, n_tokens * n_heads * cc.head_dim, dev) or not _dense(workspace, dev):
+            return _INVALID
+        return _lib.smoe_attn_decode(self.h, cc, tc, q.data_ptr(), q.element_size() == 2, step, n_heads, scale, window,
+                                     out.data_ptr(), out.element_size() == 2, _at(workspace), workspace.nbytes)
+
+    # -- sampling -------------------------------------------------------------------
+    def sample_workspace_size(self, n_rows, vocab):
+        return _lib.smoe_sample_workspace_size(n_rows, vocab)
+
+    def sample(self, logits, temperature, top_k, top_p, min_p, u, n_rows, vocab, out_tokens, out_logprobs, workspace):
+        """One token per row of logits, drawn with u in [0, 1) from what
+        temperature, top_k, top_p and min_p (a value per row, or None) keep."""
+        dev, f32, i32 = self.device, _types("f32"), _types("i32")
+        if not (_fits(logits, f32, n_rows * vocab, dev) and (temperature is None or _fits(temperature, f32, n_rows, dev))
+                and (top_k is None or _fits(top_k, i32, n_rows, dev)) and (top_p is None or _fits(top_p, f32, n_rows, dev))
+                and (min_p is None or _fits(min_p, f32, n_rows, dev)) and _fits(u, f32, n_rows, dev)
+                and _fits(out_tokens, i32, n_rows, dev) and (out_logprobs is None or _fits(out_logprobs, f32, n_rows, dev))
+                and _dense(workspace, dev)):
+            return _INVALID
+        return _lib.smoe_sample(self.h, logits.data_ptr(), _at(temperature), _at(top_k), _at(top_p), _at(min_p),
+                                u.data_ptr(), n_rows, vocab, out_tokens.data_ptr(), _at(out_logprobs), _at(workspace),
+                                workspace.nbytes)
 
     # -- expert files -------------------------------------------------------------
     def load_file(self, path, dst, offset=0, nbytes=0):

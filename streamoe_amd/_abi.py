@@ -112,6 +112,36 @@ class BeamStateC(C.Structure):
     ]
 
 
+class KvCacheC(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scales", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("page_stride", C.c_uint64),
+        ("head_stride", C.c_uint64),
+        ("slot_stride", C.c_uint64),
+        ("n_pages", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("n_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("bits", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class KvTokensC(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p),
+        ("seq", C.c_void_p),
+        ("pos", C.c_void_p),
+        ("n_seqs", C.c_uint32),
+        ("table_width", C.c_uint32),
+        ("n_tokens", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
 class FileLayout(C.Structure):
     _fields_ = [
         ("bits", C.c_uint32),
@@ -169,6 +199,13 @@ PROTOTYPES = {
     "smoe_beam_select_workspace_size": (_U64, [_U32, _U32, _U32, _U32]),
     "smoe_beam_select": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _P, _P, _U64]),
     "smoe_beam_reorder": (_I, [_P, C.POINTER(BeamStateC), _U32, _P, _U32, _U32]),
+    "smoe_kv_append": (_I, [_P, C.POINTER(KvCacheC), C.POINTER(KvTokensC), _P, _P, _I, _U64]),
+    "smoe_kv_gather": (_I, [_P, C.POINTER(KvCacheC), C.POINTER(KvTokensC), _P, _P, _I, _U64]),
+    "smoe_attn_decode_workspace_size": (_U64, [C.POINTER(KvCacheC), _U32, _U32]),
+    "smoe_attn_decode": (_I, [_P, C.POINTER(KvCacheC), C.POINTER(KvTokensC), _P, _I, _U64, _U32, C.c_float, _U32, _P,
+                              _I, _P, _U64]),
+    "smoe_sample_workspace_size": (_U64, [_U32, _U32]),
+    "smoe_sample": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32, _U32, _P, _P, _P, _U64]),
     "smoe_layer_file_layout": (_I, [_U64, _U32, _U32, _U32, _U32, _U64, _U64, C.POINTER(FileLayout)]),
     "smoe_load_file": (_I, [_P, C.c_char_p, _U64, _U64, _P, _U64, C.POINTER(_U64)]),
     "smoe_stream_read": (_I, [_P, _P, C.c_uint64, _P]),

@@ -1203,6 +1203,232 @@ int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_
   return SMOE_OK;
 }
 
+// The cache's rows as spans, and whether strides and sizes are sound: pages,
+// heads, slots and keys / values nest in some order, so no two rows overlap.
+static int check_cache(const smoe_kv_cache* c, KvView* v, Span (&rows)[4]) {
+  if (!c || !c->k || !c->v || !c->n_pages || !c->page_size || !c->n_heads || !c->head_dim || c->reserved)
+    return SMOE_ERR_INVALID_ARG;
+  if (c->bits != 16 && c->bits != 8) return SMOE_ERR_UNSUPPORTED_BITS;
+  if ((c->bits == 8) != (c->k_scales != nullptr) || (c->bits == 8) != (c->v_scales != nullptr)) return SMOE_ERR_INVALID_ARG;
+  if (c->head_dim % 16 || c->head_dim > kKvMaxDim || c->n_heads > kKvMaxHeads || c->page_size % 16 ||
+      c->page_size > kKvMaxPositions || c->slot_stride >= kKvMaxSlotStride)
+    return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(c->k, 0, 16) || !aligned(c->v, 0, 16) || !aligned(c->k_scales, 0, 16) || !aligned(c->v_scales, 0, 16) ||
+      c->page_stride % 16 || c->head_stride % 16 || c->slot_stride % 16)
+    return SMOE_ERR_MISALIGNED;
+  const uintptr_t k = (uintptr_t)c->k, w = (uintptr_t)c->v;
+  const uint64_t apart = k < w ? w - k : k - w, row = (uint64_t)c->head_dim * c->bits / 8;
+  struct Axis {
+    uint64_t stride, n;
+  } axes[4] = {{c->page_stride, c->n_pages}, {c->head_stride, c->n_heads}, {c->slot_stride, c->page_size}, {apart, 2}};
+  for (int i = 1; i < 4; ++i)
+    for (int j = i; j && axes[j].stride < axes[j - 1].stride; --j) {
+      const Axis a = axes[j];
+      axes[j] = axes[j - 1];
+      axes[j - 1] = a;
+    }
+  unsigned __int128 all = row;
+  for (const Axis& a : axes) {
+    if (a.n == 1) continue;
+    if (a.stride < all) return SMOE_ERR_INVALID_ARG;
+    all += (unsigned __int128)a.stride * (a.n - 1);
+  }
+  if (all >> 63) return SMOE_ERR_INVALID_ARG;
+  const uint64_t own = c->page_stride * (uint64_t)(c->n_pages - 1) + c->head_stride * (uint64_t)(c->n_heads - 1) +
+                       c->slot_stride * (uint64_t)(c->page_size - 1) + row;
+  const uint64_t scales = (uint64_t)c->n_pages * c->n_heads * c->page_size * 4;
+  rows[0] = {c->k, own};
+  rows[1] = {c->v, own};
+  rows[2] = {c->k_scales, scales};
+  rows[3] = {c->v_scales, scales};
+  if (overlap(rows[2], rows[3])) return SMOE_ERR_INVALID_ARG;
+  for (int i = 0; i < 2; ++i)
+    if (overlap(rows[i], rows[2]) || overlap(rows[i], rows[3])) return SMOE_ERR_INVALID_ARG;
+  v->k = (uint8_t*)c->k;
+  v->v = (uint8_t*)c->v;
+  v->ks = c->k_scales;
+  v->vs = c->v_scales;
+  // A stride over a single page, head or slot says nothing.
+  v->page = c->n_pages > 1 ? c->page_stride : 0;
+  v->head = c->n_heads > 1 ? c->head_stride : 0;
+  v->slot = c->page_size > 1 ? c->slot_stride : 0;
+  v->n_pages = c->n_pages;
+  v->page_size = c->page_size;
+  v->heads = c->n_heads;
+  v->dim = c->head_dim;
+  // n / d for n < 2^27 is n ceil(2^(27 + b) / d) >> 27 + b with 2^b >= d: the
+  // multiplier is less than 2^b / 2^(27 + b) of itself too large.
+  const uint32_t d = c->page_size / 16;
+  uint32_t b = 0;
+  while ((1u << b) < d) ++b;
+  v->div_shift = 27 + b;
+  v->div_mul = (((uint64_t)1 << v->div_shift) + d - 1) / d;
+  return SMOE_OK;
+}
+
+static int check_tokens(const smoe_kv_tokens* t, const smoe_kv_cache* c, KvTokens* v, Span (&at)[3]) {
+  if (!t || !t->table || !t->seq || !t->pos || !t->n_seqs || !t->table_width || !t->n_tokens || t->reserved)
+    return SMOE_ERR_INVALID_ARG;
+  if (t->n_tokens > kKvMaxTokens || (uint64_t)t->table_width * c->page_size > kKvMaxPositions)
+    return SMOE_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(t->table, 0, 4) || !aligned(t->seq, 0, 4) || !aligned(t->pos, 0, 4)) return SMOE_ERR_MISALIGNED;
+  at[0] = {t->table, (uint64_t)t->n_seqs * t->table_width * 4};
+  at[1] = {t->seq, (uint64_t)t->n_tokens * 4};
+  at[2] = {t->pos, (uint64_t)t->n_tokens * 4};
+  *v = {t->table, t->seq, t->pos, t->n_seqs, t->table_width, t->n_tokens, t->table_width * c->page_size};
+  return SMOE_OK;
+}
+
+// Rows of `width` elements per token, `stride` elements apart: their span.
+static int check_rows(const void* at, bool bf16, uint64_t stride, uint64_t width, uint32_t n, Span* rows) {
+  const uint64_t size = bf16 ? 2 : 4;
+  if (stride >> 60 || (n > 1 && stride < width)) return SMOE_ERR_INVALID_ARG;
+  if (!aligned(at, 0, 16) || (n > 1 && stride * size % 16)) return SMOE_ERR_MISALIGNED;
+  const unsigned __int128 all = ((unsigned __int128)stride * (n - 1) + width) * size;
+  if (all >> 63) return SMOE_ERR_INVALID_ARG;
+  *rows = {at, (uint64_t)all};
+  return SMOE_OK;
+}
+
+// Whether rows of k and v, of one stride, lie apart: side by side in one buffer or elsewhere.
+static bool rows_apart(const Span& k, const Span& v, uint64_t stride_bytes, uint64_t row_bytes) {
+  if (!overlap(k, v)) return true;
+  const uintptr_t p = (uintptr_t)k.at, q = (uintptr_t)v.at;
+  const uint64_t off = (p < q ? q - p : p - q) % stride_bytes;
+  return off >= row_bytes && off + row_bytes <= stride_bytes;
+}
+
+int smoe_kv_append(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_tokens* tokens, const void* k,
+                   const void* v, int x_is_bf16, uint64_t x_stride) {
+  if (!h || !k || !v) return SMOE_ERR_INVALID_ARG;
+  KvRowsArgs a{};
+  Span to[4], at[3], in[2];
+  if (int rc = check_cache(cache, &a.c, to)) return rc;
+  if (int rc = check_tokens(tokens, cache, &a.t, at)) return rc;
+  const uint64_t width = (uint64_t)cache->n_heads * cache->head_dim;
+  if (int rc = check_rows(k, x_is_bf16 != 0, x_stride, width, a.t.n, &in[0])) return rc;
+  if (int rc = check_rows(v, x_is_bf16 != 0, x_stride, width, a.t.n, &in[1])) return rc;
+  for (const Span& s : to)
+    for (const Span& i : {at[0], at[1], at[2], in[0], in[1]})
+      if (overlap(s, i)) return SMOE_ERR_INVALID_ARG;
+  if (int rc = use_device(h)) return rc;
+  a.k = k;
+  a.v = v;
+  a.stride = a.t.n > 1 ? x_stride : 0;
+  a.err = h->err;
+  return hip_status(launch_kv_append(a, x_is_bf16 != 0, cache->bits == 8, h->stream));
+}
+
+int smoe_kv_gather(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_tokens* tokens, void* k, void* v,
+                   int out_is_bf16, uint64_t out_stride) {
+  if (!h || !k || !v) return SMOE_ERR_INVALID_ARG;
+  KvRowsArgs a{};
+  Span in[4], at[3], to[2];
+  if (int rc = check_cache(cache, &a.c, in)) return rc;
+  if (int rc = check_tokens(tokens, cache, &a.t, at)) return rc;
+  const uint64_t width = (uint64_t)cache->n_heads * cache->head_dim, size = out_is_bf16 ? 2 : 4;
+  if (int rc = check_rows(k, out_is_bf16 != 0, out_stride, width, a.t.n, &to[0])) return rc;
+  if (int rc = check_rows(v, out_is_bf16 != 0, out_stride, width, a.t.n, &to[1])) return rc;
+  if (!rows_apart(to[0], to[1], (a.t.n > 1 ? out_stride : width) * size, width * size)) return SMOE_ERR_INVALID_ARG;
+  for (const Span& s : to)
+    for (const Span& i : {at[0], at[1], at[2], in[0], in[1], in[2], in[3]})
+      if (overlap(s, i)) return SMOE_ERR_INVALID_ARG;
+  if (int rc = use_device(h)) return rc;
+  a.ko = k;
+  a.vo = v;
+  a.stride = a.t.n > 1 ? out_stride : 0;
+  a.err = h->err;
+  return hip_status(launch_kv_gather(a, out_is_bf16 != 0, cache->bits == 8, h->stream));
+}
+
+static int check_attn(const smoe_kv_cache* c, uint32_t n_heads, uint32_t n_tokens) {
+  KvView v;
+  Span rows[4];
+  if (int rc = check_cache(c, &v, rows)) return rc;
+  if (!n_heads || !n_tokens || n_heads % c->n_heads) return SMOE_ERR_INVALID_ARG;
+  return n_heads > kAttnMaxHeads || n_tokens > kKvMaxTokens ? SMOE_ERR_UNSUPPORTED_SHAPE : SMOE_OK;
+}
+
+uint64_t smoe_attn_decode_workspace_size(const smoe_kv_cache* cache, uint32_t n_heads, uint32_t n_tokens) {
+  if (check_attn(cache, n_heads, n_tokens)) return 0;
+  return attn_workspace(cache->head_dim, n_tokens, nullptr, nullptr);
+}
+
+int smoe_attn_decode(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_tokens* tokens, const void* q,
+                     int q_is_bf16, uint64_t q_stride, uint32_t n_heads, float scale, uint32_t window, void* out,
+                     int out_is_bf16, void* workspace, uint64_t workspace_bytes) {
+  if (!h || !q || !out || !workspace) return SMOE_ERR_INVALID_ARG;
+  AttnArgs a{};
+  Span in[4], at[3], rows;
+  if (int rc = check_cache(cache, &a.c, in)) return rc;
+  if (int rc = check_tokens(tokens, cache, &a.t, at)) return rc;
+  if (int rc = check_attn(cache, n_heads, a.t.n)) return rc;
+  const uint64_t width = (uint64_t)n_heads * cache->head_dim;
+  if (int rc = check_rows(q, q_is_bf16 != 0, q_stride, width, a.t.n, &rows)) return rc;
+  if (!aligned(out, 0, 16) || !aligned(workspace, 0, 256)) return SMOE_ERR_MISALIGNED;
+  const uint64_t need = attn_workspace(cache->head_dim, a.t.n, &a, (uint8_t*)workspace);
+  if (workspace_bytes < need) return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  if (collide({{out, a.t.n * width * (out_is_bf16 ? 2 : 4)}, {workspace, need}},
+              {at[0], at[1], at[2], in[0], in[1], in[2], in[3], rows}))
+    return SMOE_ERR_INVALID_ARG;
+  if (int rc = use_device(h)) return rc;
+  a.q = q;
+  a.q_stride = a.t.n > 1 ? q_stride : 0;
+  a.heads = n_heads;
+  a.group = n_heads / cache->n_heads;
+  a.parts = (a.group + 15) / 16;
+  a.together = a.group >= 16 ? 1 : 16 / a.group;
+  a.scale = (float)((double)scale * 1.4426950408889634);
+  a.window = window;
+  a.out = out;
+  a.out_bf16 = out_is_bf16 != 0;
+  a.err = h->err;
+  const auto launch = cache->bits == 8 ? launch_attn_i8 : launch_attn_bf16;
+  const hipError_t e = launch(a, q_is_bf16 != 0, h->stream);
+  return hip_status(e == hipSuccess ? launch_attn_join(a, h->stream) : e);
+}
+
+static int check_sample(uint32_t n_rows, uint32_t vocab) {
+  if (!n_rows || !vocab) return SMOE_ERR_INVALID_ARG;
+  return n_rows > kSampleMaxRows || vocab > kSampleMaxVocab ? SMOE_ERR_UNSUPPORTED_SHAPE : SMOE_OK;
+}
+
+uint64_t smoe_sample_workspace_size(uint32_t n_rows, uint32_t vocab) {
+  if (check_sample(n_rows, vocab)) return 0;
+  return sample_workspace(n_rows, vocab, nullptr, nullptr);
+}
+
+int smoe_sample(smoe_handle* h, const float* logits, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, const float* u, uint32_t n_rows, uint32_t vocab,
+                int32_t* out_tokens, float* out_logprobs, void* workspace, uint64_t workspace_bytes) {
+  if (!h || !logits || !u || !out_tokens || !workspace) return SMOE_ERR_INVALID_ARG;
+  if (int rc = check_sample(n_rows, vocab)) return rc;
+  if (!aligned(logits, 0, 16) || !aligned(workspace, 0, 256)) return SMOE_ERR_MISALIGNED;
+  for (const void* p : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p,
+                        (const void*)u, (const void*)out_tokens, (const void*)out_logprobs})
+    if (!aligned(p, 0, 4)) return SMOE_ERR_MISALIGNED;
+  SampleArgs a{};
+  const uint64_t need = sample_workspace(n_rows, vocab, &a, (uint8_t*)workspace);
+  if (workspace_bytes < need) return SMOE_ERR_WORKSPACE_TOO_SMALL;
+  const uint64_t each = (uint64_t)n_rows * 4;
+  if (collide({{out_tokens, each}, {out_logprobs, each}, {workspace, need}},
+              {{logits, each * vocab}, {temperature, each}, {top_k, each}, {top_p, each}, {min_p, each}, {u, each}}))
+    return SMOE_ERR_INVALID_ARG;
+  if (int rc = use_device(h)) return rc;
+  a.logits = logits;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.u = u;
+  a.n = n_rows;
+  a.vocab = vocab;
+  a.tokens = out_tokens;
+  a.logprobs = out_logprobs;
+  a.err = h->err;
+  return hip_status(launch_sample(a, h->stream));
+}
+
 int smoe_synth_experts(smoe_handle* h, void* base, uint32_t n_experts, uint64_t stride,
                        const smoe_expert_shape* shape, uint64_t seed, float scale_sigma,
                        float bias_sigma) {

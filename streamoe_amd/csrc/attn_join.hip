@@ -1,0 +1,99 @@
+// attn_join.hip — the rows of the attention that several blocks had a part of,
+// and the rows that see nothing.
+#include "attn.h"
+
+namespace smoe {
+
+// A block joins a share (blockIdx.y) of one group's columns: fours of dims, each
+// by 256 / lanes threads that go through the parts in turn and are added up at
+// the end. Parts are added in their order, so a call gives the same bits again.
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, uint32_t share, uint32_t pad) {
+  __shared__ f32x4 sum[256];
+  __shared__ float2 stat[256];
+  const uint32_t tiles = a.c.heads * a.parts, row = blockIdx.x / tiles, tile = blockIdx.x - row * tiles;
+  const uint32_t t = threadIdx.x, fours = a.c.dim / 4;
+  const uint64_t before = a.before[row], units = a.before[row + 1] - before;
+  const AttnGroup grp = attn_group(a, row);
+  if (!grp.n) return;
+  const uint32_t kvh = tile / a.parts, part = tile - kvh * a.parts;
+  const uint32_t head0 = kvh * a.group + part * 16, heads = min(16u, a.group - part * 16);
+  const uint32_t all = grp.n * heads * fours, from = blockIdx.y * share, to = min(all, from + share);
+  auto put = [&](uint32_t e, f32x4 v) {
+    const uint32_t col = e / fours, token = col / heads;
+    const uint64_t at = ((uint64_t)(row + token) * a.heads + head0 + col - token * heads) * a.c.dim + (e - col * fours) * 4;
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    if (a.out_bf16)
+      *reinterpret_cast<bf16x4*>((uint16_t*)a.out + at) = __builtin_convertvector(v, bf16x4);
+    else
+      *reinterpret_cast<f32x4*>((float*)a.out + at) = v;
+  };
+  if (!units) {
+    for (uint32_t e = from + t; e < to; e += 256) put(e, f32x4{0, 0, 0, 0});
+    return;
+  }
+  const uint64_t total = a.before[a.t.n] * tiles, per = (total + a.blocks - 1) / a.blocks;
+  const uint64_t x = before * tiles + tile * units, b0 = x / per, b1 = (x + units - 1) / per;
+  if (b0 == b1) return;
+  const uint32_t parts = (uint32_t)(b1 - b0) + 1, turns = 256 / lanes, turn = t / lanes;
+  for (uint32_t e0 = from; e0 < to; e0 += lanes) {
+    const uint32_t e = e0 + t % lanes, col = min(e, all - 1) / fours, d = (min(e, all - 1) - col * fours) * 4;
+    float m = kAttnNone, l = 0.f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (uint32_t p = turn; p < parts; p += turns) {
+      const uint64_t slot = 2 * (b0 + p) + (p == 0 && x > b0 * per ? 1 : 0);
+      const float2 s = *reinterpret_cast<const float2*>(a.ml + (slot * 16 + col) * 2);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.acc + (slot * 16 + col) * pad + d);
+      const float top = fmaxf(m, s.x), f = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(s.x - top);
+      l = l * f + s.y * w;
+      acc = acc * f + v * w;
+      m = top;
+    }
+    sum[t] = acc;
+    stat[t] = float2{m, l};
+    __syncthreads();
+    if (turn == 0 && e < to) {
+      float top = m;
+      for (uint32_t i = 1; i < turns; ++i) top = fmaxf(top, stat[i * lanes + t].x);
+      float f = __builtin_amdgcn_exp2f(m - top);
+      l *= f;
+      acc *= f;
+      for (uint32_t i = 1; i < turns; ++i) {
+        const float2 s = stat[i * lanes + t];
+        f = __builtin_amdgcn_exp2f(s.x - top);
+        l += s.y * f;
+        acc += sum[i * lanes + t] * f;
+      }
+      put(e, acc * (l == 0.f ? 0.f : 1.f / l));
+    }
+    __syncthreads();
+  }
+}
+
+hipError_t launch_attn_join(const AttnArgs& a, hipStream_t st) {
+  const uint32_t items = a.t.n * a.c.heads * a.parts;
+  const uint32_t cols = min(16u, a.group) * a.together, all = cols * a.c.dim / 4;
+  // Eight fours a block where there are few rows to join, whole groups where
+  // there are many.
+  const uint32_t most = (all + 7) / 8, y = min(most, max(1u, 2048 / items));
+  const uint32_t share = (all + y - 1) / y;
+  uint32_t lanes = 8;
+  while (lanes < 256 && lanes < share) lanes *= 2;
+  const uint32_t pad = a.c.dim <= 64 ? 64 : a.c.dim <= 128 ? 128 : 256;
+  hipLaunchKernelGGL(k_attn_join, dim3(items, y), dim3(256), 0, st, a, lanes, share, pad);
+  return hipGetLastError();
+}
+
+uint64_t attn_workspace(uint32_t dim, uint32_t n, AttnArgs* a, uint8_t* base) {
+  const uint32_t pad = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  auto al = [](uint64_t b) { return (b + 255) & ~(uint64_t)255; };
+  const uint64_t before = al((uint64_t)(n + 1) * 8), ml = al((uint64_t)kAttnBlocks * 2 * 16 * 2 * 4);
+  if (a) {
+    a->blocks = kAttnBlocks;
+    a->before = (uint64_t*)base;
+    a->ml = (float*)(base + before);
+    a->acc = (float*)(base + before + ml);
+  }
+  return before + ml + (uint64_t)kAttnBlocks * 2 * 16 * pad * 4;
+}
+
+}  // namespace smoe

@@ -22,16 +22,6 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr uint32_t kBeamBlocks = 512;         // two per CU, if rows and tiles allow
 constexpr uint32_t kBeamTile = 4096;          // logits per block and round: 16 per thread
-constexpr uint32_t kOrdNegInf = 0x007FFFFFu;  // beam_ord(-inf)
-
-// Order of floats as unsigned integers; -0 as +0, NaN as -inf.
-__device__ __forceinline__ uint32_t beam_ord(float v) {
-  const uint32_t b = __float_as_uint(v == v ? v + 0.f : -INFINITY);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float beam_value(uint32_t o) {
-  return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
-}
 
 // e^x for x <= 0, from below -87 on (and for a NaN) 2^-126 (nothing beside a
 // sum of at least one): 2^p with p = x log2 e rounded, times 1 + r ln 2 for what the rounding
@@ -180,7 +170,7 @@ __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
     upto += dpp_u32<0x142, 0xA>(upto);
     upto += dpp_u32<0x143, 0xC>(upto);
     const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-    auto key = [&](float x, uint32_t token) { return (u64)beam_ord(x) << 32 | ~token; };
+    auto key = [&](float x, uint32_t token) { return (u64)float_ord(x) << 32 | ~token; };
     auto hold = [&]() {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -246,7 +236,7 @@ __global__ __launch_bounds__(256) void k_beam_slice(BeamArgs a) {
   if (t == 0) count = 0;
   __syncthreads();
   const float floor = fmaxf(fmaxf(least_of[0], least_of[1]), fmaxf(least_of[2], least_of[3]));
-  const u64 from = (u64)beam_ord(floor) << 32;
+  const u64 from = (u64)float_ord(floor) << 32;
   for (uint32_t e = lane; e < used + lane; e += 64) {
     const u64 k = e < used ? list[e] : 0;
     const u64 mask = __ballot(k >= from && k);
@@ -339,7 +329,7 @@ __global__ __launch_bounds__(256) void k_beam_pick(BeamArgs a) {
         }
         const uint32_t from = (uint32_t)__ffsll((long long)__ballot(o == mo)) - 1;
         if (lane == from) {
-          to[j] = beam_key((double)sc + ((double)beam_value(o) - lse), b, o, ~(uint32_t)head);
+          to[j] = beam_key((double)sc + ((double)ord_float(o) - lse), b, o, ~(uint32_t)head);
           ++at;
           head = at < P ? held[at * 64 + lane] : 0;
         }

@@ -27,6 +27,10 @@ constexpr int kChunk = 32;  // inputs per lane-chunk
 constexpr int kMaxK = 16;
 constexpr int kMaxSlots = kMaxK + 1;  // routed slots + shared expert
 
+// Values in 8 bits: a group whose largest magnitude is below 2^-119 (127 over
+// it would overflow) gets scale 0 and codes 0.
+constexpr float kQuantFloor = 1.5046328e-36f;
+
 __device__ __forceinline__ float bf16f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 
 template <int BITS>
@@ -515,6 +519,16 @@ __device__ __forceinline__ void store_limbs(uint32_t* p, const XLimbs& o) {
   t.w = 0;
   p4[6] = t;
 }
+
+// Order of floats as unsigned integers; -0 as +0, NaN as -inf.
+__device__ __forceinline__ uint32_t float_ord(float v) {
+  const uint32_t b = __float_as_uint(v == v ? v + 0.f : -INFINITY);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float ord_float(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+constexpr uint32_t kOrdNegInf = 0x007FFFFFu;  // float_ord(-inf)
 
 // Raises kernel fn's dynamic LDS limit to `bytes` on the current device,
 // once per device (`done` holds one bit per device index); function

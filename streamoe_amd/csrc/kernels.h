@@ -385,6 +385,78 @@ struct BeamCopy {
 uint64_t beam_copy_blocks(const BeamCopy& s, uint32_t n_rows);
 hipError_t launch_beam_copy(const BeamCopy* states, uint32_t n, const int32_t* rows, uint32_t n_rows,
                             uint32_t src_rows, uint32_t* err, hipStream_t st);
+// Paged key / value caches (cache.hip) and the attention over them (attn.h).
+constexpr uint32_t kKvMaxTokens = 16384, kKvMaxHeads = 256, kKvMaxDim = 256, kKvMaxPositions = 1u << 30;
+constexpr uint64_t kKvMaxSlotStride = 1ull << 27;
+struct KvView {
+  uint8_t *k, *v;
+  float *ks, *vs;                       // [pages, heads, page_size] with 8 bits, or null
+  uint64_t page, head, slot;            // strides in bytes
+  uint32_t n_pages, page_size, heads, dim;
+  // Sixteens of positions to pages: n / (page_size / 16) = n * div_mul >> div_shift for n < 2^27.
+  uint64_t div_mul;
+  uint32_t div_shift;
+};
+struct KvTokens {
+  const int32_t *table, *seq, *pos;
+  uint32_t n_seqs, width, n, positions;  // positions: width * page_size
+};
+struct KvRowsArgs {  // append: the cache's rows = k, v; gather: the other way round
+  KvView c;
+  KvTokens t;
+  const void *k, *v;  // append
+  void *ko, *vo;      // gather
+  uint64_t stride;    // elements between tokens of k, v, ko, vo
+  uint32_t lanes_log, per_block;  // lanes of a row, tokens of a block (append)
+  uint32_t* err;
+};
+hipError_t launch_kv_append(KvRowsArgs a, bool x_bf16, bool i8, hipStream_t st);
+hipError_t launch_kv_gather(KvRowsArgs a, bool out_bf16, bool i8, hipStream_t st);
+constexpr uint32_t kAttnMaxHeads = 4096;
+struct AttnArgs {
+  KvView c;
+  KvTokens t;
+  const void* q;
+  uint64_t q_stride;
+  uint32_t heads, group;     // query heads, and of one key head
+  uint32_t parts, together;  // tiles of up to 16 heads in a group; tokens that share a tile
+  float scale;               // times log2 e
+  uint32_t window;
+  void* out;
+  int out_bf16;
+  uint32_t* err;
+  // Workspace (attn_workspace).
+  uint32_t blocks;
+  uint64_t* before;          // [n + 1] units of the tokens before
+  float* ml;                 // [blocks, 2, 16, 2] maximum and sum of each column
+  float* acc;                // [blocks, 2, 16, padded dim] unscaled sums
+};
+uint64_t attn_workspace(uint32_t dim, uint32_t n, AttnArgs* a, uint8_t* base);
+hipError_t launch_attn_bf16(const AttnArgs& a, bool q_bf16, hipStream_t st);  // by the cache's type
+hipError_t launch_attn_i8(const AttnArgs& a, bool q_bf16, hipStream_t st);
+hipError_t launch_attn_join(const AttnArgs& a, hipStream_t st);
+// Sampling (sample.hip).
+constexpr uint32_t kSampleMaxRows = 65535, kSampleMaxVocab = 1u << 24;
+constexpr uint32_t kSampleBins = 896;  // of a logit's distance from the row's largest
+struct SampleArgs {
+  const float *logits, *temperature;  // [n, vocab]; [n] or null, as the others
+  const int32_t* top_k;
+  const float *top_p, *min_p, *u;
+  uint32_t n, vocab;
+  int32_t* tokens;
+  float* logprobs;
+  uint32_t* err;
+  // Workspace (sample_workspace).
+  uint32_t slices, slice;             // slices of a row, logits of each (a multiple of 1024)
+  double unit;                        // 2^s: what a mass of 1 is held as
+  unsigned long long *tops;           // [n, slices] largest key of a slice
+  unsigned long long *mass;           // [n, bins] of the row's logits
+  unsigned long long *kept;           // [n, slices] mass of what is kept for certain
+  unsigned long long *list;           // [n, vocab] keys of the border's bins
+  uint32_t* count;                    // [n, bins], behind them the list's length
+};
+uint64_t sample_workspace(uint32_t n, uint32_t vocab, SampleArgs* a, uint8_t* base);
+hipError_t launch_sample(const SampleArgs& a, hipStream_t st);
 // Streaming-read diagnostic over `bytes` (multiple of 16) with
 // kStreamBlocks blocks; sink: kStreamBlocks u32.
 constexpr uint32_t kStreamBlocks = 2048;

@@ -16,10 +16,6 @@ namespace smoe {
 typedef __bf16 nbf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// A group whose largest magnitude is below 2^-119 (127 over it would
-// overflow) gets scale 0 and codes 0.
-constexpr float kQuantFloor = 1.5046328e-36f;
-
 constexpr uint32_t kNormThreads = 256;
 
 // One block per row, the row in registers between its two uses, so it is read

@@ -191,6 +191,18 @@ impl Kernels {
         unsafe { sys::smoe_beam_select_workspace_size(n_requests, n_beams, vocab, n_picks) }
     }
 
+    /// Device workspace bytes an [`AttnDecodeCall`] needs (0: sizes it does
+    /// not take).
+    pub fn attn_decode_workspace_size(cache: &KvCache, n_heads: u32, n_tokens: u32) -> u64 {
+        unsafe { sys::smoe_attn_decode_workspace_size(&cache.view(), n_heads, n_tokens) }
+    }
+
+    /// Device workspace bytes a [`SampleCall`] needs (0: sizes it does not
+    /// take).
+    pub fn sample_workspace_size(n_rows: u32, vocab: u32) -> u64 {
+        unsafe { sys::smoe_sample_workspace_size(n_rows, vocab) }
+    }
+
     /// Copy a byte range of a layer file into device memory (the resident
     /// part of `ExpertFiles::open` + `attach_to_device`,
     /// io/expert_io.rs:300-420); returns the bytes copied.
@@ -847,6 +859,228 @@ impl KernelCall for BeamReorderCall<'_> {
         }
         check(unsafe {
             sys::smoe_beam_reorder(k.h, raw.as_ptr(), raw.len() as u32, rows, self.n_rows, self.src_rows)
+        }, what)
+    }
+}
+
+/// One layer's keys and values in pages: `k` and `v` start at the buffers'
+/// given offsets, rows of `head_dim` bf16 (`bits` 16) or int8 codes with an f32
+/// scale each (`bits` 8, scales `[n_pages, n_heads, page_size]`) at the strides'
+/// places, in bytes.
+#[derive(Clone, Copy, Debug)]
+pub struct KvCache<'a> {
+    pub k: &'a BufferRef,
+    pub k_offset: u64,
+    pub v: &'a BufferRef,
+    pub v_offset: u64,
+    pub scales: Option<(&'a BufferRef, &'a BufferRef)>,
+    pub page_stride: u64,
+    pub head_stride: u64,
+    pub slot_stride: u64,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub n_heads: u32,
+    pub head_dim: u32,
+    pub bits: u32,
+}
+
+impl KvCache<'_> {
+    fn view(&self) -> sys::smoe_kv_cache {
+        let at = |b: &BufferRef, o: u64| (b.ptr as *mut u8).wrapping_add(o as usize) as *mut c_void;
+        let (ks, vs) = self.scales.map_or((ptr::null_mut(), ptr::null_mut()), |(a, b)| (a.ptr as *mut f32, b.ptr as *mut f32));
+        sys::smoe_kv_cache {
+            k: at(self.k, self.k_offset),
+            v: at(self.v, self.v_offset),
+            k_scales: ks,
+            v_scales: vs,
+            page_stride: self.page_stride,
+            head_stride: self.head_stride,
+            slot_stride: self.slot_stride,
+            n_pages: self.n_pages,
+            page_size: self.page_size,
+            n_heads: self.n_heads,
+            head_dim: self.head_dim,
+            bits: self.bits,
+            reserved: 0,
+        }
+    }
+
+    /// The C view, after checking that the buffers hold every row.
+    fn raw(&self, what: &'static str) -> Result<sys::smoe_kv_cache, SmoeError> {
+        let last = |n: u32, stride: u64| (n as u64).saturating_sub(1).checked_mul(stride);
+        let extent = || {
+            let rows = last(self.n_pages, self.page_stride)?.checked_add(last(self.n_heads, self.head_stride)?)?;
+            rows.checked_add(last(self.page_size, self.slot_stride)?)?
+                .checked_add(self.head_dim as u64 * self.bits as u64 / 8)
+        };
+        let bytes = extent().unwrap_or(u64::MAX);
+        self.k.span(self.k_offset, bytes, what)?;
+        self.v.span(self.v_offset, bytes, what)?;
+        if let Some((a, b)) = self.scales {
+            let n = (self.n_pages as u64 * self.n_heads as u64).checked_mul(self.page_size as u64).unwrap_or(u64::MAX);
+            a.f32_span(0, n, what)?;
+            b.f32_span(0, n, what)?;
+        }
+        Ok(self.view())
+    }
+}
+
+/// The tokens of a call: position `pos[t]` of sequence `seq[t]` (-1: a padding
+/// row), position `p` of sequence `s` in page `table[s, p / page_size]`. What is
+/// out of range is reported by the next [`Kernels::sync`].
+#[derive(Clone, Copy, Debug)]
+pub struct KvTokens<'a> {
+    pub table: &'a BufferRef,
+    pub seq: &'a BufferRef,
+    pub pos: &'a BufferRef,
+    pub n_seqs: u32,
+    pub table_width: u32,
+    pub n_tokens: u32,
+}
+
+impl KvTokens<'_> {
+    fn raw(&self, what: &'static str) -> Result<sys::smoe_kv_tokens, SmoeError> {
+        let n = self.n_tokens as u64;
+        Ok(sys::smoe_kv_tokens {
+            table: opt_span(Some(self.table), self.n_seqs as u64 * self.table_width as u64, 4, what)? as *const i32,
+            seq: opt_span(Some(self.seq), n, 4, what)? as *const i32,
+            pos: opt_span(Some(self.pos), n, 4, what)? as *const i32,
+            n_seqs: self.n_seqs,
+            table_width: self.table_width,
+            n_tokens: self.n_tokens,
+            reserved: 0,
+        })
+    }
+
+    /// `n_tokens` rows of `width` elements, `stride` apart, from `offset` bytes
+    /// into the buffer on.
+    fn rows(&self, b: &BufferRef, offset: u64, stride: u64, width: u64, is_bf16: bool,
+            what: &'static str) -> Result<*mut c_void, SmoeError> {
+        let last = (self.n_tokens as u64).saturating_sub(1).checked_mul(stride);
+        let bytes = last.and_then(|n| n.checked_add(width)).and_then(|n| n.checked_mul(if is_bf16 { 2 } else { 4 }));
+        b.span(offset, bytes.unwrap_or(u64::MAX), what)
+    }
+}
+
+/// The cache's rows of every token = rows of `k` and `v` (`n_heads * head_dim`
+/// bf16 or f32, `stride` elements from one token's to the next, at byte offsets
+/// into their buffers). A position named twice gets the last row.
+pub struct KvAppendCall<'a> {
+    pub cache: KvCache<'a>,
+    pub tokens: KvTokens<'a>,
+    pub k: &'a BufferRef,
+    pub k_offset: u64,
+    pub v: &'a BufferRef,
+    pub v_offset: u64,
+    pub input_is_bf16: bool,
+    pub stride: u64,
+}
+
+impl KernelCall for KvAppendCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_kv_append";
+        let (c, t) = (self.cache.raw(what)?, self.tokens.raw(what)?);
+        let width = self.cache.n_heads as u64 * self.cache.head_dim as u64;
+        let kp = self.tokens.rows(self.k, self.k_offset, self.stride, width, self.input_is_bf16, what)?;
+        let vp = self.tokens.rows(self.v, self.v_offset, self.stride, width, self.input_is_bf16, what)?;
+        check(unsafe {
+            sys::smoe_kv_append(k.h, &c, &t, kp, vp, self.input_is_bf16 as c_int, self.stride)
+        }, what)
+    }
+}
+
+/// [`KvAppendCall`]'s other direction: rows of `k` and `v` = the cache's.
+pub struct KvGatherCall<'a> {
+    pub cache: KvCache<'a>,
+    pub tokens: KvTokens<'a>,
+    pub k: &'a BufferRef,
+    pub k_offset: u64,
+    pub v: &'a BufferRef,
+    pub v_offset: u64,
+    pub output_is_bf16: bool,
+    pub stride: u64,
+}
+
+impl KernelCall for KvGatherCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_kv_gather";
+        let (c, t) = (self.cache.raw(what)?, self.tokens.raw(what)?);
+        let width = self.cache.n_heads as u64 * self.cache.head_dim as u64;
+        let kp = self.tokens.rows(self.k, self.k_offset, self.stride, width, self.output_is_bf16, what)?;
+        let vp = self.tokens.rows(self.v, self.v_offset, self.stride, width, self.output_is_bf16, what)?;
+        check(unsafe {
+            sys::smoe_kv_gather(k.h, &c, &t, kp, vp, self.output_is_bf16 as c_int, self.stride)
+        }, what)
+    }
+}
+
+/// Attention of every token's queries over its sequence's cache, its own
+/// position included; `window` 0: all of them. Workspace:
+/// [`Kernels::attn_decode_workspace_size`] bytes.
+pub struct AttnDecodeCall<'a> {
+    pub cache: KvCache<'a>,
+    pub tokens: KvTokens<'a>,
+    pub queries: &'a BufferRef,
+    pub queries_offset: u64,
+    pub queries_are_bf16: bool,
+    pub stride: u64,
+    pub n_heads: u32,
+    pub scale: f32,
+    pub window: u32,
+    pub output: &'a BufferRef,
+    pub output_is_bf16: bool,
+    pub workspace: &'a BufferRef,
+}
+
+impl KernelCall for AttnDecodeCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_attn_decode";
+        let (c, t) = (self.cache.raw(what)?, self.tokens.raw(what)?);
+        let width = self.n_heads as u64 * self.cache.head_dim as u64;
+        let q = self.tokens.rows(self.queries, self.queries_offset, self.stride, width, self.queries_are_bf16, what)?;
+        let out = self.tokens.rows(self.output, 0, width, width, self.output_is_bf16, what)?;
+        check(unsafe {
+            sys::smoe_attn_decode(k.h, &c, &t, q, self.queries_are_bf16 as c_int, self.stride, self.n_heads,
+                                  self.scale, self.window, out, self.output_is_bf16 as c_int, self.workspace.ptr,
+                                  self.workspace.len)
+        }, what)
+    }
+}
+
+/// One token per row of logits, drawn with the row's `u` in [0, 1) from what
+/// the filters keep (`None`: temperature 1, no filter); the reference samples
+/// greedily (io/gpu_lm_head.rs:130-193). Workspace:
+/// [`Kernels::sample_workspace_size`] bytes.
+pub struct SampleCall<'a> {
+    pub logits: &'a BufferRef,
+    pub temperature: Option<&'a BufferRef>,
+    pub top_k: Option<&'a BufferRef>,
+    pub top_p: Option<&'a BufferRef>,
+    pub min_p: Option<&'a BufferRef>,
+    pub u: &'a BufferRef,
+    pub n_rows: u32,
+    pub vocab: u32,
+    pub out_tokens: &'a BufferRef,
+    pub out_logprobs: Option<&'a BufferRef>,
+    pub workspace: &'a BufferRef,
+}
+
+impl KernelCall for SampleCall<'_> {
+    fn encode(&self, k: &Kernels) -> Result<(), SmoeError> {
+        let what = "smoe_sample";
+        let n = self.n_rows as u64;
+        let logits = self.logits.f32_span(0, n * self.vocab as u64, what)?;
+        let t = opt_span(self.temperature, n, 4, what)?;
+        let kk = opt_span(self.top_k, n, 4, what)?;
+        let p = opt_span(self.top_p, n, 4, what)?;
+        let m = opt_span(self.min_p, n, 4, what)?;
+        let u = self.u.f32_span(0, n, what)?;
+        let tokens = self.out_tokens.f32_span(0, n, what)?;
+        let logprobs = opt_span(self.out_logprobs, n, 4, what)?;
+        check(unsafe {
+            sys::smoe_sample(k.h, logits, t as *const f32, kk as *const i32, p as *const f32, m as *const f32, u,
+                             self.n_rows, self.vocab, tokens as *mut i32, logprobs as *mut f32, self.workspace.ptr,
+                             self.workspace.len)
         }, what)
     }
 }

@@ -117,6 +117,36 @@ pub struct smoe_beam_state {
     pub reserved: u32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct smoe_kv_cache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scales: *mut f32,
+    pub v_scales: *mut f32,
+    pub page_stride: u64,
+    pub head_stride: u64,
+    pub slot_stride: u64,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub n_heads: u32,
+    pub head_dim: u32,
+    pub bits: u32,
+    pub reserved: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct smoe_kv_tokens {
+    pub table: *const i32,
+    pub seq: *const i32,
+    pub pos: *const i32,
+    pub n_seqs: u32,
+    pub table_width: u32,
+    pub n_tokens: u32,
+    pub reserved: u32,
+}
+
 extern "C" {
     pub fn smoe_strerror(status: c_int) -> *const c_char;
     pub fn smoe_abi_version() -> u32;
@@ -197,6 +227,20 @@ extern "C" {
                             workspace: *mut c_void, workspace_bytes: u64) -> c_int;
     pub fn smoe_beam_reorder(h: *mut smoe_handle, states: *const smoe_beam_state, n_states: u32, rows: *const i32,
                              n_rows: u32, src_rows: u32) -> c_int;
+    pub fn smoe_kv_append(h: *mut smoe_handle, cache: *const smoe_kv_cache, tokens: *const smoe_kv_tokens,
+                          k: *const c_void, v: *const c_void, x_is_bf16: c_int, x_stride: u64) -> c_int;
+    pub fn smoe_kv_gather(h: *mut smoe_handle, cache: *const smoe_kv_cache, tokens: *const smoe_kv_tokens,
+                          k: *mut c_void, v: *mut c_void, out_is_bf16: c_int, out_stride: u64) -> c_int;
+    pub fn smoe_attn_decode_workspace_size(cache: *const smoe_kv_cache, n_heads: u32, n_tokens: u32) -> u64;
+    pub fn smoe_attn_decode(h: *mut smoe_handle, cache: *const smoe_kv_cache, tokens: *const smoe_kv_tokens,
+                            q: *const c_void, q_is_bf16: c_int, q_stride: u64, n_heads: u32, scale: f32,
+                            window: u32, out: *mut c_void, out_is_bf16: c_int, workspace: *mut c_void,
+                            workspace_bytes: u64) -> c_int;
+    pub fn smoe_sample_workspace_size(n_rows: u32, vocab: u32) -> u64;
+    pub fn smoe_sample(h: *mut smoe_handle, logits: *const f32, temperature: *const f32, top_k: *const i32,
+                       top_p: *const f32, min_p: *const f32, u: *const f32, n_rows: u32, vocab: u32,
+                       out_tokens: *mut i32, out_logprobs: *mut f32, workspace: *mut c_void,
+                       workspace_bytes: u64) -> c_int;
     pub fn smoe_layer_file_layout(file_bytes: u64, n_experts: u32, hidden: u32, inter: u32, group: u32,
                                   declared_size: u64, declared_stride: u64,
                                   out: *mut smoe_file_layout) -> c_int;
