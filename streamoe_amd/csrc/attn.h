@@ -34,42 +34,57 @@ typedef __bf16 abf16x8 __attribute__((ext_vector_type(8)));
 typedef float af32x8 __attribute__((ext_vector_type(8), aligned(16)));
 
 constexpr uint32_t kAttnUnit = 128;     // positions of a unit: 32 of each wave
-constexpr uint32_t kAttnBlocks = 512;   // two per CU
 constexpr float kAttnNone = -3.0e38f;   // maximum of no scores
 
-// The tokens that share a tile with token r: up to `together` of one sequence at
-// positions that follow one another, from a multiple of it on.
-struct AttnGroup {
-  uint32_t n;        // tokens; 0: r is not the first of its group
-  int32_t lo, hi;    // positions that one of them sees; hi < lo: none
-  uint32_t units;
-};
+// Positions that token (seq, pos) sees.
 __device__ __forceinline__ void attn_range(const AttnArgs& a, int32_t seq, int32_t pos, int32_t* lo, int32_t* hi) {
   bool wrong;
   const bool in = kv_token(a.t, seq, pos, &wrong);
   *hi = in ? pos : -1;
   *lo = in && a.window && (uint32_t)pos >= a.window ? pos - (int32_t)a.window + 1 : 0;
 }
-__device__ __forceinline__ bool attn_follows(const AttnArgs& a, uint32_t r) {
-  return r % a.together && a.t.seq[r] == a.t.seq[r - 1] && (uint32_t)a.t.pos[r] == (uint32_t)a.t.pos[r - 1] + 1u;
-}
-__device__ __forceinline__ AttnGroup attn_group(const AttnArgs& a, uint32_t r) {
-  AttnGroup g = {0, 0, -1, 0};
-  if (attn_follows(a, r)) return g;
-  const int32_t s = a.t.seq[r];
-  uint32_t lo = ~0u;
-  do {
-    int32_t l, h;
-    attn_range(a, s, a.t.pos[r + g.n], &l, &h);
-    if (h >= 0) lo = min(lo, (uint32_t)l), g.hi = max(g.hi, h);
-    ++g.n;
-  } while (r + g.n < a.t.n && attn_follows(a, r + g.n));
-  if (g.hi >= 0) {
-    g.lo = (int32_t)lo;
-    g.units = (uint32_t)g.hi / kAttnUnit - lo / kAttnUnit + 1;
+
+// The tokens that share a tile with token r: up to `together` of one sequence at
+// positions that follow one another, from a multiple of it on. A block keeps the
+// call's first tokens in LDS: what it asks again and again of them is a chain of
+// loads otherwise.
+struct AttnGroup {
+  uint32_t n;        // tokens; 0: r is not the first of its group
+  int32_t lo, hi;    // positions that one of them sees; hi < lo: none
+  uint32_t units;
+};
+constexpr uint32_t kAttnHeld = 1024;
+struct AttnTokens {
+  const AttnArgs& a;
+  const int32_t *held_seq, *held_pos;
+  __device__ int32_t seq(uint32_t r) const { return r < kAttnHeld ? held_seq[r] : a.t.seq[r]; }
+  __device__ int32_t pos(uint32_t r) const { return r < kAttnHeld ? held_pos[r] : a.t.pos[r]; }
+  __device__ bool follows(uint32_t r) const {
+    return r % a.together && seq(r) == seq(r - 1) && (uint32_t)pos(r) == (uint32_t)pos(r - 1) + 1u;
   }
-  return g;
-}
+  __device__ AttnGroup group(uint32_t r) const {
+    AttnGroup g = {0, 0, -1, 0};
+    if (follows(r)) return g;
+    const int32_t s = seq(r);
+    uint32_t lo = ~0u;
+    do {
+      int32_t l, h;
+      attn_range(a, s, pos(r + g.n), &l, &h);
+      if (h >= 0) lo = min(lo, (uint32_t)l), g.hi = max(g.hi, h);
+      ++g.n;
+    } while (r + g.n < a.t.n && follows(r + g.n));
+    if (g.hi >= 0) {
+      g.lo = (int32_t)lo;
+      g.units = (uint32_t)g.hi / kAttnUnit - lo / kAttnUnit + 1;
+    }
+    return g;
+  }
+};
+
+// Waves per SIMD that the kernel's registers leave room for, so blocks per CU:
+// keys, values and outputs of dims up to 256 alone take 192 of a wave's.
+constexpr uint32_t attn_blocks_per_cu(uint32_t d) { return d == 256 ? 1 : 2; }
+constexpr uint32_t kAttnCus = 256;
 
 template <int D, bool I8>
 constexpr int attn_dim(int c, int j) {  // dim of output j of lane c of 16
@@ -109,10 +124,15 @@ __device__ __forceinline__ float column_sum(float v) { return swap32_add(swap16_
 
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
 
+// Units of a block.
+__device__ __forceinline__ uint64_t attn_per(uint64_t units, uint32_t blocks_log) {
+  return (units + (1u << blocks_log) - 1) >> blocks_log;
+}
+
 // D: head_dim up to it (FULL: equal). QP: parts of a query value (1: bf16 rows,
 // 3: f32).
 template <int D, bool I8, bool FULL, int QP>
-__global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
+__global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a) {
   constexpr int KS = D / 32;                    // key steps of 32 dims
   constexpr int VJ = D / 16;                    // dims per lane of a value row
   constexpr int KW = I8 ? 2 : 4, VW = I8 ? VJ / 4 : VJ / 2;  // words of a lane: a key step, a value row
@@ -122,14 +142,19 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
   __shared__ uint64_t sums[4];
   __shared__ uint32_t start_row;
   __shared__ uint64_t start_units;
+  __shared__ int32_t held_seq[kAttnHeld], held_pos[kAttnHeld];
   const uint32_t t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t n = a.t.n, tiles = a.c.heads * a.parts, hd = a.c.dim;
 
+  for (uint32_t r = t; r < min(n, kAttnHeld); r += 256) held_seq[r] = a.t.seq[r], held_pos[r] = a.t.pos[r];
+  __syncthreads();
+  const AttnTokens tokens = {a, held_seq, held_pos};
+
   // Units before every token, and where this block's begin.
   const uint32_t each = (n + 255) / 256, r0 = t * each;
   uint64_t own = 0;
-  for (uint32_t r = r0; r < min(n, r0 + each); ++r) own += attn_group(a, r).units;
+  for (uint32_t r = r0; r < min(n, r0 + each); ++r) own += tokens.group(r).units;
   uint64_t upto = own;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -149,22 +174,22 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
     uint64_t u = mine;
     for (uint32_t r = r0; r < min(n, r0 + each); ++r) {
       a.before[r] = u;
-      u += attn_group(a, r).units;
+      u += tokens.group(r).units;
       bool wrong;
-      kv_token(a.t, a.t.seq[r], a.t.pos[r], &wrong);
+      kv_token(a.t, tokens.seq(r), tokens.pos(r), &wrong);
       if (wrong) *a.err = 2u;
     }
     if (t == 0) a.before[n] = all;
   }
   all *= tiles;
-  const uint64_t per = (all + a.blocks - 1) / a.blocks;
+  const uint64_t per = attn_per(all, a.blocks_log);
   uint64_t x = blockIdx.x * per;
   const uint64_t end = min(all, x + per);
   if (x >= end) return;
   if (mine * tiles <= x && x < (mine + own) * tiles) {
     uint64_t u = mine;
     for (uint32_t r = r0;; ++r) {
-      const uint64_t more = attn_group(a, r).units;
+      const uint64_t more = tokens.group(r).units;
       if (x < (u + more) * tiles) {
         start_row = r;
         start_units = u;
@@ -179,7 +204,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
   uint64_t base = start_units * tiles;
   const uint64_t block_x = x;
   while (x < end) {
-    const AttnGroup grp = attn_group(a, row);
+    const AttnGroup grp = tokens.group(row);
     const uint32_t units = __builtin_amdgcn_readfirstlane(grp.units);
     if (x >= base + (uint64_t)units * tiles) {  // another group's token, or padding
       base += (uint64_t)units * tiles;
@@ -188,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
     }
     const uint32_t together = __builtin_amdgcn_readfirstlane(grp.n);
     const int32_t lo = __builtin_amdgcn_readfirstlane(grp.lo), hi = __builtin_amdgcn_readfirstlane(grp.hi);
-    const int32_t seq = __builtin_amdgcn_readfirstlane(a.t.seq[row]);
+    const int32_t seq = __builtin_amdgcn_readfirstlane(tokens.seq(row));
     const uint32_t tile = (uint32_t)(x - base) / units, first = (uint32_t)(x - base) - tile * units;
     const uint32_t count = (uint32_t)min((uint64_t)(units - first), end - x);
     const uint32_t kvh = tile / a.parts, part = tile - kvh * a.parts;
@@ -198,12 +223,12 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
     // This lane's column: its token and what it sees.
     const uint32_t my_token = min(col / heads, together - 1);
     int32_t see_lo, see_hi;
-    attn_range(a, seq, a.t.pos[row + my_token], &see_lo, &see_hi);
+    attn_range(a, seq, tokens.pos(row + my_token), &see_lo, &see_hi);
     // What all see.
     int32_t all_lo = 0, all_hi = 0x7FFFFFFF;
     for (uint32_t i = 0; i < together; ++i) {
       int32_t l, h;
-      attn_range(a, seq, __builtin_amdgcn_readfirstlane(a.t.pos[row + i]), &l, &h);
+      attn_range(a, seq, __builtin_amdgcn_readfirstlane(tokens.pos(row + i)), &l, &h);
       all_lo = max(all_lo, l);
       all_hi = min(all_hi, h);
     }
@@ -425,7 +450,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnArgs a) {
           // themselves.
           for (uint32_t i = 0; i < together; ++i) {
             int32_t tl, th;
-            attn_range(a, seq, __builtin_amdgcn_readfirstlane(a.t.pos[row + i]), &tl, &th);
+            attn_range(a, seq, __builtin_amdgcn_readfirstlane(tokens.pos(row + i)), &tl, &th);
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
               uint32_t both = 0;
@@ -521,7 +546,7 @@ template <int D, bool I8>
 static hipError_t attn_go(const AttnArgs& a, bool q_bf16, hipStream_t st) {
   const auto fn = a.c.dim == D ? (q_bf16 ? k_attn<D, I8, true, 1> : k_attn<D, I8, true, 3>)
                                : (q_bf16 ? k_attn<D, I8, false, 1> : k_attn<D, I8, false, 3>);
-  hipLaunchKernelGGL(fn, dim3(a.blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(fn, dim3(1u << a.blocks_log), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 template <bool I8>

@@ -12,12 +12,16 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
   __shared__ float2 stat[256];
   const uint32_t tiles = a.c.heads * a.parts, row = blockIdx.x / tiles, tile = blockIdx.x - row * tiles;
   const uint32_t t = threadIdx.x, fours = a.c.dim / 4;
-  const uint64_t before = a.before[row], units = a.before[row + 1] - before;
-  const AttnGroup grp = attn_group(a, row);
-  if (!grp.n) return;
+  const uint64_t before = a.before[row], units = a.before[row + 1] - before, all_units = a.before[a.t.n];
+  // The group, all of its tokens at once.
+  const uint32_t i = t & 15, r = min(row + i, a.t.n - 1);
+  const bool follows = r % a.together && a.t.seq[r] == a.t.seq[r - 1] && (uint32_t)a.t.pos[r] == (uint32_t)a.t.pos[r - 1] + 1u;
+  const uint32_t mask = (uint32_t)__ballot(follows && row + i < a.t.n) & 0xFFFFu;
+  if (mask & 1) return;  // another group's token
+  const uint32_t n = __builtin_ctz(~(mask >> 1)) + 1;
   const uint32_t kvh = tile / a.parts, part = tile - kvh * a.parts;
   const uint32_t head0 = kvh * a.group + part * 16, heads = min(16u, a.group - part * 16);
-  const uint32_t all = grp.n * heads * fours, from = blockIdx.y * share, to = min(all, from + share);
+  const uint32_t all = n * heads * fours, from = blockIdx.y * share, to = min(all, from + share);
   auto put = [&](uint32_t e, f32x4 v) {
     const uint32_t col = e / fours, token = col / heads;
     const uint64_t at = ((uint64_t)(row + token) * a.heads + head0 + col - token * heads) * a.c.dim + (e - col * fours) * 4;
@@ -31,16 +35,24 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
     for (uint32_t e = from + t; e < to; e += 256) put(e, f32x4{0, 0, 0, 0});
     return;
   }
-  const uint64_t total = a.before[a.t.n] * tiles, per = (total + a.blocks - 1) / a.blocks;
-  const uint64_t x = before * tiles + tile * units, b0 = x / per, b1 = (x + units - 1) / per;
+  const uint64_t total = all_units * tiles, per = attn_per(total, a.blocks_log), x = before * tiles + tile * units;
+  uint32_t b0, b1;
+  if (total >> 32) {
+    b0 = (uint32_t)(x / per);
+    b1 = (uint32_t)((x + units - 1) / per);
+  } else {
+    b0 = (uint32_t)x / (uint32_t)per;
+    b1 = (uint32_t)(x + units - 1) / (uint32_t)per;
+  }
   if (b0 == b1) return;
-  const uint32_t parts = (uint32_t)(b1 - b0) + 1, turns = 256 / lanes, turn = t / lanes;
+  const uint32_t parts = b1 - b0 + 1, turns = 256 / lanes, turn = t / lanes;
   for (uint32_t e0 = from; e0 < to; e0 += lanes) {
     const uint32_t e = e0 + t % lanes, col = min(e, all - 1) / fours, d = (min(e, all - 1) - col * fours) * 4;
     float m = kAttnNone, l = 0.f;
     f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
     for (uint32_t p = turn; p < parts; p += turns) {
-      const uint64_t slot = 2 * (b0 + p) + (p == 0 && x > b0 * per ? 1 : 0);
+      const uint64_t slot = 2 * (uint64_t)(b0 + p) + (p == 0 && x > (uint64_t)b0 * per ? 1 : 0);
       const float2 s = *reinterpret_cast<const float2*>(a.ml + (slot * 16 + col) * 2);
       const f32x4 v = *reinterpret_cast<const f32x4*>(a.acc + (slot * 16 + col) * pad + d);
       const float top = fmaxf(m, s.x), f = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(s.x - top);
@@ -86,14 +98,15 @@ hipError_t launch_attn_join(const AttnArgs& a, hipStream_t st) {
 uint64_t attn_workspace(uint32_t dim, uint32_t n, AttnArgs* a, uint8_t* base) {
   const uint32_t pad = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
   auto al = [](uint64_t b) { return (b + 255) & ~(uint64_t)255; };
-  const uint64_t before = al((uint64_t)(n + 1) * 8), ml = al((uint64_t)kAttnBlocks * 2 * 16 * 2 * 4);
+  const uint32_t blocks = kAttnCus * attn_blocks_per_cu(pad);
+  const uint64_t before = al((uint64_t)(n + 1) * 8), ml = al((uint64_t)blocks * 2 * 16 * 2 * 4);
   if (a) {
-    a->blocks = kAttnBlocks;
+    a->blocks_log = 31 - __builtin_clz(blocks);
     a->before = (uint64_t*)base;
     a->ml = (float*)(base + before);
     a->acc = (float*)(base + before + ml);
   }
-  return before + ml + (uint64_t)kAttnBlocks * 2 * 16 * pad * 4;
+  return before + ml + (uint64_t)blocks * 2 * 16 * pad * 4;
 }
 
 }  // namespace smoe

@@ -426,7 +426,7 @@ struct AttnArgs {
   int out_bf16;
   uint32_t* err;
   // Workspace (attn_workspace).
-  uint32_t blocks;
+  uint32_t blocks_log;       // of the launch
   uint64_t* before;          // [n + 1] units of the tokens before
   float* ml;                 // [blocks, 2, 16, 2] maximum and sum of each column
   float* acc;                // [blocks, 2, 16, padded dim] unscaled sums
