@@ -1377,7 +1377,8 @@ int smoe_attn_decode(smoe_handle* h, const smoe_kv_cache* cache, const smoe_kv_t
   a.heads = n_heads;
   a.group = n_heads / cache->n_heads;
   a.parts = (a.group + 15) / 16;
-  a.together = a.group >= 16 ? 1 : 16 / a.group;
+  a.together = 1;
+  while (a.together * 2 * a.group <= 16) a.together *= 2;
   a.scale = (float)((double)scale * 1.4426950408889634);
   a.window = window;
   a.out = out;

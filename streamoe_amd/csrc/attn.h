@@ -36,49 +36,71 @@ typedef float af32x8 __attribute__((ext_vector_type(8), aligned(16)));
 constexpr uint32_t kAttnUnit = 128;     // positions of a unit: 32 of each wave
 constexpr float kAttnNone = -3.0e38f;   // maximum of no scores
 
-// Positions that token (seq, pos) sees.
-__device__ __forceinline__ void attn_range(const AttnArgs& a, int32_t seq, int32_t pos, int32_t* lo, int32_t* hi) {
-  bool wrong;
-  const bool in = kv_token(a.t, seq, pos, &wrong);
+typedef unsigned long long attn_u64;
+
+// Positions [lo, hi] that position pos of a sequence sees; hi < lo: none.
+__device__ __forceinline__ void attn_range(const AttnArgs& a, bool seq_in, int32_t pos, int32_t* lo, int32_t* hi) {
+  const bool in = seq_in && (uint32_t)pos < a.t.positions;
   *hi = in ? pos : -1;
   *lo = in && a.window && (uint32_t)pos >= a.window ? pos - (int32_t)a.window + 1 : 0;
 }
+// Whether token r goes on where the one before it ends, and shares its tile.
+__device__ __forceinline__ bool attn_follows(const AttnArgs& a, uint32_t r, int32_t seq, int32_t pos, int32_t seq_before,
+                                             int32_t pos_before) {
+  return (r & (a.together - 1)) && seq == seq_before && pos_before != 0x7FFFFFFF && pos == pos_before + 1;
+}
+__device__ __forceinline__ attn_u64 wave_scan_u64(attn_u64 v) {  // inclusive, on DPP
+  auto step = [&](uint32_t lo, uint32_t hi) { v += (attn_u64)hi << 32 | lo; };
+  step(dpp_u32<0x111, 0xF>((uint32_t)v), dpp_u32<0x111, 0xF>((uint32_t)(v >> 32)));
+  step(dpp_u32<0x112, 0xF>((uint32_t)v), dpp_u32<0x112, 0xF>((uint32_t)(v >> 32)));
+  step(dpp_u32<0x114, 0xF>((uint32_t)v), dpp_u32<0x114, 0xF>((uint32_t)(v >> 32)));
+  step(dpp_u32<0x118, 0xF>((uint32_t)v), dpp_u32<0x118, 0xF>((uint32_t)(v >> 32)));
+  step(dpp_u32<0x142, 0xA>((uint32_t)v), dpp_u32<0x142, 0xA>((uint32_t)(v >> 32)));
+  step(dpp_u32<0x143, 0xC>((uint32_t)v), dpp_u32<0x143, 0xC>((uint32_t)(v >> 32)));
+  return v;
+}
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, uint32_t lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane);
+}
+__device__ __forceinline__ attn_u64 lane_u64(attn_u64 v, uint32_t lane) {
+  return (attn_u64)lane_u32((uint32_t)(v >> 32), lane) << 32 | lane_u32((uint32_t)v, lane);
+}
 
-// The tokens that share a tile with token r: up to `together` of one sequence at
-// positions that follow one another, from a multiple of it on. A block keeps the
-// call's first tokens in LDS: what it asks again and again of them is a chain of
-// loads otherwise.
-struct AttnGroup {
-  uint32_t n;        // tokens; 0: r is not the first of its group
-  int32_t lo, hi;    // positions that one of them sees; hi < lo: none
-  uint32_t units;
+// Sixty-four tokens, one per lane. Tokens of one sequence at positions that
+// follow one another share a tile, up to `together` (a power of two) from a
+// multiple of it on: the lane of the first has their number and their units.
+struct AttnChunk {
+  uint32_t first;    // token of lane 0
+  int32_t seq, pos;
+  uint32_t n, units;
+  attn_u64 before;   // units of the lanes before, from the chunk's start
+  bool wrong;        // out of range
+  __device__ void load(const AttnArgs& a, uint32_t from) {
+    const uint32_t lane = threadIdx.x & 63, r = from + lane;
+    const bool in = r < a.t.n;
+    first = from;
+    seq = in ? a.t.seq[r] : -1;
+    pos = in ? a.t.pos[r] : 0;
+    const int32_t s = __shfl_up(seq, 1, kWave), p = __shfl_up(pos, 1, kWave);
+    const bool follows = in && attn_follows(a, r, seq, pos, s, p);
+    const attn_u64 mask = __ballot(follows);
+    n = follows || !in ? 0u : (uint32_t)__builtin_ctzll(~((mask >> 1) >> lane)) + 1;
+    const bool seq_in = (uint32_t)seq < a.t.n_seqs;
+    wrong = in && seq != -1 && !(seq_in && (uint32_t)pos < a.t.positions);
+    int32_t lo, hi;
+    attn_range(a, seq_in && n, max(pos, 0), &lo, &hi);
+    hi = min(pos + (int32_t)n - 1, (int32_t)a.t.positions - 1);
+    units = seq_in && n && hi >= max(pos, 0) ? (uint32_t)hi / kAttnUnit - (uint32_t)lo / kAttnUnit + 1 : 0u;
+    before = wave_scan_u64(units) - units;
+  }
+  __device__ attn_u64 all() const { return lane_u64(before + units, 63); }
 };
-constexpr uint32_t kAttnHeld = 1024;
-struct AttnTokens {
-  const AttnArgs& a;
-  const int32_t *held_seq, *held_pos;
-  __device__ int32_t seq(uint32_t r) const { return r < kAttnHeld ? held_seq[r] : a.t.seq[r]; }
-  __device__ int32_t pos(uint32_t r) const { return r < kAttnHeld ? held_pos[r] : a.t.pos[r]; }
-  __device__ bool follows(uint32_t r) const {
-    return r % a.together && seq(r) == seq(r - 1) && (uint32_t)pos(r) == (uint32_t)pos(r - 1) + 1u;
-  }
-  __device__ AttnGroup group(uint32_t r) const {
-    AttnGroup g = {0, 0, -1, 0};
-    if (follows(r)) return g;
-    const int32_t s = seq(r);
-    uint32_t lo = ~0u;
-    do {
-      int32_t l, h;
-      attn_range(a, s, pos(r + g.n), &l, &h);
-      if (h >= 0) lo = min(lo, (uint32_t)l), g.hi = max(g.hi, h);
-      ++g.n;
-    } while (r + g.n < a.t.n && follows(r + g.n));
-    if (g.hi >= 0) {
-      g.lo = (int32_t)lo;
-      g.units = (uint32_t)g.hi / kAttnUnit - lo / kAttnUnit + 1;
-    }
-    return g;
-  }
+
+// One block's part of a group's tile: units [first, first + count) of `units`.
+struct AttnPart {
+  uint32_t row, n, tile, first, count, units;
+  int32_t seq, pos;
+  bool whole, begun;  // all of the group's units; units before them are another block's
 };
 
 // Waves per SIMD that the kernel's registers leave room for, so blocks per CU:
@@ -131,429 +153,504 @@ __device__ __forceinline__ uint64_t attn_per(uint64_t units, uint32_t blocks_log
 
 // D: head_dim up to it (FULL: equal). QP: parts of a query value (1: bf16 rows,
 // 3: f32).
+//
+// The next tile's keys are asked for when this one's are used up, its values
+// likewise, over the end of a part of a group into the next: their loads are
+// always in flight.
+template <int D, bool I8, int QP>
+constexpr uint32_t attn_lds() {  // the queries; four waves' outputs
+  return (QP * (D / 32) + 4 * (D / 16)) * 1024;
+}
 template <int D, bool I8, bool FULL, int QP>
 __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a) {
   constexpr int KS = D / 32;                    // key steps of 32 dims
   constexpr int VJ = D / 16;                    // dims per lane of a value row
   constexpr int KW = I8 ? 2 : 4, VW = I8 ? VJ / 4 : VJ / 2;  // words of a lane: a key step, a value row
-  constexpr int kSwap = 2 * VJ * 64 * 16, kQ = QP * KS * 64 * 16;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kSwap > kQ ? kSwap : kQ];
-  __shared__ float ml[4][16][2];
-  __shared__ uint64_t sums[4];
-  __shared__ uint32_t start_row;
-  __shared__ uint64_t start_units;
-  __shared__ int32_t held_seq[kAttnHeld], held_pos[kAttnHeld];
+  constexpr int QN = KS < 4 ? 1 : KS / 4;       // pieces of eight query values per thread
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  u32x4* const q_lds = reinterpret_cast<u32x4*>(lds);
+  f32x4* const o_lds = reinterpret_cast<f32x4*>(lds + QP * KS * 1024);
+  __shared__ float2 ml[4][16];
+  __shared__ attn_u64 chunk_units[kKvMaxTokens / 64];
   const uint32_t t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const uint32_t n = a.t.n, tiles = a.c.heads * a.parts, hd = a.c.dim;
+  const uint32_t n = a.t.n, tiles = a.c.heads * a.parts, hd = a.c.dim, blk = blockIdx.x;
 
-  for (uint32_t r = t; r < min(n, kAttnHeld); r += 256) held_seq[r] = a.t.seq[r], held_pos[r] = a.t.pos[r];
-  __syncthreads();
-  const AttnTokens tokens = {a, held_seq, held_pos};
-
-  // Units before every token, and where this block's begin.
-  const uint32_t each = (n + 255) / 256, r0 = t * each;
-  uint64_t own = 0;
-  for (uint32_t r = r0; r < min(n, r0 + each); ++r) own += tokens.group(r).units;
-  uint64_t upto = own;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t v = __shfl_up((unsigned long long)upto, o, kWave);
-    if (lane >= (uint32_t)o) upto += v;
-  }
-  if (lane == 63) sums[wave] = upto;
-  __syncthreads();
-  uint64_t all = 0, skip = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < 4; ++w) {
-    if (w < wave) skip += sums[w];
-    all += sums[w];
-  }
-  const uint64_t mine = skip + upto - own;
-  if (blockIdx.x == 0) {
-    uint64_t u = mine;
-    for (uint32_t r = r0; r < min(n, r0 + each); ++r) {
-      a.before[r] = u;
-      u += tokens.group(r).units;
-      bool wrong;
-      kv_token(a.t, tokens.seq(r), tokens.pos(r), &wrong);
-      if (wrong) *a.err = 2u;
+  // The units in all, this block's, and the chunk of tokens in which they begin.
+  AttnChunk chunk;
+  attn_u64 chunk_at = 0, all, x, end;  // units before the chunk; units (times tiles) from x to end
+  if (n <= 64) {
+    chunk.load(a, 0);
+    all = chunk.all();
+    const attn_u64 per = attn_per(all * tiles, a.blocks_log);
+    x = blk * per;
+    end = min(all * tiles, x + per);
+    if (blk == 0 && wave == 0) {
+      if (lane < n) a.before[lane] = chunk.before;
+      if (lane == 0) a.before[n] = all;
+      if (chunk.wrong) *a.err = 2u;
     }
-    if (t == 0) a.before[n] = all;
-  }
-  all *= tiles;
-  const uint64_t per = attn_per(all, a.blocks_log);
-  uint64_t x = blockIdx.x * per;
-  const uint64_t end = min(all, x + per);
-  if (x >= end) return;
-  if (mine * tiles <= x && x < (mine + own) * tiles) {
-    uint64_t u = mine;
-    for (uint32_t r = r0;; ++r) {
-      const uint64_t more = tokens.group(r).units;
-      if (x < (u + more) * tiles) {
-        start_row = r;
-        start_units = u;
-        break;
-      }
-      u += more;
-    }
-  }
-  __syncthreads();
-
-  uint32_t row = __builtin_amdgcn_readfirstlane(start_row);
-  uint64_t base = start_units * tiles;
-  const uint64_t block_x = x;
-  while (x < end) {
-    const AttnGroup grp = tokens.group(row);
-    const uint32_t units = __builtin_amdgcn_readfirstlane(grp.units);
-    if (x >= base + (uint64_t)units * tiles) {  // another group's token, or padding
-      base += (uint64_t)units * tiles;
-      ++row;
-      continue;
-    }
-    const uint32_t together = __builtin_amdgcn_readfirstlane(grp.n);
-    const int32_t lo = __builtin_amdgcn_readfirstlane(grp.lo), hi = __builtin_amdgcn_readfirstlane(grp.hi);
-    const int32_t seq = __builtin_amdgcn_readfirstlane(tokens.seq(row));
-    const uint32_t tile = (uint32_t)(x - base) / units, first = (uint32_t)(x - base) - tile * units;
-    const uint32_t count = (uint32_t)min((uint64_t)(units - first), end - x);
-    const uint32_t kvh = tile / a.parts, part = tile - kvh * a.parts;
-    const uint32_t head0 = kvh * a.group + part * 16, heads = min(16u, a.group - part * 16);
-    const uint32_t cols = together * heads;
-
-    // This lane's column: its token and what it sees.
-    const uint32_t my_token = min(col / heads, together - 1);
-    int32_t see_lo, see_hi;
-    attn_range(a, seq, tokens.pos(row + my_token), &see_lo, &see_hi);
-    // What all see.
-    int32_t all_lo = 0, all_hi = 0x7FFFFFFF;
-    for (uint32_t i = 0; i < together; ++i) {
-      int32_t l, h;
-      attn_range(a, seq, __builtin_amdgcn_readfirstlane(tokens.pos(row + i)), &l, &h);
-      all_lo = max(all_lo, l);
-      all_hi = min(all_hi, h);
-    }
-
-    // The queries as operands: part, step, lane.
-    for (uint32_t i = t; i < (uint32_t)KS * 64; i += 256) {
-      const uint32_t c = i & 15, lg = (i >> 4) & 3, step = i >> 6;
-      const uint32_t d = I8 ? (step >> 1) * 64 + lg * 16 + (step & 1) * 8 : step * 32 + lg * 8;
-      const uint32_t token = c / heads;
-      u32x4* const to = reinterpret_cast<u32x4*>(lds) + i;
-      const bool in = c < cols && d < hd;
-      const uint64_t at = in ? (row + token) * a.q_stride + (head0 + c - token * heads) * hd + d : 0;
-      if constexpr (QP == 1) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>((const uint16_t*)a.q + at);
-        to[0] = in ? v : u32x4{0, 0, 0, 0};
-      } else {
-        const af32x8 v = *reinterpret_cast<const af32x8*>((const float*)a.q + at);
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = in ? v[j] : 0.f;
-        u32x4 p[3];
-        attn_split(f, p);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) to[j * KS * 64] = p[j];
-      }
+  } else {
+    const uint32_t chunks = (n + 63) / 64;
+    for (uint32_t c = wave; c < chunks; c += 4) {
+      chunk.load(a, c * 64);
+      const attn_u64 units = chunk.all();
+      if (lane == 0) chunk_units[c] = units;
+      if (blk == 0 && chunk.wrong) *a.err = 2u;
     }
     __syncthreads();
+    attn_u64 u[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += u[j] = 4 * lane + j < chunks ? chunk_units[4 * lane + j] : 0ull;
+    const attn_u64 upto = wave_scan_u64(sum);
+    all = lane_u64(upto, 63);
+    const attn_u64 per = attn_per(all * tiles, a.blocks_log);
+    x = blk * per;
+    end = min(all * tiles, x + per);
+    attn_u64 before = upto - sum;
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (blk == 0 && wave == 0 && 4 * lane + j < chunks) chunk_units[4 * lane + j] = before;
+      const attn_u64 here = __ballot(before * tiles <= x && x < (before + u[j]) * tiles);
+      if (here) {
+        const uint32_t l = (uint32_t)__builtin_ctzll(here);
+        c = 4 * l + j;
+        chunk_at = lane_u64(before, l);
+      }
+      before += u[j];
+    }
+    if (blk == 0) {
+      __syncthreads();
+      for (uint32_t i = wave; i < chunks; i += 4) {
+        chunk.load(a, i * 64);
+        if (i * 64 + lane < n) a.before[i * 64 + lane] = chunk_units[i] + chunk.before;
+      }
+      if (t == 0) a.before[n] = all;
+    }
+    if (x < end) chunk.load(a, c * 64);
+  }
+  if (x >= end) return;
+  const attn_u64 block_x = x;
 
-    f32x4 acc[VJ];
+  // The part that begins at unit y; y only grows.
+  auto part_at = [&](attn_u64 y) {
+    for (;;) {
+      const attn_u64 here = __ballot((chunk_at + chunk.before) * tiles <= y && y < (chunk_at + chunk.before + chunk.units) * tiles);
+      if (here) {
+        const uint32_t l = (uint32_t)__builtin_ctzll(here);
+        const attn_u64 base = (chunk_at + lane_u64(chunk.before, l)) * tiles;
+        AttnPart p;
+        p.units = lane_u32(chunk.units, l);
+        p.row = chunk.first + l;
+        p.n = lane_u32(chunk.n, l);
+        p.seq = (int32_t)lane_u32((uint32_t)chunk.seq, l);
+        p.pos = (int32_t)lane_u32((uint32_t)chunk.pos, l);
+        p.tile = (uint32_t)(y - base) / p.units;
+        p.first = (uint32_t)(y - base) - p.tile * p.units;
+        p.count = (uint32_t)min((attn_u64)(p.units - p.first), end - y);
+        p.whole = p.count == p.units;
+        p.begun = base + (attn_u64)p.tile * p.units < block_x;
+        return p;
+      }
+      chunk_at += chunk.all();
+      chunk.load(a, chunk.first + 64);
+    }
+  };
+  // What the group's tokens see: one of them, and all.
+  struct Span {
+    int32_t lo, hi, all_lo, all_hi;
+  };
+  auto span_of = [&](const AttnPart& p) {
+    Span s;
+    const int32_t last = p.pos + (int32_t)p.n - 1, top = (int32_t)a.t.positions - 1;
+    int32_t unused;
+    attn_range(a, true, max(p.pos, 0), &s.lo, &unused);
+    s.hi = min(last, top);
+    attn_range(a, true, s.hi, &s.all_lo, &unused);
+    s.all_hi = p.pos < 0 || last > top ? -1 : p.pos;
+    return s;
+  };
+  // This wave's tiles of a part: the units' 32 positions that overlap [lo, hi].
+  auto tiles_of = [&](const AttnPart& p, const Span& s, uint32_t* p0, uint32_t* left) {
+    *p0 = ((uint32_t)s.lo / kAttnUnit + p.first) * kAttnUnit + wave * 32;
+    *left = p.count;
+    if ((int32_t)*p0 + 31 < s.lo) *p0 += kAttnUnit, --*left;
+    if (*left && (int32_t)(*p0 + (*left - 1) * kAttnUnit) > s.hi) --*left;
+  };
+
+  const uint32_t slot_stride = (uint32_t)a.c.slot;
+  const uint32_t k_off = col * slot_stride + g * 16;
+  const uint32_t v_off = g * 4 * slot_stride;
+  // Dims past head_dim are read as the row's first; their queries are zero,
+  // their outputs are not written.
+  auto k_dim = [&](int s) -> uint32_t {  // bytes from the lane's offset to step s (I8: two steps)
+    const uint32_t at = s * 64;
+    return FULL || at + g * 16 < hd * (I8 ? 1 : 2) ? at : 0u - g * 16;
+  };
+  auto v_dim = [&](int half) -> uint32_t {
+    const uint32_t at = half * 256 + col * (VW < 4 ? VW * 4 : 16);
+    return FULL || at < hd * (I8 ? 1 : 2) ? at : 0u;
+  };
+  struct Page {
+    uint64_t at;     // bytes from the cache's start to the half tile's first row
+    uint64_t scale;  // index of its first scale
+    bool ok;
+  };
+  auto page = [&](int32_t seq, uint32_t kvh, uint32_t pos) {
+    Page p;
+    const uint32_t i = kv_page_of(a.c, pos >> 4);
+    // The second half of the last tile may lie past the table.
+    const int32_t id = pos < a.t.positions ? ((const_ints)a.t.table)[(uint64_t)seq * a.t.width + i] : -1;
+    const uint32_t slot = pos - i * a.c.page_size;
+    p.ok = (uint32_t)id < a.c.n_pages;
+    const uint32_t use = p.ok ? (uint32_t)id : 0u;
+    p.at = use * a.c.page + kvh * a.c.head + (p.ok ? slot : 0u) * a.c.slot;
+    p.scale = ((uint64_t)use * a.c.heads + kvh) * a.c.page_size + (p.ok ? slot : 0u);
+    return p;
+  };
+
+  uint32_t kr[2][KS][KW];
+  uint32_t vr[8][VW];
+  f32x4 ks[2], vs[2];
+  // on: whether there is a tile to load; else all lanes read its first bytes.
+  auto load_k = [&](const Page (&pg)[2], bool on) {
+    const uint32_t off = on ? k_off : 0u;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const gbytes p = as_global(a.c.k + pg[u].at);
+#pragma unroll
+      for (int s = 0; s < KS / (I8 ? 2 : 1); ++s) {
+        const u32x4 w = gld<false, u32x4>(p + (off + (FULL || on ? k_dim(s) : 0u)));
+        if constexpr (I8) {
+          kr[u][2 * s][0] = w.x, kr[u][2 * s][1] = w.y, kr[u][2 * s + 1][0] = w.z, kr[u][2 * s + 1][1] = w.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kr[u][s][i] = w[i];
+        }
+      }
+      if constexpr (I8) ks[u] = *reinterpret_cast<const f32x4*>(a.c.ks + pg[u].scale + g * 4);
+    }
+  };
+  auto load_v = [&](const Page (&pg)[2], bool on) {
+    const uint32_t off = on ? v_off : 0u, step = on ? slot_stride : 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const gbytes p = as_global(a.c.v + pg[j >> 2].at + (uint64_t)(j & 3) * step);
+      if constexpr (VW >= 4) {
+#pragma unroll
+        for (int h = 0; h < VW / 4; ++h) {
+          const u32x4 w = gld<false, u32x4>(p + (off + v_dim(h)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[j][4 * h + i] = w[i];
+        }
+      } else if constexpr (VW == 2) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 w = gld<false, u32x2>(p + (off + v_dim(0)));
+        vr[j][0] = w.x, vr[j][1] = w.y;
+      } else {
+        vr[j][0] = gld<false, uint32_t>(p + (off + v_dim(0)));
+      }
+    }
+    if constexpr (I8) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) vs[u] = *reinterpret_cast<const f32x4*>(a.c.vs + pg[u].scale + g * 4);
+    }
+  };
+  f32x4 acc[VJ];
+  // O^T += V^T P^T; SOME: of this lane's column only where it is `mine`, and with
+  // values whose mask is 0 as zeros.
+  auto add_pv = [&](const u32x4 (&p)[3], const uint32_t (&mask)[4], bool mine, auto some) {
+    constexpr bool SOME = decltype(some)::value;
+#pragma unroll
+    for (int j = 0; j < VJ; ++j) {
+      u32x4 f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (I8) {
+          f[w] = upper_halves(__float_as_uint(code_f(vr[2 * w][j / 4], j % 4)),
+                              __float_as_uint(code_f(vr[2 * w + 1][j / 4], j % 4)));
+        } else {
+          f[w] = __builtin_amdgcn_perm(vr[2 * w + 1][j / 2], vr[2 * w][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+        }
+        if constexpr (SOME) f[w] &= mask[w];
+      }
+      f32x4 sum = acc[j];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sum = attn_mfma(f, p[i], sum);
+      if constexpr (SOME) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][r] = mine ? sum[r] : acc[j][r];
+      } else {
+        acc[j] = sum;
+      }
+    }
+  };
+
+  // The queries of a part, as operands: part of the value, step, lane.
+  struct Heads {
+    uint32_t kvh, first, n, cols;
+  };
+  auto heads_of = [&](const AttnPart& p) {
+    Heads h;
+    h.kvh = p.tile / a.parts;
+    const uint32_t part = p.tile - h.kvh * a.parts;
+    h.first = h.kvh * a.group + part * 16;
+    h.n = min(16u, a.group - part * 16);
+    h.cols = p.n * h.n;
+    return h;
+  };
+  std::conditional_t<QP == 1, u32x4, af32x8> qv[QN];
+  auto load_q = [&](const AttnPart& p, const Heads& h) {
+#pragma unroll
+    for (int j = 0; j < QN; ++j) {
+      const uint32_t i = t + j * 256, c = i & 15, lg = (i >> 4) & 3, step = i >> 6;
+      const uint32_t d = I8 ? (step >> 1) * 64 + lg * 16 + (step & 1) * 8 : step * 32 + lg * 8;
+      const uint32_t token = c / h.n;
+      const uint64_t at = c < h.cols && d < hd ? (p.row + token) * a.q_stride + (h.first + c - token * h.n) * hd + d : 0;
+      if constexpr (QP == 1)
+        qv[j] = *reinterpret_cast<const u32x4*>((const uint16_t*)a.q + at);
+      else
+        qv[j] = *reinterpret_cast<const af32x8*>((const float*)a.q + at);
+    }
+  };
+  auto store_q = [&](const Heads& h) {
+#pragma unroll
+    for (int j = 0; j < QN; ++j) {
+      const uint32_t i = t + j * 256, c = i & 15, lg = (i >> 4) & 3, step = i >> 6;
+      const uint32_t d = I8 ? (step >> 1) * 64 + lg * 16 + (step & 1) * 8 : step * 32 + lg * 8;
+      const bool in = c < h.cols && d < hd;
+      if (i >= (uint32_t)KS * 64) continue;
+      if constexpr (QP == 1) {
+        q_lds[i] = in ? qv[j] : u32x4{0, 0, 0, 0};
+      } else {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = in ? qv[j][e] : 0.f;
+        u32x4 s[3];
+        attn_split(f, s);
+#pragma unroll
+        for (int e = 0; e < 3; ++e) q_lds[e * KS * 64 + i] = s[e];
+      }
+    }
+  };
+
+  AttnPart cur = part_at(x);
+  Span see = span_of(cur);
+  Heads heads = heads_of(cur);
+  uint32_t p0, left;  // this wave's next tile, and how many it has
+  tiles_of(cur, see, &p0, &left);
+  load_q(cur, heads);
+  Page now[2];
+  bool loaded = false;
+  for (;;) {
+    if (left && !loaded) {
+      now[0] = page(cur.seq, heads.kvh, p0), now[1] = page(cur.seq, heads.kvh, p0 + 16);
+      load_k(now, true);
+      load_v(now, true);
+    }
+    store_q(heads);
+    __syncthreads();
+
+    // The part behind this one.
+    x += cur.count;
+    const bool more = x < end;
+    AttnPart then = cur;
+    Span then_see = see;
+    Heads then_heads = heads;
+    uint32_t then_p0 = 0, then_left = 0;
+    if (more) {
+      then = part_at(x);
+      then_see = span_of(then);
+      then_heads = heads_of(then);
+      tiles_of(then, then_see, &then_p0, &then_left);
+    }
+    loaded = false;
+
+    // This lane's column: its token and what it sees.
+    const uint32_t my_token = min(col / heads.n, cur.n - 1);
+    int32_t see_lo, see_hi;
+    attn_range(a, true, cur.pos + (int32_t)my_token, &see_lo, &see_hi);
 #pragma unroll
     for (int j = 0; j < VJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
     float m = kAttnNone, l = 0.f;
 
-    // This wave's tiles: the units' 32 positions that overlap [lo, hi].
-    const uint32_t unit0 = (uint32_t)lo / kAttnUnit + first;
-    uint32_t p0 = unit0 * kAttnUnit + wave * 32;  // first position of a tile
-    uint32_t left = count;
-    if ((int32_t)p0 + 31 < lo) p0 += kAttnUnit, --left;
-    if (left && (int32_t)(p0 + (left - 1) * kAttnUnit) > hi) --left;
-
-    const const_ints table = (const_ints)a.t.table + (uint64_t)seq * a.t.width;
-    const uint32_t slot_stride = (uint32_t)a.c.slot;
-    const uint32_t k_off = col * slot_stride + g * 16;
-    const uint32_t v_off = g * 4 * slot_stride;
-    // Dims past head_dim are read as the row's first; their queries are zero,
-    // their outputs are not written.
-    auto k_dim = [&](int s) -> uint32_t {  // bytes from the lane's offset to step s (I8: two steps)
-      const uint32_t at = s * 64;
-      return FULL || at + g * 16 < hd * (I8 ? 1 : 2) ? at : 0u - g * 16;
-    };
-    auto v_dim = [&](int half) -> uint32_t {
-      const uint32_t at = half * 256 + col * (VW < 4 ? VW * 4 : 16);
-      return FULL || at < hd * (I8 ? 1 : 2) ? at : 0u;
-    };
-    struct Page {
-      uint64_t at;     // bytes from the cache's start to the half tile's first row
-      uint64_t scale;  // index of its first scale
-      bool ok;
-    };
-    auto page = [&](uint32_t pos) {
-      Page p;
-      const uint32_t i = kv_page_of(a.c, pos >> 4);
-      // The second half of the last tile may lie past the table.
-      const int32_t id = pos < a.t.positions ? table[i] : -1;
-      const uint32_t slot = pos - i * a.c.page_size;
-      p.ok = (uint32_t)id < a.c.n_pages;
-      const uint32_t use = p.ok ? (uint32_t)id : 0u;
-      p.at = use * a.c.page + kvh * a.c.head + (p.ok ? slot : 0u) * a.c.slot;
-      p.scale = ((uint64_t)use * a.c.heads + kvh) * a.c.page_size + (p.ok ? slot : 0u);
-      return p;
-    };
-
-    uint32_t kr[2][KS][KW];
-    uint32_t vr[8][VW];
-    f32x4 ks[2], vs[2];
-    auto load_k = [&](const Page (&pg)[2]) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const gbytes p = as_global(a.c.k + pg[u].at);
-#pragma unroll
-        for (int s = 0; s < KS / (I8 ? 2 : 1); ++s) {
-          const u32x4 w = gld<false, u32x4>(p + (k_off + k_dim(s)));
-          if constexpr (I8) {
-            kr[u][2 * s][0] = w.x, kr[u][2 * s][1] = w.y, kr[u][2 * s + 1][0] = w.z, kr[u][2 * s + 1][1] = w.w;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) kr[u][s][i] = w[i];
-          }
-        }
-        if constexpr (I8) ks[u] = *reinterpret_cast<const f32x4*>(a.c.ks + pg[u].scale + g * 4);
+    for (; left; --left, p0 += kAttnUnit) {
+      // The tile to ask for next: this part's, or the first of the one behind it.
+      const bool same = left > 1, on = same || then_left;
+      Page next[2] = {now[0], now[1]};
+      if (on) {
+        const int32_t seq = same ? cur.seq : then.seq;
+        const uint32_t kvh = same ? heads.kvh : then_heads.kvh, at = same ? p0 + kAttnUnit : then_p0;
+        next[0] = page(seq, kvh, at), next[1] = page(seq, kvh, at + 16);
       }
-    };
-    auto load_v = [&](const Page (&pg)[2]) {
+      f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const gbytes p = as_global(a.c.v + pg[j >> 2].at + (uint64_t)(j & 3) * slot_stride);
-        if constexpr (VW >= 4) {
+      for (int st = 0; st < KS; ++st) {
+        u32x4 q[QP];
 #pragma unroll
-          for (int h = 0; h < VW / 4; ++h) {
-            const u32x4 w = gld<false, u32x4>(p + (v_off + v_dim(h)));
+        for (int i = 0; i < QP; ++i) q[i] = q_lds[(i * KS + st) * 64 + lane];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vr[j][4 * h + i] = w[i];
+        for (int u = 0; u < 2; ++u) {
+          u32x4 k;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (I8)
+              k[w] = upper_halves(__float_as_uint(code_f(kr[u][st][w / 2], 2 * (w % 2))),
+                                  __float_as_uint(code_f(kr[u][st][w / 2], 2 * (w % 2) + 1)));
+            else
+              k[w] = kr[u][st][w];
           }
-        } else if constexpr (VW == 2) {
-          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-          const u32x2 w = gld<false, u32x2>(p + (v_off + v_dim(0)));
-          vr[j][0] = w.x, vr[j][1] = w.y;
-        } else {
-          vr[j][0] = gld<false, uint32_t>(p + (v_off + v_dim(0)));
+#pragma unroll
+          for (int i = 0; i < QP; ++i) s[u] = attn_mfma(k, q[i], s[u]);
         }
+        // Else all of the queries are read at once, into registers that are not there.
+        if (st % 2) __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (I8) {
+      float y[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) vs[u] = *reinterpret_cast<const f32x4*>(a.c.vs + pg[u].scale + g * 4);
-      }
-    };
-    // O^T += V^T P^T; SOME: of this lane's column only where it is `mine`, and with
-    // values whose mask is 0 as zeros.
-    auto add_pv = [&](const u32x4 (&p)[3], const uint32_t (&mask)[4], bool mine, auto some) {
-      constexpr bool SOME = decltype(some)::value;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) {
-        u32x4 f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          if constexpr (I8) {
-            f[w] = upper_halves(__float_as_uint(code_f(vr[2 * w][j / 4], j % 4)),
-                                __float_as_uint(code_f(vr[2 * w + 1][j / 4], j % 4)));
-          } else {
-            f[w] = __builtin_amdgcn_perm(vr[2 * w + 1][j / 2], vr[2 * w][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-          }
-          if constexpr (SOME) f[w] &= mask[w];
-        }
-        f32x4 sum = acc[j];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) sum = attn_mfma(f, p[i], sum);
-        if constexpr (SOME) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[j][r] = mine ? sum[r] : acc[j][r];
-        } else {
-          acc[j] = sum;
-        }
-      }
-    };
-
-    if (left) {
-      Page now[2] = {page(p0), page(p0 + 16)};
-      load_k(now);
-      load_v(now);
-      for (; left; --left, p0 += kAttnUnit) {
-        Page next[2] = {now[0], now[1]};
-        if (left > 1) next[0] = page(p0 + kAttnUnit), next[1] = page(p0 + kAttnUnit + 16);
-        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          u32x4 q[QP];
-#pragma unroll
-          for (int i = 0; i < QP; ++i) q[i] = reinterpret_cast<const u32x4*>(lds)[(i * KS + st) * 64 + lane];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            u32x4 k;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              if constexpr (I8)
-                k[w] = upper_halves(__float_as_uint(code_f(kr[u][st][w / 2], 2 * (w % 2))),
-                                    __float_as_uint(code_f(kr[u][st][w / 2], 2 * (w % 2) + 1)));
-              else
-                k[w] = kr[u][st][w];
-            }
-#pragma unroll
-            for (int i = 0; i < QP; ++i) s[u] = attn_mfma(k, q[i], s[u]);
-          }
-        }
-        float y[8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[4 * u + r] = s[u][r] * a.scale * (I8 ? ks[u][r] : 1.f);
-        load_k(next);
-        const bool whole = (int32_t)p0 >= all_lo && (int32_t)p0 + 31 <= all_hi && now[0].ok && now[1].ok;
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int32_t pos = (int32_t)(p0 + (j >> 2) * 16 + g * 4 + (j & 3));
-            y[j] = pos >= see_lo && pos <= see_hi && now[j >> 2].ok ? y[j] : -INFINITY;
-          }
-          if (!(now[0].ok && now[1].ok) && lane == 0) {
-            const bool bad = (!now[0].ok && (int32_t)p0 + 15 >= lo && (int32_t)p0 <= hi) ||
-                             (!now[1].ok && (int32_t)p0 + 31 >= lo && (int32_t)p0 + 16 <= hi);
-            if (bad) *a.err = 2u;
-          }
-        }
-        float top = y[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, y[j]);
-        const float bigger = fmaxf(m, column_max(top));
-        if (__any(bigger > m)) {
-          const float f = __builtin_amdgcn_exp2f(m - bigger);
-          l *= f;
-#pragma unroll
-          for (int j = 0; j < VJ; ++j) acc[j] *= f;
-          m = bigger;
-        }
-        float w[8];
+        for (int r = 0; r < 4; ++r) y[4 * u + r] = s[u][r] * a.scale * (I8 ? ks[u][r] : 1.f);
+      load_k(next, on);
+      const bool whole = (int32_t)p0 >= see.all_lo && (int32_t)p0 + 31 <= see.all_hi && now[0].ok && now[1].ok;
+      if (!whole) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          w[j] = __builtin_amdgcn_exp2f(y[j] - m);
-          l += w[j];
-          if constexpr (I8) w[j] = whole || y[j] > -INFINITY || y[j] != y[j] ? w[j] * vs[j >> 2][j & 3] : 0.f;
+          const int32_t pos = (int32_t)(p0 + (j >> 2) * 16 + g * 4 + (j & 3));
+          y[j] = pos >= see_lo && pos <= see_hi && now[j >> 2].ok ? y[j] : -INFINITY;
         }
-        u32x4 p[3];
-        attn_split(w, p);
-        uint32_t mask[4] = {0, 0, 0, 0};
-        if (whole) {
-          add_pv(p, mask, true, std::false_type{});
-        } else {
-          // A position that only some of the tokens see may hold anything, a NaN
-          // too, which no weight of zero keeps out: each token's columns by
-          // themselves.
-          for (uint32_t i = 0; i < together; ++i) {
-            int32_t tl, th;
-            attn_range(a, seq, __builtin_amdgcn_readfirstlane(tokens.pos(row + i)), &tl, &th);
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              uint32_t both = 0;
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = 2 * h + e;
-                const int32_t pos = (int32_t)(p0 + (j >> 2) * 16 + g * 4 + (j & 3));
-                if (pos >= tl && pos <= th && now[j >> 2].ok) both |= e ? 0xFFFF0000u : 0xFFFFu;
-              }
-              mask[h] = both;
-            }
-            add_pv(p, mask, my_token == i, std::true_type{});
-          }
+        if (!(now[0].ok && now[1].ok) && lane == 0) {
+          const bool bad = (!now[0].ok && (int32_t)p0 + 15 >= see.lo && (int32_t)p0 <= see.hi) ||
+                           (!now[1].ok && (int32_t)p0 + 31 >= see.lo && (int32_t)p0 + 16 <= see.hi);
+          if (bad) *a.err = 2u;
         }
-        load_v(next);
-        now[0] = next[0], now[1] = next[1];
       }
+      float top = y[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, y[j]);
+      const float bigger = fmaxf(m, column_max(top));
+      if (__any(bigger > m)) {
+        const float f = __builtin_amdgcn_exp2f(m - bigger);
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) acc[j] *= f;
+        m = bigger;
+      }
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = __builtin_amdgcn_exp2f(y[j] - m);
+        l += w[j];
+        if constexpr (I8) w[j] = whole || y[j] > -INFINITY || y[j] != y[j] ? w[j] * vs[j >> 2][j & 3] : 0.f;
+      }
+      u32x4 p[3];
+      attn_split(w, p);
+      uint32_t mask[4] = {0, 0, 0, 0};
+      if (whole) {
+        add_pv(p, mask, true, std::false_type{});
+      } else {
+        // A position that only some of the tokens see may hold anything, a NaN
+        // too, which no weight of zero keeps out: each token's columns by
+        // themselves.
+        for (uint32_t i = 0; i < cur.n; ++i) {
+          int32_t tl, th;
+          attn_range(a, true, cur.pos + (int32_t)i, &tl, &th);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t both = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int j = 2 * h + e;
+              const int32_t pos = (int32_t)(p0 + (j >> 2) * 16 + g * 4 + (j & 3));
+              if (pos >= tl && pos <= th && now[j >> 2].ok) both |= e ? 0xFFFF0000u : 0xFFFFu;
+            }
+            mask[h] = both;
+          }
+          add_pv(p, mask, my_token == i, std::true_type{});
+        }
+      }
+      load_v(next, on);
+      now[0] = next[0], now[1] = next[1];
+      loaded = on && !same;
     }
+    if (more) load_q(then, then_heads);
 
-    // The four waves' columns into one.
+    // The four waves' columns into one, a quarter of the dims in each.
     l = column_sum(l);
-    if (g == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
+    if (g == 0) ml[wave][col] = float2{m, l};
+#pragma unroll
+    for (int j = 0; j < VJ; ++j) o_lds[(wave * VJ + j) * 64 + lane] = acc[j];
     __syncthreads();  // ends the use of the queries, too
-    const float m0 = ml[0][col][0], m1 = ml[1][col][0], m2 = ml[2][col][0], m3 = ml[3][col][0];
-    const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-    const float total = ml[0][col][1] * __builtin_amdgcn_exp2f(m0 - top) + ml[1][col][1] * __builtin_amdgcn_exp2f(m1 - top) +
-                        ml[2][col][1] * __builtin_amdgcn_exp2f(m2 - top) + ml[3][col][1] * __builtin_amdgcn_exp2f(m3 - top);
-    const float f = __builtin_amdgcn_exp2f(m - top);
+    const float2 s0 = ml[0][col], s1 = ml[1][col], s2 = ml[2][col], s3 = ml[3][col];
+    const float top = fmaxf(fmaxf(s0.x, s1.x), fmaxf(s2.x, s3.x));
+    float f[4] = {__builtin_amdgcn_exp2f(s0.x - top), __builtin_amdgcn_exp2f(s1.x - top), __builtin_amdgcn_exp2f(s2.x - top),
+                  __builtin_amdgcn_exp2f(s3.x - top)};
+    const float total = s0.y * f[0] + s1.y * f[1] + s2.y * f[2] + s3.y * f[3];
+    const attn_u64 slot = 2 * blk + (cur.begun || x - cur.count == block_x ? 0 : 1);
+    // A column without weights (nothing seen): zeros.
+    const float scale = !cur.whole ? 1.f : total == 0.f ? 0.f : 1.f / total;
+    constexpr int RUN = VJ / 4;  // dims next to each other
+    float o[RUN][4];
 #pragma unroll
-    for (int j = 0; j < VJ; ++j) acc[j] *= f;
-    f32x4* const swap = reinterpret_cast<f32x4*>(lds) + (wave & 1) * VJ * 64 + lane;
-    if (wave >= 2) {
+    for (int j = 0; j < RUN; ++j) {
+      f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) swap[j * 64] = acc[j];
+      for (int w = 0; w < 4; ++w) sum += o_lds[(w * VJ + wave * RUN + j) * 64 + lane] * f[w];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[j][r] = sum[r] * scale;
     }
-    __syncthreads();
-    if (wave < 2) {
+    if (col < heads.cols) {
+      const uint32_t token = col / heads.n;
+      const uint64_t at = cur.whole ? ((uint64_t)(cur.row + token) * a.heads + heads.first + col - token * heads.n) * hd
+                                    : (slot * 16 + col) * D;
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) acc[j] += swap[j * 64];
-    }
-    __syncthreads();
-    if (wave == 1) {
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t d = attn_dim<D, I8>(g * 4 + r, wave * RUN);
+        if (cur.whole && !FULL && d >= hd) continue;
+        typedef float run_f __attribute__((ext_vector_type(RUN < 2 ? 2 : RUN)));
+        typedef __bf16 run_b __attribute__((ext_vector_type(RUN < 2 ? 2 : RUN)));
+        if constexpr (RUN == 1) {
+          if (cur.whole && a.out_bf16)
+            ((__bf16*)a.out)[at + d] = (__bf16)o[0][r];
+          else
+            (cur.whole ? (float*)a.out : a.acc)[at + d] = o[0][r];
+        } else {
+          run_f v;
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) swap[j * 64] = acc[j];
-    }
-    __syncthreads();
-    if (wave == 0) {
-      const bool done = first == 0 && count == units;
-      const uint64_t slot = 2 * blockIdx.x + (base + (uint64_t)tile * units > block_x ? 1 : 0);
-      // A column without weights (nothing seen): zeros.
-      const float scale = done ? (total == 0.f ? 0.f : 1.f / total) : 1.f;
-#pragma unroll
-      for (int j = 0; j < VJ; ++j) acc[j] = (acc[j] + swap[VJ * 64 + j * 64]) * scale;
-      if (col < cols) {
-        const uint32_t token = col / heads;
-        const uint64_t at = done ? (uint64_t)(row + token) * a.heads * hd + (head0 + col - token * heads) * hd
-                                 : (slot * 16 + col) * D;
-        float* const to = (done ? (float*)a.out : a.acc) + at;
-        constexpr int RUN = VJ < 8 ? VJ : 8;  // dims next to each other
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int b = 0; b < VJ; b += RUN) {
-            const uint32_t d = attn_dim<D, I8>(g * 4 + r, b);
-            if (done && !FULL && d >= hd) continue;
-            if (done && a.out_bf16) {
-#pragma unroll
-              for (int j = 0; j < RUN; j += 4) {
-                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-                const f32x4 v = {acc[b + j][r], acc[b + j + 1][r], acc[b + j + 2][r], acc[b + j + 3][r]};
-                *reinterpret_cast<bf16x4*>((uint16_t*)a.out + at + d + j) = __builtin_convertvector(v, bf16x4);
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < RUN; j += 4)
-                *reinterpret_cast<f32x4*>(to + d + j) = f32x4{acc[b + j][r], acc[b + j + 1][r], acc[b + j + 2][r], acc[b + j + 3][r]};
-            }
-          }
-        if (!done && g == 0) {
-          float* const s = a.ml + (slot * 16 + col) * 2;
-          s[0] = top;
-          s[1] = total;
+          for (int j = 0; j < RUN; ++j) v[j] = o[j][r];
+          if (cur.whole && a.out_bf16)
+            *reinterpret_cast<run_b*>((uint16_t*)a.out + at + d) = __builtin_convertvector(v, run_b);
+          else
+            *reinterpret_cast<run_f*>((cur.whole ? (float*)a.out : a.acc) + at + d) = v;
         }
       }
+      if (!cur.whole && wave == 0 && g == 0) *reinterpret_cast<float2*>(a.ml + (slot * 16 + col) * 2) = float2{top, total};
     }
-    x += count;
-    if (x == base + (uint64_t)units * tiles) base = x, ++row;
-    if (x < end) __syncthreads();
+    if (!more) return;
+    cur = then, see = then_see, heads = then_heads, p0 = then_p0, left = then_left;
   }
 }
 
-template <int D, bool I8>
-static hipError_t attn_go(const AttnArgs& a, bool q_bf16, hipStream_t st) {
-  const auto fn = a.c.dim == D ? (q_bf16 ? k_attn<D, I8, true, 1> : k_attn<D, I8, true, 3>)
-                               : (q_bf16 ? k_attn<D, I8, false, 1> : k_attn<D, I8, false, 3>);
-  hipLaunchKernelGGL(fn, dim3(1u << a.blocks_log), dim3(256), 0, st, a);
+template <int D, bool I8, bool FULL, int QP>
+static hipError_t attn_go(const AttnArgs& a, hipStream_t st) {
+  static std::atomic<uint64_t> raised{0};
+  constexpr uint32_t bytes = attn_lds<D, I8, QP>();
+  const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(&k_attn<D, I8, FULL, QP>), bytes, raised);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((k_attn<D, I8, FULL, QP>), dim3(1u << a.blocks_log), dim3(256), bytes, st, a);
   return hipGetLastError();
+}
+template <int D, bool I8>
+static hipError_t attn_of(const AttnArgs& a, bool q_bf16, hipStream_t st) {
+  if (a.c.dim == D) return q_bf16 ? attn_go<D, I8, true, 1>(a, st) : attn_go<D, I8, true, 3>(a, st);
+  return q_bf16 ? attn_go<D, I8, false, 1>(a, st) : attn_go<D, I8, false, 3>(a, st);
 }
 template <bool I8>
 static hipError_t launch_attn(const AttnArgs& a, bool q_bf16, hipStream_t st) {
-  if (a.c.dim <= 64) return attn_go<64, I8>(a, q_bf16, st);
-  if (a.c.dim <= 128) return attn_go<128, I8>(a, q_bf16, st);
-  return attn_go<256, I8>(a, q_bf16, st);
+  if (a.c.dim <= 64) return attn_of<64, I8>(a, q_bf16, st);
+  if (a.c.dim <= 128) return attn_of<128, I8>(a, q_bf16, st);
+  return attn_of<256, I8>(a, q_bf16, st);
 }
 
 }  // namespace smoe

@@ -14,8 +14,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
   const uint32_t t = threadIdx.x, fours = a.c.dim / 4;
   const uint64_t before = a.before[row], units = a.before[row + 1] - before, all_units = a.before[a.t.n];
   // The group, all of its tokens at once.
-  const uint32_t i = t & 15, r = min(row + i, a.t.n - 1);
-  const bool follows = r % a.together && a.t.seq[r] == a.t.seq[r - 1] && (uint32_t)a.t.pos[r] == (uint32_t)a.t.pos[r - 1] + 1u;
+  const uint32_t i = t & 15, r = min(row + i, a.t.n - 1), r1 = r ? r - 1 : 0;
+  const bool follows = attn_follows(a, r, a.t.seq[r], a.t.pos[r], a.t.seq[r1], a.t.pos[r1]);
   const uint32_t mask = (uint32_t)__ballot(follows && row + i < a.t.n) & 0xFFFFu;
   if (mask & 1) return;  // another group's token
   const uint32_t n = __builtin_ctz(~(mask >> 1)) + 1;
@@ -60,21 +60,24 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
       acc = acc * f + v * w;
       m = top;
     }
+    auto add = [&](float om, float ol, f32x4 oacc) {
+      const float top = fmaxf(m, om), f = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(om - top);
+      l = l * f + ol * w;
+      acc = acc * f + oacc * w;
+      m = top;
+    };
+    // Turns of one wave, then of the waves.
+    for (uint32_t o = lanes; o < 64; o <<= 1) {
+      f32x4 other;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) other[j] = __shfl_xor(acc[j], (int)o, kWave);
+      add(__shfl_xor(m, (int)o, kWave), __shfl_xor(l, (int)o, kWave), other);
+    }
     sum[t] = acc;
     stat[t] = float2{m, l};
     __syncthreads();
     if (turn == 0 && e < to) {
-      float top = m;
-      for (uint32_t i = 1; i < turns; ++i) top = fmaxf(top, stat[i * lanes + t].x);
-      float f = __builtin_amdgcn_exp2f(m - top);
-      l *= f;
-      acc *= f;
-      for (uint32_t i = 1; i < turns; ++i) {
-        const float2 s = stat[i * lanes + t];
-        f = __builtin_amdgcn_exp2f(s.x - top);
-        l += s.y * f;
-        acc += sum[i * lanes + t] * f;
-      }
+      for (uint32_t i = max(64u, lanes); i < 256; i += max(64u, lanes)) add(stat[t + i].x, stat[t + i].y, sum[t + i]);
       put(e, acc * (l == 0.f ? 0.f : 1.f / l));
     }
     __syncthreads();
