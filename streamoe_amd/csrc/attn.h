@@ -7,15 +7,16 @@
 // unscaled output of every column (a token's head) stay in registers; a larger
 // maximum scales l and the output by e^(old - new).
 //
-// Work is a list of units of 128 positions: for every group of up to 16 columns
+// Work is a list of units of 32 positions: for every group of up to 16 columns
 // (tokens of one sequence next to each other times the query heads of one key
-// head) the units its positions touch, group after group. Block b takes the
-// units [b per, (b + 1) per), so batches of any lengths are split evenly and one
-// long row over the whole chip; a group cut between blocks leaves each one's m,
-// l and output in the workspace, which k_attn_join adds up. Nothing is decided
-// on the host, whose knowledge of lengths would need a wait.
+// head) the units its positions touch, group after group, with kAttnOver more
+// in front of each that stand for what a group costs by itself. Block b takes
+// the units [b per, (b + 1) per), so batches of any lengths are split evenly and
+// one long row over the whole chip; a group cut between blocks leaves each one's
+// m, l and output in the workspace, which k_attn_join adds up. Nothing is
+// decided on the host, whose knowledge of lengths would need a wait.
 //
-// A wave has 32 positions of a unit. S^T = K Q^T: A the keys (a row per lane of
+// A block's four waves take its units in turn. S^T = K Q^T: A the keys (a row per lane of
 // 16, 8 dims per lane sixteen), B the queries out of LDS; the result has a
 // column per lane of 16 and positions 4 g + r of both halves in lane sixteen g.
 // O^T = V^T P^T takes P as it lies there: contraction slot j of lane sixteen g is
@@ -33,7 +34,12 @@ namespace smoe {
 typedef __bf16 abf16x8 __attribute__((ext_vector_type(8)));
 typedef float af32x8 __attribute__((ext_vector_type(8), aligned(16)));
 
-constexpr uint32_t kAttnUnit = 128;     // positions of a unit: 32 of each wave
+constexpr uint32_t kAttnUnit = 32;      // positions of a unit
+// What a group costs by itself (queries, first loads, the exchange between the
+// waves, a part for the join), in units: 61 rows of very different lengths take
+// 60 us with 0, 57 with 2, 51 with 4, 48 with 6, 48 with 8, 50 with 12; 48 rows
+// of 16 key heads 100, 65, 59, 56, 58 and 60.
+constexpr uint32_t kAttnOver = 6;
 constexpr float kAttnNone = -3.0e38f;   // maximum of no scores
 
 typedef unsigned long long attn_u64;
@@ -72,7 +78,7 @@ __device__ __forceinline__ attn_u64 lane_u64(attn_u64 v, uint32_t lane) {
 struct AttnChunk {
   uint32_t first;    // token of lane 0
   int32_t seq, pos;
-  uint32_t n, units;
+  uint32_t n, units;  // kAttnOver among them; 0: sees nothing
   attn_u64 before;   // units of the lanes before, from the chunk's start
   bool wrong;        // out of range
   __device__ void load(const AttnArgs& a, uint32_t from) {
@@ -90,15 +96,15 @@ struct AttnChunk {
     int32_t lo, hi;
     attn_range(a, seq_in && n, max(pos, 0), &lo, &hi);
     hi = min(pos + (int32_t)n - 1, (int32_t)a.t.positions - 1);
-    units = seq_in && n && hi >= max(pos, 0) ? (uint32_t)hi / kAttnUnit - (uint32_t)lo / kAttnUnit + 1 : 0u;
+    units = seq_in && n && hi >= max(pos, 0) ? (uint32_t)hi / kAttnUnit - (uint32_t)lo / kAttnUnit + 1 + kAttnOver : 0u;
     before = wave_scan_u64(units) - units;
   }
   __device__ attn_u64 all() const { return lane_u64(before + units, 63); }
 };
 
-// One block's part of a group's tile: units [first, first + count) of `units`.
+// One block's part of a group's tile: units [first, first + count) of its positions'.
 struct AttnPart {
-  uint32_t row, n, tile, first, count, units;
+  uint32_t row, n, tile, first, count;
   int32_t seq, pos;
   bool whole, begun;  // all of the group's units; units before them are another block's
 };
@@ -158,8 +164,8 @@ __device__ __forceinline__ uint64_t attn_per(uint64_t units, uint32_t blocks_log
 // likewise, over the end of a part of a group into the next: their loads are
 // always in flight.
 template <int D, bool I8, int QP>
-constexpr uint32_t attn_lds() {  // the queries; four waves' outputs
-  return (QP * (D / 32) + 4 * (D / 16)) * 1024;
+constexpr uint32_t attn_lds() {  // two parts' queries; four waves' outputs
+  return (2 * QP * (D / 32) + 4 * (D / 16)) * 1024;
 }
 template <int D, bool I8, bool FULL, int QP>
 __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a) {
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
   constexpr int QN = KS < 4 ? 1 : KS / 4;       // pieces of eight query values per thread
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   u32x4* const q_lds = reinterpret_cast<u32x4*>(lds);
-  f32x4* const o_lds = reinterpret_cast<f32x4*>(lds + QP * KS * 1024);
+  f32x4* const o_lds = reinterpret_cast<f32x4*>(lds + 2 * QP * KS * 1024);
   __shared__ float2 ml[4][16];
   __shared__ attn_u64 chunk_units[kKvMaxTokens / 64];
   const uint32_t t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
@@ -231,31 +237,35 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
     if (x < end) chunk.load(a, c * 64);
   }
   if (x >= end) return;
-  const attn_u64 block_x = x;
 
-  // The part that begins at unit y; y only grows.
-  auto part_at = [&](attn_u64 y) {
-    for (;;) {
-      const attn_u64 here = __ballot((chunk_at + chunk.before) * tiles <= y && y < (chunk_at + chunk.before + chunk.units) * tiles);
-      if (here) {
-        const uint32_t l = (uint32_t)__builtin_ctzll(here);
-        const attn_u64 base = (chunk_at + lane_u64(chunk.before, l)) * tiles;
-        AttnPart p;
-        p.units = lane_u32(chunk.units, l);
-        p.row = chunk.first + l;
-        p.n = lane_u32(chunk.n, l);
-        p.seq = (int32_t)lane_u32((uint32_t)chunk.seq, l);
-        p.pos = (int32_t)lane_u32((uint32_t)chunk.pos, l);
-        p.tile = (uint32_t)(y - base) / p.units;
-        p.first = (uint32_t)(y - base) - p.tile * p.units;
-        p.count = (uint32_t)min((attn_u64)(p.units - p.first), end - y);
-        p.whole = p.count == p.units;
-        p.begun = base + (attn_u64)p.tile * p.units < block_x;
-        return p;
+  // The next part from unit x on, x then behind it; false: there is none.
+  auto next_part = [&](AttnPart& p) {
+    while (x < end) {
+      const attn_u64 at = (chunk_at + chunk.before) * tiles;
+      const attn_u64 here = __ballot(at <= x && x < at + (attn_u64)chunk.units * tiles);
+      if (!here) {
+        chunk_at += chunk.all();
+        chunk.load(a, chunk.first + 64);
+        continue;
       }
-      chunk_at += chunk.all();
-      chunk.load(a, chunk.first + 64);
+      const uint32_t l = (uint32_t)__builtin_ctzll(here), units = lane_u32(chunk.units, l);
+      const attn_u64 off = x - lane_u64(at, l);
+      p.tile = off >> 32 ? (uint32_t)(off / units) : (uint32_t)off / units;
+      const uint32_t from = (uint32_t)(off - (attn_u64)p.tile * units);
+      const uint32_t to = (uint32_t)min((attn_u64)units, from + (end - x));
+      x += to - from;
+      if (to <= kAttnOver) continue;
+      p.row = chunk.first + l;
+      p.n = lane_u32(chunk.n, l);
+      p.seq = (int32_t)lane_u32((uint32_t)chunk.seq, l);
+      p.pos = (int32_t)lane_u32((uint32_t)chunk.pos, l);
+      p.begun = from > kAttnOver;
+      p.first = p.begun ? from - kAttnOver : 0u;
+      p.count = to - kAttnOver - p.first;
+      p.whole = !p.begun && to == units;
+      return true;
     }
+    return false;
   };
   // What the group's tokens see: one of them, and all.
   struct Span {
@@ -271,12 +281,12 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
     s.all_hi = p.pos < 0 || last > top ? -1 : p.pos;
     return s;
   };
-  // This wave's tiles of a part: the units' 32 positions that overlap [lo, hi].
+  // This wave's units of a part, every fourth: where its first begins, how many.
+  uint32_t turn = wave;  // units until this wave's next
   auto tiles_of = [&](const AttnPart& p, const Span& s, uint32_t* p0, uint32_t* left) {
-    *p0 = ((uint32_t)s.lo / kAttnUnit + p.first) * kAttnUnit + wave * 32;
-    *left = p.count;
-    if ((int32_t)*p0 + 31 < s.lo) *p0 += kAttnUnit, --*left;
-    if (*left && (int32_t)(*p0 + (*left - 1) * kAttnUnit) > s.hi) --*left;
+    *p0 = ((uint32_t)s.lo / kAttnUnit + p.first + turn) * kAttnUnit;
+    *left = p.count > turn ? (p.count - turn + 3) / 4 : 0u;
+    turn = (turn - p.count) & 3;
   };
 
   const uint32_t slot_stride = (uint32_t)a.c.slot;
@@ -362,16 +372,21 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
   // values whose mask is 0 as zeros.
   auto add_pv = [&](const u32x4 (&p)[3], const uint32_t (&mask)[4], bool mine, auto some) {
     constexpr bool SOME = decltype(some)::value;
+    // (A zero that the compiler does not know, so that it does not form the
+    // operands of all tokens' rounds ahead, in as many registers again.)
+    uint32_t zero = 0;
+    if constexpr (SOME) asm volatile("" : "+v"(zero));
+    auto v = [&](int j, int i) { return SOME ? vr[j][i] ^ zero : vr[j][i]; };
 #pragma unroll
     for (int j = 0; j < VJ; ++j) {
       u32x4 f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         if constexpr (I8) {
-          f[w] = upper_halves(__float_as_uint(code_f(vr[2 * w][j / 4], j % 4)),
-                              __float_as_uint(code_f(vr[2 * w + 1][j / 4], j % 4)));
+          f[w] = upper_halves(__float_as_uint(code_f(v(2 * w, j / 4), j % 4)),
+                              __float_as_uint(code_f(v(2 * w + 1, j / 4), j % 4)));
         } else {
-          f[w] = __builtin_amdgcn_perm(vr[2 * w + 1][j / 2], vr[2 * w][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+          f[w] = __builtin_amdgcn_perm(v(2 * w + 1, j / 2), v(2 * w, j / 2), j % 2 ? 0x07060302u : 0x05040100u);
         }
         if constexpr (SOME) f[w] &= mask[w];
       }
@@ -414,7 +429,8 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
         qv[j] = *reinterpret_cast<const af32x8*>((const float*)a.q + at);
     }
   };
-  auto store_q = [&](const Heads& h) {
+  uint32_t q_at = 0;  // this part's queries in LDS: of two places in turn
+  auto store_q = [&](const Heads& h, uint32_t to) {
 #pragma unroll
     for (int j = 0; j < QN; ++j) {
       const uint32_t i = t + j * 256, c = i & 15, lg = (i >> 4) & 3, step = i >> 6;
@@ -422,7 +438,7 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
       const bool in = c < h.cols && d < hd;
       if (i >= (uint32_t)KS * 64) continue;
       if constexpr (QP == 1) {
-        q_lds[i] = in ? qv[j] : u32x4{0, 0, 0, 0};
+        q_lds[to + i] = in ? qv[j] : u32x4{0, 0, 0, 0};
       } else {
         float f[8];
 #pragma unroll
@@ -430,42 +446,41 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
         u32x4 s[3];
         attn_split(f, s);
 #pragma unroll
-        for (int e = 0; e < 3; ++e) q_lds[e * KS * 64 + i] = s[e];
+        for (int e = 0; e < 3; ++e) q_lds[to + e * KS * 64 + i] = s[e];
       }
     }
   };
 
-  AttnPart cur = part_at(x);
+  AttnPart cur;
+  if (!next_part(cur)) return;
   Span see = span_of(cur);
   Heads heads = heads_of(cur);
   uint32_t p0, left;  // this wave's next tile, and how many it has
   tiles_of(cur, see, &p0, &left);
   load_q(cur, heads);
   Page now[2];
-  bool loaded = false;
+  auto load_first = [&] {
+    now[0] = page(cur.seq, heads.kvh, p0), now[1] = page(cur.seq, heads.kvh, p0 + 16);
+    load_k(now, true);
+    load_v(now, true);
+  };
+  if (left) load_first();
+  store_q(heads, 0);
+  __syncthreads();
   for (;;) {
-    if (left && !loaded) {
-      now[0] = page(cur.seq, heads.kvh, p0), now[1] = page(cur.seq, heads.kvh, p0 + 16);
-      load_k(now, true);
-      load_v(now, true);
-    }
-    store_q(heads);
-    __syncthreads();
-
     // The part behind this one.
-    x += cur.count;
-    const bool more = x < end;
     AttnPart then = cur;
+    const bool more = next_part(then);
     Span then_see = see;
     Heads then_heads = heads;
     uint32_t then_p0 = 0, then_left = 0;
     if (more) {
-      then = part_at(x);
       then_see = span_of(then);
       then_heads = heads_of(then);
       tiles_of(then, then_see, &then_p0, &then_left);
     }
-    loaded = false;
+    load_q(then, then_heads);
+    bool loaded = false;  // the part behind's first tile
 
     // This lane's column: its token and what it sees.
     const uint32_t my_token = min(col / heads.n, cur.n - 1);
@@ -475,13 +490,13 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
     for (int j = 0; j < VJ; ++j) acc[j] = f32x4{0, 0, 0, 0};
     float m = kAttnNone, l = 0.f;
 
-    for (; left; --left, p0 += kAttnUnit) {
+    for (; left; --left, p0 += 4 * kAttnUnit) {
       // The tile to ask for next: this part's, or the first of the one behind it.
       const bool same = left > 1, on = same || then_left;
       Page next[2] = {now[0], now[1]};
       if (on) {
         const int32_t seq = same ? cur.seq : then.seq;
-        const uint32_t kvh = same ? heads.kvh : then_heads.kvh, at = same ? p0 + kAttnUnit : then_p0;
+        const uint32_t kvh = same ? heads.kvh : then_heads.kvh, at = same ? p0 + 4 * kAttnUnit : then_p0;
         next[0] = page(seq, kvh, at), next[1] = page(seq, kvh, at + 16);
       }
       f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
@@ -489,7 +504,7 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
       for (int st = 0; st < KS; ++st) {
         u32x4 q[QP];
 #pragma unroll
-        for (int i = 0; i < QP; ++i) q[i] = q_lds[(i * KS + st) * 64 + lane];
+        for (int i = 0; i < QP; ++i) q[i] = q_lds[q_at + (i * KS + st) * 64 + lane];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           u32x4 k;
@@ -574,20 +589,20 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
       now[0] = next[0], now[1] = next[1];
       loaded = on && !same;
     }
-    if (more) load_q(then, then_heads);
+    store_q(then_heads, q_at ^ (QP * KS * 64));
 
     // The four waves' columns into one, a quarter of the dims in each.
     l = column_sum(l);
     if (g == 0) ml[wave][col] = float2{m, l};
 #pragma unroll
     for (int j = 0; j < VJ; ++j) o_lds[(wave * VJ + j) * 64 + lane] = acc[j];
-    __syncthreads();  // ends the use of the queries, too
+    __syncthreads();  // the next queries are there, too
     const float2 s0 = ml[0][col], s1 = ml[1][col], s2 = ml[2][col], s3 = ml[3][col];
     const float top = fmaxf(fmaxf(s0.x, s1.x), fmaxf(s2.x, s3.x));
     float f[4] = {__builtin_amdgcn_exp2f(s0.x - top), __builtin_amdgcn_exp2f(s1.x - top), __builtin_amdgcn_exp2f(s2.x - top),
                   __builtin_amdgcn_exp2f(s3.x - top)};
     const float total = s0.y * f[0] + s1.y * f[1] + s2.y * f[2] + s3.y * f[3];
-    const attn_u64 slot = 2 * blk + (cur.begun || x - cur.count == block_x ? 0 : 1);
+    const attn_u64 slot = 2 * blk + (cur.begun ? 0 : 1);
     // A column without weights (nothing seen): zeros.
     const float scale = !cur.whole ? 1.f : total == 0.f ? 0.f : 1.f / total;
     constexpr int RUN = VJ / 4;  // dims next to each other
@@ -600,6 +615,7 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[j][r] = sum[r] * scale;
     }
+    if (more) __syncthreads();  // the outputs' place is free
     if (col < heads.cols) {
       const uint32_t token = col / heads.n;
       const uint64_t at = cur.whole ? ((uint64_t)(cur.row + token) * a.heads + heads.first + col - token * heads.n) * hd
@@ -629,6 +645,8 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
     }
     if (!more) return;
     cur = then, see = then_see, heads = then_heads, p0 = then_p0, left = then_left;
+    q_at ^= QP * KS * 64;
+    if (left && !loaded) load_first();
   }
 }
 

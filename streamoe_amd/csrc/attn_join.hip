@@ -7,7 +7,7 @@ namespace smoe {
 // A block joins a share (blockIdx.y) of one group's columns: fours of dims, each
 // by 256 / lanes threads that go through the parts in turn and are added up at
 // the end. Parts are added in their order, so a call gives the same bits again.
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, uint32_t share, uint32_t pad) {
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t pad) {
   __shared__ f32x4 sum[256];
   __shared__ float2 stat[256];
   const uint32_t tiles = a.c.heads * a.parts, row = blockIdx.x / tiles, tile = blockIdx.x - row * tiles;
@@ -21,7 +21,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
   const uint32_t n = __builtin_ctz(~(mask >> 1)) + 1;
   const uint32_t kvh = tile / a.parts, part = tile - kvh * a.parts;
   const uint32_t head0 = kvh * a.group + part * 16, heads = min(16u, a.group - part * 16);
-  const uint32_t all = n * heads * fours, from = blockIdx.y * share, to = min(all, from + share);
+  const uint32_t all = n * heads * fours, share = (all + gridDim.y - 1) / gridDim.y;
+  const uint32_t from = blockIdx.y * share, to = min(all, from + share);
   auto put = [&](uint32_t e, f32x4 v) {
     const uint32_t col = e / fours, token = col / heads;
     const uint64_t at = ((uint64_t)(row + token) * a.heads + head0 + col - token * heads) * a.c.dim + (e - col * fours) * 4;
@@ -35,30 +36,56 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
     for (uint32_t e = from + t; e < to; e += 256) put(e, f32x4{0, 0, 0, 0});
     return;
   }
-  const uint64_t total = all_units * tiles, per = attn_per(total, a.blocks_log), x = before * tiles + tile * units;
+  const uint64_t total = all_units * tiles, per = attn_per(total, a.blocks_log);
+  const uint64_t x = before * tiles + tile * units + kAttnOver, last = x + units - kAttnOver - 1;
   uint32_t b0, b1;
   if (total >> 32) {
     b0 = (uint32_t)(x / per);
-    b1 = (uint32_t)((x + units - 1) / per);
+    b1 = (uint32_t)(last / per);
   } else {
     b0 = (uint32_t)x / (uint32_t)per;
-    b1 = (uint32_t)(x + units - 1) / (uint32_t)per;
+    b1 = (uint32_t)last / (uint32_t)per;
   }
   if (b0 == b1) return;
-  const uint32_t parts = b1 - b0 + 1, turns = 256 / lanes, turn = t / lanes;
+  const uint32_t parts = b1 - b0 + 1;
+  uint32_t lanes = 8;
+  while (lanes < 256 && lanes < share) lanes *= 2;
+  const uint32_t turns = 256 / lanes, turn = t / lanes;
   for (uint32_t e0 = from; e0 < to; e0 += lanes) {
-    const uint32_t e = e0 + t % lanes, col = min(e, all - 1) / fours, d = (min(e, all - 1) - col * fours) * 4;
+    const uint32_t e = e0 + t % lanes, in = min(e, all - 1), col = in / fours, d = (in - col * fours) * 4;
     float m = kAttnNone, l = 0.f;
     f32x4 acc = {0, 0, 0, 0};
-#pragma unroll 4
-    for (uint32_t p = turn; p < parts; p += turns) {
-      const uint64_t slot = 2 * (uint64_t)(b0 + p) + (p == 0 && x > (uint64_t)b0 * per ? 1 : 0);
-      const float2 s = *reinterpret_cast<const float2*>(a.ml + (slot * 16 + col) * 2);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.acc + (slot * 16 + col) * pad + d);
-      const float top = fmaxf(m, s.x), f = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(s.x - top);
-      l = l * f + s.y * w;
-      acc = acc * f + v * w;
+    // K parts of this turn from p on, their loads together.
+    auto take = [&](uint32_t p0, auto count) {
+      constexpr uint32_t K = decltype(count)::value;
+      float2 s[K];
+      f32x4 v[K];
+#pragma unroll
+      for (uint32_t i = 0; i < K; ++i) {
+        const uint32_t p = min(p0 + i * turns, parts - 1);
+        const uint64_t slot = 2 * (uint64_t)(b0 + p) + (p == 0 ? 1 : 0);
+        s[i] = *reinterpret_cast<const float2*>(a.ml + (slot * 16 + col) * 2);
+        v[i] = *reinterpret_cast<const f32x4*>(a.acc + (slot * 16 + col) * pad + d);
+      }
+      float top = m;
+#pragma unroll
+      for (uint32_t i = 0; i < K; ++i) top = fmaxf(top, s[i].x);
+      const float f = __builtin_amdgcn_exp2f(m - top);
+      l *= f;
+      acc *= f;
       m = top;
+#pragma unroll
+      for (uint32_t i = 0; i < K; ++i) {
+        if (p0 + i * turns >= parts) continue;
+        const float w = __builtin_amdgcn_exp2f(s[i].x - top);
+        l += s[i].y * w;
+        acc += v[i] * w;
+      }
+    };
+    if (parts <= turns) {
+      if (turn < parts) take(turn, std::integral_constant<uint32_t, 1>{});
+    } else {
+      for (uint32_t p = turn; p < parts; p += 4 * turns) take(p, std::integral_constant<uint32_t, 4>{});
     }
     auto add = [&](float om, float ol, f32x4 oacc) {
       const float top = fmaxf(m, om), f = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(om - top);
@@ -86,15 +113,11 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t lanes, u
 
 hipError_t launch_attn_join(const AttnArgs& a, hipStream_t st) {
   const uint32_t items = a.t.n * a.c.heads * a.parts;
-  const uint32_t cols = min(16u, a.group) * a.together, all = cols * a.c.dim / 4;
-  // Eight fours a block where there are few rows to join, whole groups where
+  // A share of eight fours where there are few rows to join, whole groups where
   // there are many.
-  const uint32_t most = (all + 7) / 8, y = min(most, max(1u, 2048 / items));
-  const uint32_t share = (all + y - 1) / y;
-  uint32_t lanes = 8;
-  while (lanes < 256 && lanes < share) lanes *= 2;
+  const uint32_t most = (min(16u, a.group) * a.together * a.c.dim / 4 + 7) / 8, y = min(most, max(1u, 2048 / items));
   const uint32_t pad = a.c.dim <= 64 ? 64 : a.c.dim <= 128 ? 128 : 256;
-  hipLaunchKernelGGL(k_attn_join, dim3(items, y), dim3(256), 0, st, a, lanes, share, pad);
+  hipLaunchKernelGGL(k_attn_join, dim3(items, y), dim3(256), 0, st, a, pad);
   return hipGetLastError();
 }
 
