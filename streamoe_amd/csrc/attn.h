@@ -11,7 +11,7 @@
 // (tokens of one sequence next to each other times the query heads of one key
 // head) the units its positions touch, group after group, with kAttnOver more
 // in front of each that stand for what a group costs by itself. Block b takes
-// the units [b per, (b + 1) per), so batches of any lengths are split evenly and
+// an equal part of them, so batches of any lengths are split evenly and
 // one long row over the whole chip; a group cut between blocks leaves each one's
 // m, l and output in the workspace, which k_attn_join adds up. Nothing is
 // decided on the host, whose knowledge of lengths would need a wait.
@@ -152,9 +152,16 @@ __device__ __forceinline__ float column_sum(float v) { return swap32_add(swap16_
 
 typedef const __attribute__((address_space(4))) int32_t* const_ints;
 
-// Units of a block.
-__device__ __forceinline__ uint64_t attn_per(uint64_t units, uint32_t blocks_log) {
-  return (units + (1u << blocks_log) - 1) >> blocks_log;
+// Block b takes the units from attn_from(all, b) to attn_from(all, b + 1): as many
+// as the others or one more, one each where there are fewer than blocks.
+__device__ __forceinline__ attn_u64 attn_from(attn_u64 units, uint32_t block, uint32_t blocks_log) {
+  return units >> blocks_log ? (units * block) >> blocks_log : min((attn_u64)block, units);
+}
+// The block that has unit x: the last that begins at or before it.
+__device__ __forceinline__ uint32_t attn_block_of(attn_u64 x, attn_u64 units, uint32_t blocks_log) {
+  if (!(units >> blocks_log)) return (uint32_t)x;
+  const attn_u64 y = ((x + 1) << blocks_log) - 1;
+  return y >> 32 ? (uint32_t)(y / units) : (uint32_t)y / (uint32_t)units;
 }
 
 // D: head_dim up to it (FULL: equal). QP: parts of a query value (1: bf16 rows,
@@ -188,9 +195,8 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
   if (n <= 64) {
     chunk.load(a, 0);
     all = chunk.all();
-    const attn_u64 per = attn_per(all * tiles, a.blocks_log);
-    x = blk * per;
-    end = min(all * tiles, x + per);
+    x = attn_from(all * tiles, blk, a.blocks_log);
+    end = attn_from(all * tiles, blk + 1, a.blocks_log);
     if (blk == 0 && wave == 0) {
       if (lane < n) a.before[lane] = chunk.before;
       if (lane == 0) a.before[n] = all;
@@ -210,9 +216,8 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
     for (int j = 0; j < 4; ++j) sum += u[j] = 4 * lane + j < chunks ? chunk_units[4 * lane + j] : 0ull;
     const attn_u64 upto = wave_scan_u64(sum);
     all = lane_u64(upto, 63);
-    const attn_u64 per = attn_per(all * tiles, a.blocks_log);
-    x = blk * per;
-    end = min(all * tiles, x + per);
+    x = attn_from(all * tiles, blk, a.blocks_log);
+    end = attn_from(all * tiles, blk + 1, a.blocks_log);
     attn_u64 before = upto - sum;
     uint32_t c = 0;
 #pragma unroll
@@ -465,9 +470,7 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
     load_v(now, true);
   };
   if (left) load_first();
-  store_q(heads, 0);
-  __syncthreads();
-  for (;;) {
+  for (bool begin = true;; begin = false) {
     // The part behind this one.
     AttnPart then = cur;
     const bool more = next_part(then);
@@ -478,6 +481,10 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
       then_see = span_of(then);
       then_heads = heads_of(then);
       tiles_of(then, then_see, &then_p0, &then_left);
+    }
+    if (begin) {  // the first part's queries, its loads still on their way
+      store_q(heads, 0);
+      __syncthreads();
     }
     load_q(then, then_heads);
     bool loaded = false;  // the part behind's first tile

@@ -36,16 +36,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t pad) {
     for (uint32_t e = from + t; e < to; e += 256) put(e, f32x4{0, 0, 0, 0});
     return;
   }
-  const uint64_t total = all_units * tiles, per = attn_per(total, a.blocks_log);
-  const uint64_t x = before * tiles + tile * units + kAttnOver, last = x + units - kAttnOver - 1;
-  uint32_t b0, b1;
-  if (total >> 32) {
-    b0 = (uint32_t)(x / per);
-    b1 = (uint32_t)(last / per);
-  } else {
-    b0 = (uint32_t)x / (uint32_t)per;
-    b1 = (uint32_t)last / (uint32_t)per;
-  }
+  const uint64_t total = all_units * tiles, x = before * tiles + tile * units + kAttnOver, last = x + units - kAttnOver - 1;
+  const uint32_t b0 = attn_block_of(x, total, a.blocks_log), b1 = attn_block_of(last, total, a.blocks_log);
   if (b0 == b1) return;
   const uint32_t parts = b1 - b0 + 1;
   uint32_t lanes = 8;
