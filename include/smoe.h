@@ -767,7 +767,7 @@ uint64_t smoe_sample_workspace_size(uint32_t n_rows, uint32_t vocab);
  * exceeds u times their sum. Temperature 0: the first of the order. A logit of
  * -inf or NaN is never kept; a row with +inf has e = 1 there and 0 elsewhere.
  * e is computed in f64 and held as an integer of 2^-s, s = 62 - bits of vocab (44
- * for 2^18 tokens), so sums do not depend on their order and borders within
+ * for 2^18 tokens) but at most 51, so sums do not depend on their order and borders within
  * 2^-s of the sum are told by the rounded values.
  * logits: device f32[n_rows, vocab], 16-byte aligned; temperature, top_p, min_p,
  * u: device f32[n_rows], top_k: device int32[n_rows]; temperature NULL: 1, top_k

@@ -55,16 +55,6 @@ __device__ __forceinline__ bool attn_follows(const AttnArgs& a, uint32_t r, int3
                                              int32_t pos_before) {
   return (r & (a.together - 1)) && seq == seq_before && pos_before != 0x7FFFFFFF && pos == pos_before + 1;
 }
-__device__ __forceinline__ attn_u64 wave_scan_u64(attn_u64 v) {  // inclusive, on DPP
-  auto step = [&](uint32_t lo, uint32_t hi) { v += (attn_u64)hi << 32 | lo; };
-  step(dpp_u32<0x111, 0xF>((uint32_t)v), dpp_u32<0x111, 0xF>((uint32_t)(v >> 32)));
-  step(dpp_u32<0x112, 0xF>((uint32_t)v), dpp_u32<0x112, 0xF>((uint32_t)(v >> 32)));
-  step(dpp_u32<0x114, 0xF>((uint32_t)v), dpp_u32<0x114, 0xF>((uint32_t)(v >> 32)));
-  step(dpp_u32<0x118, 0xF>((uint32_t)v), dpp_u32<0x118, 0xF>((uint32_t)(v >> 32)));
-  step(dpp_u32<0x142, 0xA>((uint32_t)v), dpp_u32<0x142, 0xA>((uint32_t)(v >> 32)));
-  step(dpp_u32<0x143, 0xC>((uint32_t)v), dpp_u32<0x143, 0xC>((uint32_t)(v >> 32)));
-  return v;
-}
 __device__ __forceinline__ uint32_t lane_u32(uint32_t v, uint32_t lane) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane);
 }

@@ -304,6 +304,31 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   return __longlong_as_double((long long)(hi << 32 | lo));
 }
 
+// 64-bit integers over the wave, the same way: sums of the lanes up to each one,
+// and the largest, in lane 63.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_u64(unsigned long long v) {
+  return (unsigned long long)dpp_u32<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp_u32<CTRL, ROWS>((uint32_t)v);
+}
+__device__ __forceinline__ unsigned long long wave_scan_u64(unsigned long long v) {
+  v += dpp_u64<0x111, 0xF>(v);
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
+  v += dpp_u64<0x142, 0xA>(v);
+  v += dpp_u64<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ unsigned long long wave_max_last_u64(unsigned long long v) {
+  v = max(v, dpp_u64<0x111, 0xF>(v));
+  v = max(v, dpp_u64<0x112, 0xF>(v));
+  v = max(v, dpp_u64<0x114, 0xF>(v));
+  v = max(v, dpp_u64<0x118, 0xF>(v));
+  v = max(v, dpp_u64<0x142, 0xA>(v));
+  v = max(v, dpp_u64<0x143, 0xC>(v));
+  return v;
+}
+
 // Transposed reductions: several per-lane partial sums reduced at once, each
 // exchange halving the values per lane while every lane stays busy.
 // swap32_add(a, b): lanes 0-31 hold a's partial over lanes {l, l + 32},

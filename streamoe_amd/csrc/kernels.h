@@ -451,6 +451,7 @@ struct SampleArgs {
   double unit;                        // 2^s: what a mass of 1 is held as
   unsigned long long *tops;           // [n, slices] largest key of a slice
   unsigned long long *mass;           // [n, bins] of the row's logits
+  unsigned long long *slice_mass;     // [n, slices, bins] of a slice's
   unsigned long long *kept;           // [n, slices] mass of what is kept for certain
   unsigned long long *list;           // [n, vocab] keys of the border's bins
   uint32_t* count;                    // [n, bins], behind them the list's length

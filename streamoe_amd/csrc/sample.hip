@@ -3,20 +3,22 @@
 //
 //   k_sample_top   a slice's largest key; clears the row's sums
 //   k_sample_bins  the row's logits by their distance from its largest: counts
-//                  and masses per bin (rows with top-k or top-p)
+//                  and masses per bin, of the row and (masses) of the slice
 //   k_sample_list  the keys of the bins in which a border lies, and each slice's
 //                  mass of what is kept for certain
 //   k_sample_pick  the borders themselves, the sum, and the token
 //
 // A logit becomes 32 bits in an order that integers compare, and a key with the
 // complement of its token below it, so keys are unique and the order of the
-// filters is that of falling keys. Its distance from the row's largest is an
-// integer too; bins are 32 to every power of two of it, so that they are finest
-// where the mass is. All three filters keep a first part of the order: what
-// decides is one key, and only the bins around it have to be looked into.
+// filters is that of falling keys. Bins are by the distance d from the row's
+// largest logit (a rounded difference, but it never falls as logits fall): 64 to
+// every power of two of d from 1/64 to 256, so that they are finest where the
+// mass is. All three filters keep a first part of the order: what decides is one
+// key, and only the bins around it have to be looked into.
 //
 // A mass e^((logit - max) / T) is f64 and then an integer of 2^-s: sums of
-// integers are the same in any order, so atomics may form them.
+// integers are the same in any order, so atomics may form them. Masses of whole
+// bins are formed once; rows with top-k alone need those of the few kept.
 #include "common.h"
 #include "kernels.h"
 
@@ -25,26 +27,17 @@ namespace smoe {
 typedef unsigned long long u64;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr uint32_t kSampleThreads = 256;
+constexpr uint32_t kSampleThreads = 256, kPickThreads = 512;
 constexpr uint32_t kSampleSlices = 128;  // of a row at most
 constexpr uint32_t kCountStride = kSampleBins + 4;
 constexpr uint32_t kNoBin = kSampleBins;
 
-// Bin of a distance: itself below 32, else 32 to a power of two.
-__device__ __forceinline__ uint32_t sample_bin(uint32_t d) {
-  if (d < 32) return d;
-  const uint32_t e = 31 - __builtin_clz(d);
-  return (e - 4) * 32 + ((d >> (e - 5)) & 31);
-}
-// First distance of a bin, and the binary digits that its distances differ in.
-__device__ __forceinline__ void sample_bin_range(uint32_t bin, uint32_t* first, uint32_t* bits) {
-  if (bin < 32) {
-    *first = bin;
-    *bits = 0;
-    return;
-  }
-  *bits = bin / 32 - 1;
-  *first = (32 + bin % 32) << *bits;
+// Bin of a logit, 0 the largest's.
+__device__ __forceinline__ uint32_t sample_bin(float max, float l) {
+  constexpr uint32_t kFirst = (127 - 6) << 6;  // the upper bits of 1/64
+  const float d = max - l;                     // NaN where both are infinite: 0
+  const uint32_t b = d > 0.f ? __float_as_uint(d) >> 17 : 0u;
+  return b < kFirst ? 0u : min(b - kFirst, kSampleBins - 1);
 }
 
 // e^x for -46 <= x <= 0: x = n ln 2 + r, the series of e^r to r^11 (what is left
@@ -63,6 +56,7 @@ struct SampleRow {
   uint32_t k;              // kept at most; 0: all
   double inv_t, top_p, min_p, u;
   __device__ bool by_mass() const { return top_p < 1.0; }
+  __device__ bool masses() const { return by_mass() || !k; }  // of all bins
 };
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, uint32_t row) {
   SampleRow r;
@@ -81,11 +75,11 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, uint32_t ro
 
 // What a row's largest logit makes of the others.
 struct SampleScale {
-  uint32_t top;       // its order
+  float top;
   double max, inv_t, unit, least, min_p;
   bool infinite;
   __device__ SampleScale(const SampleArgs& a, const SampleRow& r, uint32_t o)
-      : top(o), max(ord_float(o)), inv_t(r.inv_t), unit(a.unit), min_p(r.min_p), infinite(o == 0xFF800000u) {
+      : top(ord_float(o)), max(top), inv_t(r.inv_t), unit(a.unit), min_p(r.min_p), infinite(o == 0xFF800000u) {
     // Below it a mass rounds to zero.
     least = -0.6931471805599453 * (2 + __builtin_amdgcn_frexp_exp(a.unit));
   }
@@ -98,41 +92,64 @@ struct SampleScale {
     const double x = log_mass(l);
     const double e = x > least ? sample_exp(x) : 0.0;
     *kept = e >= min_p;
-    return (u64)__builtin_rint(e * unit);
+    // The sum's last place is 1: its lower bits are the rounded product.
+    return (u64)__double_as_longlong(__builtin_fma(e, unit, 0x1p52)) - 0x4330000000000000ull;
   }
 };
 
 __device__ __forceinline__ u64 sample_key(float l, uint32_t token) { return (u64)float_ord(l) << 32 | (uint32_t)~token; }
 __device__ __forceinline__ uint32_t key_token(u64 key) { return ~(uint32_t)key; }
 
-// Over the block's 256 threads; lds: 4 of T. Every thread gets the result.
+// Over the block's T threads; lds: T / 64 words. Every thread gets the result.
+template <uint32_t T>
 __device__ __forceinline__ u64 block_max(u64 v, u64* lds) {
+  v = wave_max_last_u64(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (u64)__shfl_xor(v, o, kWave));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+  for (uint32_t w = 1; w < T / 64; ++w) v = max(v, lds[w]);
+  return v;
 }
-// Sum of the threads before this one; *all: of all.
+// Sums of the threads before this one, of two values (lds: 2 T / 64 words);
+// all: of all.
+template <uint32_t T, uint32_t N>
+__device__ __forceinline__ void block_before(u64 (&v)[N], u64 (&all)[N], u64* lds) {
+  u64 s[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) s[i] = wave_scan_u64(v[i]);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) lds[(threadIdx.x >> 6) * N + i] = s[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    u64 skip = 0, sum = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < T / 64; ++w) {
+      const u64 x = lds[w * N + i];
+      if (w < threadIdx.x >> 6) skip += x;
+      sum += x;
+    }
+    all[i] = sum;
+    v[i] = skip + s[i] - v[i];
+  }
+}
+template <uint32_t T>
+__device__ __forceinline__ u64 block_sum(u64 v, u64* lds) {
+  u64 a[1] = {v}, s[1];
+  block_before<T, 1>(a, s, lds);
+  return s[0];
+}
+template <uint32_t T>
 __device__ __forceinline__ u64 block_before(u64 v, u64* all, u64* lds) {
-  u64 s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 w = __shfl_up(s, o, kWave);
-    if ((threadIdx.x & 63) >= (uint32_t)o) s += w;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = s;
-  __syncthreads();
-  u64 skip = 0;
-  *all = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < 4; ++w) {
-    if (w < threadIdx.x >> 6) skip += lds[w];
-    *all += lds[w];
-  }
-  return skip + s - v;
+  u64 a[1] = {v}, s[1];
+  block_before<T, 1>(a, s, lds);
+  *all = s[0];
+  return a[0];
 }
 
 // Thread t's four logits of a thousand from `first` on, -inf behind the row.
@@ -145,8 +162,9 @@ __device__ __forceinline__ f32x4 sample_load(const float* row, uint32_t at, uint
   return v;
 }
 
+template <uint32_t T>
 __device__ __forceinline__ u64 row_top(const SampleArgs& a, uint32_t row, u64* lds) {
-  return block_max(threadIdx.x < a.slices ? a.tops[row * a.slices + threadIdx.x] : 0ull, lds);
+  return block_max<T>(threadIdx.x < a.slices ? a.tops[row * a.slices + threadIdx.x] : 0ull, lds);
 }
 
 __global__ __launch_bounds__(kSampleThreads) void k_sample_top(SampleArgs a) {
@@ -163,7 +181,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_top(SampleArgs a) {
       if (v[j] > -INFINITY && key > top) top = key;
     }
   }
-  top = block_max(top, lds);
+  top = block_max<kSampleThreads>(top, lds);
   if (t == 0) a.tops[blockIdx.x] = top;
   for (uint32_t i = slice * kSampleThreads + t; i < kCountStride; i += a.slices * kSampleThreads) {
     a.count[(uint64_t)row * kCountStride + i] = 0;
@@ -177,22 +195,23 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs a) {
   __shared__ u64 lds[4];
   const uint32_t t = threadIdx.x, row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const SampleRow r = sample_row(a, row);
-  if (!r.good || r.greedy || !(r.k || r.by_mass())) return;
-  const u64 top = row_top(a, row, lds);
+  if (!r.good || r.greedy) return;
+  const u64 top = row_top<kSampleThreads>(a, row, lds);
   if (!top) return;
   for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
   __syncthreads();
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
   const float* const l = a.logits + (uint64_t)row * a.vocab;
   const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
+  const bool counts = r.k, masses = r.masses();
   for (uint32_t i = from + t * 4; i < to; i += kSampleThreads * 4) {
     const f32x4 v = sample_load(l, i, a.vocab);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
       if (!(v[j] > -INFINITY)) continue;
-      const uint32_t bin = sample_bin(scale.top - float_ord(v[j]));
-      atomicAdd(&count[bin], 1u);
-      if (r.by_mass()) {
+      const uint32_t bin = sample_bin(scale.top, v[j]);
+      if (counts) atomicAdd(&count[bin], 1u);
+      if (masses) {
         bool kept;
         const u64 m = scale.mass(v[j], &kept);
         if (m) atomicAdd(&mass[bin], m);
@@ -200,10 +219,11 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs a) {
     }
   }
   __syncthreads();
+  u64* const own = a.slice_mass + (uint64_t)blockIdx.x * kSampleBins;
   for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) {
-    if (!count[i]) continue;
-    atomicAdd(a.count + (uint64_t)row * kCountStride + i, count[i]);
+    if (count[i]) atomicAdd(a.count + (uint64_t)row * kCountStride + i, count[i]);
     if (mass[i]) atomicAdd(a.mass + (uint64_t)row * kSampleBins + i, mass[i]);
+    if (masses) own[i] = mass[i];
   }
 }
 
@@ -212,11 +232,15 @@ struct SampleBorder {
   uint32_t k_bin, k_before;     // top-k's, and tokens before it
   u64 k_mass;                   // mass before it, or of all
   uint32_t p_first, p_last;     // top-p's is one of these
-  __device__ bool certain(uint32_t bin) const { return bin < min(k_bin, p_first); }
-  __device__ bool listed(uint32_t bin) const { return bin == k_bin || (bin >= p_first && bin <= p_last); }
+  u64 p_before;                 // mass before the first of them
+  uint32_t m_first, m_last;     // min-p's is one of these
+  __device__ uint32_t certain() const { return min(min(k_bin, p_first), m_first); }  // bins below it are kept
+  __device__ bool listed(uint32_t bin) const {
+    return bin == k_bin || (bin >= p_first && bin <= p_last) || (bin >= m_first && bin <= m_last);
+  }
 };
 struct SampleBorderLds {
-  u64 part[4];
+  u64 part[2 * kPickThreads / 64];
   SampleBorder b;
   u64 k_own;
 };
@@ -224,34 +248,41 @@ __device__ __forceinline__ u64 share_of(double p, u64 of) {  // at least one
   const double v = __builtin_ceil(p * (double)of);
   return v >= 1.0 ? (u64)v : 1ull;
 }
-// Thread t has bins 4 t .. 4 t + 3; before: mass ahead of its first, m: of each.
-__device__ __forceinline__ SampleBorder sample_border(const SampleArgs& a, const SampleRow& r, uint32_t row,
-                                                      SampleBorderLds* lds, u64* before, u64 (&m)[4]) {
+// Thread t of T has the B bins from B t on; before: mass ahead of its first, m: of each.
+template <uint32_t T, uint32_t B = (kSampleBins + T - 1) / T>
+__device__ __forceinline__ SampleBorder sample_border(const SampleArgs& a, const SampleRow& r, const SampleScale& scale,
+                                                      uint32_t row, SampleBorderLds* lds, u64* before, u64 (&m)[B]) {
   const uint32_t t = threadIdx.x;
-  uint32_t c[4] = {0, 0, 0, 0};
+  uint32_t c[B];
+  u64 own[2] = {0, 0}, all[2];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) m[j] = 0;
-  if (4 * t < kSampleBins) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      c[j] = a.count[(uint64_t)row * kCountStride + 4 * t + j];
-      m[j] = a.mass[(uint64_t)row * kSampleBins + 4 * t + j];
-    }
+  for (uint32_t j = 0; j < B; ++j) {
+    const bool in = B * t + j < kSampleBins;
+    c[j] = in ? a.count[(uint64_t)row * kCountStride + B * t + j] : 0u;
+    m[j] = in ? a.mass[(uint64_t)row * kSampleBins + B * t + j] : 0ull;
+    own[0] += c[j];
+    own[1] += m[j];
   }
-  u64 all, all_count;
-  u64 n = block_before((u64)c[0] + c[1] + c[2] + c[3], &all_count, lds->part);
-  *before = block_before(m[0] + m[1] + m[2] + m[3], &all, lds->part);
+  block_before<T, 2>(own, all, lds->part);
+  u64 n = own[0];
+  *before = own[1];
   if (t == 0) {
-    lds->b = SampleBorder{kNoBin, 0, all, kNoBin, kNoBin};
+    lds->b = SampleBorder{kNoBin, 0, all[1], kNoBin, kNoBin, 0, kNoBin, kNoBin};
     lds->k_own = 0;
+    if (r.min_p > 0.0 && !scale.infinite) {
+      // The last logit that min-p keeps, to within more than its roundings.
+      const double x = log(r.min_p), at = scale.max + x / r.inv_t, off = (fabs(scale.max) + fabs(at)) * 0x1p-22 + fabs(x / r.inv_t) * 0x1p-40;
+      lds->b.m_first = sample_bin(scale.top, (float)(at + off));
+      lds->b.m_last = sample_bin(scale.top, (float)(at - off));
+    }
   }
   __syncthreads();
   if (r.k) {
     u64 w = *before;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (uint32_t j = 0; j < B; ++j) {
       if (n < r.k && r.k <= n + c[j]) {
-        lds->b.k_bin = 4 * t + j;
+        lds->b.k_bin = B * t + j;
         lds->b.k_before = (uint32_t)n;
         lds->b.k_mass = w;
         lds->k_own = m[j];
@@ -265,115 +296,160 @@ __device__ __forceinline__ SampleBorder sample_border(const SampleArgs& a, const
     const u64 lo = share_of(r.top_p, lds->b.k_mass), hi = share_of(r.top_p, lds->b.k_mass + lds->k_own);
     u64 w = *before;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (w < lo && lo <= w + m[j]) lds->b.p_first = 4 * t + j;
-      if (w < hi && hi <= w + m[j]) lds->b.p_last = 4 * t + j;
+    for (uint32_t j = 0; j < B; ++j) {
+      if (w < lo && lo <= w + m[j]) {
+        lds->b.p_first = B * t + j;
+        lds->b.p_before = w;
+      }
+      if (w < hi && hi <= w + m[j]) lds->b.p_last = B * t + j;
       w += m[j];
     }
   }
   __syncthreads();
-  return lds->b;
+  SampleBorder b = lds->b;
+  // Behind the other borders min-p's does not count.
+  if (b.m_first > min(b.k_bin, b.p_last)) b.m_first = b.m_last = kNoBin;
+  return b;
 }
 
+// A block gathers its keys in LDS first: one addition to the row's count per
+// block, not per key (thousands to one place are one after another).
+constexpr uint32_t kListHeld = 2048;
 __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   __shared__ u64 lds[4];
   __shared__ SampleBorderLds border_lds;
+  __shared__ u64 held[kListHeld];
+  __shared__ uint32_t n_held, list_at;
   const uint32_t t = threadIdx.x, row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const SampleRow r = sample_row(a, row);
   if (!r.good || r.greedy) return;
-  const u64 top = row_top(a, row, lds);
+  const u64 top = row_top<kSampleThreads>(a, row, lds);
   if (!top) return;
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
-  SampleBorder b = {kNoBin, 0, 0, kNoBin, kNoBin};
-  if (r.k || r.by_mass()) {
-    u64 before, m[4];
-    b = sample_border(a, r, row, &border_lds, &before, m);
-  }
+  u64 before, m[4];
+  const SampleBorder b = sample_border<kSampleThreads>(a, r, scale, row, &border_lds, &before, m);
+  if (t == 0) n_held = 0;
+  __syncthreads();
+  uint32_t* const count = a.count + (uint64_t)row * kCountStride + kSampleBins;
+  u64* const list = a.list + (uint64_t)row * a.vocab;
   const float* const l = a.logits + (uint64_t)row * a.vocab;
-  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
+  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice), certain = b.certain();
   u64 sum = 0;
-  for (uint32_t i = from + t * 4; i < to; i += kSampleThreads * 4) {
+  const bool masses = r.masses();
+  if (masses) {
+    const u64* const own = a.slice_mass + (uint64_t)blockIdx.x * kSampleBins;
+    for (uint32_t i = t; i < certain; i += kSampleThreads) sum += own[i];
+  }
+  // Nothing to list: the slice need not be read.
+  for (uint32_t i = from + t * 4; i < (certain < kNoBin ? to : 0u); i += kSampleThreads * 4) {
     const f32x4 v = sample_load(l, i, a.vocab);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      if (!(v[j] > -INFINITY)) continue;
-      const uint32_t bin = sample_bin(scale.top - float_ord(v[j]));
-      if (b.certain(bin)) {
+      const uint32_t bin = sample_bin(scale.top, v[j]);
+      if (bin < certain) {
+        if (masses || !(v[j] > -INFINITY)) continue;
         bool kept;
-        const u64 m = scale.mass(v[j], &kept);
-        if (kept) sum += m;
-      } else if (b.listed(bin)) {
-        const uint32_t at = atomicAdd(a.count + (uint64_t)row * kCountStride + kSampleBins, 1u);
-        a.list[(uint64_t)row * a.vocab + at] = sample_key(v[j], i + j);
+        sum += scale.mass(v[j], &kept);
+      } else if (b.listed(bin) && v[j] > -INFINITY) {
+        const uint32_t at = atomicAdd(&n_held, 1u);
+        if (at < kListHeld)
+          held[at] = sample_key(v[j], i + j);
+        else
+          list[atomicAdd(count, 1u)] = sample_key(v[j], i + j);
       }
     }
   }
   u64 all;
-  block_before(sum, &all, lds);
+  block_before<kSampleThreads>(sum, &all, lds);
   if (t == 0) a.kept[blockIdx.x] = all;
+  const uint32_t n = min(n_held, kListHeld);
+  if (!n) return;
+  if (t == 0) list_at = atomicAdd(count, n);
+  __syncthreads();
+  for (uint32_t i = t; i < n; i += kSampleThreads) list[list_at + i] = held[i];
 }
 
-// The list's entries of one bin, in order; a place is distance and token in one
-// number, the first of the order the smallest.
-struct SamplePlaces {
-  u64 thr;        // only keys from it on
-  uint32_t bin, top, first, bits, token_bits;
-  __device__ bool place(u64 key, u64* p) const {
-    const uint32_t d = top - (uint32_t)(key >> 32);
-    if (key < thr || sample_bin(d) != bin) return false;
-    *p = (u64)(d - first) << token_bits | key_token(key);
-    return true;
+// The row's list: its first keys in LDS with their masses, if it has no more.
+constexpr uint32_t kPickHeld = 4096, kPickBins = (kSampleBins + kPickThreads - 1) / kPickThreads;
+struct SampleList {
+  const u64* list;
+  u64 *keys, *masses;  // LDS
+  uint32_t n;
+  __device__ bool held() const { return n <= kPickHeld; }
+  __device__ u64 key(uint32_t i) const { return held() ? keys[i] : list[i]; }
+  // A key's mass; 0 where min_p does not keep it (if `kept`).
+  __device__ static u64 mass_of(u64 key, const SampleScale& scale, bool kept_only) {
+    bool kept;
+    const u64 m = scale.mass(ord_float((uint32_t)(key >> 32)), &kept);
+    return kept || !kept_only ? m : 0ull;
   }
+  __device__ u64 mass(uint32_t i, const SampleScale& scale) const { return held() ? masses[i] : mass_of(list[i], scale, false); }
+};
+
+// Its entries of one bin, in order; a place is the distance from `first` (in
+// steps of the order) and the token in one number, the first of the order the
+// smallest.
+struct SamplePlaces {
+  u64 thr;              // only keys from it on
+  float max;
+  uint32_t bin, first;  // the bin's largest logit in the list
+  uint32_t token_bits;
+  __device__ bool in(u64 key) const { return key >= thr && sample_bin(max, ord_float((uint32_t)(key >> 32))) == bin; }
+  __device__ u64 place(u64 key) const { return (u64)(first - (uint32_t)(key >> 32)) << token_bits | key_token(key); }
   __device__ u64 key(u64 p) const {
-    const uint32_t d = first + (uint32_t)(p >> token_bits), token = (uint32_t)(p & ((1ull << token_bits) - 1));
-    return (u64)(top - d) << 32 | (uint32_t)~token;
+    return (u64)(first - (uint32_t)(p >> token_bits)) << 32 | (uint32_t)~(uint32_t)(p & ((1ull << token_bits) - 1));
   }
 };
 
-constexpr uint32_t kDigit = 10;
+constexpr int kDigit = 9;
+static_assert(1u << kDigit == kPickThreads, "a digit's value per thread");
 struct SelectLds {
   u64 weight[1u << kDigit];
   uint32_t count[1u << kDigit];
-  u64 part[4];
+  u64 part[kPickThreads / 64];
   u64 prefix, rest, found;
   uint32_t left;
 };
 // Key of the first place up to which the weights (masses, or 1 each) add up to
 // `target` or more, digit after digit of the places from the top; there is one.
 template <bool MASS>
-__device__ u64 sample_select(const u64* list, uint32_t n, const SamplePlaces& s, const SampleScale& scale, u64 target,
-                             SelectLds* lds) {
+__device__ u64 sample_select(const SampleList& list, SamplePlaces s, const SampleScale& scale, u64 target, SelectLds* lds) {
   const uint32_t t = threadIdx.x;
-  int shift = (int)(s.bits + s.token_bits);
+  // What the bin's entries span.
+  u64 hi = 0, lo = 0;  // lo: of complements
+  for (uint32_t i = t; i < list.n; i += kPickThreads) {
+    const u64 key = list.key(i);
+    if (s.in(key)) hi = max(hi, key), lo = max(lo, ~key);
+  }
+  hi = block_max<kPickThreads>(hi, lds->part);
+  lo = ~block_max<kPickThreads>(lo, lds->part);
+  s.first = (uint32_t)(hi >> 32);
+  const uint32_t span = s.first - (uint32_t)(lo >> 32);
+  int shift = (int)((span ? 32 - __builtin_clz(span) : 0) + s.token_bits);
   u64 prefix = 0;  // the digits above shift
   for (;;) {
-    const int width = min(shift, (int)kDigit);
+    const int width = min(shift, kDigit);
     shift -= width;
-    for (uint32_t i = t; i < 1u << kDigit; i += kSampleThreads) lds->weight[i] = 0, lds->count[i] = 0;
+    lds->weight[t] = 0;
+    lds->count[t] = 0;
     __syncthreads();
-    for (uint32_t i = t; i < n; i += kSampleThreads) {
-      u64 p;
-      if (!s.place(list[i], &p) || p >> (shift + width) != prefix) continue;
+    for (uint32_t i = t; i < list.n; i += kPickThreads) {
+      const u64 key = list.key(i);
+      if (!s.in(key)) continue;
+      const u64 p = s.place(key);
+      if (p >> (shift + width) != prefix) continue;
       const uint32_t digit = (uint32_t)(p >> shift) & ((1u << width) - 1);
       atomicAdd(&lds->count[digit], 1u);
-      if constexpr (MASS) {
-        bool kept;
-        atomicAdd(&lds->weight[digit], scale.mass(ord_float((uint32_t)(list[i] >> 32)), &kept));
-      }
+      if constexpr (MASS) atomicAdd(&lds->weight[digit], list.mass(i, scale));
     }
     __syncthreads();
-    u64 w[4], all, sum = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum += w[j] = MASS ? lds->weight[4 * t + j] : lds->count[4 * t + j];
-    u64 before = block_before(sum, &all, lds->part);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (before < target && target <= before + w[j]) {
-        lds->prefix = prefix << width | (4 * t + j);
-        lds->rest = target - before;
-        lds->left = lds->count[4 * t + j];
-      }
-      before += w[j];
+    const u64 w = MASS ? lds->weight[t] : lds->count[t];
+    u64 all;
+    const u64 before = block_before<kPickThreads>(w, &all, lds->part);
+    if (before < target && target <= before + w) {
+      lds->prefix = prefix << width | t;
+      lds->rest = target - before;
+      lds->left = lds->count[t];
     }
     __syncthreads();
     prefix = lds->prefix;
@@ -383,24 +459,25 @@ __device__ u64 sample_select(const u64* list, uint32_t n, const SamplePlaces& s,
     __syncthreads();
   }
   // One place has these digits.
-  for (uint32_t i = t; i < n; i += kSampleThreads) {
-    u64 p;
-    if (s.place(list[i], &p) && p >> shift == prefix) lds->found = list[i];
+  for (uint32_t i = t; i < list.n; i += kPickThreads) {
+    const u64 key = list.key(i);
+    if (s.in(key) && s.place(key) >> shift == prefix) lds->found = key;
   }
   __syncthreads();
   return lds->found;
 }
 
-__global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
-  __shared__ u64 lds[4];
+__global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
+  extern __shared__ __attribute__((aligned(16))) u64 held[];  // kPickHeld keys, as many masses
+  __shared__ u64 lds[kPickThreads / 64];
   __shared__ SampleBorderLds border_lds;
   __shared__ SelectLds select_lds;
   __shared__ u64 kept_of[kSampleSlices];
-  __shared__ uint32_t the_slice;
+  __shared__ uint32_t the_one;
   __shared__ u64 the_rest;
   const uint32_t t = threadIdx.x, row = blockIdx.x;
   const SampleRow r = sample_row(a, row);
-  const u64 top = row_top(a, row, lds);
+  const u64 top = row_top<kPickThreads>(a, row, lds);
   if (!r.good || !top || r.greedy) {
     if (t == 0) {
       if (!r.good) *a.err = 2u;
@@ -412,91 +489,121 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   }
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
   u64 thr = 0;  // keys from it on are kept
-  const u64* const list = a.list + (uint64_t)row * a.vocab;
-  uint32_t n = 0;
-  if (r.k || r.by_mass()) {
-    u64 before, m[4];
-    const SampleBorder b = sample_border(a, r, row, &border_lds, &before, m);
-    n = a.count[(uint64_t)row * kCountStride + kSampleBins];
+  SampleList list = {a.list + (uint64_t)row * a.vocab, held, held + kPickHeld, 0};
+  if (t < a.slices) kept_of[t] = a.kept[(uint64_t)row * a.slices + t];
+  u64 mass_before, m[kPickBins];
+  const SampleBorder b = sample_border<kPickThreads>(a, r, scale, row, &border_lds, &mass_before, m);
+  list.n = b.certain() < kNoBin ? a.count[(uint64_t)row * kCountStride + kSampleBins] : 0u;
+  if (list.held())
+    for (uint32_t i = t; i < list.n; i += kPickThreads) {
+      const u64 key = list.list[i];
+      list.keys[i] = key;
+      list.masses[i] = SampleList::mass_of(key, scale, false);
+    }
+  __syncthreads();
+  if (b.k_bin == kNoBin && b.p_first == kNoBin) {
+    // No border but min-p's.
+  } else if (list.n <= kPickThreads) {
+    // Few keys: sorted by counting the larger ones, which puts the bins in order
+    // and top-k's last.
+    const u64 key = t < list.n ? list.keys[t] : 0ull, mass = t < list.n ? list.masses[t] : 0ull;
+    uint32_t rank = 0;
+    for (uint32_t i = 0; i < list.n; ++i) rank += list.keys[i] > key;
+    __syncthreads();
+    if (t < list.n) {
+      list.keys[rank] = key;
+      list.masses[rank] = mass;
+    }
+    __syncthreads();
+    const u64 mine = t < list.n ? list.keys[t] : 0ull, here = t < list.n ? list.masses[t] : 0ull;
+    const uint32_t bin = t < list.n ? sample_bin(scale.top, ord_float((uint32_t)(mine >> 32))) : kNoBin;
+    // Where top-k's bin begins in the list (others with min-p's alone may lie behind it: none are kept).
+    const uint32_t k_from = (uint32_t)block_sum<kPickThreads>(bin < b.k_bin, lds);
+    uint32_t last = list.n;  // keys from it on are not kept
+    u64 sums[2] = {bin >= b.p_first && bin <= b.p_last ? here : 0ull, 0}, all[2];
+    if (b.k_bin != kNoBin) last = k_from + (r.k - b.k_before);
+    sums[1] = t >= k_from && t < last && b.k_bin != kNoBin ? here : 0ull;
+    block_before<kPickThreads, 2>(sums, all, border_lds.part);
+    if (r.by_mass()) {
+      // Kept: with less mass before it than top-p asks for.
+      const u64 target = share_of(r.top_p, b.k_mass + all[1]);
+      const bool kept = t < last && (bin < b.p_first || (bin <= b.p_last && b.p_before + sums[0] < target));
+      last = (uint32_t)block_sum<kPickThreads>(kept, lds);
+    }
+    thr = list.keys[last - 1];  // the first key of top-k's or top-p's bin is kept
+  } else {
     SamplePlaces s;
     s.thr = 0;
-    s.top = scale.top;
+    s.max = scale.top;
     s.token_bits = a.vocab > 1 ? 32 - __builtin_clz(a.vocab - 1) : 0;
     u64 own = 0;  // mass of top-k's bin that is kept
     if (b.k_bin != kNoBin) {
       s.bin = b.k_bin;
-      sample_bin_range(s.bin, &s.first, &s.bits);
-      thr = s.thr = sample_select<false>(list, n, s, scale, r.k - b.k_before, &select_lds);
+      thr = s.thr = sample_select<false>(list, s, scale, r.k - b.k_before, &select_lds);
       if (r.by_mass()) {
         u64 sum = 0;
-        for (uint32_t i = t; i < n; i += kSampleThreads) {
-          u64 p;
-          bool kept;
-          if (s.place(list[i], &p)) sum += scale.mass(ord_float((uint32_t)(list[i] >> 32)), &kept);
-        }
-        block_before(sum, &own, lds);
+        for (uint32_t i = t; i < list.n; i += kPickThreads)
+          if (s.in(list.key(i))) sum += list.mass(i, scale);
+        own = block_sum<kPickThreads>(sum, lds);
       }
     }
     if (r.by_mass()) {
       const u64 target = share_of(r.top_p, b.k_mass + own);
-      u64 w = before;
+      u64 w = mass_before;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 mass = 4 * t + j == b.k_bin ? own : m[j];
+      for (uint32_t j = 0; j < kPickBins; ++j) {
+        const uint32_t bin = kPickBins * t + j;
+        const u64 mass = bin == b.k_bin ? own : m[j];
         if (w < target && target <= w + mass) {
-          the_slice = 4 * t + j;
+          the_one = bin;
           the_rest = target - w;
         }
         w += mass;
       }
       __syncthreads();
-      s.bin = the_slice;
-      sample_bin_range(s.bin, &s.first, &s.bits);
-      thr = sample_select<true>(list, n, s, scale, the_rest, &select_lds);
+      s.bin = the_one;
+      thr = sample_select<true>(list, s, scale, the_rest, &select_lds);
     }
   }
   // Every slice's kept mass: what is certain, and what of the list is kept.
-  if (t < a.slices) kept_of[t] = a.kept[(uint64_t)row * a.slices + t];
   __syncthreads();
-  for (uint32_t i = t; i < n; i += kSampleThreads) {
-    const u64 key = list[i];
-    bool kept;
-    const u64 m = scale.mass(ord_float((uint32_t)(key >> 32)), &kept);
-    if (key >= thr && kept && m) atomicAdd(&kept_of[key_token(key) / a.slice], m);
+  for (uint32_t i = t; i < list.n; i += kPickThreads) {
+    const u64 key = list.key(i);
+    if (key < thr) continue;
+    const u64 m = SampleList::mass_of(key, scale, true);
+    if (m) atomicAdd(&kept_of[key_token(key) / a.slice], m);
   }
   __syncthreads();
   const u64 own = t < a.slices ? kept_of[t] : 0ull;
   u64 total;
-  u64 before = block_before(own, &total, lds);
+  u64 before = block_before<kPickThreads>(own, &total, lds);
   // u < 1 and total >= 2^s: the product stays below the total.
   u64 target = (u64)(r.u * (double)total);
   target = min(target, total - 1);
   if (before <= target && target < before + own) {
-    the_slice = t;
+    the_one = t;
     the_rest = target - before;
   }
   __syncthreads();
-  const uint32_t slice = the_slice;
+  const uint32_t slice = the_one;
   target = the_rest;
   const float* const l = a.logits + (uint64_t)row * a.vocab;
-  const uint32_t run = a.slice / kSampleThreads, from = slice * a.slice + t * run;
-  auto mass_at = [&](float v, uint32_t token) -> u64 {
+  const uint32_t run = a.slice / kPickThreads, from = slice * a.slice + t * run;
+  auto mass_at = [&](uint32_t token) -> u64 {
+    const float v = l[token];
     if (!(v > -INFINITY) || sample_key(v, token) < thr) return 0;
     bool kept;
     const u64 m = scale.mass(v, &kept);
     return kept ? m : 0ull;
   };
   u64 sum = 0;
-  for (uint32_t i = from; i < min(a.vocab, from + run); i += 4) {
-    const f32x4 v = sample_load(l, i, a.vocab);
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) sum += mass_at(v[j], i + j);
-  }
+  const uint32_t to = min(a.vocab, from + run);
+  for (uint32_t i = from; i < to; ++i) sum += mass_at(i);
   u64 all;
-  before = block_before(sum, &all, lds);
+  before = block_before<kPickThreads>(sum, &all, lds);
   if (before <= target && target < before + sum) {
     for (uint32_t i = from;; ++i) {
-      const u64 m = mass_at(l[i], i);
+      const u64 m = mass_at(i);
       if (target < before + m) {
         a.tokens[row] = (int32_t)i;
         if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(l[i]) - log((double)total / a.unit));
@@ -520,27 +627,33 @@ uint64_t sample_workspace(uint32_t n, uint32_t vocab, SampleArgs* a, uint8_t* ba
   auto al = [](uint64_t b) { return (b + 255) & ~(uint64_t)255; };
   const uint64_t rows = n, tops = al(rows * slices * 8), mass = al(rows * kSampleBins * 8);
   const uint64_t count = al(rows * kCountStride * 4), list = al(rows * vocab * 8);
+  const uint64_t slice_mass = rows * slices * kSampleBins * 8;
   if (a) {
     uint32_t bits = 0;
     while (((uint64_t)1 << bits) < vocab) ++bits;
     a->slice = slice;
     a->slices = slices;
-    a->unit = (double)((uint64_t)1 << (62 - bits));
+    a->unit = (double)((uint64_t)1 << (bits < 11 ? 51 : 62 - bits));
     a->tops = (u64*)base;
     a->kept = (u64*)(base + tops);
     a->mass = (u64*)(base + 2 * tops);
     a->list = (u64*)(base + 2 * tops + mass);
     a->count = (uint32_t*)(base + 2 * tops + mass + list);
+    a->slice_mass = (u64*)(base + 2 * tops + mass + list + count);
   }
-  return 2 * tops + mass + list + count;
+  return 2 * tops + mass + list + count + slice_mass;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
   const dim3 grid(a.n * a.slices), block(kSampleThreads);
   hipLaunchKernelGGL(k_sample_top, grid, block, 0, st, a);
-  if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, a);
+  hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, a);
   hipLaunchKernelGGL(k_sample_list, grid, block, 0, st, a);
-  hipLaunchKernelGGL(k_sample_pick, dim3(a.n), block, 0, st, a);
+  static std::atomic<uint64_t> raised{0};
+  constexpr uint32_t bytes = 2 * kPickHeld * sizeof(u64);
+  const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(&k_sample_pick), bytes, raised);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k_sample_pick, dim3(a.n), dim3(kPickThreads), bytes, st, a);
   return hipGetLastError();
 }
 
