@@ -11,8 +11,8 @@
 // A logit becomes 32 bits in an order that integers compare, and a key with the
 // complement of its token below it, so keys are unique and the order of the
 // filters is that of falling keys. Bins are by the distance d from the row's
-// largest logit (a rounded difference, but it never falls as logits fall): 64 to
-// every power of two of d from 1/64 to 256, so that they are finest where the
+// largest logit (a rounded difference, but it never falls as logits fall): 128 to
+// every power of two of d from 1/32 to 128, so that they are finest where the
 // mass is. All three filters keep a first part of the order: what decides is one
 // key, and only the bins around it have to be looked into.
 //
@@ -34,21 +34,23 @@ constexpr uint32_t kNoBin = kSampleBins;
 
 // Bin of a logit, 0 the largest's.
 __device__ __forceinline__ uint32_t sample_bin(float max, float l) {
-  constexpr uint32_t kFirst = (127 - 6) << 6;  // the upper bits of 1/64
+  constexpr uint32_t kFirst = (127 - 5) << 7;  // the upper bits of 1/32
   const float d = max - l;                     // NaN where both are infinite: 0
-  const uint32_t b = d > 0.f ? __float_as_uint(d) >> 17 : 0u;
+  const uint32_t b = d > 0.f ? __float_as_uint(d) >> 16 : 0u;
   return b < kFirst ? 0u : min(b - kFirst, kSampleBins - 1);
 }
 
-// e^x for -46 <= x <= 0: x = n ln 2 + r, the series of e^r to r^11 (what is left
-// out is below 2^-47 of it).
-__device__ __forceinline__ double sample_exp(double x) {
-  const double n = __builtin_rint(x * 1.4426950408889634), r = __builtin_fma(n, -0.6931471805599453, x);
-  double e = 1.0 / 39916800;
-  constexpr double c[11] = {1, 1, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800};
+// 2^t for -66 <= t <= 0, to 2^-44 of it: t = n + f, and (2^f - 1) / f as the
+// polynomial that agrees with it at nine Chebyshev points of [-1/2, 1/2].
+__device__ __forceinline__ double sample_exp2(double t) {
+  constexpr double c[9] = {0.6931471805599453,     0.2402265069581299,      0.055504108664760424,
+                           0.009618129159402558,   0.0013333558179043112,   0.00015403455852453838,
+                           1.525268684626772e-05,  1.3255224878668817e-06,  1.0203121063391729e-07};
+  const double n = __builtin_rint(t), f = t - n;
+  double e = c[8];
 #pragma unroll
-  for (int i = 10; i >= 0; --i) e = __builtin_fma(e, r, c[i]);
-  return __builtin_ldexp(e, (int)n);
+  for (int i = 7; i >= 0; --i) e = __builtin_fma(e, f, c[i]);
+  return __builtin_ldexp(__builtin_fma(e, f, 1.0), (int)n);
 }
 
 struct SampleRow {
@@ -76,24 +78,33 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, uint32_t ro
 // What a row's largest logit makes of the others.
 struct SampleScale {
   float top;
-  double max, inv_t, unit, least, min_p;
+  double max, inv_t, inv_t2, unit, least, min_p;
   bool infinite;
   __device__ SampleScale(const SampleArgs& a, const SampleRow& r, uint32_t o)
-      : top(ord_float(o)), max(top), inv_t(r.inv_t), unit(a.unit), min_p(r.min_p), infinite(o == 0xFF800000u) {
+      : top(ord_float(o)), max(top), inv_t(r.inv_t), inv_t2(r.inv_t * 1.4426950408889634), unit(a.unit), min_p(r.min_p), infinite(o == 0xFF800000u) {
     // Below it a mass rounds to zero.
-    least = -0.6931471805599453 * (2 + __builtin_amdgcn_frexp_exp(a.unit));
+    least = -2 - __builtin_amdgcn_frexp_exp(a.unit);
   }
   __device__ double log_mass(float l) const {
-    if (infinite) return l == INFINITY ? 0.0 : -INFINITY;
-    return ((double)l - max) * inv_t;
+    return infinite ? (l == INFINITY ? 0.0 : -INFINITY) : ((double)l - max) * inv_t;
   }
-  // The mass as an integer; *kept: whether min_p keeps it.
+  // The mass as an integer; *kept: whether min_p keeps it. No branches, so that
+  // several logits' series are formed side by side (one is a chain of eleven).
   __device__ u64 mass(float l, bool* kept) const {
-    const double x = log_mass(l);
-    const double e = x > least ? sample_exp(x) : 0.0;
-    *kept = e >= min_p;
+    const double x = infinite ? (l == INFINITY ? 0.0 : -INFINITY) : ((double)l - max) * inv_t2;
+    const double e = sample_exp2(fmax(x, least)), in = x > least ? e : 0.0;  // -inf and NaN: 0
+    *kept = in >= min_p;
     // The sum's last place is 1: its lower bits are the rounded product.
-    return (u64)__double_as_longlong(__builtin_fma(e, unit, 0x1p52)) - 0x4330000000000000ull;
+    return (u64)__double_as_longlong(__builtin_fma(in, unit, 0x1p52)) - 0x4330000000000000ull;
+  }
+  // Of four logits; 0 where min_p does not keep it (if `kept_only`).
+  __device__ void masses(f32x4 l, u64 (&m)[4], bool kept_only) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bool kept;
+      m[j] = mass(l[j], &kept);
+      m[j] = kept || !kept_only ? m[j] : 0ull;
+    }
   }
 };
 
@@ -162,9 +173,9 @@ __device__ __forceinline__ f32x4 sample_load(const float* row, uint32_t at, uint
   return v;
 }
 
-template <uint32_t T>
-__device__ __forceinline__ u64 row_top(const SampleArgs& a, uint32_t row, u64* lds) {
-  return block_max<T>(threadIdx.x < a.slices ? a.tops[row * a.slices + threadIdx.x] : 0ull, lds);
+// What a thread asks for first: all of it is on its way at once.
+__device__ __forceinline__ u64 slice_top(const SampleArgs& a, uint32_t row) {
+  return threadIdx.x < a.slices ? a.tops[row * a.slices + threadIdx.x] : 0ull;
 }
 
 __global__ __launch_bounds__(kSampleThreads) void k_sample_top(SampleArgs a) {
@@ -195,27 +206,26 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs a) {
   __shared__ u64 lds[4];
   const uint32_t t = threadIdx.x, row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const SampleRow r = sample_row(a, row);
-  if (!r.good || r.greedy) return;
-  const u64 top = row_top<kSampleThreads>(a, row, lds);
-  if (!top) return;
-  for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
-  __syncthreads();
-  const SampleScale scale(a, r, (uint32_t)(top >> 32));
+  u64 top = slice_top(a, row);
   const float* const l = a.logits + (uint64_t)row * a.vocab;
   const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
+  f32x4 next = sample_load(l, from + t * 4, a.vocab);
+  if (!r.good || r.greedy) return;
+  for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
+  top = block_max<kSampleThreads>(top, lds);
+  if (!top) return;
+  const SampleScale scale(a, r, (uint32_t)(top >> 32));
   const bool counts = r.k, masses = r.masses();
   for (uint32_t i = from + t * 4; i < to; i += kSampleThreads * 4) {
-    const f32x4 v = sample_load(l, i, a.vocab);
+    const f32x4 v = next;
+    next = sample_load(l, i + kSampleThreads * 4, a.vocab);
+    u64 m[4] = {0, 0, 0, 0};
+    if (masses) scale.masses(v, m, false);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      if (!(v[j] > -INFINITY)) continue;
       const uint32_t bin = sample_bin(scale.top, v[j]);
-      if (counts) atomicAdd(&count[bin], 1u);
-      if (masses) {
-        bool kept;
-        const u64 m = scale.mass(v[j], &kept);
-        if (m) atomicAdd(&mass[bin], m);
-      }
+      if (counts && v[j] > -INFINITY) atomicAdd(&count[bin], 1u);
+      if (m[j]) atomicAdd(&mass[bin], m[j]);
     }
   }
   __syncthreads();
@@ -248,24 +258,37 @@ __device__ __forceinline__ u64 share_of(double p, u64 of) {  // at least one
   const double v = __builtin_ceil(p * (double)of);
   return v >= 1.0 ? (u64)v : 1ull;
 }
-// Thread t of T has the B bins from B t on; before: mass ahead of its first, m: of each.
-template <uint32_t T, uint32_t B = (kSampleBins + T - 1) / T>
-__device__ __forceinline__ SampleBorder sample_border(const SampleArgs& a, const SampleRow& r, const SampleScale& scale,
-                                                      uint32_t row, SampleBorderLds* lds, u64* before, u64 (&m)[B]) {
-  const uint32_t t = threadIdx.x;
+// Thread t of T has the B bins from B t on.
+template <uint32_t T>
+struct SampleShare {
+  static constexpr uint32_t B = (kSampleBins + T - 1) / T;
   uint32_t c[B];
+  u64 m[B], before;  // counts; masses; mass of the bins ahead
+  __device__ __forceinline__ void load(const SampleArgs& a, uint32_t row) {
+#pragma unroll
+    for (uint32_t j = 0; j < B; ++j) {
+      const uint32_t i = B * threadIdx.x + j;
+      c[j] = i < kSampleBins ? a.count[(uint64_t)row * kCountStride + i] : 0u;
+      m[j] = i < kSampleBins ? a.mass[(uint64_t)row * kSampleBins + i] : 0ull;
+    }
+  }
+};
+template <uint32_t T>
+__device__ __forceinline__ SampleBorder sample_border(const SampleRow& r, const SampleScale& scale, SampleBorderLds* lds,
+                                                      SampleShare<T>& share) {
+  constexpr uint32_t B = SampleShare<T>::B;
+  const uint32_t t = threadIdx.x;
   u64 own[2] = {0, 0}, all[2];
 #pragma unroll
   for (uint32_t j = 0; j < B; ++j) {
-    const bool in = B * t + j < kSampleBins;
-    c[j] = in ? a.count[(uint64_t)row * kCountStride + B * t + j] : 0u;
-    m[j] = in ? a.mass[(uint64_t)row * kSampleBins + B * t + j] : 0ull;
-    own[0] += c[j];
-    own[1] += m[j];
+    own[0] += share.c[j];
+    own[1] += share.m[j];
   }
   block_before<T, 2>(own, all, lds->part);
+  const auto& c = share.c;
+  const auto& m = share.m;
   u64 n = own[0];
-  *before = own[1];
+  share.before = own[1];
   if (t == 0) {
     lds->b = SampleBorder{kNoBin, 0, all[1], kNoBin, kNoBin, 0, kNoBin, kNoBin};
     lds->k_own = 0;
@@ -278,7 +301,7 @@ __device__ __forceinline__ SampleBorder sample_border(const SampleArgs& a, const
   }
   __syncthreads();
   if (r.k) {
-    u64 w = *before;
+    u64 w = share.before;
 #pragma unroll
     for (uint32_t j = 0; j < B; ++j) {
       if (n < r.k && r.k <= n + c[j]) {
@@ -294,7 +317,7 @@ __device__ __forceinline__ SampleBorder sample_border(const SampleArgs& a, const
   }
   if (r.by_mass()) {
     const u64 lo = share_of(r.top_p, lds->b.k_mass), hi = share_of(r.top_p, lds->b.k_mass + lds->k_own);
-    u64 w = *before;
+    u64 w = share.before;
 #pragma unroll
     for (uint32_t j = 0; j < B; ++j) {
       if (w < lo && lo <= w + m[j]) {
@@ -322,18 +345,22 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   __shared__ uint32_t n_held, list_at;
   const uint32_t t = threadIdx.x, row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const SampleRow r = sample_row(a, row);
+  u64 top = slice_top(a, row);
+  SampleShare<kSampleThreads> share;
+  share.load(a, row);
+  const float* const l = a.logits + (uint64_t)row * a.vocab;
+  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
+  f32x4 next = sample_load(l, from + t * 4, a.vocab);
   if (!r.good || r.greedy) return;
-  const u64 top = row_top<kSampleThreads>(a, row, lds);
+  top = block_max<kSampleThreads>(top, lds);
   if (!top) return;
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
-  u64 before, m[4];
-  const SampleBorder b = sample_border<kSampleThreads>(a, r, scale, row, &border_lds, &before, m);
+  const SampleBorder b = sample_border<kSampleThreads>(r, scale, &border_lds, share);
   if (t == 0) n_held = 0;
   __syncthreads();
   uint32_t* const count = a.count + (uint64_t)row * kCountStride + kSampleBins;
   u64* const list = a.list + (uint64_t)row * a.vocab;
-  const float* const l = a.logits + (uint64_t)row * a.vocab;
-  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice), certain = b.certain();
+  const uint32_t certain = b.certain();
   u64 sum = 0;
   const bool masses = r.masses();
   if (masses) {
@@ -342,15 +369,24 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   }
   // Nothing to list: the slice need not be read.
   for (uint32_t i = from + t * 4; i < (certain < kNoBin ? to : 0u); i += kSampleThreads * 4) {
-    const f32x4 v = sample_load(l, i, a.vocab);
+    const f32x4 v = next;
+    next = sample_load(l, i + kSampleThreads * 4, a.vocab);
+    uint32_t bin[4];
+    bool sure = false;
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      const uint32_t bin = sample_bin(scale.top, v[j]);
-      if (bin < certain) {
-        if (masses || !(v[j] > -INFINITY)) continue;
-        bool kept;
-        sum += scale.mass(v[j], &kept);
-      } else if (b.listed(bin) && v[j] > -INFINITY) {
+      bin[j] = sample_bin(scale.top, v[j]);
+      sure |= bin[j] < certain;
+    }
+    if (!masses && __any(sure)) {
+      u64 m[4];
+      scale.masses(v, m, false);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) sum += bin[j] < certain ? m[j] : 0ull;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      if (bin[j] >= certain && b.listed(bin[j]) && v[j] > -INFINITY) {
         const uint32_t at = atomicAdd(&n_held, 1u);
         if (at < kListHeld)
           held[at] = sample_key(v[j], i + j);
@@ -382,6 +418,10 @@ struct SampleList {
     bool kept;
     const u64 m = scale.mass(ord_float((uint32_t)(key >> 32)), &kept);
     return kept || !kept_only ? m : 0ull;
+  }
+  // Masses of keys held by all filters but min-p, which is asked where there is one.
+  __device__ u64 kept(uint32_t i, const SampleScale& scale) const {
+    return scale.min_p > 0.0 ? mass_of(key(i), scale, true) : mass(i, scale);
   }
   __device__ u64 mass(uint32_t i, const SampleScale& scale) const { return held() ? masses[i] : mass_of(list[i], scale, false); }
 };
@@ -477,7 +517,12 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   __shared__ u64 the_rest;
   const uint32_t t = threadIdx.x, row = blockIdx.x;
   const SampleRow r = sample_row(a, row);
-  const u64 top = row_top<kPickThreads>(a, row, lds);
+  SampleList list = {a.list + (uint64_t)row * a.vocab, held, held + kPickHeld, a.count[(uint64_t)row * kCountStride + kSampleBins]};
+  const u64 kept_own = t < a.slices ? a.kept[(uint64_t)row * a.slices + t] : 0ull;
+  const u64 first_key = t < a.vocab ? list.list[t] : 0ull;  // if it is one
+  SampleShare<kPickThreads> share;
+  share.load(a, row);
+  const u64 top = block_max<kPickThreads>(slice_top(a, row), lds);
   if (!r.good || !top || r.greedy) {
     if (t == 0) {
       if (!r.good) *a.err = 2u;
@@ -489,14 +534,12 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   }
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
   u64 thr = 0;  // keys from it on are kept
-  SampleList list = {a.list + (uint64_t)row * a.vocab, held, held + kPickHeld, 0};
-  if (t < a.slices) kept_of[t] = a.kept[(uint64_t)row * a.slices + t];
-  u64 mass_before, m[kPickBins];
-  const SampleBorder b = sample_border<kPickThreads>(a, r, scale, row, &border_lds, &mass_before, m);
-  list.n = b.certain() < kNoBin ? a.count[(uint64_t)row * kCountStride + kSampleBins] : 0u;
+  if (t < a.slices) kept_of[t] = kept_own;
+  const SampleBorder b = sample_border<kPickThreads>(r, scale, &border_lds, share);
+  if (b.certain() == kNoBin) list.n = 0;
   if (list.held())
     for (uint32_t i = t; i < list.n; i += kPickThreads) {
-      const u64 key = list.list[i];
+      const u64 key = i < kPickThreads ? first_key : list.list[i];
       list.keys[i] = key;
       list.masses[i] = SampleList::mass_of(key, scale, false);
     }
@@ -549,11 +592,11 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     }
     if (r.by_mass()) {
       const u64 target = share_of(r.top_p, b.k_mass + own);
-      u64 w = mass_before;
+      u64 w = share.before;
 #pragma unroll
       for (uint32_t j = 0; j < kPickBins; ++j) {
         const uint32_t bin = kPickBins * t + j;
-        const u64 mass = bin == b.k_bin ? own : m[j];
+        const u64 mass = bin == b.k_bin ? own : share.m[j];
         if (w < target && target <= w + mass) {
           the_one = bin;
           the_rest = target - w;
@@ -570,7 +613,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   for (uint32_t i = t; i < list.n; i += kPickThreads) {
     const u64 key = list.key(i);
     if (key < thr) continue;
-    const u64 m = SampleList::mass_of(key, scale, true);
+    const u64 m = list.kept(i, scale);
     if (m) atomicAdd(&kept_of[key_token(key) / a.slice], m);
   }
   __syncthreads();
@@ -587,30 +630,66 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   __syncthreads();
   const uint32_t slice = the_one;
   target = the_rest;
+  // Each wave has a stretch of the slice, 256 tokens at a time; then the wave in
+  // whose stretch the sum passes u goes through it again.
   const float* const l = a.logits + (uint64_t)row * a.vocab;
-  const uint32_t run = a.slice / kPickThreads, from = slice * a.slice + t * run;
-  auto mass_at = [&](uint32_t token) -> u64 {
-    const float v = l[token];
-    if (!(v > -INFINITY) || sample_key(v, token) < thr) return 0;
-    bool kept;
-    const u64 m = scale.mass(v, &kept);
-    return kept ? m : 0ull;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  constexpr uint32_t kStep = 256;
+  const uint32_t stretch = (a.slice / (kPickThreads / 64) + kStep - 1) / kStep * kStep;
+  const uint32_t begin = slice * a.slice, from = begin + min(a.slice, wave * stretch);
+  const uint32_t to = min(min(a.vocab, begin + a.slice), from + stretch);
+  // Kept masses of this lane's four tokens from i on.
+  auto masses_at = [&](f32x4 v, uint32_t i, u64 (&m)[4]) {
+    bool in[4], any = false;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) any |= in[j] = i + j < to && sample_key(v[j], i + j) >= thr;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) m[j] = 0;
+    if (!__any(any)) return;
+    scale.masses(v, m, true);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) m[j] = in[j] ? m[j] : 0ull;
   };
   u64 sum = 0;
-  const uint32_t to = min(a.vocab, from + run);
-  for (uint32_t i = from; i < to; ++i) sum += mass_at(i);
-  u64 all;
-  before = block_before<kPickThreads>(sum, &all, lds);
-  if (before <= target && target < before + sum) {
-    for (uint32_t i = from;; ++i) {
-      const u64 m = mass_at(i);
-      if (target < before + m) {
-        a.tokens[row] = (int32_t)i;
-        if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(l[i]) - log((double)total / a.unit));
-        break;
+  f32x4 next = sample_load(l, from + lane * 4, a.vocab);
+  for (uint32_t i = from; i < to; i += kStep) {
+    const f32x4 v = next;
+    next = sample_load(l, i + kStep + lane * 4, a.vocab);
+    u64 m[4];
+    masses_at(v, i + lane * 4, m);
+    sum += m[0] + m[1] + m[2] + m[3];
+  }
+  sum = wave_scan_u64(sum);
+  if (lane == 63) lds[wave] = sum;
+  __syncthreads();
+  for (uint32_t w = 0; w < wave; ++w) {
+    const u64 m = lds[w];
+    if (target < m) return;  // another wave's
+    target -= m;
+  }
+  if (target >= lds[wave]) return;
+  for (uint32_t i = from;; i += kStep) {
+    const f32x4 v = sample_load(l, i + lane * 4, a.vocab);
+    u64 m[4];
+    masses_at(v, i + lane * 4, m);
+    const u64 own4 = m[0] + m[1] + m[2] + m[3];
+    const u64 upto = wave_scan_u64(own4);
+    const u64 here = __ballot(target < upto);
+    if (here) {
+      if (lane == (uint32_t)__builtin_ctzll(here)) {
+        u64 at = upto - own4;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          if (target >= at && target < at + m[j]) {
+            a.tokens[row] = (int32_t)(i + lane * 4 + j);
+            if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(v[j]) - log((double)total / a.unit));
+          }
+          at += m[j];
+        }
       }
-      before += m;
+      return;
     }
+    target -= (u64)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   }
 }
 
