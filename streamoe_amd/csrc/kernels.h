@@ -448,7 +448,7 @@ struct SampleArgs {
   uint32_t* err;
   // Workspace (sample_workspace).
   uint32_t slices, slice;             // slices of a row, logits of each (a multiple of 1024)
-  double unit;                        // 2^s: what a mass of 1 is held as
+  int up;                             // a mass of 1 is held as 2^up
   unsigned long long *tops;           // [n, slices] largest key of a slice
   unsigned long long *mass;           // [n, bins] of the row's logits
   unsigned long long *slice_mass;     // [n, slices, bins] of a slice's

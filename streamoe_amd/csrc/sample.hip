@@ -18,7 +18,9 @@
 //
 // A mass e^((logit - max) / T) is f64 and then an integer of 2^-s: sums of
 // integers are the same in any order, so atomics may form them. Masses of whole
-// bins are formed once; rows with top-k alone need those of the few kept.
+// bins are formed once. A row with a small top-k needs no masses but of those
+// tokens: all of them are listed, and the list sorted (one row with top-k 20: 24
+// -> XX us). A larger top-k alone needs the masses of what it keeps.
 #include "common.h"
 #include "kernels.h"
 
@@ -31,6 +33,7 @@ constexpr uint32_t kSampleThreads = 256, kPickThreads = 512;
 constexpr uint32_t kSampleSlices = 128;  // of a row at most
 constexpr uint32_t kCountStride = kSampleBins + 4;
 constexpr uint32_t kNoBin = kSampleBins;
+constexpr uint32_t kSmallK = 448;  // with the tokens that share its bin, mostly, a block's threads
 
 // Bin of a logit, 0 the largest's.
 __device__ __forceinline__ uint32_t sample_bin(float max, float l) {
@@ -40,17 +43,21 @@ __device__ __forceinline__ uint32_t sample_bin(float max, float l) {
   return b < kFirst ? 0u : min(b - kFirst, kSampleBins - 1);
 }
 
-// 2^t for -66 <= t <= 0, to 2^-44 of it: t = n + f, and (2^f - 1) / f as the
-// polynomial that agrees with it at nine Chebyshev points of [-1/2, 1/2].
-__device__ __forceinline__ double sample_exp2(double t) {
+// 2^(t + up) for -70 <= t <= 0, to 2^-44 of it: t = n + f, and (2^f - 1) / f as
+// the polynomial that agrees with it at nine Chebyshev points of [-1/2, 1/2]. n
+// is the lower word of t + 1.5 2^52 and goes into the exponent: conversions and
+// the scaling instruction take four times as long as an addition.
+__device__ __forceinline__ double sample_exp2(double t, int up) {
   constexpr double c[9] = {0.6931471805599453,     0.2402265069581299,      0.055504108664760424,
                            0.009618129159402558,   0.0013333558179043112,   0.00015403455852453838,
                            1.525268684626772e-05,  1.3255224878668817e-06,  1.0203121063391729e-07};
-  const double n = __builtin_rint(t), f = t - n;
+  const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);
   double e = c[8];
 #pragma unroll
   for (int i = 7; i >= 0; --i) e = __builtin_fma(e, f, c[i]);
-  return __builtin_ldexp(__builtin_fma(e, f, 1.0), (int)n);
+  const u64 bits = (u64)__double_as_longlong(__builtin_fma(e, f, 1.0));
+  const uint32_t n = (uint32_t)__double_as_longlong(whole) + (uint32_t)up;
+  return __longlong_as_double((long long)(bits + ((u64)(n << 20) << 32)));
 }
 
 struct SampleRow {
@@ -58,7 +65,8 @@ struct SampleRow {
   uint32_t k;              // kept at most; 0: all
   double inv_t, top_p, min_p, u;
   __device__ bool by_mass() const { return top_p < 1.0; }
-  __device__ bool masses() const { return by_mass() || !k; }  // of all bins
+  __device__ bool small() const { return k && k <= kSmallK; }
+  __device__ bool masses() const { return !small() && (by_mass() || !k); }  // of all bins
 };
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, uint32_t row) {
   SampleRow r;
@@ -78,24 +86,22 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, uint32_t ro
 // What a row's largest logit makes of the others.
 struct SampleScale {
   float top;
-  double max, inv_t, inv_t2, unit, least, min_p;
-  bool infinite;
+  bool infinite;            // +inf: 0 beside the others' -inf
+  double max, inv_t, inv_t2, least;  // 1 / T, also for powers of two; what min_p keeps, in units
+  int up;                   // a mass of 1 is 2^up
   __device__ SampleScale(const SampleArgs& a, const SampleRow& r, uint32_t o)
-      : top(ord_float(o)), max(top), inv_t(r.inv_t), inv_t2(r.inv_t * 1.4426950408889634), unit(a.unit), min_p(r.min_p), infinite(o == 0xFF800000u) {
-    // Below it a mass rounds to zero.
-    least = -2 - __builtin_amdgcn_frexp_exp(a.unit);
-  }
-  __device__ double log_mass(float l) const {
-    return infinite ? (l == INFINITY ? 0.0 : -INFINITY) : ((double)l - max) * inv_t;
-  }
-  // The mass as an integer; *kept: whether min_p keeps it. No branches, so that
-  // several logits' series are formed side by side (one is a chain of eleven).
+      : top(ord_float(o)), infinite(o == 0xFF800000u), max(infinite ? 0.0 : (double)top), inv_t(r.inv_t),
+        inv_t2(r.inv_t * 1.4426950408889634), least(__builtin_ldexp(r.min_p, a.up)), up(a.up) {}
+  __device__ float finite(float l) const { return infinite ? (l == INFINITY ? 0.f : -INFINITY) : l; }
+  __device__ double log_mass(float l) const { return ((double)finite(l) - max) * inv_t; }
+  // The mass as an integer; *kept: whether min_p keeps it. 0 below 2^-70, as for
+  // -inf and NaN. No branches, so that several logits' series are formed side by
+  // side.
   __device__ u64 mass(float l, bool* kept) const {
-    const double x = infinite ? (l == INFINITY ? 0.0 : -INFINITY) : ((double)l - max) * inv_t2;
-    const double e = sample_exp2(fmax(x, least)), in = x > least ? e : 0.0;  // -inf and NaN: 0
-    *kept = in >= min_p;
+    const double e = sample_exp2(fmax(((double)finite(l) - max) * inv_t2, -70.0), up);
+    *kept = e >= least;
     // The sum's last place is 1: its lower bits are the rounded product.
-    return (u64)__double_as_longlong(__builtin_fma(in, unit, 0x1p52)) - 0x4330000000000000ull;
+    return (u64)__double_as_longlong(e + 0x1p52) - 0x4330000000000000ull;
   }
   // Of four logits; 0 where min_p does not keep it (if `kept_only`).
   __device__ void masses(f32x4 l, u64 (&m)[4], bool kept_only) const {
@@ -173,6 +179,34 @@ __device__ __forceinline__ f32x4 sample_load(const float* row, uint32_t at, uint
   return v;
 }
 
+// A thread's fours of a slice in turn, two thousands at a time, the next two on
+// their way (16 waves of a CU and 1 KB each would be 2 TB/s).
+constexpr uint32_t kAhead = 2;
+struct SampleFours {
+  f32x4 next[kAhead];
+  uint32_t at;
+  __device__ __forceinline__ void load(const float* row, uint32_t from, uint32_t vocab) {
+    at = from;
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) next[j] = sample_load(row, from + j * kSampleThreads * 4, vocab);
+  }
+  // each(logits, first token), from `from` + 4 t on as loaded up to `to`.
+  template <class F>
+  __device__ __forceinline__ void go(const float* row, uint32_t to, uint32_t vocab, F each) {
+    for (; at < to; at += kAhead * kSampleThreads * 4) {
+      f32x4 v[kAhead];
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j) {
+        v[j] = next[j];
+        next[j] = sample_load(row, at + (kAhead + j) * kSampleThreads * 4, vocab);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j)
+        if (at + j * kSampleThreads * 4 < to) each(v[j], at + j * kSampleThreads * 4);
+    }
+  }
+};
+
 // What a thread asks for first: all of it is on its way at once.
 __device__ __forceinline__ u64 slice_top(const SampleArgs& a, uint32_t row) {
   return threadIdx.x < a.slices ? a.tops[row * a.slices + threadIdx.x] : 0ull;
@@ -184,14 +218,15 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_top(SampleArgs a) {
   const float* const l = a.logits + (uint64_t)row * a.vocab;
   u64 top = 0;
   const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
-  for (uint32_t i = from + t * 4; i < to; i += kSampleThreads * 4) {
-    const f32x4 v = sample_load(l, i, a.vocab);
+  SampleFours fours;
+  fours.load(l, from + t * 4, a.vocab);
+  fours.go(l, to, a.vocab, [&](f32x4 v, uint32_t i) {
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
       const u64 key = sample_key(v[j], i + j);
       if (v[j] > -INFINITY && key > top) top = key;
     }
-  }
+  });
   top = block_max<kSampleThreads>(top, lds);
   if (t == 0) a.tops[blockIdx.x] = top;
   for (uint32_t i = slice * kSampleThreads + t; i < kCountStride; i += a.slices * kSampleThreads) {
@@ -209,16 +244,15 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs a) {
   u64 top = slice_top(a, row);
   const float* const l = a.logits + (uint64_t)row * a.vocab;
   const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
-  f32x4 next = sample_load(l, from + t * 4, a.vocab);
+  SampleFours fours;
+  fours.load(l, from + t * 4, a.vocab);
   if (!r.good || r.greedy) return;
   for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
   top = block_max<kSampleThreads>(top, lds);
   if (!top) return;
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
   const bool counts = r.k, masses = r.masses();
-  for (uint32_t i = from + t * 4; i < to; i += kSampleThreads * 4) {
-    const f32x4 v = next;
-    next = sample_load(l, i + kSampleThreads * 4, a.vocab);
+  fours.go(l, to, a.vocab, [&](f32x4 v, uint32_t) {
     u64 m[4] = {0, 0, 0, 0};
     if (masses) scale.masses(v, m, false);
 #pragma unroll
@@ -227,7 +261,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs a) {
       if (counts && v[j] > -INFINITY) atomicAdd(&count[bin], 1u);
       if (m[j]) atomicAdd(&mass[bin], m[j]);
     }
-  }
+  });
   __syncthreads();
   u64* const own = a.slice_mass + (uint64_t)blockIdx.x * kSampleBins;
   for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) {
@@ -244,8 +278,10 @@ struct SampleBorder {
   uint32_t p_first, p_last;     // top-p's is one of these
   u64 p_before;                 // mass before the first of them
   uint32_t m_first, m_last;     // min-p's is one of these
-  __device__ uint32_t certain() const { return min(min(k_bin, p_first), m_first); }  // bins below it are kept
+  bool small;                   // all of top-k is listed
+  __device__ uint32_t certain() const { return small ? 0u : min(min(k_bin, p_first), m_first); }  // bins below it are kept
   __device__ bool listed(uint32_t bin) const {
+    if (small) return bin <= k_bin;
     return bin == k_bin || (bin >= p_first && bin <= p_last) || (bin >= m_first && bin <= m_last);
   }
 };
@@ -290,9 +326,9 @@ __device__ __forceinline__ SampleBorder sample_border(const SampleRow& r, const 
   u64 n = own[0];
   share.before = own[1];
   if (t == 0) {
-    lds->b = SampleBorder{kNoBin, 0, all[1], kNoBin, kNoBin, 0, kNoBin, kNoBin};
+    lds->b = SampleBorder{kNoBin, 0, all[1], kNoBin, kNoBin, 0, kNoBin, kNoBin, r.small()};
     lds->k_own = 0;
-    if (r.min_p > 0.0 && !scale.infinite) {
+    if (!r.small() && r.min_p > 0.0 && !scale.infinite) {
       // The last logit that min-p keeps, to within more than its roundings.
       const double x = log(r.min_p), at = scale.max + x / r.inv_t, off = (fabs(scale.max) + fabs(at)) * 0x1p-22 + fabs(x / r.inv_t) * 0x1p-40;
       lds->b.m_first = sample_bin(scale.top, (float)(at + off));
@@ -315,7 +351,7 @@ __device__ __forceinline__ SampleBorder sample_border(const SampleRow& r, const 
     }
     __syncthreads();
   }
-  if (r.by_mass()) {
+  if (r.by_mass() && !r.small()) {
     const u64 lo = share_of(r.top_p, lds->b.k_mass), hi = share_of(r.top_p, lds->b.k_mass + lds->k_own);
     u64 w = share.before;
 #pragma unroll
@@ -350,7 +386,8 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   share.load(a, row);
   const float* const l = a.logits + (uint64_t)row * a.vocab;
   const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
-  f32x4 next = sample_load(l, from + t * 4, a.vocab);
+  SampleFours fours;
+  fours.load(l, from + t * 4, a.vocab);
   if (!r.good || r.greedy) return;
   top = block_max<kSampleThreads>(top, lds);
   if (!top) return;
@@ -368,9 +405,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
     for (uint32_t i = t; i < certain; i += kSampleThreads) sum += own[i];
   }
   // Nothing to list: the slice need not be read.
-  for (uint32_t i = from + t * 4; i < (certain < kNoBin ? to : 0u); i += kSampleThreads * 4) {
-    const f32x4 v = next;
-    next = sample_load(l, i + kSampleThreads * 4, a.vocab);
+  fours.go(l, certain < kNoBin ? to : 0u, a.vocab, [&](f32x4 v, uint32_t i) {
     uint32_t bin[4];
     bool sure = false;
 #pragma unroll
@@ -378,7 +413,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
       bin[j] = sample_bin(scale.top, v[j]);
       sure |= bin[j] < certain;
     }
-    if (!masses && __any(sure)) {
+    if (!masses && __any(sure)) {  // top-k alone
       u64 m[4];
       scale.masses(v, m, false);
 #pragma unroll
@@ -394,7 +429,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
           list[atomicAdd(count, 1u)] = sample_key(v[j], i + j);
       }
     }
-  }
+  });
   u64 all;
   block_before<kSampleThreads>(sum, &all, lds);
   if (t == 0) a.kept[blockIdx.x] = all;
@@ -421,7 +456,7 @@ struct SampleList {
   }
   // Masses of keys held by all filters but min-p, which is asked where there is one.
   __device__ u64 kept(uint32_t i, const SampleScale& scale) const {
-    return scale.min_p > 0.0 ? mass_of(key(i), scale, true) : mass(i, scale);
+    return scale.least > 0.0 ? mass_of(key(i), scale, true) : mass(i, scale);
   }
   __device__ u64 mass(uint32_t i, const SampleScale& scale) const { return held() ? masses[i] : mass_of(list[i], scale, false); }
 };
@@ -432,9 +467,9 @@ struct SampleList {
 struct SamplePlaces {
   u64 thr;              // only keys from it on
   float max;
-  uint32_t bin, first;  // the bin's largest logit in the list
+  uint32_t bin, first;  // kNoBin: all of them; the bin's largest logit in the list
   uint32_t token_bits;
-  __device__ bool in(u64 key) const { return key >= thr && sample_bin(max, ord_float((uint32_t)(key >> 32))) == bin; }
+  __device__ bool in(u64 key) const { return bin == kNoBin || (key >= thr && sample_bin(max, ord_float((uint32_t)(key >> 32))) == bin); }
   __device__ u64 place(u64 key) const { return (u64)(first - (uint32_t)(key >> 32)) << token_bits | key_token(key); }
   __device__ u64 key(u64 p) const {
     return (u64)(first - (uint32_t)(p >> token_bits)) << 32 | (uint32_t)~(uint32_t)(p & ((1ull << token_bits) - 1));
@@ -544,7 +579,29 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
       list.masses[i] = SampleList::mass_of(key, scale, false);
     }
   __syncthreads();
-  if (b.k_bin == kNoBin && b.p_first == kNoBin) {
+  SamplePlaces s;
+  s.thr = 0;
+  s.max = scale.top;
+  s.token_bits = a.vocab > 1 ? 32 - __builtin_clz(a.vocab - 1) : 0;
+  if (b.small && list.n > kPickThreads) {
+    // More tokens in top-k's bin than there is room for: the k largest alone.
+    s.bin = kNoBin;
+    const u64 least = sample_select<false>(list, s, scale, r.k, &select_lds);
+    if (t == 0) the_one = 0;
+    __syncthreads();
+    for (uint32_t i = t; i < list.n; i += kPickThreads) {
+      const u64 key = list.key(i);
+      if (key >= least) select_lds.weight[atomicAdd(&the_one, 1u)] = key;
+    }
+    __syncthreads();
+    list.n = r.k;
+    if (t < list.n) {
+      list.keys[t] = select_lds.weight[t];
+      list.masses[t] = SampleList::mass_of(list.keys[t], scale, false);
+    }
+    __syncthreads();
+  }
+  if (!b.small && b.k_bin == kNoBin && b.p_first == kNoBin) {
     // No border but min-p's.
   } else if (list.n <= kPickThreads) {
     // Few keys: sorted by counting the larger ones, which puts the bins in order
@@ -560,25 +617,21 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     __syncthreads();
     const u64 mine = t < list.n ? list.keys[t] : 0ull, here = t < list.n ? list.masses[t] : 0ull;
     const uint32_t bin = t < list.n ? sample_bin(scale.top, ord_float((uint32_t)(mine >> 32))) : kNoBin;
-    // Where top-k's bin begins in the list (others with min-p's alone may lie behind it: none are kept).
-    const uint32_t k_from = (uint32_t)block_sum<kPickThreads>(bin < b.k_bin, lds);
-    uint32_t last = list.n;  // keys from it on are not kept
-    u64 sums[2] = {bin >= b.p_first && bin <= b.p_last ? here : 0ull, 0}, all[2];
-    if (b.k_bin != kNoBin) last = k_from + (r.k - b.k_before);
-    sums[1] = t >= k_from && t < last && b.k_bin != kNoBin ? here : 0ull;
+    // Keys from `last` on are not top-k's.
+    const uint32_t k_from = b.small ? 0u : (uint32_t)block_sum<kPickThreads>(bin < b.k_bin, lds);
+    uint32_t last = b.small ? min(r.k, list.n) : b.k_bin != kNoBin ? k_from + (r.k - b.k_before) : list.n;
+    const bool in_k = t < last && t >= k_from && (b.small || b.k_bin != kNoBin);
+    u64 sums[2] = {b.small || (bin >= b.p_first && bin <= b.p_last) ? here : 0ull, in_k ? here : 0ull}, all[2];
     block_before<kPickThreads, 2>(sums, all, border_lds.part);
     if (r.by_mass()) {
       // Kept: with less mass before it than top-p asks for.
-      const u64 target = share_of(r.top_p, b.k_mass + all[1]);
-      const bool kept = t < last && (bin < b.p_first || (bin <= b.p_last && b.p_before + sums[0] < target));
+      const u64 target = share_of(r.top_p, (b.small ? 0ull : b.k_mass) + all[1]);
+      const bool under = (b.small ? 0ull : b.p_before) + sums[0] < target;
+      const bool kept = t < last && (b.small ? under : bin < b.p_first || (bin <= b.p_last && under));
       last = (uint32_t)block_sum<kPickThreads>(kept, lds);
     }
     thr = list.keys[last - 1];  // the first key of top-k's or top-p's bin is kept
   } else {
-    SamplePlaces s;
-    s.thr = 0;
-    s.max = scale.top;
-    s.token_bits = a.vocab > 1 ? 32 - __builtin_clz(a.vocab - 1) : 0;
     u64 own = 0;  // mass of top-k's bin that is kept
     if (b.k_bin != kNoBin) {
       s.bin = b.k_bin;
@@ -682,7 +735,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
         for (uint32_t j = 0; j < 4; ++j) {
           if (target >= at && target < at + m[j]) {
             a.tokens[row] = (int32_t)(i + lane * 4 + j);
-            if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(v[j]) - log((double)total / a.unit));
+            if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(v[j]) - log(__builtin_ldexp((double)total, -a.up)));
           }
           at += m[j];
         }
@@ -712,7 +765,7 @@ uint64_t sample_workspace(uint32_t n, uint32_t vocab, SampleArgs* a, uint8_t* ba
     while (((uint64_t)1 << bits) < vocab) ++bits;
     a->slice = slice;
     a->slices = slices;
-    a->unit = (double)((uint64_t)1 << (bits < 11 ? 51 : 62 - bits));
+    a->up = bits < 11 ? 51 : 62 - (int)bits;
     a->tops = (u64*)base;
     a->kept = (u64*)(base + tops);
     a->mass = (u64*)(base + 2 * tops);
