@@ -35,9 +35,10 @@ constexpr uint32_t kCountStride = kSampleBins + 4;
 constexpr uint32_t kNoBin = kSampleBins;
 constexpr uint32_t kSmallK = 448;  // with the tokens that share its bin, mostly, a block's threads
 
-// Bin of a logit, 0 the largest's.
+// Bin of a logit, 0 the largest's; least distance of a bin (not of 0).
+constexpr uint32_t kFirst = (127 - 5) << 7;  // the upper bits of 1/32
+__device__ __forceinline__ float sample_bin_from(uint32_t bin) { return __uint_as_float((kFirst + bin) << 16); }
 __device__ __forceinline__ uint32_t sample_bin(float max, float l) {
-  constexpr uint32_t kFirst = (127 - 5) << 7;  // the upper bits of 1/32
   const float d = max - l;                     // NaN where both are infinite: 0
   const uint32_t b = d > 0.f ? __float_as_uint(d) >> 16 : 0u;
   return b < kFirst ? 0u : min(b - kFirst, kSampleBins - 1);
@@ -179,30 +180,38 @@ __device__ __forceinline__ f32x4 sample_load(const float* row, uint32_t at, uint
   return v;
 }
 
-// A thread's fours of a slice in turn, two thousands at a time, the next two on
-// their way (16 waves of a CU and 1 KB each would be 2 TB/s).
-constexpr uint32_t kAhead = 2;
+// A thread's fours of a slice, a thousand logits of the block at a time, two of
+// these on their way. Kernels that follow one another go through a slice in
+// turns (BACK: from its end): what an XCD's L2 still holds is what the one before
+// read last.
+template <bool BACK>
 struct SampleFours {
+  static constexpr uint32_t kAhead = 2, kStep = kSampleThreads * 4;
+  const float* row;
+  uint32_t vocab, first, steps, at;  // this thread's place in the first step; steps of the slice
   f32x4 next[kAhead];
-  uint32_t at;
-  __device__ __forceinline__ void load(const float* row, uint32_t from, uint32_t vocab) {
-    at = from;
+  __device__ __forceinline__ uint32_t place(uint32_t i) const { return first + (BACK ? steps - 1 - i : i) * kStep; }
+  __device__ __forceinline__ SampleFours(const SampleArgs& a, uint32_t r, uint32_t slice)
+      : row(a.logits + (uint64_t)r * a.vocab), vocab(a.vocab), first(slice * a.slice + threadIdx.x * 4),
+        steps((min(a.slice, a.vocab - slice * a.slice) + kStep - 1) / kStep), at(0) {
 #pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j) next[j] = sample_load(row, from + j * kSampleThreads * 4, vocab);
+    for (uint32_t j = 0; j < kAhead; ++j) next[j] = load(j);
   }
-  // each(logits, first token), from `from` + 4 t on as loaded up to `to`.
+  __device__ __forceinline__ f32x4 load(uint32_t i) const {
+    return i < steps ? sample_load(row, place(i), vocab) : f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  }
   template <class F>
-  __device__ __forceinline__ void go(const float* row, uint32_t to, uint32_t vocab, F each) {
-    for (; at < to; at += kAhead * kSampleThreads * 4) {
+  __device__ __forceinline__ void go(F each) {  // each(logits, first token)
+    for (; at < steps; at += kAhead) {
       f32x4 v[kAhead];
 #pragma unroll
       for (uint32_t j = 0; j < kAhead; ++j) {
         v[j] = next[j];
-        next[j] = sample_load(row, at + (kAhead + j) * kSampleThreads * 4, vocab);
+        next[j] = load(at + kAhead + j);
       }
 #pragma unroll
       for (uint32_t j = 0; j < kAhead; ++j)
-        if (at + j * kSampleThreads * 4 < to) each(v[j], at + j * kSampleThreads * 4);
+        if (at + j < steps) each(v[j], place(at + j));
     }
   }
 };
@@ -215,12 +224,9 @@ __device__ __forceinline__ u64 slice_top(const SampleArgs& a, uint32_t row) {
 __global__ __launch_bounds__(kSampleThreads) void k_sample_top(SampleArgs a) {
   __shared__ u64 lds[4];
   const uint32_t t = threadIdx.x, row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
-  const float* const l = a.logits + (uint64_t)row * a.vocab;
   u64 top = 0;
-  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
-  SampleFours fours;
-  fours.load(l, from + t * 4, a.vocab);
-  fours.go(l, to, a.vocab, [&](f32x4 v, uint32_t i) {
+  SampleFours<false> fours(a, row, slice);
+  fours.go([&](f32x4 v, uint32_t i) {
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
       const u64 key = sample_key(v[j], i + j);
@@ -242,17 +248,14 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs a) {
   const uint32_t t = threadIdx.x, row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const SampleRow r = sample_row(a, row);
   u64 top = slice_top(a, row);
-  const float* const l = a.logits + (uint64_t)row * a.vocab;
-  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
-  SampleFours fours;
-  fours.load(l, from + t * 4, a.vocab);
+  SampleFours<true> fours(a, row, slice);
   if (!r.good || r.greedy) return;
   for (uint32_t i = t; i < kSampleBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
   top = block_max<kSampleThreads>(top, lds);
   if (!top) return;
   const SampleScale scale(a, r, (uint32_t)(top >> 32));
   const bool counts = r.k, masses = r.masses();
-  fours.go(l, to, a.vocab, [&](f32x4 v, uint32_t) {
+  fours.go([&](f32x4 v, uint32_t) {
     u64 m[4] = {0, 0, 0, 0};
     if (masses) scale.masses(v, m, false);
 #pragma unroll
@@ -280,6 +283,12 @@ struct SampleBorder {
   uint32_t m_first, m_last;     // min-p's is one of these
   bool small;                   // all of top-k is listed
   __device__ uint32_t certain() const { return small ? 0u : min(min(k_bin, p_first), m_first); }  // bins below it are kept
+  // Bins from it on are neither kept nor listed.
+  __device__ uint32_t end() const {
+    uint32_t e = k_bin + 1;  // top-p's border is not behind it
+    if (k_bin == kNoBin) e = p_first == kNoBin ? 0u : p_last + 1;
+    return min(max(e, m_first == kNoBin ? 0u : m_last + 1), kNoBin);
+  }
   __device__ bool listed(uint32_t bin) const {
     if (small) return bin <= k_bin;
     return bin == k_bin || (bin >= p_first && bin <= p_last) || (bin >= m_first && bin <= m_last);
@@ -384,10 +393,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   u64 top = slice_top(a, row);
   SampleShare<kSampleThreads> share;
   share.load(a, row);
-  const float* const l = a.logits + (uint64_t)row * a.vocab;
-  const uint32_t from = slice * a.slice, to = min(a.vocab, from + a.slice);
-  SampleFours fours;
-  fours.load(l, from + t * 4, a.vocab);
+  SampleFours<false> fours(a, row, slice);
   if (!r.good || r.greedy) return;
   top = block_max<kSampleThreads>(top, lds);
   if (!top) return;
@@ -404,8 +410,19 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
     const u64* const own = a.slice_mass + (uint64_t)blockIdx.x * kSampleBins;
     for (uint32_t i = t; i < certain; i += kSampleThreads) sum += own[i];
   }
-  // Nothing to list: the slice need not be read.
-  fours.go(l, certain < kNoBin ? to : 0u, a.vocab, [&](f32x4 v, uint32_t i) {
+  // Distances of what has to be looked at (most logits are behind it); nothing
+  // to list: the slice need not be read.
+  const uint32_t last = b.end();
+  const float near = !masses || certain == 0 ? -INFINITY : sample_bin_from(certain);
+  const float far = scale.infinite || last == kNoBin || b.small && b.k_bin == kNoBin ? INFINITY : sample_bin_from(last);
+  if (certain < kNoBin) fours.go([&](f32x4 v, uint32_t i) {
+    bool look = scale.infinite;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const float d = scale.top - v[j];
+      look |= d >= near && d < far;
+    }
+    if (!__any(look)) return;
     uint32_t bin[4];
     bool sure = false;
 #pragma unroll
@@ -419,15 +436,28 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) sum += bin[j] < certain ? m[j] : 0ull;
     }
+    // A place for each key to list, one addition per wave.
+    u64 hits[4];
+    uint32_t n = 0;
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      if (bin[j] >= certain && b.listed(bin[j]) && v[j] > -INFINITY) {
-        const uint32_t at = atomicAdd(&n_held, 1u);
-        if (at < kListHeld)
-          held[at] = sample_key(v[j], i + j);
+      hits[j] = __ballot(bin[j] >= certain && b.listed(bin[j]) && v[j] > -INFINITY);
+      n += (uint32_t)__popcll(hits[j]);
+    }
+    if (!n) return;
+    uint32_t at = 0;
+    if ((t & 63) == 0) at = atomicAdd(&n_held, n);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      if (hits[j] >> (t & 63) & 1) {
+        const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits[j], 0u));
+        if (to < kListHeld)
+          held[to] = sample_key(v[j], i + j);
         else
           list[atomicAdd(count, 1u)] = sample_key(v[j], i + j);
       }
+      at += (uint32_t)__popcll(hits[j]);
     }
   });
   u64 all;
