@@ -437,7 +437,7 @@ hipError_t launch_attn_i8(const AttnArgs& a, bool q_bf16, hipStream_t st);
 hipError_t launch_attn_join(const AttnArgs& a, hipStream_t st);
 // Sampling (sample.hip).
 constexpr uint32_t kSampleMaxRows = 65535, kSampleMaxVocab = 1u << 24;
-constexpr uint32_t kSampleBins = 1536;  // of a logit's distance from the row's largest
+constexpr uint32_t kSampleBins = 640;  // of a logit's distance from the row's largest
 struct SampleArgs {
   const float *logits, *temperature;  // [n, vocab]; [n] or null, as the others
   const int32_t* top_k;

@@ -11,8 +11,8 @@
 // A logit becomes 32 bits in an order that integers compare, and a key with the
 // complement of its token below it, so keys are unique and the order of the
 // filters is that of falling keys. Bins are by the distance d from the row's
-// largest logit (a rounded difference, but it never falls as logits fall): 128 to
-// every power of two of d from 1/32 to 128, so that they are finest where the
+// largest logit (a rounded difference, but it never falls as logits fall): 64 to
+// every power of two of d from 1/16 to 64, so that they are finest where the
 // mass is. All three filters keep a first part of the order: what decides is one
 // key, and only the bins around it have to be looked into.
 //
@@ -36,11 +36,11 @@ constexpr uint32_t kNoBin = kSampleBins;
 constexpr uint32_t kSmallK = 448;  // with the tokens that share its bin, mostly, a block's threads
 
 // Bin of a logit, 0 the largest's; least distance of a bin (not of 0).
-constexpr uint32_t kFirst = (127 - 5) << 7;  // the upper bits of 1/32
-__device__ __forceinline__ float sample_bin_from(uint32_t bin) { return __uint_as_float((kFirst + bin) << 16); }
+constexpr uint32_t kFirst = (127 - 4) << 6;  // the upper bits of 1/16
+__device__ __forceinline__ float sample_bin_from(uint32_t bin) { return __uint_as_float((kFirst + bin) << 17); }
 __device__ __forceinline__ uint32_t sample_bin(float max, float l) {
   const float d = max - l;                     // NaN where both are infinite: 0
-  const uint32_t b = d > 0.f ? __float_as_uint(d) >> 16 : 0u;
+  const uint32_t b = d > 0.f ? __float_as_uint(d) >> 17 : 0u;
   return b < kFirst ? 0u : min(b - kFirst, kSampleBins - 1);
 }
 
