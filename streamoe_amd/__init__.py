@@ -275,13 +275,17 @@ class KvCache:
 def _row_stride(t, types, n, width, device):
     """Elements from a row of t to the next, if t holds n rows of `width` dense
     elements of `types` on `device` ([n, width] or [n, heads, dim]); else None."""
-    if t is None or t.dtype not in types or t.get_device() != device or t.dim() not in (2, 3) or t.shape[0] < n:
+    if t is None or t.dtype not in types or t.get_device() != device:
         return None
-    if t.dim() == 2:
-        dense = t.shape[1] == width and (t.stride(1) == 1 or width == 1)
+    shape, step = t.shape, t.stride()
+    if len(shape) == 3:
+        _, heads, dim = shape
+        dense = heads * dim == width and step[2] == 1 and (heads == 1 or step[1] == dim)
     else:
-        dense = t.shape[1] * t.shape[2] == width and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2])
-    return None if not dense else t.stride(0) if n > 1 else width
+        dense = len(shape) == 2 and shape[1] == width and step[1] == 1
+    if not dense or shape[0] < n:
+        return None
+    return step[0] if n > 1 else width
 
 
 @dataclass
@@ -570,9 +574,9 @@ class Kernels:
 
     def _kv_rows(self, cc, k, v, n_tokens):
         """Row stride of k and v, or None where they are no rows of one kind."""
-        width = cc.n_heads * cc.head_dim
-        step = _row_stride(k, _types("f32_bf16"), n_tokens, width, self.device)
-        if step is None or k.dtype != v.dtype or _row_stride(v, _types("f32_bf16"), n_tokens, width, self.device) != step:
+        width, either = cc.n_heads * cc.head_dim, _types("f32_bf16")
+        step = _row_stride(k, either, n_tokens, width, self.device)
+        if step is None or v is None or k.dtype != v.dtype or _row_stride(v, either, n_tokens, width, self.device) != step:
             return None
         return step
 
