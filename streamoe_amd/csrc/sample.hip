@@ -470,25 +470,43 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   for (uint32_t i = t; i < n; i += kSampleThreads) list[list_at + i] = held[i];
 }
 
-// The row's list: its first keys in LDS with their masses, if it has no more.
-constexpr uint32_t kPickHeld = 4096, kPickBins = (kSampleBins + kPickThreads - 1) / kPickThreads;
+// The row's list: with their masses in registers, up to eight keys of a thread;
+// a longer one (ties, logits past 64 from the largest) out of memory, again and
+// again.
+constexpr uint32_t kPickEach = 8, kPickBins = (kSampleBins + kPickThreads - 1) / kPickThreads;
 struct SampleList {
   const u64* list;
-  u64 *keys, *masses;  // LDS
   uint32_t n;
-  __device__ bool held() const { return n <= kPickHeld; }
-  __device__ u64 key(uint32_t i) const { return held() ? keys[i] : list[i]; }
-  // A key's mass; 0 where min_p does not keep it (if `kept`).
-  __device__ static u64 mass_of(u64 key, const SampleScale& scale, bool kept_only) {
-    bool kept;
-    const u64 m = scale.mass(ord_float((uint32_t)(key >> 32)), &kept);
-    return kept || !kept_only ? m : 0ull;
+  u64 keys[kPickEach], masses[kPickEach];
+  __device__ static float logit(u64 key) { return ord_float((uint32_t)(key >> 32)); }
+  __device__ bool held() const { return n <= kPickEach * kPickThreads; }
+  __device__ __forceinline__ void hold(const SampleScale& scale) {  // keys[0] is there
+    if (!held()) return;
+#pragma unroll
+    for (uint32_t h = 0; h < kPickEach; h += 4) {
+      if (n <= h * kPickThreads) break;
+#pragma unroll
+      for (uint32_t j = h ? h : 1; j < h + 4; ++j) keys[j] = threadIdx.x + j * kPickThreads < n ? list[threadIdx.x + j * kPickThreads] : 0ull;
+      u64 m[4];
+      scale.masses(f32x4{logit(keys[h]), logit(keys[h + 1]), logit(keys[h + 2]), logit(keys[h + 3])}, m, false);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) masses[h + j] = m[j];
+    }
   }
-  // Masses of keys held by all filters but min-p, which is asked where there is one.
-  __device__ u64 kept(uint32_t i, const SampleScale& scale) const {
-    return scale.least > 0.0 ? mass_of(key(i), scale, true) : mass(i, scale);
+  // f(key, mass) of this thread's.
+  template <class F>
+  __device__ __forceinline__ void each(const SampleScale& scale, F f) const {
+    if (held()) {
+#pragma unroll
+      for (uint32_t j = 0; j < kPickEach; ++j)
+        if (threadIdx.x + j * kPickThreads < n) f(keys[j], masses[j]);
+    } else {
+      for (uint32_t i = threadIdx.x; i < n; i += kPickThreads) {
+        bool kept;
+        f(list[i], scale.mass(logit(list[i]), &kept));
+      }
+    }
   }
-  __device__ u64 mass(uint32_t i, const SampleScale& scale) const { return held() ? masses[i] : mass_of(list[i], scale, false); }
 };
 
 // Its entries of one bin, in order; a place is the distance from `first` (in
@@ -522,10 +540,9 @@ __device__ u64 sample_select(const SampleList& list, SamplePlaces s, const Sampl
   const uint32_t t = threadIdx.x;
   // What the bin's entries span.
   u64 hi = 0, lo = 0;  // lo: of complements
-  for (uint32_t i = t; i < list.n; i += kPickThreads) {
-    const u64 key = list.key(i);
+  list.each(scale, [&](u64 key, u64) {
     if (s.in(key)) hi = max(hi, key), lo = max(lo, ~key);
-  }
+  });
   hi = block_max<kPickThreads>(hi, lds->part);
   lo = ~block_max<kPickThreads>(lo, lds->part);
   s.first = (uint32_t)(hi >> 32);
@@ -538,15 +555,13 @@ __device__ u64 sample_select(const SampleList& list, SamplePlaces s, const Sampl
     lds->weight[t] = 0;
     lds->count[t] = 0;
     __syncthreads();
-    for (uint32_t i = t; i < list.n; i += kPickThreads) {
-      const u64 key = list.key(i);
-      if (!s.in(key)) continue;
+    list.each(scale, [&](u64 key, u64 mass) {
       const u64 p = s.place(key);
-      if (p >> (shift + width) != prefix) continue;
+      if (!s.in(key) || p >> (shift + width) != prefix) return;
       const uint32_t digit = (uint32_t)(p >> shift) & ((1u << width) - 1);
       atomicAdd(&lds->count[digit], 1u);
-      if constexpr (MASS) atomicAdd(&lds->weight[digit], list.mass(i, scale));
-    }
+      if constexpr (MASS) atomicAdd(&lds->weight[digit], mass);
+    });
     __syncthreads();
     const u64 w = MASS ? lds->weight[t] : lds->count[t];
     u64 all;
@@ -564,16 +579,15 @@ __device__ u64 sample_select(const SampleList& list, SamplePlaces s, const Sampl
     __syncthreads();
   }
   // One place has these digits.
-  for (uint32_t i = t; i < list.n; i += kPickThreads) {
-    const u64 key = list.key(i);
+  list.each(scale, [&](u64 key, u64) {
     if (s.in(key) && s.place(key) >> shift == prefix) lds->found = key;
-  }
+  });
   __syncthreads();
   return lds->found;
 }
 
 __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
-  extern __shared__ __attribute__((aligned(16))) u64 held[];  // kPickHeld keys, as many masses
+  __shared__ u64 keys[kPickThreads], masses[kPickThreads];
   __shared__ u64 lds[kPickThreads / 64];
   __shared__ SampleBorderLds border_lds;
   __shared__ SelectLds select_lds;
@@ -582,9 +596,11 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   __shared__ u64 the_rest;
   const uint32_t t = threadIdx.x, row = blockIdx.x;
   const SampleRow r = sample_row(a, row);
-  SampleList list = {a.list + (uint64_t)row * a.vocab, held, held + kPickHeld, a.count[(uint64_t)row * kCountStride + kSampleBins]};
+  SampleList list;
+  list.list = a.list + (uint64_t)row * a.vocab;
+  list.n = a.count[(uint64_t)row * kCountStride + kSampleBins];
   const u64 kept_own = t < a.slices ? a.kept[(uint64_t)row * a.slices + t] : 0ull;
-  const u64 first_key = t < a.vocab ? list.list[t] : 0ull;  // if it is one
+  list.keys[0] = t < a.vocab ? list.list[t] : 0ull;  // if it is one
   SampleShare<kPickThreads> share;
   share.load(a, row);
   const u64 top = block_max<kPickThreads>(slice_top(a, row), lds);
@@ -602,13 +618,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   if (t < a.slices) kept_of[t] = kept_own;
   const SampleBorder b = sample_border<kPickThreads>(r, scale, &border_lds, share);
   if (b.certain() == kNoBin) list.n = 0;
-  if (list.held())
-    for (uint32_t i = t; i < list.n; i += kPickThreads) {
-      const u64 key = i < kPickThreads ? first_key : list.list[i];
-      list.keys[i] = key;
-      list.masses[i] = SampleList::mass_of(key, scale, false);
-    }
-  __syncthreads();
+  list.hold(scale);
   SamplePlaces s;
   s.thr = 0;
   s.max = scale.top;
@@ -619,16 +629,14 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     const u64 least = sample_select<false>(list, s, scale, r.k, &select_lds);
     if (t == 0) the_one = 0;
     __syncthreads();
-    for (uint32_t i = t; i < list.n; i += kPickThreads) {
-      const u64 key = list.key(i);
-      if (key >= least) select_lds.weight[atomicAdd(&the_one, 1u)] = key;
-    }
+    list.each(scale, [&](u64 key, u64) {
+      if (key >= least) keys[atomicAdd(&the_one, 1u)] = key;
+    });
     __syncthreads();
     list.n = r.k;
-    if (t < list.n) {
-      list.keys[t] = select_lds.weight[t];
-      list.masses[t] = SampleList::mass_of(list.keys[t], scale, false);
-    }
+    list.keys[0] = t < list.n ? keys[t] : 0ull;
+    bool kept;
+    list.masses[0] = scale.mass(SampleList::logit(list.keys[0]), &kept);
     __syncthreads();
   }
   if (!b.small && b.k_bin == kNoBin && b.p_first == kNoBin) {
@@ -636,17 +644,20 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   } else if (list.n <= kPickThreads) {
     // Few keys: sorted by counting the larger ones, which puts the bins in order
     // and top-k's last.
-    const u64 key = t < list.n ? list.keys[t] : 0ull, mass = t < list.n ? list.masses[t] : 0ull;
+    const u64 key = list.keys[0];
+    keys[t] = key;
+    __syncthreads();
     uint32_t rank = 0;
-    for (uint32_t i = 0; i < list.n; ++i) rank += list.keys[i] > key;
+#pragma unroll 8
+    for (uint32_t i = 0; i < list.n; ++i) rank += keys[i] > key;
     __syncthreads();
     if (t < list.n) {
-      list.keys[rank] = key;
-      list.masses[rank] = mass;
+      keys[rank] = key;
+      masses[rank] = list.masses[0];
     }
     __syncthreads();
-    const u64 mine = t < list.n ? list.keys[t] : 0ull, here = t < list.n ? list.masses[t] : 0ull;
-    const uint32_t bin = t < list.n ? sample_bin(scale.top, ord_float((uint32_t)(mine >> 32))) : kNoBin;
+    const u64 mine = t < list.n ? keys[t] : 0ull, here = t < list.n ? masses[t] : 0ull;
+    const uint32_t bin = t < list.n ? sample_bin(scale.top, SampleList::logit(mine)) : kNoBin;
     // Keys from `last` on are not top-k's.
     const uint32_t k_from = b.small ? 0u : (uint32_t)block_sum<kPickThreads>(bin < b.k_bin, lds);
     uint32_t last = b.small ? min(r.k, list.n) : b.k_bin != kNoBin ? k_from + (r.k - b.k_before) : list.n;
@@ -660,7 +671,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
       const bool kept = t < last && (b.small ? under : bin < b.p_first || (bin <= b.p_last && under));
       last = (uint32_t)block_sum<kPickThreads>(kept, lds);
     }
-    thr = list.keys[last - 1];  // the first key of top-k's or top-p's bin is kept
+    thr = keys[last - 1];  // the first key of top-k's or top-p's bin is kept
   } else {
     u64 own = 0;  // mass of top-k's bin that is kept
     if (b.k_bin != kNoBin) {
@@ -668,8 +679,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
       thr = s.thr = sample_select<false>(list, s, scale, r.k - b.k_before, &select_lds);
       if (r.by_mass()) {
         u64 sum = 0;
-        for (uint32_t i = t; i < list.n; i += kPickThreads)
-          if (s.in(list.key(i))) sum += list.mass(i, scale);
+        list.each(scale, [&](u64 key, u64 mass) { sum += s.in(key) ? mass : 0ull; });
         own = block_sum<kPickThreads>(sum, lds);
       }
     }
@@ -693,12 +703,11 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   }
   // Every slice's kept mass: what is certain, and what of the list is kept.
   __syncthreads();
-  for (uint32_t i = t; i < list.n; i += kPickThreads) {
-    const u64 key = list.key(i);
-    if (key < thr) continue;
-    const u64 m = list.kept(i, scale);
-    if (m) atomicAdd(&kept_of[key_token(key) / a.slice], m);
-  }
+  list.each(scale, [&](u64 key, u64 mass) {
+    bool kept = true;
+    if (key >= thr && scale.least > 0.0) scale.mass(SampleList::logit(key), &kept);  // min-p
+    if (key >= thr && kept && mass) atomicAdd(&kept_of[key_token(key) / a.slice], mass);
+  });
   __syncthreads();
   const u64 own = t < a.slices ? kept_of[t] : 0ull;
   u64 total;
@@ -811,11 +820,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(k_sample_top, grid, block, 0, st, a);
   hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, a);
   hipLaunchKernelGGL(k_sample_list, grid, block, 0, st, a);
-  static std::atomic<uint64_t> raised{0};
-  constexpr uint32_t bytes = 2 * kPickHeld * sizeof(u64);
-  const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(&k_sample_pick), bytes, raised);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k_sample_pick, dim3(a.n), dim3(kPickThreads), bytes, st, a);
+  hipLaunchKernelGGL(k_sample_pick, dim3(a.n), dim3(kPickThreads), 0, st, a);
   return hipGetLastError();
 }
 
