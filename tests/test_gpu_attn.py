@@ -105,6 +105,30 @@ def test_many_rows(kernels, n):
     _check(cache, tok, q, 0.125, 0, got, True)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,bits", [(256, 256, 16, 8), (4096, 1, 16, 16), (480, 240, 32, 16), (4080, 240, 16, 8)])
+def test_many_heads(kernels, heads, kv_heads, dim, bits):
+    rng = np.random.default_rng(heads)
+    cache = Cache([70, 200], kv_heads, dim, bits, 16, seed=heads, spare=1)
+    tok = np.array([(1, 199), (0, 69), (-1, 0), (0, 3)])
+    q = _queries(rng, 4, heads, dim, True)
+    got = _run(kernels, cache, tok, q, 0.25, 0, False, heads)
+    _check(cache, tok, q, 0.25, 0, got, False)
+
+
+def test_the_most_tokens(kernels):
+    """16384 rows: prompts of many sequences in one call, one row in seven padding."""
+    rng = np.random.default_rng(16)
+    lens = [64] * 220
+    cache = Cache(lens, 1, 64, 16, 32, seed=16)
+    tok = np.array([(s, p) for s in range(220) for p in range(64)], np.int64)
+    tok = np.concatenate([tok, np.full((16384 - len(tok), 2), -1)])
+    tok[::7, 0] = -1
+    q = _queries(rng, len(tok), 4, 64, True)
+    got = _run(kernels, cache, tok, q, 0.125, 0, False, 4)
+    some = np.sort(rng.permutation(len(tok))[:700])
+    _check(cache, tok[some], q[some], 0.125, 0, got[some], False)
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("length,page", [(70001, 64), (66000, 16), (65536, 1 << 17)])
 def test_one_long_sequence(kernels, bits, length, page):

@@ -194,6 +194,33 @@ def test_rows_without_a_value_and_bad_numbers(kernels):
             assert tok[i] == want_of(x[i], 1.0, 10, np.float32(0.9), np.float32(0.1), 0.5)[0]
 
 
+def test_the_most_rows(kernels):
+    rng = np.random.default_rng(65)
+    n, V = 65535, 7
+    l = (rng.standard_normal((n, V)) * 2).astype(np.float32)
+    t, k = rng.choice([0.0, 1.0, 2.0], n).astype(np.float32), rng.choice([0, 1, 3], n)
+    p, u = rng.choice([1.0, 0.7], n).astype(np.float32), rng.random(n).astype(np.float32)
+    tok, _ = _run(kernels, l, t, k, p, np.zeros(n), u, V)
+    kernels.sync()
+    for i in rng.permutation(n)[:3000]:
+        a, _, near = want_of(l[i], t[i], k[i], p[i], 0.0, u[i])
+        assert tok[i] == a or near < 1e-9, i
+
+
+@pytest.mark.parametrize("V", [400, 3000, 20000])
+def test_more_ties_than_top_k(kernels, V):
+    """Top-k's bin holds more tokens than a block sorts: a few larger ones, then
+    thousands of equal ones, with every filter."""
+    rng = np.random.default_rng(V)
+    n = 8
+    l = np.full((n, V), 0.5, np.float32)
+    at = rng.permutation(V)[:37]
+    l[:, at] = (2 + rng.random((n, 37))).astype(np.float32)
+    k = [38, 50, 448, 449, 300, 700, 37, 1]
+    p = [1.0, 0.9, 1.0, 1.0, 0.97, 0.99, 0.5, 1.0]
+    _check(kernels, l, np.ones(n), k, p, [0.0, 0.0, 0.0, 0.0, 0.05, 0.0, 0.9, 0.0], rng.random(n), apart=1e-9)
+
+
 def test_the_same_bits_again(kernels):
     rng = np.random.default_rng(12)
     l = np.round(rng.standard_normal((40, 30011)) * 3).astype(np.float32)

@@ -93,6 +93,7 @@ def test_attn(k):  # noqa: F811
     for w in (None, On(64, dtype=torch.uint8, dev=1), On(64, dtype=torch.uint8, step=(2,))):
         _refused(k, lambda: go(w=w))
     _refused(k, lambda: go(tok=_tok(3)))
+    _refused(k, lambda: k.attn_decode(_cache(), *_tok(), q(), 0.1, -1, On(5, 8, 64), 8, 5, ws))
 
 
 def test_sample(k):  # noqa: F811
