@@ -19,8 +19,16 @@
 // A mass e^((logit - max) / T) is f64 and then an integer of 2^-s: sums of
 // integers are the same in any order, so atomics may form them. Masses of whole
 // bins are formed once. A row with a small top-k needs no masses but of those
-// tokens: all of them are listed, and the list sorted (one row with top-k 20: 24
-// -> XX us). A larger top-k alone needs the masses of what it keeps.
+// tokens: all of them are listed, the list is sorted and the token found in it
+// (one row of 151936 with top-k 20: 19 us, with bins of masses and the slice gone
+// through again 24). A larger top-k alone needs the masses of what it keeps.
+//
+// The reads (39 MB of 64 rows of 151936: 8 us) are what a call cannot do without;
+// later passes find most of them in the memory-side cache. What bounds the four
+// is: top, the reads, 9 us at 64 rows; bins, the series in f64 and the additions
+// in LDS, 14; list, three comparisons a logit, 13; pick, one block's chain of
+// loads, scans and selections, 14. A launch in between takes 1.5 (sums in the
+// last block of the one before need no launch, but every block a ticket).
 #include "common.h"
 #include "kernels.h"
 
@@ -380,11 +388,15 @@ __device__ __forceinline__ SampleBorder sample_border(const SampleRow& r, const 
   return b;
 }
 
-// A block gathers its keys in LDS first: one addition to the row's count per
-// block, not per key (thousands to one place are one after another).
+// A block gathers in LDS the keys of all distances that it has to look at, three
+// comparisons a logit, and sorts them out afterwards, a key per thread: masses
+// of what is kept for certain (top-k alone), the list, one addition to the row's
+// count per block (thousands to one place are one after another). Bins, masses
+// and lists a step at a time took 10 us of blocks of wide nuclei (10 thousand
+// logits) instead of 5.
 constexpr uint32_t kListHeld = 2048;
 __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
-  __shared__ u64 lds[4];
+  __shared__ u64 lds[2 * kSampleThreads / 64];
   __shared__ SampleBorderLds border_lds;
   __shared__ u64 held[kListHeld];
   __shared__ uint32_t n_held, list_at;
@@ -410,64 +422,87 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
     const u64* const own = a.slice_mass + (uint64_t)blockIdx.x * kSampleBins;
     for (uint32_t i = t; i < certain; i += kSampleThreads) sum += own[i];
   }
-  // Distances of what has to be looked at (most logits are behind it); nothing
-  // to list: the slice need not be read.
+  // Distances of what has to be looked at (most logits are behind it). Beside
+  // +inf (distances of infinity and NaN) all.
   const uint32_t last = b.end();
-  const float near = !masses || certain == 0 ? -INFINITY : sample_bin_from(certain);
-  const float far = scale.infinite || last == kNoBin || b.small && b.k_bin == kNoBin ? INFINITY : sample_bin_from(last);
+  const float near = !masses || certain == 0 || scale.infinite ? -INFINITY : sample_bin_from(certain);
+  const float far = scale.infinite                                           ? __builtin_nanf("")
+                    : last == kNoBin || (b.small && b.k_bin == kNoBin) ? INFINITY
+                                                                             : sample_bin_from(last);
+  // Nothing to list: the slice need not be read.
   if (certain < kNoBin) fours.go([&](f32x4 v, uint32_t i) {
-    bool look = scale.infinite;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const float d = scale.top - v[j];
-      look |= d >= near && d < far;
-    }
-    if (!__any(look)) return;
-    uint32_t bin[4];
-    bool sure = false;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      bin[j] = sample_bin(scale.top, v[j]);
-      sure |= bin[j] < certain;
-    }
-    if (!masses && __any(sure)) {  // top-k alone
-      u64 m[4];
-      scale.masses(v, m, false);
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) sum += bin[j] < certain ? m[j] : 0ull;
-    }
-    // A place for each key to list, one addition per wave.
     u64 hits[4];
     uint32_t n = 0;
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      hits[j] = __ballot(bin[j] >= certain && b.listed(bin[j]) && v[j] > -INFINITY);
+      const float d = scale.top - v[j];
+      hits[j] = __ballot(!(d < near) && !(d >= far) && v[j] > -INFINITY);
       n += (uint32_t)__popcll(hits[j]);
     }
     if (!n) return;
+    // A place for each, one addition per wave.
     uint32_t at = 0;
     if ((t & 63) == 0) at = atomicAdd(&n_held, n);
     at = __builtin_amdgcn_readfirstlane(at);
+    if (at + n <= kListHeld) {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        if (hits[j] >> (t & 63) & 1)
+          held[__builtin_amdgcn_mbcnt_hi((uint32_t)(hits[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits[j], at))] = sample_key(v[j], i + j);
+        at += (uint32_t)__popcll(hits[j]);
+      }
+      return;
+    }
+    // No room.
+    u64 m[4] = {0, 0, 0, 0};
+    if (!masses && certain) scale.masses(v, m, false);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t place = __builtin_amdgcn_mbcnt_hi((uint32_t)(hits[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits[j], at));
       if (hits[j] >> (t & 63) & 1) {
-        const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits[j], 0u));
-        if (to < kListHeld)
-          held[to] = sample_key(v[j], i + j);
-        else
+        const uint32_t bin = sample_bin(scale.top, v[j]);
+        if (place < kListHeld)
+          held[place] = sample_key(v[j], i + j);
+        else if (bin < certain)
+          sum += m[j];
+        else if (b.listed(bin))
           list[atomicAdd(count, 1u)] = sample_key(v[j], i + j);
       }
       at += (uint32_t)__popcll(hits[j]);
     }
   });
-  u64 all;
-  block_before<kSampleThreads>(sum, &all, lds);
-  if (t == 0) a.kept[blockIdx.x] = all;
-  const uint32_t n = min(n_held, kListHeld);
-  if (!n) return;
-  if (t == 0) list_at = atomicAdd(count, n);
   __syncthreads();
-  for (uint32_t i = t; i < n; i += kSampleThreads) list[list_at + i] = held[i];
+  const uint32_t n = min(n_held, kListHeld);
+  // Where no bin between the first and the last listed one is not, all are.
+  const bool plain = !scale.infinite && (b.small || (masses && (b.k_bin != kNoBin) + (b.p_first != kNoBin) + (b.m_first != kNoBin) == 1));
+  u64 own[2] = {sum, 0}, all[2];
+  if (plain) {
+    if (t == 0 && n) list_at = atomicAdd(count, n);
+  } else {
+    for (uint32_t i = t; i < n; i += kSampleThreads) {
+      const float l = ord_float((uint32_t)(held[i] >> 32));
+      const uint32_t bin = sample_bin(scale.top, l);
+      bool kept;
+      if (bin < certain)
+        own[0] += scale.mass(l, &kept);
+      else
+        own[1] += b.listed(bin);
+    }
+  }
+  block_before<kSampleThreads, 2>(own, all, lds);
+  if (t == 0) a.kept[blockIdx.x] = all[0];
+  if (plain) {
+    for (uint32_t i = t; i < n; i += kSampleThreads) list[list_at + i] = held[i];
+    return;
+  }
+  if (!all[1]) return;
+  if (t == 0) list_at = atomicAdd(count, (uint32_t)all[1]);
+  __syncthreads();
+  uint32_t to = list_at + (uint32_t)own[1];
+  for (uint32_t i = t; i < n; i += kSampleThreads) {
+    const uint32_t bin = sample_bin(scale.top, ord_float((uint32_t)(held[i] >> 32)));
+    if (bin >= certain && b.listed(bin)) list[to++] = held[i];
+  }
 }
 
 // The row's list: with their masses in registers, up to eight keys of a thread;
@@ -535,8 +570,8 @@ struct SelectLds {
 };
 // Key of the first place up to which the weights (masses, or 1 each) add up to
 // `target` or more, digit after digit of the places from the top; there is one.
-template <bool MASS>
-__device__ u64 sample_select(const SampleList& list, SamplePlaces s, const SampleScale& scale, u64 target, SelectLds* lds) {
+__device__ __forceinline__ u64 sample_select(const SampleList& list, SamplePlaces s, const SampleScale& scale, u64 target, bool by_mass,
+                                             SelectLds* lds) {
   const uint32_t t = threadIdx.x;
   // What the bin's entries span.
   u64 hi = 0, lo = 0;  // lo: of complements
@@ -560,10 +595,10 @@ __device__ u64 sample_select(const SampleList& list, SamplePlaces s, const Sampl
       if (!s.in(key) || p >> (shift + width) != prefix) return;
       const uint32_t digit = (uint32_t)(p >> shift) & ((1u << width) - 1);
       atomicAdd(&lds->count[digit], 1u);
-      if constexpr (MASS) atomicAdd(&lds->weight[digit], mass);
+      if (by_mass) atomicAdd(&lds->weight[digit], mass);
     });
     __syncthreads();
-    const u64 w = MASS ? lds->weight[t] : lds->count[t];
+    const u64 w = by_mass ? lds->weight[t] : lds->count[t];
     u64 all;
     const u64 before = block_before<kPickThreads>(w, &all, lds->part);
     if (before < target && target <= before + w) {
@@ -586,8 +621,20 @@ __device__ u64 sample_select(const SampleList& list, SamplePlaces s, const Sampl
   return lds->found;
 }
 
+// u of the total; u < 1 and total >= 2^s: the product stays below the total.
+__device__ __forceinline__ u64 sample_target(const SampleRow& r, u64 total) {
+  return min((u64)(r.u * (double)total), total - 1);
+}
+__device__ __forceinline__ void sample_out(const SampleArgs& a, uint32_t row, const SampleScale& scale, float l, uint32_t token, u64 total) {
+  a.tokens[row] = (int32_t)token;
+  if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(l) - log(__builtin_ldexp((double)total, -a.up)));
+}
+
 __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
-  __shared__ u64 keys[kPickThreads], masses[kPickThreads];
+  constexpr uint32_t kStep = 256, kScan = 8;  // of the last part
+  __shared__ alignas(16) u64 keys[kPickThreads];
+  __shared__ u64 masses[kPickThreads];
+  __shared__ u64 scan[kPickThreads / 64][kScan][64];
   __shared__ u64 lds[kPickThreads / 64];
   __shared__ SampleBorderLds border_lds;
   __shared__ SelectLds select_lds;
@@ -623,33 +670,69 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   s.thr = 0;
   s.max = scale.top;
   s.token_bits = a.vocab > 1 ? 32 - __builtin_clz(a.vocab - 1) : 0;
-  if (b.small && list.n > kPickThreads) {
-    // More tokens in top-k's bin than there is room for: the k largest alone.
-    s.bin = kNoBin;
-    const u64 least = sample_select<false>(list, s, scale, r.k, &select_lds);
-    if (t == 0) the_one = 0;
-    __syncthreads();
-    list.each(scale, [&](u64 key, u64) {
-      if (key >= least) keys[atomicAdd(&the_one, 1u)] = key;
-    });
-    __syncthreads();
-    list.n = r.k;
-    list.keys[0] = t < list.n ? keys[t] : 0ull;
-    bool kept;
-    list.masses[0] = scale.mass(SampleList::logit(list.keys[0]), &kept);
-    __syncthreads();
+  // Of more keys than a block sorts: top-k's last (of all where all of top-k are
+  // listed), then top-p's.
+  const bool border = b.small || b.k_bin != kNoBin || b.p_first != kNoBin;  // but min-p's
+  bool by_k = b.small || b.k_bin != kNoBin;
+  u64 own_k = 0;  // mass of top-k's bin that is kept
+#pragma unroll 1
+  for (bool more = border && list.n > kPickThreads; more;) {
+    u64 target = b.small ? r.k : r.k - b.k_before;
+    s.bin = b.small ? kNoBin : b.k_bin;
+    if (!by_k) {
+      target = share_of(r.top_p, b.k_mass + own_k);
+      u64 w = share.before;
+#pragma unroll
+      for (uint32_t j = 0; j < kPickBins; ++j) {
+        const uint32_t bin = kPickBins * t + j;
+        const u64 mass = bin == b.k_bin ? own_k : share.m[j];
+        if (w < target && target <= w + mass) {
+          the_one = bin;
+          the_rest = target - w;
+        }
+        w += mass;
+      }
+      __syncthreads();
+      s.bin = the_one;
+      target = the_rest;
+    }
+    thr = sample_select(list, s, scale, target, !by_k, &select_lds);
+    more = by_k && r.by_mass() && !b.small;
+    if (by_k && b.small) {
+      // The k largest alone.
+      if (t == 0) the_one = 0;
+      __syncthreads();
+      list.each(scale, [&](u64 key, u64) {
+        if (key >= thr) keys[atomicAdd(&the_one, 1u)] = key;
+      });
+      __syncthreads();
+      list.n = r.k;
+      list.keys[0] = t < list.n ? keys[t] : 0ull;
+      bool kept;
+      list.masses[0] = scale.mass(SampleList::logit(list.keys[0]), &kept);
+    } else if (more) {
+      s.thr = thr;
+      u64 sum = 0;
+      list.each(scale, [&](u64 key, u64 mass) { sum += s.in(key) ? mass : 0ull; });
+      own_k = block_sum<kPickThreads>(sum, lds);
+    }
+    by_k = false;
   }
-  if (!b.small && b.k_bin == kNoBin && b.p_first == kNoBin) {
-    // No border but min-p's.
-  } else if (list.n <= kPickThreads) {
+  if (border && list.n <= kPickThreads) {
     // Few keys: sorted by counting the larger ones, which puts the bins in order
     // and top-k's last.
-    const u64 key = list.keys[0];
+    const u64 key = t < list.n ? list.keys[0] : 0ull;
+    __syncthreads();
     keys[t] = key;
     __syncthreads();
     uint32_t rank = 0;
-#pragma unroll 8
-    for (uint32_t i = 0; i < list.n; ++i) rank += keys[i] > key;
+    if ((t & ~63u) < list.n) {
+#pragma unroll 4
+      for (uint32_t i = 0; i < list.n; i += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + i);
+        rank += (two.x > key) + (two.y > key);
+      }
+    }
     __syncthreads();
     if (t < list.n) {
       keys[rank] = key;
@@ -672,33 +755,23 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
       last = (uint32_t)block_sum<kPickThreads>(kept, lds);
     }
     thr = keys[last - 1];  // the first key of top-k's or top-p's bin is kept
-  } else {
-    u64 own = 0;  // mass of top-k's bin that is kept
-    if (b.k_bin != kNoBin) {
-      s.bin = b.k_bin;
-      thr = s.thr = sample_select<false>(list, s, scale, r.k - b.k_before, &select_lds);
-      if (r.by_mass()) {
-        u64 sum = 0;
-        list.each(scale, [&](u64 key, u64 mass) { sum += s.in(key) ? mass : 0ull; });
-        own = block_sum<kPickThreads>(sum, lds);
-      }
-    }
-    if (r.by_mass()) {
-      const u64 target = share_of(r.top_p, b.k_mass + own);
-      u64 w = share.before;
-#pragma unroll
-      for (uint32_t j = 0; j < kPickBins; ++j) {
-        const uint32_t bin = kPickBins * t + j;
-        const u64 mass = bin == b.k_bin ? own : share.m[j];
-        if (w < target && target <= w + mass) {
-          the_one = bin;
-          the_rest = target - w;
-        }
-        w += mass;
-      }
+    if (b.small) {
+      // All that may be kept is here: the token by the masses of lower tokens.
+      bool kept;
+      if (r.min_p > 0.0) scale.mass(SampleList::logit(mine), &kept);
+      const u64 w = t < last && (r.min_p <= 0.0 || kept) ? here : 0ull;
+      masses[t] = w;
       __syncthreads();
-      s.bin = the_one;
-      thr = sample_select<true>(list, s, scale, the_rest, &select_lds);
+      u64 before = 0, total = 0;
+#pragma unroll 4
+      for (uint32_t i = 0; i < last; ++i) {
+        const u64 m = masses[i];
+        total += m;
+        before += key_token(keys[i]) < key_token(mine) ? m : 0ull;
+      }
+      const u64 target = sample_target(r, total);
+      if (before <= target && target < before + w) sample_out(a, row, scale, SampleList::logit(mine), key_token(mine), total);
+      return;
     }
   }
   // Every slice's kept mass: what is certain, and what of the list is kept.
@@ -712,9 +785,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   const u64 own = t < a.slices ? kept_of[t] : 0ull;
   u64 total;
   u64 before = block_before<kPickThreads>(own, &total, lds);
-  // u < 1 and total >= 2^s: the product stays below the total.
-  u64 target = (u64)(r.u * (double)total);
-  target = min(target, total - 1);
+  u64 target = sample_target(r, total);
   if (before <= target && target < before + own) {
     the_one = t;
     the_rest = target - before;
@@ -722,11 +793,11 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   __syncthreads();
   const uint32_t slice = the_one;
   target = the_rest;
-  // Each wave has a stretch of the slice, 256 tokens at a time; then the wave in
-  // whose stretch the sum passes u goes through it again.
+  // Each wave has a stretch of the slice, 256 tokens a step; then the wave in
+  // whose stretch the sum passes u looks for the step and the token. The masses
+  // of the first steps stay in LDS.
   const float* const l = a.logits + (uint64_t)row * a.vocab;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
-  constexpr uint32_t kStep = 256;
   const uint32_t stretch = (a.slice / (kPickThreads / 64) + kStep - 1) / kStep * kStep;
   const uint32_t begin = slice * a.slice, from = begin + min(a.slice, wave * stretch);
   const uint32_t to = min(min(a.vocab, begin + a.slice), from + stretch);
@@ -744,12 +815,15 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   };
   u64 sum = 0;
   f32x4 next = sample_load(l, from + lane * 4, a.vocab);
-  for (uint32_t i = from; i < to; i += kStep) {
+#pragma unroll 1
+  for (uint32_t i = from, step = 0; i < to; i += kStep, ++step) {
     const f32x4 v = next;
     next = sample_load(l, i + kStep + lane * 4, a.vocab);
     u64 m[4];
     masses_at(v, i + lane * 4, m);
-    sum += m[0] + m[1] + m[2] + m[3];
+    const u64 own4 = m[0] + m[1] + m[2] + m[3];
+    if (step < kScan) scan[wave][step][lane] = own4;
+    sum += own4;
   }
   sum = wave_scan_u64(sum);
   if (lane == 63) lds[wave] = sum;
@@ -760,35 +834,46 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     target -= m;
   }
   if (target >= lds[wave]) return;
-  for (uint32_t i = from;; i += kStep) {
+#pragma unroll 1
+  for (uint32_t i = from, step = 0; i < to; i += kStep, ++step) {
     const f32x4 v = sample_load(l, i + lane * 4, a.vocab);
-    u64 m[4];
-    masses_at(v, i + lane * 4, m);
-    const u64 own4 = m[0] + m[1] + m[2] + m[3];
-    const u64 upto = wave_scan_u64(own4);
-    const u64 here = __ballot(target < upto);
-    if (here) {
-      if (lane == (uint32_t)__builtin_ctzll(here)) {
-        u64 at = upto - own4;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          if (target >= at && target < at + m[j]) {
-            a.tokens[row] = (int32_t)(i + lane * 4 + j);
-            if (a.logprobs) a.logprobs[row] = (float)(scale.log_mass(v[j]) - log(__builtin_ldexp((double)total, -a.up)));
-          }
-          at += m[j];
-        }
-      }
-      return;
+    u64 m[4], own4;
+    if (step < kScan) {
+      own4 = scan[wave][step][lane];
+    } else {
+      masses_at(v, i + lane * 4, m);
+      own4 = m[0] + m[1] + m[2] + m[3];
     }
-    target -= (u64)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    const u64 upto = wave_scan_u64(own4), here = __ballot(target < upto);
+    if (!here) {
+      target -= (u64)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+      continue;
+    }
+    masses_at(v, i + lane * 4, m);
+    if (lane == (uint32_t)__builtin_ctzll(here)) {
+      u64 before4 = upto - own4;
+      float l_at = 0.f;
+      uint32_t token = 0;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        if (target >= before4 && target < before4 + m[j]) l_at = v[j], token = i + lane * 4 + j;
+        before4 += m[j];
+      }
+      sample_out(a, row, scale, l_at, token, total);
+    }
+    return;
   }
 }
 
-// Slices of whole thousands, about a thousand blocks in all.
+// Slices of whole thousands (of 1024), for about a thousand blocks in all but
+// not above five each: longer ones leave the pick much to go through alone and
+// the CUs with blocks that end far apart (10 thousands: 64 rows of 151936 62 us
+// instead of 54; 38: 256 rows 209 instead of 124), shorter ones are mostly
+// prologue (one thousand instead of two: 64 rows of 32000 37 us instead of 34;
+// two instead of five: 64 rows of 151936 61).
 static void sample_slices(uint32_t n, uint32_t vocab, uint32_t* slice, uint32_t* slices) {
-  const uint32_t want = n >= 1024 ? 1 : n * kSampleSlices <= 1024 ? kSampleSlices : 1024 / n;
-  *slice = ((vocab + want - 1) / want + 1023) / 1024 * 1024;
+  const uint32_t want = n >= 1024 ? 1 : min(kSampleSlices, 1024 / n), most = max(5u, (vocab + kSampleSlices * 1024 - 1) / (kSampleSlices * 1024));
+  *slice = min(most, ((vocab + want - 1) / want + 1023) / 1024) * 1024;
   *slices = (vocab + *slice - 1) / *slice;
 }
 
