@@ -766,9 +766,10 @@ uint64_t smoe_sample_workspace_size(uint32_t n_rows, uint32_t vocab);
  * the token is the first, by rising token, at which the kept e's running sum
  * exceeds u times their sum. Temperature 0: the first of the order. A logit of
  * -inf or NaN is never kept; a row with +inf has e = 1 there and 0 elsewhere.
- * e is computed in f64 and held as an integer of 2^-s, s = 62 - bits of vocab (44
- * for 2^18 tokens) but at most 51, so sums do not depend on their order and borders within
- * 2^-s of the sum are told by the rounded values.
+ * e is computed in f64, to 2^-44 of it (0 below 2^-70), and held as an integer of
+ * 2^-s, s = 62 - bits of vocab (44 for 2^18 tokens) but at most 51: sums do not
+ * depend on their order, and a border that lies closer than these roundings to
+ * top_p, min_p or u is told by the rounded values.
  * logits: device f32[n_rows, vocab], 16-byte aligned; temperature, top_p, min_p,
  * u: device f32[n_rows], top_k: device int32[n_rows]; temperature NULL: 1, top_k
  * NULL: 0, top_p NULL: 1, min_p NULL: 0. out_tokens: device int32[n_rows];
