@@ -740,9 +740,10 @@ uint64_t smoe_attn_decode_workspace_size(const smoe_kv_cache* cache, uint32_t n_
  * are f32. A padding row gives zeros; so do a row whose scores are all -inf and
  * a token whose sequence or position is out of range; a page out of range is
  * left out (the next smoe_sync returns SMOE_ERR_INVALID_ARG for these two). What
- * an infinity or NaN in a query, key or value makes shows in the rows that see
- * it only. n_heads a multiple of cache->n_heads, up to
- * 4096. The last bits of a row depend on the lengths of the call's other rows.
+ * an infinity or NaN in a query, key or value makes (an infinity may act as a
+ * NaN) shows in the rows that see it only; scores beyond 2e38 may count as
+ * infinite. n_heads a multiple of cache->n_heads, up to 4096. The last bits of a
+ * row depend on the lengths of the call's other rows.
  * out and the workspace overlap nothing (SMOE_ERR_INVALID_ARG); workspace:
  * device, 256-byte aligned, one call's at a time. Enqueue-only, allocates
  * nothing, capturable in a HIP graph. */

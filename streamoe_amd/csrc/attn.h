@@ -247,6 +247,8 @@ __global__ __launch_bounds__(256, attn_blocks_per_cu(D)) void k_attn(AttnArgs a)
       const attn_u64 at = (chunk_at + chunk.before) * tiles;
       const attn_u64 here = __ballot(at <= x && x < at + (attn_u64)chunk.units * tiles);
       if (!here) {
+        // (Not behind the last token, should positions change meanwhile.)
+        if (chunk.first + 64 >= n) return false;
         chunk_at += chunk.all();
         chunk.load(a, chunk.first + 64);
         continue;

@@ -423,13 +423,13 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
     const u64* const own = a.slice_mass + (uint64_t)blockIdx.x * kSampleBins;
     for (uint32_t i = t; i < certain; i += kSampleThreads) sum += own[i];
   }
-  // Distances of what has to be looked at (most logits are behind it). Beside
-  // +inf (distances of infinity and NaN) all.
+  // Distances of what has to be looked at (most logits are behind it). A NaN
+  // bounds none: distances of finite logits may be infinite, those beside +inf
+  // are infinity and NaN.
   const uint32_t last = b.end();
   const float near = !masses || certain == 0 || scale.infinite ? -INFINITY : sample_bin_from(certain);
-  const float far = scale.infinite                                           ? __builtin_nanf("")
-                    : last == kNoBin || (b.small && b.k_bin == kNoBin) ? INFINITY
-                                                                             : sample_bin_from(last);
+  const bool no_far = scale.infinite || last == kNoBin || (b.small && b.k_bin == kNoBin);
+  const float far = no_far ? __builtin_nanf("") : sample_bin_from(last);
   // Nothing to list: the slice need not be read.
   if (certain < kNoBin) fours.go([&](f32x4 v, uint32_t i) {
     u64 hits[4];
@@ -775,7 +775,10 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
       return;
     }
   }
-  // Every slice's kept mass: what is certain, and what of the list is kept.
+  // Every slice's kept mass: what is certain, and what of the list is kept. (The
+  // slice and the rest are numbers whatever happens: logits that another stream
+  // writes meanwhile give a wrong token, not a read outside of the row.)
+  if (t == 0) the_one = 0, the_rest = 0;
   __syncthreads();
   list.each(scale, [&](u64 key, u64 mass) {
     bool kept = true;

@@ -176,6 +176,29 @@ def test_replayed_with_eager_work_between(kernels, bits):
         other.pos += other.one
 
 
+def test_two_graphs_share_workspaces(kernels):
+    """Captured steps of two batches with the same workspaces, replayed in turn."""
+    import torch
+
+    import streamoe_amd as sa
+
+    a, b = Step(kernels, 8, 16), Step(kernels, 9, 8)
+    b.aws, b.sws = a.aws, a.sws
+    graphs = [sa.capture_graph(kernels, s.run) for s in (a, b)]
+    for i in range(4):
+        for s, graph in ((a, graphs[0]), (b, graphs[1])):
+            s.x.normal_()
+            s.u.uniform_(0, 0.999)
+            before = s.all_held()
+            graph.replay()
+            if i % 2:
+                a.aws.fill_(255)  # holds nothing between calls
+                a.sws.fill_(255)
+            torch.cuda.synchronize()
+            s.check(before)
+            s.pos += s.one
+
+
 def test_two_handles_at_once(kernels):
     import torch
 

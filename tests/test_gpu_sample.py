@@ -164,6 +164,34 @@ def test_rows_of_all_kinds(kernels, kind):
     _check(kernels, l, t, k, p, m, u, apart=1e-9)
 
 
+@pytest.mark.parametrize("V", [700, 5003, 40001])
+def test_logits_further_apart_than_f32_goes(kernels, V):
+    """Distances from the largest overflow, logits and masses do not."""
+    rng = np.random.default_rng(V + 1)
+    n = 10
+    l = ((rng.random((n, V)) * 2 - 1) * 3.3e38).astype(np.float32)
+    l[:, ::7] = -np.inf
+    t = [3e38, 1e38, 3e38, 3e38, 1.0, 3e38, 1e38, 3e38, 3e38, 3e38]
+    k = [0, 0, V // 2, V * 4 // 5, V // 2, 300, 448, 449, V // 3, 0]
+    p = [1.0, 0.9, 0.9, 1.0, 1.0, 0.99, 1.0, 0.99, 1.0, 0.999]
+    m = [0.0, 0.0, 0.0, 0.0, 0.0, 0.1, 0.0, 0.0, 0.3, 0.2]
+    _check(kernels, l, t, k, p, m, rng.random(n), apart=1e-9)
+
+
+def test_extreme_numbers(kernels):
+    rng = np.random.default_rng(66)
+    V = 3001
+    l = np.round(rng.standard_normal((12, V)) * 4, 1)
+    l[:, 17] = l.max(1)  # two largest at least
+    top = np.float32(1 - 2.0 ** -24)
+    t = [1e-40, 1e-38, 3e38, 1.0, 1.0, 1.0, 1e-3, 1.0, 1.0, 1.0, 1e-45, 0.5]
+    k = [0, 5, 0, 2 ** 31 - 1, -2 ** 31, V, 0, V - 1, 0, 0, 600, 600]
+    p = [1.0, 1e-38, 1.0, np.finfo(np.float32).max, 1.0, np.inf, 0.5, 0.999, 1e-45, top, 0.5, 1.0]
+    m = [1e-45, 1.0, 0.0, 1.0, 1e-38, 0.0, 1.0, 0.0, 0.0, 0.0, 0.0, 1e-30]
+    u = [top, 0.0, 0.3, top, 1e-45, top, 0.4, 0.7, 0.2, 0.6, 0.9, top]
+    _check(kernels, l, t, k, p, m, u, apart=None)
+
+
 def test_rows_without_a_value_and_bad_numbers(kernels):
     import streamoe_amd as sa
 
