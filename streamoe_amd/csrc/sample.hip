@@ -42,6 +42,9 @@ constexpr uint32_t kSampleThreads = 256, kPickThreads = 512;
 constexpr uint32_t kSampleSlices = 128;  // of a row at most
 constexpr uint32_t kCountStride = kSampleBins + 4;
 constexpr uint32_t kNoBin = kSampleBins;
+// Longer lists are not sorted but selected from (16 rows of wide nuclei, lists of
+// 360 to 770: 27 us; with up to 512 sorted 30; up to 64 as here).
+constexpr uint32_t kSort = 256;
 constexpr uint32_t kSmallK = 448;  // with the tokens that share its bin, mostly, a block's threads
 
 // Bin of a logit, 0 the largest's; least distance of a bin (not of 0).
@@ -551,8 +554,8 @@ struct SampleList {
 struct SamplePlaces {
   u64 thr;              // only keys from it on
   float max;
-  uint32_t bin, first;  // kNoBin: all of them; the bin's largest logit in the list
-  uint32_t token_bits;
+  uint32_t bin, end;    // kNoBin: all of them, up to bin end; else the same
+  uint32_t first, token_bits;
   __device__ bool in(u64 key) const { return bin == kNoBin || (key >= thr && sample_bin(max, ord_float((uint32_t)(key >> 32))) == bin); }
   __device__ u64 place(u64 key) const { return (u64)(first - (uint32_t)(key >> 32)) << token_bits | key_token(key); }
   __device__ u64 key(u64 p) const {
@@ -567,22 +570,24 @@ struct SelectLds {
   uint32_t count[1u << kDigit];
   u64 part[kPickThreads / 64];
   u64 prefix, rest, found;
-  uint32_t left;
+  u64 few[64], few_weight[64];
+  uint32_t left, n_few;
 };
 // Key of the first place up to which the weights (masses, or 1 each) add up to
 // `target` or more, digit after digit of the places from the top; there is one.
+// When 64 keys or fewer share the digits, a wave compares them with one another:
+// two digits less, 1.2 us each, for 1.
 __device__ __forceinline__ u64 sample_select(const SampleList& list, SamplePlaces s, const SampleScale& scale, u64 target, bool by_mass,
                                              SelectLds* lds) {
   const uint32_t t = threadIdx.x;
-  // What the bin's entries span.
-  u64 hi = 0, lo = 0;  // lo: of complements
-  list.each(scale, [&](u64 key, u64) {
-    if (s.in(key)) hi = max(hi, key), lo = max(lo, ~key);
-  });
-  hi = block_max<kPickThreads>(hi, lds->part);
-  lo = ~block_max<kPickThreads>(lo, lds->part);
-  s.first = (uint32_t)(hi >> 32);
-  const uint32_t span = s.first - (uint32_t)(lo >> 32);
+  // The values that the bins may hold, to within more than a distance's rounding.
+  s.first = float_ord(s.max);
+  uint32_t last = kOrdNegInf;
+  if (!scale.infinite) {
+    if (s.bin != kNoBin && s.bin) s.first = float_ord((float)(scale.max - sample_bin_from(s.bin) * (1 - 0x1p-22))) + 1;
+    if (s.end < kSampleBins - 1) last = float_ord((float)(scale.max - sample_bin_from(s.end + 1) * (1 + 0x1p-22))) - 1;
+  }
+  const uint32_t span = s.first - last;
   int shift = (int)((span ? 32 - __builtin_clz(span) : 0) + s.token_bits);
   u64 prefix = 0;  // the digits above shift
   for (;;) {
@@ -590,6 +595,7 @@ __device__ __forceinline__ u64 sample_select(const SampleList& list, SamplePlace
     shift -= width;
     lds->weight[t] = 0;
     lds->count[t] = 0;
+    if (t == 0) lds->n_few = 0;
     __syncthreads();
     list.each(scale, [&](u64 key, u64 mass) {
       const u64 p = s.place(key);
@@ -611,13 +617,23 @@ __device__ __forceinline__ u64 sample_select(const SampleList& list, SamplePlace
     prefix = lds->prefix;
     target = lds->rest;
     if (shift == 0) return s.key(prefix);
-    if (lds->left == 1) break;
+    if (lds->left <= 64) break;
     __syncthreads();
   }
-  // One place has these digits.
-  list.each(scale, [&](u64 key, u64) {
-    if (s.in(key) && s.place(key) >> shift == prefix) lds->found = key;
+  list.each(scale, [&](u64 key, u64 mass) {
+    if (!s.in(key) || s.place(key) >> shift != prefix) return;
+    const uint32_t i = atomicAdd(&lds->n_few, 1u);
+    if (i < 64) lds->few[i] = key, lds->few_weight[i] = by_mass ? mass : 1ull;
   });
+  __syncthreads();
+  if (t < 64) {
+    const uint32_t n = min(lds->n_few, 64u);
+    const u64 key = lds->few[t], w = lds->few_weight[t];
+    u64 before = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < n; ++i) before += lds->few[i] > key ? lds->few_weight[i] : 0ull;
+    if (t < n && before < target && target <= before + w) lds->found = key;
+  }
   __syncthreads();
   return lds->found;
 }
@@ -671,15 +687,17 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
   s.thr = 0;
   s.max = scale.top;
   s.token_bits = a.vocab > 1 ? 32 - __builtin_clz(a.vocab - 1) : 0;
-  // Of more keys than a block sorts: top-k's last (of all where all of top-k are
+  // Of more keys than are sorted: top-k's last (of all where all of top-k are
   // listed), then top-p's.
   const bool border = b.small || b.k_bin != kNoBin || b.p_first != kNoBin;  // but min-p's
   bool by_k = b.small || b.k_bin != kNoBin;
   u64 own_k = 0;  // mass of top-k's bin that is kept
+  const bool sort = b.small || list.n <= kSort;
 #pragma unroll 1
-  for (bool more = border && list.n > kPickThreads; more;) {
+  for (bool more = border && (!sort || list.n > kPickThreads); more;) {
     u64 target = b.small ? r.k : r.k - b.k_before;
     s.bin = b.small ? kNoBin : b.k_bin;
+    s.end = b.k_bin;
     if (!by_k) {
       target = share_of(r.top_p, b.k_mass + own_k);
       u64 w = share.before;
@@ -694,7 +712,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
         w += mass;
       }
       __syncthreads();
-      s.bin = the_one;
+      s.bin = s.end = the_one;
       target = the_rest;
     }
     thr = sample_select(list, s, scale, target, !by_k, &select_lds);
@@ -719,7 +737,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a) {
     }
     by_k = false;
   }
-  if (border && list.n <= kPickThreads) {
+  if (border && sort) {
     // Few keys: sorted by counting the larger ones, which puts the bins in order
     // and top-k's last.
     const u64 key = t < list.n ? list.keys[0] : 0ull;
