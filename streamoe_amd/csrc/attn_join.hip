@@ -7,7 +7,7 @@ namespace smoe {
 // A block joins a share (blockIdx.y) of one group's columns: fours of dims, each
 // by 256 / lanes threads that go through the parts in turn and are added up at
 // the end. Parts are added in their order, so a call gives the same bits again.
-// 4 to 6 us: the launch and a chain of three loads (the units before the group,
+// 4 to 5 us: the launch and a chain of three loads (the units before the group,
 // then m, l and the outputs of its parts, a few MB); where a row is cut into 128
 // parts, 64 blocks share its columns. The last block of a group joining them
 // would need counters that start at zero, which the workspace has not.

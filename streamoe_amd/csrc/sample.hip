@@ -29,7 +29,7 @@
 // later passes find most of them in the memory-side cache. What bounds the four
 // is: top, the reads, 9 us at 64 rows; bins, the series in f64 and the additions
 // in LDS, 14; list, three comparisons a logit, 13; pick, one block's chain of
-// loads, scans and selections, 18 (one row: 2.7, 4.5, 5.5 and 6.6).
+// loads, scans and selections, 16 (one row: 2.7, 4.4, 5.5 and 6.5).
 #include "common.h"
 #include "kernels.h"
 
