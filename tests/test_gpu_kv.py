@@ -118,7 +118,7 @@ def test_gather(kernels, heads, dim, page, bits, out_bf16, layout):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
-@pytest.mark.parametrize("n", [1, 2, 300, 1000, 5001, 16384])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 300, 1000, 1025, 1030, 2049, 5001, 16384])
 def test_the_last_of_a_position_stays(kernels, bits, n):
     """Few positions, named over and over: each holds its last row, whole."""
     import torch
