@@ -21,7 +21,8 @@ LIB = os.path.join(HERE, "libsmoe.so")
 SOURCES = ["api.hip", "attn_bf16.hip", "attn_i8.hip", "attn_join.hip", "beam.hip", "cache.hip", "decode.hip",
            "fused.hip", "limb.hip", "loader.hip", "lora.hip", "norm.hip", "phase.hip", "prefill.hip", "router.hip",
            "rows8_q3.hip", "rows8_q4.hip", "rows8_q8.hip", "sample.hip", "synth.hip"]
-HEADERS = ["attn.h", "common.h", "handle.h", "kernels.h", "kv.h", "rows8.h", os.path.join("..", "..", "include", "smoe.h")]
+HEADERS = ["attn.h", "attn_plan.h", "common.h", "handle.h", "kernels.h", "kv.h", "rows8.h",
+           os.path.join("..", "..", "include", "smoe.h")]
 ARCH = "gfx950"
 
 FLAGS = [
