@@ -82,7 +82,7 @@ __device__ __forceinline__ attn_u64 attn_from(attn_u64 units, uint32_t block, ui
 __device__ __forceinline__ uint32_t attn_block_of(attn_u64 x, attn_u64 units, uint32_t blocks_log) {
   if (!(units >> blocks_log)) return (uint32_t)x;
   const attn_u64 y = ((x + 1) << blocks_log) - 1;
-  return y >> 32 ? (uint32_t)(y / units) : (uint32_t)y / (uint32_t)units;
+  return (y | units) >> 32 ? (uint32_t)(y / units) : (uint32_t)y / (uint32_t)units;
 }
 
 // A block's place in the list of units, the same in all of its waves.

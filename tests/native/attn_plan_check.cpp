@@ -182,8 +182,42 @@ static void plans(unsigned seed) {
   }
 }
 
+// attn_block_of against attn_from, whose blocks are wide integers' quotients: units
+// next to the blocks' borders and far from them, totals of few units to the most
+// that a call can have (16384 rows of 2^30 positions and 482 tiles each, below 2^49).
+static void blocks() {
+  std::mt19937_64 rng(1);
+  std::vector<uint64_t> totals = {1, 255, 256, 257, 511, 512, 513, 70001, (1ull << 32) + 786432, (1ull << 32) + 5000};
+  for (int bit = 20; bit <= 48; ++bit)
+    for (int64_t off : {-513, -1, 0, 1, 2, 511, 512}) totals.push_back((1ull << bit) + (uint64_t)off);
+  for (int i = 0; i < 500; ++i) totals.push_back(1 + (rng() >> (15 + rng() % 48)));
+  for (uint64_t total : totals)
+    for (uint32_t log : {8u, 9u}) {
+      const uint32_t n = 1u << log;
+      std::vector<uint64_t> units;
+      for (uint32_t b = 0; b <= n; ++b) {
+        const uint64_t from = attn_from(total, b, log);
+        const uint64_t want = total < n ? std::min<uint64_t>(b, total) : (uint64_t)((unsigned __int128)total * b >> log);
+        CHECK(from == want, "total %llu block %u", (unsigned long long)total, b);
+        for (uint64_t x : {from - 1, from, from + 1}) units.push_back(x);
+      }
+      for (int i = 0; i < 2000; ++i) units.push_back(rng() >> (rng() % 64));
+      for (uint64_t x : units) {
+        if (x >= total) continue;
+        const uint32_t b = attn_block_of(x, total, log);
+        CHECK(b < n && attn_from(total, b, log) <= x && x < attn_from(total, b + 1, log), "unit %llu of %llu: block %u of %u",
+              (unsigned long long)x, (unsigned long long)total, b, n);
+      }
+    }
+}
+
 int main(int argc, char** argv) {
-  for (int i = 1; i < argc; ++i) plans((unsigned)atoi(argv[i]));
+  for (int i = 1; i < argc; ++i) {
+    if (!strcmp(argv[i], "blocks"))
+      blocks();
+    else
+      plans((unsigned)atoi(argv[i]));
+  }
   printf("failures=%d\n", failures);
   return failures != 0;
 }

@@ -22,3 +22,9 @@ def checker(tmp_path_factory):
 def test_every_unit_has_one_block_and_waves_agree(checker, seed):
     r = subprocess.run([checker, str(seed)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_a_unit_s_block_and_a_block_s_units_agree(checker):
+    """Totals up to the most that a call can have, past 32 bits."""
+    r = subprocess.run([checker, "blocks"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
