@@ -59,7 +59,7 @@ struct AttnChunk {
     wrong = in && seq != -1 && !(seq_in && (uint32_t)pos < a.t.positions);
     int32_t lo, hi;
     attn_range(a, seq_in && n, max(pos, 0), &lo, &hi);
-    hi = min(pos + (int32_t)n - 1, (int32_t)a.t.positions - 1);
+    hi = min((int32_t)((uint32_t)pos + n - 1), (int32_t)a.t.positions - 1);  // pos + n may pass 2^31
     units = seq_in && n && hi >= max(pos, 0) ? (uint32_t)hi / kAttnUnit - (uint32_t)lo / kAttnUnit + 1 + kAttnOver : 0u;
     before = wave_scan_u64(units) - units;
   }

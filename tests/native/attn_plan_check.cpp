@@ -166,6 +166,21 @@ static void plans(unsigned seed) {
       check_plan(what, a, seq, pos, order);
     }
   }
+  // Positions next to the largest number, alone, in runs, and before others.
+  for (uint32_t together : {1u, 2u, 16u}) {
+    AttnArgs a{};
+    a.blocks_log = 2;
+    a.c.heads = a.parts = 1;
+    a.together = together;
+    a.t.n_seqs = 2;
+    a.t.positions = 1u << 30;
+    const std::vector<int32_t> seq = {0, 0, 0, 1, 1, 1, 1, -1, 0, 0, 1};
+    const std::vector<int32_t> pos = {INT32_MAX, INT32_MAX - 1, INT32_MAX, 100, INT32_MIN, INT32_MIN + 1, INT32_MAX, 0, -1, 0, (1 << 30) - 1};
+    check_plan("positions that are far", a, seq, pos, orders[0]);
+    a.t.positions = 4096;
+    a.window = 100;
+    check_plan("positions that are far, a window", a, seq, pos, orders[0]);
+  }
   // Nothing but padding, and one row that sees something behind it.
   for (uint32_t n : {5u, 64u, 65u, 300u}) {
     AttnArgs a{};
