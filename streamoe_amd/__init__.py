@@ -610,8 +610,8 @@ class Kernels:
         cc, dev, either = cache.c(), self.device, _types("f32_bf16")
         tc = self._kv_tokens(cache, table, seq, pos, n_tokens)
         step = _row_stride(q, either, n_tokens, n_heads * cc.head_dim, dev)
-        if (tc is None or step is None or window < 0 or not _fits(out, either, n_tokens * n_heads * cc.head_dim, dev)
-                or not _dense(workspace, dev)):
+        if (tc is None or step is None or not 0 <= window < 1 << 32
+                or not _fits(out, either, n_tokens * n_heads * cc.head_dim, dev) or not _dense(workspace, dev)):
             return _INVALID
         return _lib.smoe_attn_decode(self.h, cc, tc, q.data_ptr(), q.element_size() == 2, step, n_heads, scale, window,
                                      out.data_ptr(), out.element_size() == 2, _at(workspace), workspace.nbytes)
