@@ -664,7 +664,9 @@ int smoe_beam_reorder(smoe_handle* h, const smoe_beam_state* states, uint32_t n_
  * i * slot_stride, head_dim values in bf16 (bits 16), or in 8 bits (bits 8):
  * int8 codes with one f32 scale per row, value = code * scale, scales in
  * k_scales (v_scales) [n_pages, n_heads, page_size]. Pages, heads and slots may
- * lie in any order, keys and values in one buffer or two; no two rows overlap.
+ * lie in any order, keys and values in one buffer or two, as long as these four
+ * axes nest (each one's stride spans all of those with smaller ones): no two rows
+ * overlap.
  * A cache that is no pool of pages is one page per sequence. */
 typedef struct {
   void* k;              /* device, 16-byte aligned */
@@ -730,8 +732,11 @@ uint64_t smoe_attn_decode_workspace_size(const smoe_kv_cache* cache, uint32_t n_
  * position included:
  *   out[t, h] = sum_p w_p v[p, h / g] / sum_p w_p,  w_p = exp(scale * q[t, h] . k[p, h / g])
  * over pos[t] - window < p <= pos[t] (window 0: from 0 on), g = n_heads /
- * cache->n_heads. Tokens of one sequence at positions that follow one
- * another share reads of the cache; each sees its own positions only, whatever the others' hold.
+ * cache->n_heads. Tokens of one sequence at positions that follow one another
+ * share reads of the cache: as many as fit into 16 columns with their g heads, a
+ * power of two, from a row t on that is a multiple of it. Each sees its own
+ * positions only, whatever the others' hold. A prompt is taken so, too, its prefix
+ * read again for every 16 columns.
  * q: device rows of n_heads * head_dim values, bf16 when q_is_bf16 else f32,
  * q_stride elements from one token's to the next, 16-byte aligned; out: device
  * [n_tokens, n_heads, head_dim], bf16 when out_is_bf16 else f32, 16-byte aligned.
@@ -781,8 +786,9 @@ uint64_t smoe_sample_workspace_size(uint32_t n_rows, uint32_t vocab);
  * the latter the next smoe_sync returns SMOE_ERR_INVALID_ARG. n_rows up to 65535, vocab
  * up to 2^24 (SMOE_ERR_UNSUPPORTED_SHAPE). Outputs and workspace overlap nothing
  * (SMOE_ERR_INVALID_ARG); workspace: device, 256-byte aligned, one call's at a
- * time. The same bits on every run. Enqueue-only, allocates nothing, capturable
- * in a HIP graph. No counterpart in the reference, whose sampling is greedy
+ * time, 8 bytes for every logit and 5 KB for every one to five thousand (88 MB for
+ * 64 rows of 151936, 2 for one). The same bits on every run. Enqueue-only,
+ * allocates nothing, capturable in a HIP graph. No counterpart in the reference, whose sampling is greedy
  * (io/gpu_lm_head.rs:130-193). */
 int smoe_sample(smoe_handle* h, const float* logits, const float* temperature, const int32_t* top_k,
                 const float* top_p, const float* min_p, const float* u, uint32_t n_rows, uint32_t vocab,

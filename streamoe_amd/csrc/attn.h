@@ -30,7 +30,7 @@
 // vector units 14 and 19. 61 rows of up to 9001 positions in 8 bits, 154 MB, take
 // 39 us, 3.9 TB/s: twice the positions to a byte (vector units 32 %) and a part
 // more per row. Short ones are bound by the chain plan, table, keys, values,
-// exchange: 700 positions 9.5 us, a window of 1000 in 8 sequences 15.
+// exchange: 700 positions 9.6 us, a window of 1000 in 8 sequences 15.
 #pragma once
 
 #include <type_traits>
@@ -47,7 +47,9 @@ typedef float af32x8 __attribute__((ext_vector_type(8), aligned(16)));
 constexpr float kAttnNone = -3.0e38f;   // maximum of no scores
 
 // Waves per SIMD that the kernel's registers leave room for, so blocks per CU:
-// keys, values and outputs of dims up to 256 alone take 192 of a wave's.
+// keys, values and outputs of dims up to 256 alone take 192 of a wave's in bf16; 128
+// in 8 bits, where the kernel as a whole still has 380 to 392. No vector register is
+// spilled; 112 to 143 scalars (the plan, spans, arguments) lie in vector lanes.
 constexpr uint32_t attn_blocks_per_cu(uint32_t d) { return d == 256 ? 1 : 2; }
 constexpr uint32_t kAttnCus = 256;
 

@@ -9,8 +9,9 @@ namespace smoe {
 // the end. Parts are added in their order, so a call gives the same bits again.
 // 4 to 5 us: the launch and a chain of three loads (the units before the group,
 // then m, l and the outputs of its parts, a few MB); where a row is cut into 128
-// parts, 64 blocks share its columns. The last block of a group joining them
-// would need counters that start at zero, which the workspace has not.
+// parts, 64 blocks share its columns. The last block of a group joining them would
+// need counters that start at zero: the workspace holds anything, the handle's
+// memory could have them if each group's last block put its own back.
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t pad) {
   __shared__ f32x4 sum[256];
   __shared__ float2 stat[256];
@@ -110,9 +111,9 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, uint32_t pad) {
 hipError_t launch_attn_join(const AttnArgs& a, hipStream_t st) {
   const uint32_t items = a.t.n * a.c.heads * a.parts;
   // A share of eight fours where there are few rows to join, whole groups where
-  // there are many; a thousand blocks in all (61 rows of 2 key heads 47.3 us, with
-  // two thousand 49.7, 500 48.4; 8 sequences' 4 tokens each of 8 key heads 20.5, 21.7
-  // and 20.6).
+  // there are many; a thousand blocks in all (captured calls of 61 rows of 2
+  // key heads 48.8 us, with two thousand 49.4, 500 48.9; 48 rows of 16 key heads
+  // 55.6, 56.6 and 55.7; 8 sequences' 4 tokens each of 8 key heads 20.6, 22.0 and 22.3).
   const uint32_t most = (min(16u, a.group) * a.together * a.c.dim / 4 + 7) / 8, y = min(most, max(1u, 1024 / items));
   const uint32_t pad = a.c.dim <= 64 ? 64 : a.c.dim <= 128 ? 128 : 256;
   hipLaunchKernelGGL(k_attn_join, dim3(items, y), dim3(256), 0, st, a, pad);
