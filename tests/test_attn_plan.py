@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 
 @pytest.fixture(scope="module")
-def checker(tmp_path_factory):
+def program(tmp_path_factory):
     exe = str(tmp_path_factory.mktemp("plan") / "attn_plan_check")
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wno-unknown-pragmas", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-o", exe,
                     os.path.join(HERE, "native", "attn_plan_check.cpp")], check=True)
@@ -19,12 +19,12 @@ def checker(tmp_path_factory):
 
 
 @pytest.mark.parametrize("seed", range(3))
-def test_every_unit_has_one_block_and_waves_agree(checker, seed):
-    r = subprocess.run([checker, str(seed)], capture_output=True, text=True, timeout=300)
+def test_every_unit_has_one_block_and_waves_agree(program, seed):
+    r = subprocess.run([program, str(seed)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
 
 
-def test_a_unit_s_block_and_a_block_s_units_agree(checker):
+def test_a_unit_s_block_and_a_block_s_units_agree(program):
     """Totals up to the most that a call can have, past 32 bits."""
-    r = subprocess.run([checker, "blocks"], capture_output=True, text=True, timeout=300)
+    r = subprocess.run([program, "blocks"], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
