@@ -297,8 +297,8 @@ struct SampleBorder {
   __device__ uint32_t certain() const { return small ? 0u : min(min(k_bin, p_first), m_first); }  // bins below it are kept
   // Bins from it on are neither kept nor listed.
   __device__ uint32_t end() const {
-    uint32_t e = k_bin + 1;  // top-p's border is not behind it
-    if (k_bin == kNoBin) e = p_first == kNoBin ? 0u : p_last + 1;
+    if (k_bin == kNoBin && p_first == kNoBin) return m_first == kNoBin ? kNoBin : m_last + 1;
+    const uint32_t e = k_bin == kNoBin ? p_last + 1 : k_bin + 1;  // top-p's border is not behind top-k's
     return min(max(e, m_first == kNoBin ? 0u : m_last + 1), kNoBin);
   }
   __device__ bool listed(uint32_t bin) const {
@@ -433,8 +433,10 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs a) {
   const float near = !masses || certain == 0 || scale.infinite ? -INFINITY : sample_bin_from(certain);
   const bool no_far = scale.infinite || last == kNoBin || (b.small && b.k_bin == kNoBin);
   const float far = no_far ? __builtin_nanf("") : sample_bin_from(last);
-  // Nothing to list: the slice need not be read.
-  if (certain < kNoBin) fours.go([&](f32x4 v, uint32_t i) {
+  // Nothing to list, and masses of bins: the slice need not be read. (Without them
+  // the masses of all that is kept are formed here, also where no border was found:
+  // a top-k of more than there are.)
+  if (certain < kNoBin || !masses) fours.go([&](f32x4 v, uint32_t i) {
     u64 hits[4];
     uint32_t n = 0;
 #pragma unroll
